@@ -11,11 +11,28 @@ several experts of one rank): ``layout="rank_major"`` gives toks [n, max_tokens,
 index) and ``layout="flat"`` gives the received tokens packed as [n*max_tokens, hidden]; both also return the routing
 rows ``ep.recv_topk_idx`` (expert ids that are local to this rank, else -1) and ``ep.recv_topk_weights``. The caller
 applies its local experts and the weights and gives one pre-reduced row per received token to ``combine``.
+
+The rest of a mixture-of-experts layer, forward and backward, on the rows of the default layout (``fp8=False``):
+
+    idx, weights = ep.route(logits, topk, score="sigmoid", bias=balance, groups=8, keep_groups=4, group_score="top2", scale=2.5)
+    toks, _, counts = ep.dispatch(x, idx, weights, fp8=False)
+    pre = torch.empty(ep.El, ep.cap, 2 * ffn, dtype=torch.bfloat16, device="cuda")
+    act = ep.expert_linear(toks, w_gate_up, counts, activation="swiglu", pre=pre)       # w_gate_up [El, 2 * ffn, hidden]
+    y = ep.expert_linear(act, w_down, counts)                                           # w_down [El, hidden, ffn]
+    out = ep.combine(y)
+
+    rows = ep.dispatch_rows()                                                           # (before the next dispatch)
+    dy, dweights = ep.combine_backward(dout, y, weights, rows)
+    dact, dw_down, _ = ep.expert_linear_backward(dy, act, w_down, counts)
+    dtoks, dw_gate_up, _ = ep.expert_linear_backward(dact, toks, w_gate_up, counts, pre=pre, activation="swiglu")
+    dx = ep.dispatch_backward(dtoks, rows)
+    dlogits = ep.route_backward(dweights, logits, idx, score="sigmoid", scale=2.5)
 """
 import ctypes
+import functools
 
 from .. import _lib
-from ..core import INT64, current_stream
+from ..core import BF16, FP16, FP32, INT64, current_stream
 
 EP_MAGIC = 0xC00FFFEE
 TENSOR_MAGIC = 0xCAFECAFE
@@ -67,6 +84,11 @@ class CombIO(ctypes.Structure):
     _fields_ = [("size", ctypes.c_uint), ("magic", ctypes.c_uint), ("tokens", ctypes.POINTER(EpTensor)), ("topk_weights", ctypes.POINTER(EpTensor))]
 
 
+class RouteCfg(ctypes.Structure):
+    _fields_ = [("size", ctypes.c_uint), ("magic", ctypes.c_uint), ("score", ctypes.c_int), ("groups", ctypes.c_int), ("keep_groups", ctypes.c_int),
+                ("group_score", ctypes.c_int), ("renormalize", ctypes.c_int), ("scale", ctypes.c_float)]
+
+
 def _tensor(t, code):
     sizes = (ctypes.c_size_t * t.dim())(*t.shape)
     et = EpTensor(ctypes.sizeof(EpTensor), TENSOR_MAGIC, t.dim(), code, t.data_ptr(), None, 0, sizes)
@@ -82,6 +104,9 @@ def _hdr(s):
 
 class ExpertParallel:
     LAYOUTS = {"expert_major": 1, "rank_major": 2, "flat": 3}
+    SCORES = {"softmax": 0, "sigmoid": 1}
+    GROUP_SCORES = {"max": 0, "top2": 1}
+    ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "silu": 3, "swiglu": 4, "geglu": 5}
 
     def __init__(self, comm, num_experts, max_tokens, hidden, max_sms=0, timeout_ms=0, enable_mask=False, layout="expert_major"):
         import torch
@@ -123,6 +148,7 @@ class ExpertParallel:
         fast = _lib.fastcall()
         entries = [_lib.address(L, name) for name in ("b200EpDispatch", "b200EpCombine")]
         self._fast = (fast.invoke, *entries) if fast and all(entries) else None
+        self._moe_protos(fast)
         self.handle = None
         self._keep = None
         self.recv_total = None
@@ -207,4 +233,197 @@ class ExpertParallel:
             rc = L.b200EpCombine(self.handle, y.data_ptr(), *self._dims(y), out.data_ptr(), *self._dims(out), int(send_only), self._stream())
         _lib.check(rc, "ncclEpCombine", L)
         self._keep_c = (y, out)
+        return out
+
+    # ------------------------------------------------------------------ routing, the experts' products, and the gradients across the exchange
+    def _moe_protos(self, fast):
+        L, P, I = self.lib, ctypes.c_void_p, ctypes.c_int
+        types = {"ncclEpRoute": [P, P, I, P, P, P, I, I, I, P, P], "ncclEpRouteBackward": [P, P, P, I, P, P, I, I, I, P, P],
+                 "ncclEpExpertLinear": [P] * 8 + [I] * 5 + [P], "ncclEpExpertLinearBackward": [P] * 10 + [I] * 5 + [P],
+                 "ncclEpDispatchRows": [P, P, P], "ncclEpCombineBackward": [P] * 7 + [I] * 4 + [P], "ncclEpDispatchBackward": [P] * 4 + [I] * 4 + [P]}
+        self._moe = {}
+        for name, args in types.items():
+            fn = getattr(L, name, None)
+            if fn is None:
+                continue   # a library without them
+            fn.argtypes = args
+            entry = _lib.address(L, name) if fast else None
+            self._moe[name] = functools.partial(fast.invoke, entry) if entry else fn
+        if self._moe:
+            L.ncclEpExpertLinearBackwardWork.argtypes = [P, I, I, I, I, I]
+            L.ncclEpExpertLinearBackwardWork.restype = ctypes.c_size_t
+        dev = ctypes.c_int()
+        _lib.check(L.ncclCommCuDevice(self.comm.handle, ctypes.byref(dev)), "ncclCommCuDevice", L)
+        self._device = dev.value
+        self._route_cfgs = {}
+        torch = self.torch
+        self._logit_codes = {torch.float32: FP32, torch.float16: FP16, torch.bfloat16: BF16}
+
+    def _moe_call(self, name, *args):
+        _lib.check(self._moe[name](*args, current_stream(self._device)), name, self.lib)
+
+    def _need(self, name, t, dtype, shape):
+        """Checks a tensor: type, shape, contiguous, on the group's GPU."""
+        if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or not t.is_cuda or t.device.index != self._device:
+            raise ValueError("%s must be a contiguous %s tensor %s on cuda:%d, not %s %s%s on %s" % (
+                name, str(dtype).replace("torch.", ""), list(shape), self._device, str(t.dtype).replace("torch.", ""), list(t.shape),
+                "" if t.is_contiguous() else " (strided)", t.device))
+
+    def _result(self, name, t, dtype, shape):
+        if t is None:
+            return self.torch.empty(shape, dtype=dtype, device=self._device)
+        self._need(name, t, dtype, shape)
+        return t
+
+    def _route_cfg(self, *rule):
+        """Address of the configuration; the group keeps it."""
+        cfg = self._route_cfgs.get(rule)
+        if cfg is None:
+            score, groups, keep, group_score, renormalize, scale = rule
+            if score not in self.SCORES:
+                raise ValueError("score must be one of %s, not %r" % (", ".join(map(repr, self.SCORES)), score))
+            if group_score not in self.GROUP_SCORES:
+                raise ValueError("group_score must be one of %s, not %r" % (", ".join(map(repr, self.GROUP_SCORES)), group_score))
+            cfg = _hdr(RouteCfg())
+            cfg.score, cfg.groups, cfg.keep_groups, cfg.group_score = self.SCORES[score], groups, keep, self.GROUP_SCORES[group_score]
+            cfg.renormalize, cfg.scale = int(bool(renormalize)), scale
+            if len(self._route_cfgs) >= 64:
+                self._route_cfgs.clear()
+            self._route_cfgs[rule] = cfg
+        return ctypes.addressof(cfg)
+
+    def _logits(self, logits):
+        code = self._logit_codes.get(logits.dtype)
+        if code is None or logits.dim() != 2 or logits.shape[1] != self.E:
+            raise ValueError("logits must be an fp32, fp16 or bf16 tensor [tokens, %d], not %s %s" % (self.E, str(logits.dtype).replace("torch.", ""), list(logits.shape)))
+        self._need("logits", logits, logits.dtype, logits.shape)
+        return code
+
+    def route(self, logits, topk, score="softmax", bias=None, groups=1, keep_groups=None, group_score="max", renormalize=True, scale=1.0, idx=None, weights=None):
+        """What ``dispatch`` takes: (int64 [tokens, topk] expert ids, fp32 [tokens, topk] weights) from router logits [tokens, num_experts].
+
+        Scores are the softmax or sigmoid of the logits (fp32, fp16 or bf16). Experts are ranked by score + ``bias`` (fp32 [num_experts]; it
+        chooses and does not weigh) among the ``keep_groups`` best of ``groups`` equal runs of experts; a group counts as its best expert
+        (``group_score="max"``) or the sum of its two best ("top2"). Best first; equal ones by index. Weights are ``scale`` * score, with
+        ``renormalize`` divided by the sum of the taken experts' scores. Experts whose logit is -inf or NaN are never taken: entries that
+        find none are -1 with weight 0, which ``dispatch`` leaves out (rows of -inf stand for padding)."""
+        code = self._logits(logits)
+        topk = int(topk)
+        T, i64, f32 = logits.shape[0], self.torch.int64, self.torch.float32
+        if bias is not None:
+            self._need("bias", bias, f32, (self.E,))
+        cfg = self._route_cfg(score, groups, groups if keep_groups is None else keep_groups, group_score, renormalize, scale)
+        idx, weights = self._result("idx", idx, i64, (T, topk)), self._result("weights", weights, f32, (T, topk))
+        self._moe_call("ncclEpRoute", self.group, logits.data_ptr(), code, None if bias is None else bias.data_ptr(), idx.data_ptr(), weights.data_ptr(), T, self.E, topk, cfg)
+        return idx, weights
+
+    def route_backward(self, dweights, logits, idx, score="softmax", renormalize=True, scale=1.0, out=None):
+        """Gradient of the logits (their type) from that of the weights; ``idx`` and the rule as ``route`` had them. The choice has no gradient."""
+        code = self._logits(logits)
+        T, topk = idx.shape
+        self._need("dweights", dweights, self.torch.float32, (T, topk))
+        self._need("idx", idx, self.torch.int64, (logits.shape[0], topk))
+        cfg = self._route_cfg(score, 1, 1, "max", renormalize, scale)
+        out = self._result("out", out, logits.dtype, logits.shape)
+        self._moe_call("ncclEpRouteBackward", self.group, dweights.data_ptr(), logits.data_ptr(), code, idx.data_ptr(), out.data_ptr(), T, self.E, topk, cfg)
+        return out
+
+    def _linear(self, x, w, counts, activation):
+        """(experts, rows, n, k, columns of the result, code of the activation) of a product, its operands checked."""
+        torch = self.torch
+        if activation not in self.ACTIVATIONS:
+            raise ValueError("activation must be one of %s, not %r" % (", ".join(map(repr, self.ACTIVATIONS)), activation))
+        if x.dim() != 3 or w.dim() != 3:
+            raise ValueError("x must be [experts, rows, k] and w [experts, n, k], not %s and %s" % (list(x.shape), list(w.shape)))
+        E, rows, k = x.shape
+        n = w.shape[1]
+        gated = activation in ("swiglu", "geglu")
+        if n % (16 if gated else 8) or k % 8 or not 0 < E <= 256:
+            raise ValueError("%d experts (at most 256), n = %d must be a multiple of %d and k = %d of 8" % (E, n, 16 if gated else 8, k))
+        self._need("x", x, torch.bfloat16, (E, rows, k))
+        self._need("w", w, torch.bfloat16, (E, n, k))
+        if counts is not None:
+            self._need("counts", counts, torch.int32, (E,))
+        return E, rows, n, k, n // 2 if gated else n, self.ACTIVATIONS[activation]
+
+    def expert_linear(self, x, w, counts, bias=None, activation=None, residual=None, out=None, pre=None):
+        """act(x w^T + bias) + residual for every expert over its rows in use, as ``dispatch`` packs and counts them; bf16 with fp32 sums.
+
+        x [experts, rows, k], w [experts, n, k], counts int32 [experts] (None: all rows), bias [experts, n], residual and the result [experts, rows, n].
+        activation: None, "relu", "gelu" (by erf), "silu", or gated, "swiglu" and "geglu": w is then gate rows and up rows one after the other, and
+        the result, silu(gate) * up or gelu(gate) * up, has n / 2 columns. n and k are multiples of 8 (gated: n of 16). ``pre``
+        [experts, rows, n] gets x w^T + bias for the backward pass. Rows behind an expert's last are not written; ``residual`` may be ``out``."""
+        torch = self.torch
+        E, rows, n, k, cols, act = self._linear(x, w, counts, activation)
+        bf16, ptr = torch.bfloat16, lambda t: None if t is None else t.data_ptr()   # noqa: E731
+        if bias is not None:
+            self._need("bias", bias, bf16, (E, n))
+        if residual is not None:
+            self._need("residual", residual, bf16, (E, rows, cols))
+        if pre is not None:
+            self._need("pre", pre, bf16, (E, rows, n))
+        out = self._result("out", out, bf16, (E, rows, cols))
+        self._moe_call("ncclEpExpertLinear", self.group, x.data_ptr(), w.data_ptr(), ptr(counts), ptr(bias), ptr(residual), out.data_ptr(), ptr(pre), E, rows, n, k, act)
+        return out
+
+    def expert_linear_backward(self, dout, x, w, counts, pre=None, activation=None, need_dx=True, need_dw=True, need_dbias=False, dx=None, dw=None, dbias=None):
+        """(dx, dw, dbias) of ``expert_linear``, None for those that are not needed; the residual's gradient is ``dout`` itself. ``pre`` as the
+        forward call filled it (not needed without an activation). dx has the rows in use only; dw and dbias are zero for experts without rows."""
+        torch = self.torch
+        E, rows, n, k, cols, act = self._linear(x, w, counts, activation)
+        bf16, ptr = torch.bfloat16, lambda t: None if t is None else t.data_ptr()   # noqa: E731
+        self._need("dout", dout, bf16, (E, rows, cols))
+        if act:
+            if pre is None:
+                raise ValueError("the gradient of an activation needs what it was applied to: give expert_linear and this call the same `pre`")
+            self._need("pre", pre, bf16, (E, rows, n))
+        dx = self._result("dx", dx, bf16, (E, rows, k)) if need_dx else None
+        dw = self._result("dw", dw, bf16, (E, n, k)) if need_dw else None
+        dbias = self._result("dbias", dbias, bf16, (E, n)) if need_dbias else None
+        size = self.lib.ncclEpExpertLinearBackwardWork(self.group, E, rows, n, act, int(need_dbias))
+        work = torch.empty(size, dtype=torch.uint8, device=self._device) if size else None
+        self._moe_call("ncclEpExpertLinearBackward", self.group, dout.data_ptr(), x.data_ptr(), w.data_ptr(), ptr(counts), ptr(pre) if act else None, ptr(dx), ptr(dw),
+                       ptr(dbias), ptr(work), E, rows, n, k, act)
+        return dx, dw, dbias
+
+    def dispatch_rows(self, rows=None):
+        """int32 [tokens, topk]: the row of the dispatched tensor (as [experts * capacity, hidden]) that holds each entry of the last ``dispatch``, -1
+        for entries without an expert. Groups of one rank with the expert-major layout; the next dispatch moves the rows."""
+        if self.handle is None:
+            raise ValueError("nothing has been dispatched yet")
+        idx = self._keep[1]
+        rows = self._result("rows", rows, self.torch.int32, tuple(idx.shape))
+        self._moe_call("ncclEpDispatchRows", self.handle, rows.data_ptr())
+        return rows
+
+    def combine_backward(self, dout, y, weights, rows, dy=None, dweights=None):
+        """(dy, dweights) of ``combine`` from the gradient [tokens, hidden] of its result: dy[row] = weight * dout[token] for the rows that
+        ``rows`` (see ``dispatch_rows``) names, each by one entry; dweights[t, k] = <dout[t], y[row]>. dy is like y and may be y."""
+        torch = self.torch
+        if dout.dim() != 2 or y.dim() < 2 or weights.dim() != 2:
+            raise ValueError("dout must be [tokens, hidden], y [..., hidden], weights [tokens, topk], not %s, %s, %s" % (list(dout.shape), list(y.shape), list(weights.shape)))
+        (T, H), K, bf16 = dout.shape, weights.shape[1], torch.bfloat16
+        if H % 8 or not 0 < K <= 16:
+            raise ValueError("hidden = %d must be a multiple of 8, topk = %d at most 16" % (H, K))
+        self._need("dout", dout, bf16, (T, H))
+        self._need("y", y, bf16, (*y.shape[:-1], H))
+        self._need("weights", weights, torch.float32, (T, K))
+        self._need("rows", rows, torch.int32, (T, K))
+        dy, dweights = self._result("dy", dy, bf16, y.shape), self._result("dweights", dweights, torch.float32, (T, K))
+        self._moe_call("ncclEpCombineBackward", self.group, dout.data_ptr(), y.data_ptr(), weights.data_ptr(), rows.data_ptr(), dy.data_ptr(), dweights.data_ptr(), T, K, H,
+                       y.numel() // H if H else 0)
+        return dy, dweights
+
+    def dispatch_backward(self, dtoks, rows, out=None):
+        """Gradient of the tokens, [tokens, hidden], from that of the dispatched rows: the sum over the token's rows."""
+        torch = self.torch
+        if dtoks.dim() < 2 or rows.dim() != 2:
+            raise ValueError("dtoks must be [..., hidden] and rows [tokens, topk], not %s and %s" % (list(dtoks.shape), list(rows.shape)))
+        (T, K), H = rows.shape, dtoks.shape[-1]
+        if H == 0 or H % 8 or not 0 < K <= 16:
+            raise ValueError("hidden = %d must be a multiple of 8, topk = %d at most 16" % (H, K))
+        self._need("dtoks", dtoks, torch.bfloat16, dtoks.shape)
+        self._need("rows", rows, torch.int32, (T, K))
+        out = self._result("out", out, torch.bfloat16, (T, H))
+        self._moe_call("ncclEpDispatchBackward", self.group, dtoks.data_ptr(), rows.data_ptr(), out.data_ptr(), T, K, H, dtoks.numel() // H)
         return out

@@ -1,0 +1,96 @@
+// Internal interface between the host code of the mixture-of-experts operators (moe_ops.cc) and their kernels.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace b200 {
+
+// ---------------------------------------------------------------- routing (route.cu)
+constexpr int kRouteMaxExperts = 1024, kRouteMaxTopk = 16, kRouteMaxGroups = 32;
+
+struct RouteArgs {
+  const void* logits;         // [tokens][experts]
+  const float* bias;          // [experts] or null
+  int64_t* idx;               // [tokens][topk], -1 = no expert
+  float* weights;             // [tokens][topk]
+  const float* dweights;      // backward: [tokens][topk]
+  void* dlogits;              // backward: [tokens][experts]
+  int tokens, experts, topk;
+  int groups, keep, perGroup; // groups of perGroup experts next to each other, of which `keep` stay
+  uint32_t groupMagic;        // ceil(2^32 / perGroup): expert / perGroup is the high word of the product (0: perGroup is 1)
+  int sigmoid, top2, renormalize;
+  float scale;
+  int wide;                   // rows of logits may be read in packs of 16 bytes
+};
+
+enum RouteType : int { ROUTE_F32 = 0, ROUTE_F16 = 1, ROUTE_BF16 = 2 };
+const void* routeKernelFn(int type, int experts);
+const void* routeBackwardKernelFn(int type, int experts);
+int routeWarps();             // warps of a CTA, one token each
+
+// ---------------------------------------------------------------- the experts' products (expert_gemm_sm100.cu)
+enum ExpertAct : int { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_SILU = 3, ACT_SWIGLU = 4, ACT_GEGLU = 5 };
+inline bool actGated(int act) { return act == ACT_SWIGLU || act == ACT_GEGLU; }
+
+// Which of the three products of a linear layer: rows x W^T, their gradient dz W, or the weights' gradient dz^T x.
+enum ExpertMode : int { EXPERT_FORWARD = 0, EXPERT_DX = 1, EXPERT_DW = 2 };
+
+constexpr int kExpertMax = 256;   // experts of a call: the tile counts of all of them are held in shared memory
+
+struct ExpertGemmArgs {
+  const int* counts;          // [experts] rows in use (null: all of them)
+  int experts, cap;           // rows that the tensors have for each expert
+  int outRows;                // DW: rows of the result (of W); else the rows in use
+  int cols;                   // columns of the result
+  int depth;                  // length of the sums (DW: cap; the rows in use count)
+  int gated, act;             // forward: gate rows of W, then up rows, `cols` of each
+  const void* bias;           // bf16 [experts][cols, twice when gated] or null
+  const void* residual;       // bf16, laid out like out, or null
+  void* out;                  // bf16 [experts][cap or outRows][cols]
+  void* pre;                  // bf16 [experts][cap][cols, twice when gated]: what the activation is applied to, or null
+  uint32_t* status;           // {code, kind, what, CTA} of the communicator, written when a wait runs out
+};
+
+const void* expertGemmKernelFn(int mode);
+size_t expertGemmSmemBytes();
+int expertGemmThreads();
+
+// ---------------------------------------------------------------- row kernels (moe_backward.cu)
+struct ExpertActArgs {
+  const int* counts;
+  const void* dout;           // bf16 [experts][cap][cols]
+  const void* pre;            // bf16 [experts][cap][cols, twice when gated]; not read without an activation
+  void* dz;                   // as pre; null without an activation
+  float* partial;             // [slices][experts][cols, twice when gated] sums of dz over the rows of a slice, or null
+  void* dbias;                // bf16 [experts][cols, twice when gated] or null
+  int experts, cap, cols, act, slices;
+};
+const void* expertActKernelFn(int act);
+const void* expertBiasKernelFn();
+constexpr int kActCols = 256, kActThreads = 256;   // columns and threads of a CTA
+
+struct MoeRowsArgs {
+  const void* dout;           // [tokens][hidden] bf16
+  const void* y;              // rows of the experts, bf16
+  const float* weights;       // [tokens][topk]
+  const int* rows;            // [tokens][topk], negative = no row
+  void* dy;
+  float* dweights;
+  void* dx;                   // dispatch's backward: [tokens][hidden]
+  int tokens, topk, hidden, numRows;
+};
+const void* combineBackwardKernelFn(int topk);
+const void* dispatchBackwardKernelFn();
+constexpr int kMoeRowThreads = 256;
+
+struct DispatchRowsArgs {
+  const int64_t* idx;         // [tokens][topk] of the last dispatch
+  const int* rowOf;
+  const int2* srcInfo;
+  const int* counts;
+  int* rows;
+  int entries, experts, cap, rank;
+};
+const void* dispatchRowsKernelFn();
+
+}  // namespace b200

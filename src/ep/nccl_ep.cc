@@ -6,28 +6,9 @@
 
 #include <algorithm>
 
-#include "../comm/device_plane.h"
-#include "ep_kernels.cuh"
+#include "ep_group.h"
 
 using namespace b200;
-
-struct ncclEpGroup {
-  ncclComm* comm = nullptr;
-  ncclEpGroupConfig_t cfg;
-  int n = 1, E = 0, El = 0, H = 0, maxTokens = 0, K = 0;
-  size_t slotBytes = 0, zoneBytes = 0, combZoneBytes = 0;
-  char* recvZone = nullptr;           // 2 zones (epoch parity)
-  SymWindow* recvWin = nullptr;
-  char* ctl = nullptr;                // counts [2][El][n] u64, combine flags [n] u64
-  SymWindow* ctlWin = nullptr;
-  char* combZone = nullptr;           // 2 zones, allocated with the first handle (needs top-k)
-  SymWindow* combWin = nullptr;
-  uint32_t* state = nullptr;
-  uint32_t* mask = nullptr;           // [n] device words: non-zero = that rank is left out of dispatch / combine
-  int smCount = 0;
-  int lastError = 0;
-  int layoutClass = 0;                // 0 none yet, 1 expert-major, 2 per-rank (rank-major / flat)
-};
 
 // Buffers that only this rank touches come from the group's allocator hooks when the configuration gives them
 // (ncclEpGroupConfig_t::alloc); memory that peers map stays with the library's own allocator, which makes it exportable.
@@ -40,25 +21,6 @@ static void epFree(const ncclEpAllocConfig_t& a, void* p) {
   if (a.alloc_fn) a.free_fn(p, a.context);
   else cudaFree(p);
 }
-
-struct ncclEpHandle {
-  ncclEpGroup* g = nullptr;
-  ncclEpLayout_t layout;
-  int K = 0, T = 0;
-  int outSlots = 0;                   // flat layout: rows of the last dispatch's outputs
-  const int64_t* topkIdx = nullptr;
-  const float* topkW = nullptr;
-  int2* srcInfo = nullptr;
-  int* rowOf = nullptr;               // one-rank groups, expert-major: where (token, k) went
-  int* expertCount = nullptr;
-  ncclEpAllocConfig_t alloc = {};     // the group's hooks, kept here so that a handle can outlive its group's record
-  // a send_only call leaves its receiving half to ncclEpComplete
-  int pending = 0;                    // 0 nothing, 1 dispatch, 2 combine
-  EpArgs pendingArgs;
-  int pendingCtas = 0;
-  size_t pendingSmem = 0;
-  void* pendingCounters = nullptr;    // layout_info->expert_counters of the pending dispatch
-};
 
 static bool cfgOk(const void* p) {
   const unsigned int* u = (const unsigned int*)p;
@@ -114,17 +76,6 @@ static bool onThisGpu(const void* p, int dev) {
   cudaPointerAttributes attr;
   if (cudaPointerGetAttributes(&attr, p) != cudaSuccess) { (void)cudaGetLastError(); return false; }
   return attr.type == cudaMemoryTypeDevice && attr.device == dev;
-}
-
-struct Span {
-  const void* data;
-  size_t bytes;
-};
-static bool overlap(std::initializer_list<Span> outputs, std::initializer_list<Span> inputs) {
-  for (const Span& o : outputs)
-    for (const Span& i : inputs)
-      if (o.data && i.data && (const char*)o.data < (const char*)i.data + i.bytes && (const char*)i.data < (const char*)o.data + o.bytes) return true;
-  return false;
 }
 
 // `want`: CTAs that have something to do. Two CTAs per SM, or the caller's number of SMs with one each.
