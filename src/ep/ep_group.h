@@ -2,6 +2,7 @@
 #pragma once
 #include "nccl_ep.h"
 
+#include <atomic>
 #include <initializer_list>
 
 #include "../comm/device_plane.h"
@@ -25,6 +26,7 @@ struct ncclEpGroup {
   uint32_t* mask = nullptr;           // [n] device words: non-zero = that rank is left out of dispatch / combine
   int smCount = 0;
   int lastError = 0;
+  std::atomic<int> expertPairs{-1};   // clusters of the experts' products on CTA pairs that can be resident at once (-1: not asked yet)
   int layoutClass = 0;                // 0 none yet, 1 expert-major, 2 per-rank (rank-major / flat)
 };
 

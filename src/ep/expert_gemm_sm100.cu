@@ -6,13 +6,17 @@
 // Only the device knows the counts: every CTA reads them, counts the tiles of all experts and walks its share of them, so that one launch
 // serves a single token and a full batch alike.
 //
-// One persistent CTA per SM, 320 threads in three roles:
-//   warp 0      TMA producer: 128 x 64 tiles of the first operand and up to 256 x 64 of the second (128-byte swizzle) through a ring in
-//               shared memory. Of few rows only the boxes of 32 that hold some are fetched; the rows behind them in shared memory are
-//               whatever was there: they reach only results that nobody stores.
-//   warp 1      MMA issuer: tcgen05.mma 128 x BN x 16 into one of two accumulators in tensor memory.
-//   warps 2-9   epilogue, two warps to 32 rows: bias, activation, residual, rounding, stores of whole 128-byte lines.
-// The last step of DW's sum may hold rows behind the expert's last: the issuing warp writes zeros over them in shared memory.
+// Two kernels. expertGemmPairKernel: CTA pairs (clusters of two, tcgen05 cta_group::2) on tiles of 256 rows x up to 256 columns; each CTA stages
+// its 128 rows of the first operand and its half of the second per 64 steps of the sum, and keeps the results of its rows. A CTA alone
+// would need 48 KiB where one of a pair needs 32, more than level 2 delivers while the tensor cores work on them (4 x 2048 rows, 4096 x 4096:
+// 1142 TFLOP/s). expertGemmKernel: one CTA per tile of 128 rows, where no expert can have more: there the weights are the traffic.
+//
+// Persistent CTAs, one per SM, in roles:
+//   warp 0      TMA producer: operand tiles (128-byte swizzle) through a ring in shared memory
+//   warp 1      MMA issuer (of a pair: the first CTA's) into one of two accumulators in tensor memory
+//   warps 2-9   epilogue, two warps to 32 rows: bias, activation, residual, rounding, stores of whole 128-byte lines
+//   warp 10     DW: the last step of a sum may hold rows behind the expert's last; zeros are written over them in shared memory
+// Rows of the first operand that were not fetched, or lie behind the last, are whatever shared memory held: they reach only results that nobody stores.
 // Every wait is bounded; on expiry the kernel records a status, waits for its copies in flight, frees its tensor memory and returns.
 #include "../kernels/common.cuh"
 #include "../tp/gemm_sm100.cuh"
@@ -25,22 +29,48 @@ using namespace sm100;
 
 namespace {
 
-constexpr int kBM = 128, kBK = 64, kUmmaK = 16, kMaxBN = 256;
-constexpr int kThreads = 320, kEpiWarps = 8;
+constexpr int kBK = 64, kUmmaK = 16, kMaxBN = 256;
+constexpr int kEpiWarps = 8, kFirstEpiWarp = 2, kFixWarp = kFirstEpiWarp + kEpiWarps;
+constexpr int kThreads = kFixWarp * 32, kPairThreads = kThreads + 32;
 constexpr uint32_t kTmemCols = 512, kAccCols = 256;
-constexpr uint32_t kRingBytes = 4 * (kBM + kMaxBN) * kBK * 2;
-constexpr int kMaxStages = 12;
-constexpr uint32_t kBlockBytes = 64 * kBK * 2;   // of a box of 64 x 64
-constexpr size_t kCtrlBytes = 512;
-static_assert((2 * kMaxStages + 4) * 8 + 8 <= kCtrlBytes, "control block too small");
-constexpr size_t kTableBytes = (kExpertMax + 1) * 4 + 12;
-constexpr size_t kSmemBytes = 1024 + kRingBytes + kEpiWarps * 4096 + kCtrlBytes + kTableBytes;
-static_assert(kSmemBytes <= 227 * 1024, "shared memory");
+constexpr uint32_t kRingBytes = 192 << 10;
+constexpr int kMaxStages = 12, kPairStages = 6;
+constexpr uint32_t kHalfBytes = 128 * kBK * 2;   // 128 rows (or columns) of an operand, 64 steps
+constexpr uint32_t kBlockBytes = 64 * kBK * 2;   // a box of 64 x 64
+constexpr size_t kEpiBytes = kEpiWarps * 4096, kCtrlBytes = 512, kTableBytes = (kExpertMax + 1) * 4 + 12;
+constexpr size_t kSmemBytes = 1024 + kRingBytes + kEpiBytes + kCtrlBytes + kTableBytes;
+static_assert((2 * kMaxStages + 4) * 8 + 8 <= kCtrlBytes && (4 * kPairStages + 4) * 8 + 8 <= kCtrlBytes, "control block too small");
+static_assert(kPairStages * 2 * kHalfBytes <= kRingBytes && kSmemBytes <= 227 * 1024, "shared memory");
 
 __device__ __forceinline__ void tmaLoad3d(uint32_t dstSmem, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
       ::"r"(dstSmem), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+}
+// The same, counted on an mbarrier of either CTA of the pair (cluster address). No multicast.
+__device__ __forceinline__ void tmaLoad3dPair(uint32_t dstSmem, const CUtensorMap* map, int c0, int c1, int c2, uint32_t barCluster) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dstSmem), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(barCluster) : "memory");
+}
+
+// Arrival at an mbarrier of the pair that publishes no memory: with release it waits until all of the warp's stores are done (DW over experts of
+// 64 rows, 32 x 4096 x 7168: 681 us, RELAXED_US with this one).
+__device__ __forceinline__ void mbarArriveRelaxed(uint32_t clusterAddr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(clusterAddr) : "memory");
+}
+// As mbarWait, for what the other CTA of the pair wrote before it arrived.
+__device__ __forceinline__ bool mbarWaitCluster(uint32_t bar, uint32_t parity, uint32_t limit = 1u << 24) {
+  for (uint32_t i = 0; i < limit; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (ok) return true;
+  }
+  return false;
 }
 
 // An operand that lies across the sum, in boxes of 64 values x 64 steps with 128-byte swizzle: the next 64 values are a box further, the
@@ -54,30 +84,212 @@ __device__ __forceinline__ uint64_t descAcross(uint32_t smemByteAddr) {
   d |= (uint64_t)2 << 61;
   return d;
 }
+template <bool ACROSS> __device__ __forceinline__ uint64_t descOf(uint32_t addr) { return ACROSS ? descAcross(addr) : umDescK128(addr); }
+template <bool ACROSS> constexpr uint64_t kNextDesc = (ACROSS ? kUmmaK * 128 : kUmmaK * 2) >> 4;   // 16 steps on, in 16-byte units
+
+template <int MODE> constexpr bool kAcrossA = MODE == EXPERT_DW;
+template <int MODE> constexpr bool kAcrossB = MODE != EXPERT_FORWARD;
 
 struct Tile {
   int e, rows, row0, col0, steps;   // expert, its rows in use, first row and column of the result, 64-wide steps of the sum
 };
 
+// The tiles of all experts and their order.
+template <int MODE, int BM>
+struct Tiles {
+  const ExpertGemmArgs& a;
+  const int* start;          // [experts + 1] row tiles in front of each expert's
+  int bn, parts;             // columns of a tile's accumulator, and of how many parts (gate and up) they are
+  int outCols, tilesN, count;
+
+  __device__ __forceinline__ static int rowsOf(const ExpertGemmArgs& a, int e) { return a.counts ? min(max(a.counts[e], 0), a.cap) : a.cap; }
+
+  // One warp fills the table.
+  __device__ static void fill(const ExpertGemmArgs& a, int* start, int lane) {
+    int before = 0;
+    for (int e0 = 0; e0 < a.experts; e0 += 32) {
+      const int e = e0 + lane;
+      const int mine = e < a.experts ? ((MODE == EXPERT_DW ? a.outRows : rowsOf(a, e)) + BM - 1) / BM : 0;
+      int n = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(~0u, n, o);
+        if (lane >= o) n += v;
+      }
+      if (e < a.experts) start[e] = before + n - mine;
+      before += __shfl_sync(~0u, n, 31);
+    }
+    if (lane == 0) start[a.experts] = before;
+  }
+
+  // Width of the tiles, from kMaxBN down in steps of `step`: what `workers` CTAs or pairs finish first, a wave of tiles taken to cost `cost(width)`. The sums do
+  // not depend on it.
+  template <typename Cost>
+  __device__ __forceinline__ Tiles(const ExpertGemmArgs& args, const int* table, int workers, int narrowest, int step, Cost cost) : a(args), start(table) {
+    parts = MODE == EXPERT_FORWARD && a.gated ? 2 : 1;
+    const int rowTiles = start[a.experts];
+    float best = 0.0f;
+    bn = kMaxBN;
+    for (int w = kMaxBN; w >= narrowest; w -= step) {
+      const int n = rowTiles * ((a.cols + w / parts - 1) / (w / parts));
+      const float all = (n + workers - 1) / workers * cost(w);
+      if (w == kMaxBN || all < best) { best = all; bn = w; }
+    }
+    outCols = bn / parts;
+    tilesN = (a.cols + outCols - 1) / outCols;
+    count = rowTiles * tilesN;
+  }
+
+  // Panels of 8 row tiles: those in flight share both operands.
+  __device__ __forceinline__ Tile at(int t) const {
+    Tile r;
+    int lo = 0, hi = a.experts;
+    while (hi - lo > 1) {   // the last expert whose tiles begin at or before t
+      const int mid = (lo + hi) / 2;
+      if (start[mid] * tilesN <= t) lo = mid;
+      else hi = mid;
+    }
+    r.e = lo;
+    r.rows = rowsOf(a, lo);
+    const int j = t - start[lo] * tilesN, mine = start[lo + 1] - start[lo];
+    const int panel = j / (8 * tilesN), width = min(8, mine - panel * 8), k = j - panel * 8 * tilesN;
+    r.row0 = (panel * 8 + k % width) * BM;
+    r.col0 = k / width * outCols;
+    r.steps = ((MODE == EXPERT_DW ? r.rows : a.depth) + kBK - 1) / kBK;
+    return r;
+  }
+  __device__ __forceinline__ int rowLimit(const Tile& c) const { return MODE == EXPERT_DW ? a.outRows : c.rows; }
+  __device__ __forceinline__ int length(const Tile& c) const { return MODE == EXPERT_DW ? c.rows : a.depth; }
+};
+
+__device__ __forceinline__ void reportTimeout(const ExpertGemmArgs& a, uint32_t what) {
+  if (a.status && ldRelaxedSys(a.status) == DEV_OK) {
+    a.status[1] = WAIT_TILE;
+    a.status[2] = what;
+    a.status[3] = blockIdx.x;
+    __threadfence_system();
+    stRelaxedSys(a.status, DEV_TIMEOUT);
+  }
+}
+
+// Epilogue of one warp for its 32 rows, `row` the first of them, and every other 64 columns of the tile: tBase is the tensor-memory address of the
+// warp's first lane and the tile's first column, the columns of `up` begin partCols behind those of `gate`. A lane has a row of the accumulator; 64 columns at a time pass through 4 KiB of shared memory (16-byte chunks
+// XOR-swizzled by row), so that memory sees 128 contiguous bytes of a row.
+template <int MODE, typename T>
+__device__ __forceinline__ void storeTile(const ExpertGemmArgs& a, const T& tiles, const Tile& c, int row, int partCols, uint32_t tBase, uint8_t* wbuf, int half, int lane) {
+  const int parts = tiles.parts, outCols = tiles.outCols, left = tiles.rowLimit(c) - row;   // rows from here on
+  const size_t first = (size_t)c.e * (MODE == EXPERT_DW ? a.outRows : a.cap) + row;
+  for (int cc = half * 64; cc < outCols && c.col0 + cc < a.cols && left > 0; cc += 128) {
+    const int col = c.col0 + cc, width = min(min(64, outCols - cc), a.cols - col);   // a multiple of 8
+    auto chunk = [&](int r, int j) { return (uint4*)(wbuf + r * 128 + ((j ^ (r & 7)) * 16)); };
+    auto store = [&](__nv_bfloat16* to, size_t ld) {
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int r = k * 4 + (lane >> 3), j = lane & 7;
+        if (r < left && j * 8 < width) *(uint4*)(to + (size_t)r * ld + j * 8) = *chunk(r, j);
+      }
+      __syncwarp();
+    };
+    auto sums = [&](int part, int h, float (&v)[32]) {
+      uint32_t r[32];
+      tmemLd32(tBase + part * partCols + cc + h * 32, r);
+      tmemLdWait32(r);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+      if (MODE == EXPERT_FORWARD && a.bias) {
+        const __nv_bfloat16* b = (const __nv_bfloat16*)a.bias + ((size_t)c.e * parts + part) * a.cols + col + h * 32;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (h * 32 + j * 8 >= width) break;
+          float f[8];
+          unpackBf16x8(__ldg((const uint4*)b + j), f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[j * 8 + i] += f[i];
+        }
+      }
+    };
+    if (MODE == EXPERT_FORWARD && a.pre) {
+      for (int p = 0; p < parts; ++p) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h * 32 >= width) break;
+          float v[32];
+          sums(p, h, v);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) *chunk(lane, h * 4 + j) = packBf16x8(v + j * 8);
+        }
+        store((__nv_bfloat16*)a.pre + (first * parts + p) * a.cols + col, (size_t)parts * a.cols);
+      }
+    }
+    if (MODE == EXPERT_FORWARD && a.residual) {
+      const __nv_bfloat16* from = (const __nv_bfloat16*)a.residual + first * a.cols + col;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int r = k * 4 + (lane >> 3), j = lane & 7;
+        *chunk(r, j) = r < left && j * 8 < width ? *(const uint4*)(from + (size_t)r * a.cols + j * 8) : make_uint4(0, 0, 0, 0);
+      }
+      __syncwarp();
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (h * 32 >= width) break;
+      float v[32];
+      if (MODE == EXPERT_DW && c.steps == 0) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+      } else {
+        sums(0, h, v);
+      }
+      if (MODE == EXPERT_FORWARD) {
+        if (parts == 2) {
+          float u[32];
+          sums(1, h, u);
+          const int base = a.act == ACT_SWIGLU ? ACT_SILU : ACT_GELU;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = activation(base, v[i]) * u[i];
+        } else if (a.act != ACT_NONE) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = activation(a.act, v[i]);
+        }
+        if (a.residual) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float f[8];
+            unpackBf16x8(*chunk(lane, h * 4 + j), f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[j * 8 + i] += f[i];
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *chunk(lane, h * 4 + j) = packBf16x8(v + j * 8);
+    }
+    store((__nv_bfloat16*)a.out + first * a.cols + col, (size_t)a.cols);
+  }
+}
+
 }  // namespace
 
+// ---------------------------------------------------------------------------------------------- one CTA per tile of 128 rows
+// No expert has more rows than one tile (cap <= 128): FORWARD and DX, boxes of tmA as high as cap asks for. tmB has boxes of 128 rows of W (DX: 64 x 64), tmBNarrow
+// of 32, for tiles that are not wider than two of them.
 template <int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
-expertGemmKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmASmall, const __grid_constant__ CUtensorMap tmB,
-                 const __grid_constant__ CUtensorMap tmBSmall, const __grid_constant__ ExpertGemmArgs a) {
-  constexpr bool kAcrossA = MODE == EXPERT_DW, kAcrossB = MODE != EXPERT_FORWARD;
+expertGemmKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmBNarrow,
+                 const __grid_constant__ ExpertGemmArgs a) {
+  static_assert(MODE != EXPERT_DW, "DW runs on pairs");
   extern __shared__ uint8_t smemRaw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smemRaw + 1023) & ~(uintptr_t)1023);
   uint8_t* epiBuf = smem + kRingBytes;
-  uint8_t* ctrl = epiBuf + kEpiWarps * 4096;
+  uint8_t* ctrl = epiBuf + kEpiBytes;
   uint64_t* fullBar = (uint64_t*)ctrl;              // [kMaxStages]
   uint64_t* emptyBar = fullBar + kMaxStages;        // [kMaxStages]
   uint64_t* accFull = emptyBar + kMaxStages;        // [2]
   uint64_t* accEmpty = accFull + 2;                 // [2]
   uint32_t* tmemSlot = (uint32_t*)(accEmpty + 2);
   volatile uint32_t* abortFlag = tmemSlot + 1;
-  int* tileStart = (int*)(ctrl + kCtrlBytes);       // [experts + 1] row tiles in front of each expert's
-  int* mostRows = tileStart + kExpertMax + 1;       // of one expert
+  int* table = (int*)(ctrl + kCtrlBytes);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -93,282 +305,95 @@ expertGemmKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     tmemRelinquish();
   }
   pdlEnter();   // the set-up above overlaps the end of the kernel before
-
-  auto rowsOf = [&](int e) { return a.counts ? min(max(a.counts[e], 0), a.cap) : a.cap; };
-  if (warp == 0) {
-    int before = 0, most = 0;
-    for (int e0 = 0; e0 < a.experts; e0 += 32) {
-      const int e = e0 + lane, rows = e < a.experts ? rowsOf(e) : 0;
-      int n = e >= a.experts ? 0 : ((MODE == EXPERT_DW ? a.outRows : rows) + kBM - 1) / kBM;
-      most = max(most, rows);
-      const int mine = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(~0u, n, o);
-        if (lane >= o) n += v;
-      }
-      if (e < a.experts) tileStart[e] = before + n - mine;
-      before += __shfl_sync(~0u, n, 31);
-    }
-    most = __reduce_max_sync(~0u, most);
-    if (lane == 0) {
-      tileStart[a.experts] = before;
-      *mostRows = most;
-    }
-  }
+  if (warp == 0) Tiles<MODE, 128>::fill(a, table, lane);
   tcFenceBefore();
   __syncthreads();
   tcFenceAfter();
   const uint32_t tmemBase = *tmemSlot;
-
-  // Width of the tiles: the one that the SMs finish first, a wave of tiles taken to cost its columns and a fixed part for the first
-  // operand and the start. The sums do not depend on it.
-  const int parts = MODE == EXPERT_FORWARD && a.gated ? 2 : 1;
-  const int rowTiles = tileStart[a.experts];
-  int bn = kMaxBN;
-  {
-    long long best = 0;
-    for (int w = kMaxBN; w >= (MODE == EXPERT_FORWARD && parts == 1 ? 32 : 64); w >>= 1) {
-      const long long tiles = (long long)rowTiles * ((a.cols + w / parts - 1) / (w / parts));
-      const long long cost = (tiles + gridDim.x - 1) / gridDim.x * (w + 32);
-      if (w == kMaxBN || cost < best) { best = cost; bn = w; }
-    }
-  }
-  const int outCols = bn / parts;                       // columns of the result in a tile
-  const int tilesN = (a.cols + outCols - 1) / outCols;
-  // of the first operand only the boxes that hold rows are fetched: where no expert has many, the ring has more and smaller stages
-  const uint32_t aBytes = kAcrossA ? 2 * kBlockBytes : (uint32_t)min(kBM, (*mostRows + 31) / 32 * 32) * 128;
-  const uint32_t stageBytes = aBytes + (uint32_t)bn * 128;
+  // the weights are the traffic: a tile costs its columns, and about 32 for its start
+  const Tiles<MODE, 128> tiles(a, table, gridDim.x, MODE == EXPERT_FORWARD && !a.gated ? 32 : 64, 32, [](int w) { return w + 32.0f; });
+  const int bn = tiles.bn, parts = tiles.parts, outCols = tiles.outCols;
+  // rows of W that a tile fetches for each part: whole boxes, what hangs over belongs to the neighbour, who fetches it too
+  const bool narrow = MODE == EXPERT_FORWARD && outCols <= 64;
+  const int boxRows = MODE == EXPERT_FORWARD ? (narrow ? 32 : 128) : 64, boxes = (outCols + boxRows - 1) / boxRows;
+  const int partCols = boxes * boxRows;   // gate and up are one operand: what hangs over is multiplied too and not stored
+  const uint32_t aBytes = (uint32_t)a.boxRows * 128, stageBytes = aBytes + (uint32_t)(parts * partCols) * 128;
   const int stages = (int)min((uint32_t)kMaxStages, kRingBytes / stageBytes);
   const uint32_t ring = smemAddr(smem);
-  const int nTiles = rowTiles * tilesN;
-
-  // Tiles of an expert in panels of 8 row tiles: those in flight share both operands.
-  auto tileAt = [&](int t) {
-    Tile r;
-    int lo = 0, hi = a.experts;
-    while (hi - lo > 1) {   // the last expert whose tiles begin at or before t, among those with tiles
-      const int mid = (lo + hi) / 2;
-      if (tileStart[mid] * tilesN <= t) lo = mid;
-      else hi = mid;
-    }
-    r.e = lo;
-    r.rows = rowsOf(lo);
-    const int j = t - tileStart[lo] * tilesN, mine = tileStart[lo + 1] - tileStart[lo];
-    const int panel = j / (8 * tilesN), width = min(8, mine - panel * 8), k = j - panel * 8 * tilesN;
-    r.row0 = (panel * 8 + k % width) * kBM;
-    r.col0 = k / width * outCols;
-    r.steps = ((MODE == EXPERT_DW ? r.rows : a.depth) + kBK - 1) / kBK;
-    return r;
-  };
   auto fail = [&](uint32_t what) {
     *abortFlag = 1;
-    if (a.status && ldRelaxedSys(a.status) == DEV_OK) {
-      a.status[1] = WAIT_TILE;
-      a.status[2] = what;
-      a.status[3] = blockIdx.x;
-      __threadfence_system();
-      stRelaxedSys(a.status, DEV_TIMEOUT);
-    }
+    reportTimeout(a, what);
   };
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (electOne()) {
+      const CUtensorMap* map = narrow ? &tmBNarrow : &tmB;
       int s = 0, armed = 0;   // stages that were ever loaded
       uint32_t phase = 0;
-      for (int t = blockIdx.x; t < nTiles && !*abortFlag; t += gridDim.x) {
-        const Tile c = tileAt(t);
-        const int left = (MODE == EXPERT_DW ? a.outRows : c.rows) - c.row0;
-        const int aBoxes = kAcrossA ? (left > 64 ? 2 : 1) : min(kBM / 32, (left + 31) / 32);
-        const int bLeft = min(outCols, a.cols - c.col0), perPart = outCols >= 64 ? 64 : 32;
-        const int bBoxes = kAcrossB ? (bLeft + 63) / 64 : (bLeft + perPart - 1) / perPart;
-        const uint32_t bytes = (kAcrossA ? aBoxes * kBlockBytes : aBoxes * 32 * 128) + (kAcrossB ? bBoxes * kBlockBytes : (uint32_t)(parts * bBoxes * perPart) * 128);
+      for (int t = blockIdx.x; t < tiles.count && !*abortFlag; t += gridDim.x) {
+        const Tile c = tiles.at(t);
         for (int kb = 0; kb < c.steps; ++kb) {
           if (!mbarWait(smemAddr(&emptyBar[s]), phase ^ 1)) { fail(1000 + s); break; }
           if (*abortFlag) break;
-          const uint32_t full = smemAddr(&fullBar[s]), sA = ring + s * stageBytes, sB = sA + aBytes;
-          mbarExpectTx(full, bytes);
-          if (kAcrossA) {
-            for (int i = 0; i < aBoxes; ++i) tmaLoad3d(sA + i * kBlockBytes, &tmA, c.row0 + i * 64, kb * kBK, c.e, full);
-          } else if (aBoxes == kBM / 32) {
-            tmaLoad3d(sA, &tmA, kb * kBK, c.row0, c.e, full);
-          } else {
-            for (int i = 0; i < aBoxes; ++i) tmaLoad3d(sA + i * 32 * 128, &tmASmall, kb * kBK, c.row0 + i * 32, c.e, full);
-          }
-          if (kAcrossB) {
-            for (int i = 0; i < bBoxes; ++i) tmaLoad3d(sB + i * kBlockBytes, &tmB, c.col0 + i * 64, kb * kBK, c.e, full);
-          } else {
-            const CUtensorMap* map = perPart == 64 ? &tmB : &tmBSmall;
-            for (int p = 0; p < parts; ++p)
-              for (int i = 0; i < bBoxes; ++i)
-                tmaLoad3d(sB + (p * outCols + i * perPart) * 128, map, kb * kBK, p * a.cols + c.col0 + i * perPart, c.e, full);
-          }
+          const uint32_t full = smemAddr(&fullBar[s]), sA = ring + s * stageBytes;
+          uint32_t sB = sA + aBytes;
+          mbarExpectTx(full, stageBytes);
+          tmaLoad3d(sA, &tmA, kb * kBK, 0, c.e, full);
+          for (int p = 0; p < parts; ++p)
+            for (int i = 0; i < boxes; ++i, sB += boxRows * 128) {
+              if (MODE == EXPERT_FORWARD) tmaLoad3d(sB, map, kb * kBK, p * a.cols + c.col0 + i * boxRows, c.e, full);
+              else tmaLoad3d(sB, &tmB, c.col0 + i * 64, kb * kBK, c.e, full);
+            }
           armed = max(armed, s + 1);
           if (++s == stages) { s = 0; phase ^= 1; }
         }
       }
       if (*abortFlag) {
-        // copies already issued still write into shared memory: wait for them (bounded). A stage in front of s was loaded in this round, one from s on in the one before
+        // copies already issued still write into shared memory: wait for them (bounded). Stages in front of s were loaded in this round, the others in the one before
         for (int i = 0; i < armed; ++i) mbarWait(smemAddr(&fullBar[i]), i < s ? phase : phase ^ 1, 1u << 20);
       }
     }
     __syncwarp();
   } else if (warp == 1) {
-    const uint32_t idesc = umInstrBf16(kBM, bn) | (kAcrossA ? 1u << 15 : 0u) | (kAcrossB ? 1u << 16 : 0u);
-    int s = 0, it = 0;
-    uint32_t phase = 0;
-    for (int t = blockIdx.x; t < nTiles && !__any_sync(~0u, *abortFlag); t += gridDim.x) {
-      const Tile c = tileAt(t);
-      if (c.steps == 0) continue;   // nothing to add up: the epilogue writes zeros
-      const int buf = it & 1;
-      const uint32_t aph = (it >> 1) & 1;
-      ++it;
-      if (!__all_sync(~0u, mbarWait(smemAddr(&accEmpty[buf]), aph ^ 1))) { if (lane == 0) fail(2000 + buf); break; }
-      tcFenceAfter();
-      const uint32_t dT = tmemBase + buf * kAccCols;
-      const int length = MODE == EXPERT_DW ? c.rows : a.depth;
+    if (electOne()) {
+      const uint32_t idesc = umInstrBf16(128, parts == 2 ? 2 * partCols : bn) | (kAcrossB<MODE> ? 1u << 16 : 0u);
+      int s = 0, it = 0;
+      uint32_t phase = 0;
       bool bad = false;
-      for (int kb = 0; kb < c.steps; ++kb) {
-        if (!__all_sync(~0u, mbarWait(smemAddr(&fullBar[s]), phase))) { if (lane == 0) fail(3000 + s); bad = true; break; }
-        const uint32_t sA = ring + s * stageBytes, sB = sA + aBytes;
-        const int left = length - kb * kBK, chunks = min(kBK / kUmmaK, (left + kUmmaK - 1) / kUmmaK);
-        if (MODE == EXPERT_DW && left < chunks * kUmmaK) {
-          // rows behind the expert's last are somebody's old values: zeros, so that they add nothing (a row is 128 bytes of every box)
-          const int rows = chunks * kUmmaK - left, boxes = 2 + bn / 64;
-          for (int i = lane; i < boxes * rows * 8; i += 32) {
-            const int box = i / (rows * 8), r = i / 8 % rows;
-            *(uint4*)(smem + (size_t)s * stageBytes + box * kBlockBytes + (left + r) * 128 + i % 8 * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fenceProxyAsync();
-          __syncwarp();
-        }
+      for (int t = blockIdx.x; t < tiles.count && !bad && !*abortFlag; t += gridDim.x, ++it) {
+        const Tile c = tiles.at(t);
+        const int buf = it & 1;
+        if (!mbarWait(smemAddr(&accEmpty[buf]), ((it >> 1) & 1) ^ 1)) { fail(2000 + buf); break; }
         tcFenceAfter();
-        if (lane == 0) {
-          for (int k = 0; k < chunks; ++k) {
-            const uint64_t da = kAcrossA ? descAcross(sA + k * kUmmaK * 128) : umDescK128(sA + k * kUmmaK * 2);
-            const uint64_t db = kAcrossB ? descAcross(sB + k * kUmmaK * 128) : umDescK128(sB + k * kUmmaK * 2);
-            ummaBf16(dT, da, db, idesc, (kb | k) != 0);
-          }
+        const uint32_t dT = tmemBase + buf * kAccCols;
+        for (int kb = 0; kb < c.steps; ++kb) {
+          if (!mbarWait(smemAddr(&fullBar[s]), phase)) { fail(3000 + s); bad = true; break; }
+          tcFenceAfter();
+          const uint32_t sA = ring + s * stageBytes, sB = sA + aBytes;
+          const uint64_t da = umDescK128(sA), db = descOf<kAcrossB<MODE>>(sB);
+#pragma unroll
+          for (int k = 0; k < kBK / kUmmaK; ++k)   // (behind the sum's end are zeros)
+            ummaBf16(dT, da + k * kNextDesc<false>, db + k * kNextDesc<kAcrossB<MODE>>, idesc, (kb | k) != 0);
           ummaCommit(smemAddr(&emptyBar[s]));
+          if (++s == stages) { s = 0; phase ^= 1; }
         }
-        __syncwarp();
-        if (++s == stages) { s = 0; phase ^= 1; }
+        if (!bad) ummaCommit(smemAddr(&accFull[buf]));
       }
-      if (bad) break;
-      if (lane == 0) ummaCommit(smemAddr(&accFull[buf]));
-      __syncwarp();
     }
+    __syncwarp();
   } else {
-    // ---- epilogue: TMEM lanes [32q, 32q+32) belong to the warps with warp % 4 == q; of those two, each takes every other 64 columns
-    const int q = warp & 3, half = (warp - 2) >> 2;
-    uint8_t* wbuf = epiBuf + (size_t)(warp - 2) * 4096;
+    const int q = warp & 3, half = (warp - kFirstEpiWarp) >> 2;   // TMEM lanes [32q, 32q+32) belong to the warps with warp % 4 == q
+    uint8_t* wbuf = epiBuf + (size_t)(warp - kFirstEpiWarp) * 4096;
     int it = 0;
-    for (int t = blockIdx.x; t < nTiles && !__any_sync(~0u, *abortFlag); t += gridDim.x) {
-      const Tile c = tileAt(t);
+    for (int t = blockIdx.x; t < tiles.count && !__any_sync(~0u, *abortFlag); t += gridDim.x, ++it) {
+      const Tile c = tiles.at(t);
       const int buf = it & 1;
-      const uint32_t aph = (it >> 1) & 1;
-      if (c.steps) {
-        ++it;
-        if (!__all_sync(~0u, mbarWait(smemAddr(&accFull[buf]), aph))) { if (lane == 0) fail(4000 + buf); break; }
-        tcFenceAfter();
-      }
-      const int row = c.row0 + q * 32, left = (MODE == EXPERT_DW ? a.outRows : c.rows) - row;   // this warp's first row, rows from there on
-      const uint32_t tBase = tmemBase + ((uint32_t)(q * 32) << 16) + buf * kAccCols;
-      const size_t first = (size_t)c.e * (MODE == EXPERT_DW ? a.outRows : a.cap) + row;
-      for (int cc = half * 64; cc < outCols && c.col0 + cc < a.cols && left > 0; cc += 128) {
-        const int col = c.col0 + cc, width = min(min(64, outCols - cc), a.cols - col);   // a multiple of 8
-        // 64 columns of 32 rows between the lanes (a row each) and whole lines of memory, 16-byte chunks XOR-swizzled by row
-        auto chunk = [&](int r, int j) { return (uint4*)(wbuf + r * 128 + ((j ^ (r & 7)) * 16)); };
-        auto store = [&](__nv_bfloat16* to, size_t ld) {
-          __syncwarp();
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int r = k * 4 + (lane >> 3), j = lane & 7;
-            if (r < left && j * 8 < width) *(uint4*)(to + (size_t)r * ld + j * 8) = *chunk(r, j);
-          }
-          __syncwarp();
-        };
-        auto sums = [&](int part, int h, float (&v)[32]) {
-          uint32_t r[32];
-          tmemLd32(tBase + part * outCols + cc + h * 32, r);
-          tmemLdWait32(r);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-          if (MODE == EXPERT_FORWARD && a.bias) {
-            const __nv_bfloat16* b = (const __nv_bfloat16*)a.bias + ((size_t)c.e * parts + part) * a.cols + col + h * 32;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              if (h * 32 + j * 8 >= width) break;
-              float f[8];
-              unpackBf16x8(__ldg((const uint4*)b + j), f);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) v[j * 8 + i] += f[i];
-            }
-          }
-        };
-        if (MODE == EXPERT_FORWARD && a.pre) {
-          for (int p = 0; p < parts; ++p) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (h * 32 >= width) break;
-              float v[32];
-              sums(p, h, v);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) *chunk(lane, h * 4 + j) = packBf16x8(v + j * 8);
-            }
-            store((__nv_bfloat16*)a.pre + (first * parts + p) * a.cols + col, (size_t)parts * a.cols);
-          }
-        }
-        if (MODE == EXPERT_FORWARD && a.residual) {
-          const __nv_bfloat16* from = (const __nv_bfloat16*)a.residual + first * a.cols + col;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int r = k * 4 + (lane >> 3), j = lane & 7;
-            *chunk(r, j) = r < left && j * 8 < width ? *(const uint4*)(from + (size_t)r * a.cols + j * 8) : make_uint4(0, 0, 0, 0);
-          }
-          __syncwarp();
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (h * 32 >= width) break;
-          float v[32];
-          if (MODE == EXPERT_DW && c.steps == 0) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 0.0f;
-          } else {
-            sums(0, h, v);
-          }
-          if (MODE == EXPERT_FORWARD) {
-            if (parts == 2) {
-              float u[32];
-              sums(1, h, u);
-              const int base = a.act == ACT_SWIGLU ? ACT_SILU : ACT_GELU;
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = activation(base, v[i]) * u[i];
-            } else if (a.act != ACT_NONE) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = activation(a.act, v[i]);
-            }
-            if (a.residual) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                float f[8];
-                unpackBf16x8(*chunk(lane, h * 4 + j), f);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[j * 8 + i] += f[i];
-              }
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) *chunk(lane, h * 4 + j) = packBf16x8(v + j * 8);
-        }
-        store((__nv_bfloat16*)a.out + first * a.cols + col, (size_t)a.cols);
-      }
-      if (c.steps) {
-        tcFenceBefore();
-        __syncwarp();
-        if (lane == 0) mbarArrive(smemAddr(&accEmpty[buf]));
-      }
+      if (!__all_sync(~0u, mbarWait(smemAddr(&accFull[buf]), (it >> 1) & 1))) { if (lane == 0) fail(4000 + buf); break; }
+      tcFenceAfter();
+      storeTile<MODE>(a, tiles, c, q * 32, partCols, tmemBase + ((uint32_t)(q * 32) << 16) + buf * kAccCols, wbuf, half, lane);
+      tcFenceBefore();
+      __syncwarp();
+      if (lane == 0) mbarArrive(smemAddr(&accEmpty[buf]));
     }
   }
 
@@ -380,10 +405,230 @@ expertGemmKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   }
 }
 
-const void* expertGemmKernelFn(int mode) {
-  return mode == EXPERT_DW ? (const void*)expertGemmKernel<EXPERT_DW> : mode == EXPERT_DX ? (const void*)expertGemmKernel<EXPERT_DX> : (const void*)expertGemmKernel<EXPERT_FORWARD>;
+// ---------------------------------------------------------------------------------------------- CTA pairs, tiles of 256 rows
+// FORWARD: tmB has boxes of 128 rows of W, tmBNarrow of 64, half the width of a tile each; else tmB has boxes of 64 x 64.
+//   fullBar[s]   (the first CTA's copy) counts the bytes of both CTAs' loads of ring stage s;
+//   emptyBar[s]  in each CTA: a commit that signals both frees the stage;
+//   accFull[b]   in each CTA: the same publishes accumulator b to both epilogues;
+//   accEmpty[b]  (the first CTA's copy) collects the epilogue warps of both;
+//   tailBar[s]   DW, in each CTA: the bytes of its own loads of a stage whose last rows are to be zeroed;
+//   fixBar[s]    (the first CTA's copy) the other CTA has written its zeros; the first CTA's warp for that arrives at fullBar then, in the
+//                producer's place. (An arrival of both producers in every step, so that fullBar could count two, took half of DW's rate.)
+template <int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmBNarrow,
+                     const __grid_constant__ ExpertGemmArgs a) {
+  constexpr uint32_t kStageBytes = 2 * kHalfBytes;
+  extern __shared__ uint8_t smemRaw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smemRaw + 1023) & ~(uintptr_t)1023);
+  uint8_t* epiBuf = smem + kRingBytes;
+  uint8_t* ctrl = epiBuf + kEpiBytes;
+  uint64_t* fullBar = (uint64_t*)ctrl;              // [kPairStages]
+  uint64_t* emptyBar = fullBar + kPairStages;       // [kPairStages]
+  uint64_t* tailBar = emptyBar + kPairStages;       // [kPairStages]
+  uint64_t* fixBar = tailBar + kPairStages;         // [kPairStages]
+  uint64_t* accFull = fixBar + kPairStages;         // [2]
+  uint64_t* accEmpty = accFull + 2;                 // [2]
+  uint32_t* tmemSlot = (uint32_t*)(accEmpty + 2);
+  volatile uint32_t* abortFlag = tmemSlot + 1;
+  int* table = (int*)(ctrl + kCtrlBytes);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t cr = clusterCtaRank();
+  const bool leader = cr == 0;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      for (uint64_t* b : {fullBar, emptyBar, tailBar, fixBar}) mbarInit(smemAddr(&b[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) { mbarInit(smemAddr(&accFull[b]), 1); mbarInit(smemAddr(&accEmpty[b]), 2 * kEpiWarps); }
+    *abortFlag = 0;
+    mbarInitFence();
+    prefetchTensorMap(&tmA);
+    prefetchTensorMap(&tmB);
+  }
+  if (warp == 1) {
+    tmemAllocPair(smemAddr(tmemSlot), kTmemCols);
+    tmemRelinquishPair();
+  }
+  pdlEnter();   // the set-up above overlaps the end of the kernel before
+  if (warp == 0) Tiles<MODE, 256>::fill(a, table, lane);
+  tcFenceBefore();
+  __syncthreads();
+  __syncwarp();
+  clusterSync();   // both CTAs' barriers are initialised before either signals the other's
+  tcFenceAfter();
+  const uint32_t tmemBase = *tmemSlot;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  // us of a step. Half as wide a tile fetches three quarters as much: it pays where whole ones would leave most of the SMs idle
+  const Tiles<MODE, 256> tiles(a, table, pairs, 128, 128, [](int w) { return w == 256 ? 0.35f : 0.22f; });
+  const int bn = tiles.bn, parts = tiles.parts, halfCols = bn / 2;   // columns that each CTA stages
+  const uint32_t ring = smemAddr(smem);
+  auto fail = [&](uint32_t what) {
+    *abortFlag = 1;
+    stSharedCluster(mapaShared(smemAddr((const void*)abortFlag), cr ^ 1), 1u);   // the partner gives up too
+    reportTimeout(a, what);
+  };
+  // Rows of this CTA's half of the first operand in use (DW: of the result), and its first row or column of the second
+  auto rowsIn = [&](const Tile& c, int rank) { return min(128, tiles.rowLimit(c) - c.row0 - rank * 128); };
+  auto firstB = [&](const Tile& c) { return parts == 2 ? (int)cr * a.cols + c.col0 : c.col0 + (int)cr * halfCols; };
+  auto colsIn = [&](const Tile& c, int rank) { return parts == 2 ? min(halfCols, a.cols - c.col0) : min(halfCols, a.cols - c.col0 - rank * halfCols); };
+  // Bytes that CTA `rank` loads for a step: nothing of an operand where it has no row or column. With neither it still loads a box from behind the matrix (zeros, no
+  // traffic): what keeps a CTA within one round of the ring of its partner is that no step is complete without its bytes.
+  auto bytesA = [&](const Tile& c, int rank) {
+    const int n = rowsIn(c, rank);
+    return n <= 0 ? 0u : kAcrossA<MODE> && n <= 64 ? kBlockBytes : kHalfBytes;
+  };
+  auto bytesB = [&](const Tile& c, int rank) {
+    const int n = colsIn(c, rank);
+    return n <= 0 && rowsIn(c, rank) > 0 ? 0u : !kAcrossB<MODE> ? (uint32_t)halfCols * 128 : n <= 64 ? kBlockBytes : kHalfBytes;
+  };
+
+  if (warp == 0) {
+    if (electOne()) {
+      int s = 0, armed = 0, tails = 0;   // stages that were ever loaded; bit s: the last load of stage s counts on tailBar
+      uint32_t phase = 0, tailPhase = 0;
+      const CUtensorMap* mapB = kAcrossB<MODE> || bn == 256 ? &tmB : &tmBNarrow;
+      for (int t = pair; t < tiles.count && !*abortFlag; t += pairs) {
+        const Tile c = tiles.at(t);
+        const uint32_t mineA = bytesA(c, cr), mineB = bytesB(c, cr), both = bytesA(c, 0) + bytesA(c, 1) + bytesB(c, 0) + bytesB(c, 1);
+        const int row = c.row0 + (int)cr * 128, col = firstB(c);
+        for (int kb = 0; kb < c.steps; ++kb) {
+          if (!mbarWait(smemAddr(&emptyBar[s]), phase ^ 1)) { fail(1000 + s); break; }
+          if (*abortFlag) break;
+          const uint32_t sA = ring + s * kStageBytes, sB = sA + kHalfBytes;
+          const bool tail = MODE == EXPERT_DW && kb == c.steps - 1 && c.rows % kUmmaK != 0;
+          uint32_t full;
+          if (tail) {
+            full = mapaShared(smemAddr(&tailBar[s]), cr);
+            mbarExpectTx(smemAddr(&tailBar[s]), mineA + mineB);
+            tails |= 1 << s;
+            tailPhase ^= 1u << s;
+          } else {
+            full = mapaShared(smemAddr(&fullBar[s]), 0);
+            if (leader) mbarExpectTx(smemAddr(&fullBar[s]), both);
+            tails &= ~(1 << s);
+          }
+          if (kAcrossA<MODE>) {
+            if (mineA) tmaLoad3dPair(sA, &tmA, row, kb * kBK, c.e, full);
+            if (mineA > kBlockBytes) tmaLoad3dPair(sA + kBlockBytes, &tmA, row + 64, kb * kBK, c.e, full);
+          } else if (mineA) {
+            tmaLoad3dPair(sA, &tmA, kb * kBK, row, c.e, full);
+          }
+          if (kAcrossB<MODE>) {
+            if (mineB) tmaLoad3dPair(sB, &tmB, col, kb * kBK, c.e, full);
+            if (mineB > kBlockBytes) tmaLoad3dPair(sB + kBlockBytes, &tmB, col + 64, kb * kBK, c.e, full);
+          } else if (mineB) {
+            tmaLoad3dPair(sB, mapB, kb * kBK, col, c.e, full);
+          }
+          armed = max(armed, s + 1);
+          if (++s == kPairStages) { s = 0; phase ^= 1; }
+        }
+      }
+      if (*abortFlag) {
+        // copies already issued (by either CTA) still write into shared memory: wait for them (bounded). Stages in front of s were loaded in this round
+        for (int i = 0; i < armed; ++i) {
+          if (tails >> i & 1) mbarWait(smemAddr(&tailBar[i]), (tailPhase >> i & 1) ^ 1, 1u << 20);
+          else if (leader) mbarWait(smemAddr(&fullBar[i]), i < s ? phase : phase ^ 1, 1u << 20);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (leader && electOne()) {
+      const uint32_t idesc = umInstrBf16(256, bn) | (kAcrossA<MODE> ? 1u << 15 : 0u) | (kAcrossB<MODE> ? 1u << 16 : 0u);
+      int s = 0, it = 0;
+      uint32_t phase = 0;
+      bool bad = false;
+      for (int t = pair; t < tiles.count && !bad && !*abortFlag; t += pairs) {
+        const Tile c = tiles.at(t);
+        if (c.steps == 0) continue;   // nothing to add up: the epilogue writes zeros
+        const int buf = it & 1;
+        if (!mbarWait(smemAddr(&accEmpty[buf]), ((it >> 1) & 1) ^ 1)) { fail(2000 + buf); break; }
+        ++it;
+        tcFenceAfter();
+        const uint32_t dT = tmemBase + buf * kAccCols;
+        const int last = (tiles.length(c) - (c.steps - 1) * kBK + kUmmaK - 1) / kUmmaK;   // sixteens in the last step
+        for (int kb = 0; kb < c.steps; ++kb) {
+          if (!mbarWait(smemAddr(&fullBar[s]), phase)) { fail(3000 + s); bad = true; break; }
+          tcFenceAfter();
+          const uint32_t sA = ring + s * kStageBytes;
+          const uint64_t da = descOf<kAcrossA<MODE>>(sA), db = descOf<kAcrossB<MODE>>(sA + kHalfBytes);
+          const int chunks = kb == c.steps - 1 ? last : kBK / kUmmaK;
+#pragma unroll
+          for (int k = 0; k < kBK / kUmmaK; ++k)
+            if (k < chunks) ummaBf16Pair(dT, da + k * kNextDesc<kAcrossA<MODE>>, db + k * kNextDesc<kAcrossB<MODE>>, idesc, (kb | k) != 0);
+          ummaCommitPair(smemAddr(&emptyBar[s]), 3);
+          if (++s == kPairStages) { s = 0; phase ^= 1; }
+        }
+        if (!bad) ummaCommitPair(smemAddr(&accFull[buf]), 3);
+      }
+    }
+    __syncwarp();
+  } else if (warp < kFixWarp) {
+    const int q = warp & 3, half = (warp - kFirstEpiWarp) >> 2;   // TMEM lanes [32q, 32q+32) belong to the warps with warp % 4 == q
+    uint8_t* wbuf = epiBuf + (size_t)(warp - kFirstEpiWarp) * 4096;
+    int it = 0;
+    for (int t = pair; t < tiles.count && !__any_sync(~0u, *abortFlag); t += pairs) {
+      const Tile c = tiles.at(t);
+      const int buf = it & 1;
+      if (c.steps) {
+        if (!__all_sync(~0u, mbarWait(smemAddr(&accFull[buf]), (it >> 1) & 1))) { if (lane == 0) fail(4000 + buf); break; }
+        ++it;
+        tcFenceAfter();
+      }
+      storeTile<MODE>(a, tiles, c, c.row0 + (int)cr * 128 + q * 32, halfCols, tmemBase + ((uint32_t)(q * 32) << 16) + buf * kAccCols, wbuf, half, lane);
+      if (c.steps) {
+        tcFenceBefore();
+        __syncwarp();
+        if (lane == 0) mbarArriveRelaxed(mapaShared(smemAddr(&accEmpty[buf]), 0));
+      }
+    }
+  } else if (MODE == EXPERT_DW) {
+    // rows behind the expert's last are somebody's old values: zeros up to the next sixteen, so that they add nothing (a row is 128 bytes of every box)
+    int at = 0;   // steps of the tiles before
+    uint32_t phases = 0;
+    for (int t = pair; t < tiles.count && !__any_sync(~0u, *abortFlag); t += pairs) {
+      const Tile c = tiles.at(t);
+      if (c.steps == 0) continue;
+      const int s = (at + c.steps - 1) % kPairStages, rows = (kUmmaK - c.rows % kUmmaK) % kUmmaK;
+      at = (at + c.steps) % kPairStages;
+      if (rows == 0) continue;
+      const uint32_t parity = phases >> s & 1;
+      phases ^= 1u << s;
+      if (!__all_sync(~0u, mbarWait(smemAddr(&tailBar[s]), parity))) { if (lane == 0) fail(5000 + s); break; }
+      const int from = c.rows - (c.steps - 1) * kBK;
+      for (int i = lane; i < 4 * rows * 8; i += 32) {
+        const int box = i / (rows * 8), r = i / 8 % rows;
+        *(uint4*)(smem + (size_t)s * kStageBytes + box * kBlockBytes + (from + r) * 128 + i % 8 * 16) = make_uint4(0, 0, 0, 0);
+      }
+      fenceProxyAsync();
+      __syncwarp();
+      if (!leader) {
+        if (lane == 0) mbarArriveCluster(mapaShared(smemAddr(&fixBar[s]), 0));
+      } else {
+        if (!__all_sync(~0u, mbarWaitCluster(smemAddr(&fixBar[s]), parity))) { if (lane == 0) fail(6000 + s); break; }
+        if (lane == 0) mbarArrive(smemAddr(&fullBar[s]));
+      }
+    }
+  }
+
+  // the pair meets: nobody touches the partner's shared or tensor memory afterwards
+  tcFenceBefore();
+  __syncthreads();
+  __syncwarp();
+  clusterSync();
+  if (warp == 1) {
+    tcFenceAfter();
+    tmemDeallocPair(tmemBase, kTmemCols);
+  }
+}
+
+const void* expertGemmKernelFn(int mode) { return mode == EXPERT_DX ? (const void*)expertGemmKernel<EXPERT_DX> : (const void*)expertGemmKernel<EXPERT_FORWARD>; }
+const void* expertGemmPairKernelFn(int mode) {
+  return mode == EXPERT_DW ? (const void*)expertGemmPairKernel<EXPERT_DW>
+         : mode == EXPERT_DX ? (const void*)expertGemmPairKernel<EXPERT_DX> : (const void*)expertGemmPairKernel<EXPERT_FORWARD>;
 }
 size_t expertGemmSmemBytes() { return kSmemBytes; }
-int expertGemmThreads() { return kThreads; }
+int expertGemmThreads(bool pair) { return pair ? kPairThreads : kThreads; }
 
 }  // namespace b200

@@ -139,22 +139,48 @@ static ncclResult_t checkLinear(const ncclEpGroup* g, const char* what, int expe
   return ncclSuccess;
 }
 
-// A product of [experts][rowsA][innerA] and [experts][rowsB][innerB]; see expert_gemm_sm100.cu for what each mode makes of them.
+// Pairs that can be resident at once: with more the last ones would start when the first have finished all their tiles.
+static int pairsAtOnce(ncclEpGroup* g) {
+  int n = g->expertPairs.load(std::memory_order_relaxed);
+  if (n >= 0) return n;
+  n = g->smCount / 2;
+  for (int mode : {EXPERT_FORWARD, EXPERT_DX, EXPERT_DW}) {
+    const void* fn = expertGemmPairKernelFn(mode);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(g->smCount & ~1);
+    cfg.blockDim = dim3(expertGemmThreads(true));
+    cfg.dynamicSmemBytes = expertGemmSmemBytes();
+    int clusters = 0;
+    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)expertGemmSmemBytes()) == cudaSuccess &&
+        cudaOccupancyMaxActiveClusters(&clusters, fn, &cfg) == cudaSuccess && clusters > 0)
+      n = std::min(n, clusters);
+    else
+      (void)cudaGetLastError();
+  }
+  g->expertPairs.store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// A product of [experts][rowsA][innerA] and [experts][rowsB][innerB]; see expert_gemm_sm100.cu for what each mode makes of them. The host knows how many
+// rows an expert may have, not how many it has: where a tile of 128 holds them all, single CTAs take a tile each, else pairs tiles of 256.
 static ncclResult_t launchExpertGemm(ncclEpGroup* g, int mode, const void* A, int innerA, int rowsA, const void* B, int innerB, int rowsB, ExpertGemmArgs* a, cudaStream_t stream) {
-  CUtensorMap maps[4];
-  const bool acrossA = mode == EXPERT_DW, acrossB = mode != EXPERT_FORWARD;
-  NCCLCHECK(makeMap(&maps[0], A, innerA, rowsA, a->experts, acrossA ? 64 : 128));
-  if (acrossA) maps[1] = maps[0];
-  else NCCLCHECK(makeMap(&maps[1], A, innerA, rowsA, a->experts, 32));
-  NCCLCHECK(makeMap(&maps[2], B, innerB, rowsB, a->experts, 64));
-  if (acrossB) maps[3] = maps[2];
-  else NCCLCHECK(makeMap(&maps[3], B, innerB, rowsB, a->experts, 32));
+  const bool pair = mode == EXPERT_DW || a->cap > kExpertOneCtaRows;
+  a->boxRows = pair ? 128 : (a->cap + 7) / 8 * 8;
   a->status = g->comm->devStatusDev;
+  CUtensorMap maps[3];
+  NCCLCHECK(makeMap(&maps[0], A, innerA, rowsA, a->experts, mode == EXPERT_DW ? 64 : a->boxRows));
+  NCCLCHECK(makeMap(&maps[1], B, innerB, rowsB, a->experts, mode == EXPERT_FORWARD ? 128 : 64));
+  if (mode == EXPERT_FORWARD) NCCLCHECK(makeMap(&maps[2], B, innerB, rowsB, a->experts, pair ? 64 : 32));
+  else maps[2] = maps[1];
+  void* args[4] = {&maps[0], &maps[1], &maps[2], a};
   // no more CTAs than the narrowest tiles of all rows
-  const double most = (double)a->experts * (((mode == EXPERT_DW ? a->outRows : a->cap) + 127) / 128) * ((a->cols + 31) / 32);
-  const int grid = (int)std::min<double>(g->smCount, most);
-  void* args[5] = {&maps[0], &maps[1], &maps[2], &maps[3], a};
-  return launchMoe(g, expertGemmKernelFn(mode), dim3(grid), expertGemmThreads(), expertGemmSmemBytes(), args, stream);
+  const double rows = mode == EXPERT_DW ? a->outRows : a->cap, tilesN = (a->cols + 31) / 32;
+  if (pair) {
+    const int pairs = (int)std::min<double>(pairsAtOnce(g), (double)a->experts * (int)((rows + 255) / 256) * tilesN);
+    return launchMoe(g, expertGemmPairKernelFn(mode), dim3(2 * pairs), expertGemmThreads(true), expertGemmSmemBytes(), args, stream);
+  }
+  const int ctas = (int)std::min<double>(g->smCount, (double)a->experts * tilesN);
+  return launchMoe(g, expertGemmKernelFn(mode), dim3(ctas), expertGemmThreads(false), expertGemmSmemBytes(), args, stream);
 }
 
 // Slices of rows that the activation's backward works on at a time: enough CTAs to fill the chip eight times over.

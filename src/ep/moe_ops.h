@@ -43,6 +43,7 @@ struct ExpertGemmArgs {
   int outRows;                // DW: rows of the result (of W); else the rows in use
   int cols;                   // columns of the result
   int depth;                  // length of the sums (DW: cap; the rows in use count)
+  int boxRows;                // rows of a box of the first operand (the kernel on single CTAs)
   int gated, act;             // forward: gate rows of W, then up rows, `cols` of each
   const void* bias;           // bf16 [experts][cols, twice when gated] or null
   const void* residual;       // bf16, laid out like out, or null
@@ -51,9 +52,11 @@ struct ExpertGemmArgs {
   uint32_t* status;           // {code, kind, what, CTA} of the communicator, written when a wait runs out
 };
 
-const void* expertGemmKernelFn(int mode);
+constexpr int kExpertOneCtaRows = 128;   // an expert with more rows takes the kernel on CTA pairs
+const void* expertGemmKernelFn(int mode);       // FORWARD, DX; tensor maps of A, B and B in boxes of 32 rows
+const void* expertGemmPairKernelFn(int mode);   // tensor maps of A, B and B in boxes of 64 rows; clusters of two
 size_t expertGemmSmemBytes();
-int expertGemmThreads();
+int expertGemmThreads(bool pair);
 
 // ---------------------------------------------------------------- row kernels (moe_backward.cu)
 struct ExpertActArgs {

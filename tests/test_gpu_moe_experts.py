@@ -169,6 +169,20 @@ def test_large(ep, E, cap, n, k, act, counts):
     check(ep, E, cap, n, k, act, counts, bias=act is None)
 
 
+# The second CTA of a pair has neither a row nor a column of such tiles, and many steps in which to fall behind
+@pytest.mark.parametrize("n,k", [(48, 8192), (8192, 48), (64, 64)])
+def test_tiles_that_one_cta_of_a_pair_has_no_part_in(ep, n, k):
+    check(ep, 64, 160, n, k, "relu", [(7 * e) % 120 for e in range(64)])
+    x, w = torch.randn(64, 160, k, device="cuda").bfloat16(), torch.randn(64, n, k, device="cuda").bfloat16()
+    c = torch.tensor([(11 * e) % 120 + 1 for e in range(64)], dtype=torch.int32, device="cuda")
+    d = torch.randn(64, 160, n, device="cuda").bfloat16()
+    for _ in range(50):
+        ep.expert_linear(x, w, c)
+        ep.expert_linear_backward(d, x, w, c)
+    torch.cuda.synchronize()
+    assert ep.comm.async_error() == 0
+
+
 def test_residual_in_place_and_none_kept(ep):
     x, w, b, r, _, c = make(3, 50, 64, 128, "gelu", 9, True, True, [50, 0, 20])
     want = ep.expert_linear(x, w, c, bias=b, activation="gelu", residual=r, out=torch.zeros(3, 50, 64, dtype=torch.bfloat16, device="cuda"))
