@@ -254,24 +254,28 @@ class ExpertParallel:
             L.ncclEpExpertLinearBackwardWork.restype = ctypes.c_size_t
         dev = ctypes.c_int()
         _lib.check(L.ncclCommCuDevice(self.comm.handle, ctypes.byref(dev)), "ncclCommCuDevice", L)
-        self._device = dev.value
-        self._route_cfgs = {}
         torch = self.torch
+        self._device, self._place = dev.value, torch.device("cuda", dev.value)
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or current_stream
+        self._route_cfgs = {}
         self._logit_codes = {torch.float32: FP32, torch.float16: FP16, torch.bfloat16: BF16}
 
     def _moe_call(self, name, *args):
-        _lib.check(self._moe[name](*args, current_stream(self._device)), name, self.lib)
+        rc = self._moe[name](*args, self._raw_stream(self._device))
+        if rc:
+            _lib.check(rc, name, self.lib)
 
     def _need(self, name, t, dtype, shape):
         """Checks a tensor: type, shape, contiguous, on the group's GPU."""
-        if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or not t.is_cuda or t.device.index != self._device:
-            raise ValueError("%s must be a contiguous %s tensor %s on cuda:%d, not %s %s%s on %s" % (
-                name, str(dtype).replace("torch.", ""), list(shape), self._device, str(t.dtype).replace("torch.", ""), list(t.shape),
-                "" if t.is_contiguous() else " (strided)", t.device))
+        if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == self._device:
+            return
+        raise ValueError("%s must be a contiguous %s tensor %s on cuda:%d, not %s %s%s on %s" % (
+            name, str(dtype).replace("torch.", ""), list(shape), self._device, str(t.dtype).replace("torch.", ""), list(t.shape),
+            "" if t.is_contiguous() else " (strided)", t.device))
 
     def _result(self, name, t, dtype, shape):
         if t is None:
-            return self.torch.empty(shape, dtype=dtype, device=self._device)
+            return self.torch.empty(*shape, dtype=dtype, device=self._place)   # (sizes one by one: 0.7 us less than as a tuple)
         self._need(name, t, dtype, shape)
         return t
 
@@ -293,10 +297,10 @@ class ExpertParallel:
         return ctypes.addressof(cfg)
 
     def _logits(self, logits):
-        code = self._logit_codes.get(logits.dtype)
-        if code is None or logits.dim() != 2 or logits.shape[1] != self.E:
-            raise ValueError("logits must be an fp32, fp16 or bf16 tensor [tokens, %d], not %s %s" % (self.E, str(logits.dtype).replace("torch.", ""), list(logits.shape)))
-        self._need("logits", logits, logits.dtype, logits.shape)
+        code, shape = self._logit_codes.get(logits.dtype), logits.shape
+        if code is None or len(shape) != 2 or shape[1] != self.E:
+            raise ValueError("logits must be an fp32, fp16 or bf16 tensor [tokens, %d], not %s %s" % (self.E, str(logits.dtype).replace("torch.", ""), list(shape)))
+        self._need("logits", logits, logits.dtype, shape)
         return code
 
     def route(self, logits, topk, score="softmax", bias=None, groups=1, keep_groups=None, group_score="max", renormalize=True, scale=1.0, idx=None, weights=None):

