@@ -54,6 +54,28 @@ __device__ __forceinline__ void tmaLoad3dPair(uint32_t dstSmem, const CUtensorMa
       ::"r"(dstSmem), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(barCluster) : "memory");
 }
 
+// Waits of the roles: they end early when another role has given up. The flag is looked at where there is something to wait for, not in every step.
+__device__ __forceinline__ bool waitOr(uint32_t bar, uint32_t parity, volatile uint32_t* abortFlag) {
+  if (mbarTry(bar, parity)) return true;
+  for (uint32_t i = 0; i < (1u << 24) && !*abortFlag; ++i)
+    if (mbarTry(bar, parity)) return true;
+  return false;
+}
+// The same for a warp of the epilogue: one lane asks, now and then (eight warps that ask all the time slow the others' barriers down).
+__device__ __forceinline__ bool warpWaitOr(uint32_t bar, uint32_t parity, volatile uint32_t* abortFlag, int lane) {
+  bool ok = true;
+  if (lane == 0) {
+    ok = mbarTry(bar, parity);
+    for (uint32_t i = 0; i < (1u << 24) && !ok && !*abortFlag; ++i) {
+      __nanosleep(64);
+      ok = mbarTry(bar, parity);
+    }
+  }
+  ok = __shfl_sync(~0u, (int)ok, 0);
+  if (ok) mbarTry(bar, parity);   // every lane has seen the phase end
+  return ok;
+}
+
 // Arrival at an mbarrier of the pair that publishes no memory: with release it waits until all of the warp's stores are done (DW over experts of
 // 64 rows, 32 x 4096 x 7168: 598 us, 439 with this one).
 __device__ __forceinline__ void mbarArriveRelaxed(uint32_t clusterAddr) {
@@ -122,15 +144,15 @@ struct Tiles {
     if (lane == 0) start[a.experts] = before;
   }
 
-  // Width of the tiles, from kMaxBN down in steps of `step`: what `workers` CTAs or pairs finish first, a wave of tiles taken to cost `cost(width)`. The sums do
-  // not depend on it.
+  // Width of the tiles, kMaxBN or half as much and so on: what `workers` CTAs or pairs finish first, a wave of tiles taken to cost `cost(width)`. The
+  // sums do not depend on it.
   template <typename Cost>
-  __device__ __forceinline__ Tiles(const ExpertGemmArgs& args, const int* table, int workers, int narrowest, int step, Cost cost) : a(args), start(table) {
+  __device__ __forceinline__ Tiles(const ExpertGemmArgs& args, const int* table, int workers, int narrowest, Cost cost) : a(args), start(table) {
     parts = MODE == EXPERT_FORWARD && a.gated ? 2 : 1;
     const int rowTiles = start[a.experts];
     float best = 0.0f;
     bn = kMaxBN;
-    for (int w = kMaxBN; w >= narrowest; w -= step) {
+    for (int w = kMaxBN; w >= narrowest; w /= 2) {
       const int n = rowTiles * ((a.cols + w / parts - 1) / (w / parts));
       const float all = (n + workers - 1) / workers * cost(w);
       if (w == kMaxBN || all < best) { best = all; bn = w; }
@@ -173,10 +195,10 @@ __device__ __forceinline__ void reportTimeout(const ExpertGemmArgs& a, uint32_t 
 }
 
 // Epilogue of one warp for its 32 rows, `row` the first of them, and every other 64 columns of the tile: tBase is the tensor-memory address of the
-// warp's first lane and the tile's first column, the columns of `up` begin partCols behind those of `gate`. A lane has a row of the accumulator; 64 columns at a time pass through 4 KiB of shared memory (16-byte chunks
+// warp's first lane and the tile's first column. A lane has a row of the accumulator; 64 columns at a time pass through 4 KiB of shared memory (16-byte chunks
 // XOR-swizzled by row), so that memory sees 128 contiguous bytes of a row.
 template <int MODE, typename T>
-__device__ __forceinline__ void storeTile(const ExpertGemmArgs& a, const T& tiles, const Tile& c, int row, int partCols, uint32_t tBase, uint8_t* wbuf, int half, int lane) {
+__device__ __forceinline__ void storeTile(const ExpertGemmArgs& a, const T& tiles, const Tile& c, int row, uint32_t tBase, uint8_t* wbuf, int half, int lane) {
   const int parts = tiles.parts, outCols = tiles.outCols, left = tiles.rowLimit(c) - row;   // rows from here on
   const size_t first = (size_t)c.e * (MODE == EXPERT_DW ? a.outRows : a.cap) + row;
   for (int cc = half * 64; cc < outCols && c.col0 + cc < a.cols && left > 0; cc += 128) {
@@ -193,7 +215,7 @@ __device__ __forceinline__ void storeTile(const ExpertGemmArgs& a, const T& tile
     };
     auto sums = [&](int part, int h, float (&v)[32]) {
       uint32_t r[32];
-      tmemLd32(tBase + part * partCols + cc + h * 32, r);
+      tmemLd32(tBase + part * outCols + cc + h * 32, r);
       tmemLdWait32(r);
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
@@ -272,8 +294,8 @@ __device__ __forceinline__ void storeTile(const ExpertGemmArgs& a, const T& tile
 }  // namespace
 
 // ---------------------------------------------------------------------------------------------- one CTA per tile of 128 rows
-// No expert has more rows than one tile (cap <= 128): FORWARD and DX, boxes of tmA as high as cap asks for. tmB has boxes of 128 rows of W (DX: 64 x 64), tmBNarrow
-// of 32, for tiles that are not wider than two of them.
+// No expert has more rows than one tile (cap <= 128): FORWARD and DX. tmA has boxes of 32 rows (of fewer, if cap is less), of which those that hold rows are fetched. tmB has
+// boxes of 128 rows of W (DX: 64 x 64), tmBNarrow of 32 (gated: 64) for narrow tiles: one or two boxes make a tile.
 template <int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
 expertGemmKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmBNarrow,
@@ -310,14 +332,14 @@ expertGemmKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   __syncthreads();
   tcFenceAfter();
   const uint32_t tmemBase = *tmemSlot;
-  // the weights are the traffic: a tile costs its columns, and about 32 for its start
-  const Tiles<MODE, 128> tiles(a, table, gridDim.x, MODE == EXPERT_FORWARD && !a.gated ? 32 : 64, 32, [](int w) { return w + 32.0f; });
+  // us of a step, where the weights come as fast as they are used. Wide tiles: 32 experts of 16 rows, 4096 x 7168 gated, 256 columns 299 us, 128 373; two
+  // experts of one row, 28672 x 4096 80 and 126. Narrow ones where they would leave SMs idle: 4096 x 14336 87, 79 and (64) NARROW_US
+  const Tiles<MODE, 128> tiles(a, table, gridDim.x, MODE != EXPERT_FORWARD ? 64 : a.gated ? 128 : 32,
+                               [](int w) { return w == 256 ? 0.33f : w == 128 ? 0.27f : w == 64 ? 0.23f : 0.2f; });
   const int bn = tiles.bn, parts = tiles.parts, outCols = tiles.outCols;
-  // rows of W that a tile fetches for each part: whole boxes, what hangs over belongs to the neighbour, who fetches it too
   const bool narrow = MODE == EXPERT_FORWARD && outCols <= 64;
-  const int boxRows = MODE == EXPERT_FORWARD ? (narrow ? 32 : 128) : 64, boxes = (outCols + boxRows - 1) / boxRows;
-  const int partCols = boxes * boxRows;   // gate and up are one operand: what hangs over is multiplied too and not stored
-  const uint32_t aBytes = (uint32_t)a.boxRows * 128, stageBytes = aBytes + (uint32_t)(parts * partCols) * 128;
+  const int boxRows = MODE != EXPERT_FORWARD ? 64 : !narrow ? 128 : parts == 2 ? 64 : 32, boxes = bn / boxRows;
+  const uint32_t aBytes = (uint32_t)((a.cap + 31) / 32 * a.boxRows) * 128, stageBytes = aBytes + (uint32_t)bn * 128;
   const int stages = (int)min((uint32_t)kMaxStages, kRingBytes / stageBytes);
   const uint32_t ring = smemAddr(smem);
   auto fail = [&](uint32_t what) {
@@ -327,47 +349,58 @@ expertGemmKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 
   if (warp == 0) {
     if (electOne()) {
-      const CUtensorMap* map = narrow ? &tmBNarrow : &tmB;
-      int s = 0, armed = 0;   // stages that were ever loaded
-      uint32_t phase = 0;
+      // one thread feeds the ring: what a step takes here is what the others wait for, so addresses are counted on and not computed
+      const uint32_t bars = smemAddr(fullBar), toEmpty = smemAddr(emptyBar) - bars, stride = boxRows * 128;
+      uint32_t phase = 0, sA = ring, bar = bars;
+      const uint32_t ringEnd = ring + stages * stageBytes;
+      bool whole = false;   // every stage was loaded once
       for (int t = blockIdx.x; t < tiles.count && !*abortFlag; t += gridDim.x) {
         const Tile c = tiles.at(t);
-        for (int kb = 0; kb < c.steps; ++kb) {
-          if (!mbarWait(smemAddr(&emptyBar[s]), phase ^ 1)) { fail(1000 + s); break; }
-          if (*abortFlag) break;
-          const uint32_t full = smemAddr(&fullBar[s]), sA = ring + s * stageBytes;
-          uint32_t sB = sA + aBytes;
-          mbarExpectTx(full, stageBytes);
-          tmaLoad3d(sA, &tmA, kb * kBK, 0, c.e, full);
-          for (int p = 0; p < parts; ++p)
-            for (int i = 0; i < boxes; ++i, sB += boxRows * 128) {
-              if (MODE == EXPERT_FORWARD) tmaLoad3d(sB, map, kb * kBK, p * a.cols + c.col0 + i * boxRows, c.e, full);
-              else tmaLoad3d(sB, &tmB, c.col0 + i * 64, kb * kBK, c.e, full);
-            }
-          armed = max(armed, s + 1);
-          if (++s == stages) { s = 0; phase ^= 1; }
+        const int second = c.col0 + (parts == 2 ? a.cols : boxRows);   // row of W in a tile's second box
+        const int aBoxes = (c.rows + 31) / 32, end = c.steps * kBK;
+        const uint32_t bytes = (uint32_t)(aBoxes * a.boxRows + bn) * 128;
+        for (int x = 0; x < end; x += kBK) {
+          if (!waitOr(bar + toEmpty, phase ^ 1, abortFlag)) { fail(1000); break; }
+          mbarExpectTx(bar, bytes);
+          tmaLoad3d(sA, &tmA, x, 0, c.e, bar);
+          if (aBoxes > 1)
+            for (int i = 1; i < aBoxes; ++i) tmaLoad3d(sA + i * 32 * 128, &tmA, x, i * 32, c.e, bar);
+          const uint32_t sB = sA + aBytes;
+          if (MODE != EXPERT_FORWARD) {
+            for (int i = 0; i < boxes; ++i) tmaLoad3d(sB + i * kBlockBytes, &tmB, c.col0 + i * 64, x, c.e, bar);
+          } else if (!narrow) {
+            tmaLoad3d(sB, &tmB, x, c.col0, c.e, bar);
+            if (boxes == 2) tmaLoad3d(sB + stride, &tmB, x, second, c.e, bar);
+          } else {
+            tmaLoad3d(sB, &tmBNarrow, x, c.col0, c.e, bar);
+            if (boxes == 2) tmaLoad3d(sB + stride, &tmBNarrow, x, second, c.e, bar);
+          }
+          sA += stageBytes;
+          bar += 8;
+          if (sA == ringEnd) { sA = ring; bar = bars; phase ^= 1; whole = true; }
         }
       }
       if (*abortFlag) {
-        // copies already issued still write into shared memory: wait for them (bounded). Stages in front of s were loaded in this round, the others in the one before
-        for (int i = 0; i < armed; ++i) mbarWait(smemAddr(&fullBar[i]), i < s ? phase : phase ^ 1, 1u << 20);
+        // copies already issued still write into shared memory: wait for them (bounded). Stages in front of the next one were loaded in this round, the others in the one before
+        for (uint32_t i = bars; i < bars + stages * 8; i += 8)
+          if (whole || i < bar) mbarWait(i, i < bar ? phase : phase ^ 1, 1u << 20);
       }
     }
     __syncwarp();
   } else if (warp == 1) {
     if (electOne()) {
-      const uint32_t idesc = umInstrBf16(128, parts == 2 ? 2 * partCols : bn) | (kAcrossB<MODE> ? 1u << 16 : 0u);
+      const uint32_t idesc = umInstrBf16(128, bn) | (kAcrossB<MODE> ? 1u << 16 : 0u);
       int s = 0, it = 0;
       uint32_t phase = 0;
       bool bad = false;
       for (int t = blockIdx.x; t < tiles.count && !bad && !*abortFlag; t += gridDim.x, ++it) {
         const Tile c = tiles.at(t);
         const int buf = it & 1;
-        if (!mbarWait(smemAddr(&accEmpty[buf]), ((it >> 1) & 1) ^ 1)) { fail(2000 + buf); break; }
+        if (!waitOr(smemAddr(&accEmpty[buf]), ((it >> 1) & 1) ^ 1, abortFlag)) { fail(2000 + buf); break; }
         tcFenceAfter();
         const uint32_t dT = tmemBase + buf * kAccCols;
         for (int kb = 0; kb < c.steps; ++kb) {
-          if (!mbarWait(smemAddr(&fullBar[s]), phase)) { fail(3000 + s); bad = true; break; }
+          if (!waitOr(smemAddr(&fullBar[s]), phase, abortFlag)) { fail(3000 + s); bad = true; break; }
           tcFenceAfter();
           const uint32_t sA = ring + s * stageBytes, sB = sA + aBytes;
           const uint64_t da = umDescK128(sA), db = descOf<kAcrossB<MODE>>(sB);
@@ -388,9 +421,9 @@ expertGemmKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     for (int t = blockIdx.x; t < tiles.count && !__any_sync(~0u, *abortFlag); t += gridDim.x, ++it) {
       const Tile c = tiles.at(t);
       const int buf = it & 1;
-      if (!__all_sync(~0u, mbarWait(smemAddr(&accFull[buf]), (it >> 1) & 1))) { if (lane == 0) fail(4000 + buf); break; }
+      if (!warpWaitOr(smemAddr(&accFull[buf]), (it >> 1) & 1, abortFlag, lane)) { if (lane == 0) fail(4000 + buf); break; }
       tcFenceAfter();
-      storeTile<MODE>(a, tiles, c, q * 32, partCols, tmemBase + ((uint32_t)(q * 32) << 16) + buf * kAccCols, wbuf, half, lane);
+      storeTile<MODE>(a, tiles, c, q * 32, tmemBase + ((uint32_t)(q * 32) << 16) + buf * kAccCols, wbuf, half, lane);
       tcFenceBefore();
       __syncwarp();
       if (lane == 0) mbarArrive(smemAddr(&accEmpty[buf]));
@@ -460,7 +493,7 @@ expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   const uint32_t tmemBase = *tmemSlot;
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   // us of a step. Half as wide a tile fetches three quarters as much: it pays where whole ones would leave most of the SMs idle
-  const Tiles<MODE, 256> tiles(a, table, pairs, 128, 128, [](int w) { return w == 256 ? 0.35f : 0.22f; });
+  const Tiles<MODE, 256> tiles(a, table, pairs, 128, [](int w) { return w == 256 ? 0.35f : 0.22f; });
   const int bn = tiles.bn, parts = tiles.parts, halfCols = bn / 2;   // columns that each CTA stages
   const uint32_t ring = smemAddr(smem);
   auto fail = [&](uint32_t what) {
@@ -485,50 +518,54 @@ expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
 
   if (warp == 0) {
     if (electOne()) {
-      int s = 0, armed = 0, tails = 0;   // stages that were ever loaded; bit s: the last load of stage s counts on tailBar
-      uint32_t phase = 0, tailPhase = 0;
-      const CUtensorMap* mapB = kAcrossB<MODE> || bn == 256 ? &tmB : &tmBNarrow;
+      const uint32_t bars = smemAddr(fullBar), toEmpty = smemAddr(emptyBar) - bars, toTail = smemAddr(tailBar) - bars;
+      const uint32_t toLeader = mapaShared(bars, 0) - bars, toOwn = mapaShared(bars, cr) - bars;   // cluster addresses of the barriers
+      const uint32_t ringEnd = ring + kPairStages * kStageBytes;
+      uint32_t phase = 0, sA = ring, bar = bars, tails = 0, tailPhase = 0;   // bit s: the last load of stage s counts on tailBar, and the phase of that
+      bool whole = false;                                                    // every stage was loaded once
       for (int t = pair; t < tiles.count && !*abortFlag; t += pairs) {
         const Tile c = tiles.at(t);
         const uint32_t mineA = bytesA(c, cr), mineB = bytesB(c, cr), both = bytesA(c, 0) + bytesA(c, 1) + bytesB(c, 0) + bytesB(c, 1);
-        const int row = c.row0 + (int)cr * 128, col = firstB(c);
-        for (int kb = 0; kb < c.steps; ++kb) {
-          if (!mbarWait(smemAddr(&emptyBar[s]), phase ^ 1)) { fail(1000 + s); break; }
-          if (*abortFlag) break;
-          const uint32_t sA = ring + s * kStageBytes, sB = sA + kHalfBytes;
-          const bool tail = MODE == EXPERT_DW && kb == c.steps - 1 && c.rows % kUmmaK != 0;
-          uint32_t full;
-          if (tail) {
-            full = mapaShared(smemAddr(&tailBar[s]), cr);
-            mbarExpectTx(smemAddr(&tailBar[s]), mineA + mineB);
-            tails |= 1 << s;
-            tailPhase ^= 1u << s;
+        const int row = c.row0 + (int)cr * 128, col = firstB(c), end = c.steps * kBK;
+        const int tailAt = MODE == EXPERT_DW && c.rows % kUmmaK != 0 ? end - kBK : -1;
+        for (int x = 0; x < end; x += kBK) {
+          if (!waitOr(bar + toEmpty, phase ^ 1, abortFlag)) { fail(1000); break; }
+          const uint32_t sB = sA + kHalfBytes;
+          uint32_t full = bar + toLeader;
+          if (MODE == EXPERT_DW && x == tailAt) {
+            full = bar + toTail + toOwn;
+            mbarExpectTx(bar + toTail, mineA + mineB);
+            tails |= 1u << (bar - bars) / 8;
+            tailPhase ^= 1u << (bar - bars) / 8;
           } else {
-            full = mapaShared(smemAddr(&fullBar[s]), 0);
-            if (leader) mbarExpectTx(smemAddr(&fullBar[s]), both);
-            tails &= ~(1 << s);
+            if (leader) mbarExpectTx(bar, both);
+            if (MODE == EXPERT_DW) tails &= ~(1u << (bar - bars) / 8);
           }
           if (kAcrossA<MODE>) {
-            if (mineA) tmaLoad3dPair(sA, &tmA, row, kb * kBK, c.e, full);
-            if (mineA > kBlockBytes) tmaLoad3dPair(sA + kBlockBytes, &tmA, row + 64, kb * kBK, c.e, full);
+            if (mineA) tmaLoad3dPair(sA, &tmA, row, x, c.e, full);
+            if (mineA > kBlockBytes) tmaLoad3dPair(sA + kBlockBytes, &tmA, row + 64, x, c.e, full);
           } else if (mineA) {
-            tmaLoad3dPair(sA, &tmA, kb * kBK, row, c.e, full);
+            tmaLoad3dPair(sA, &tmA, x, row, c.e, full);
           }
           if (kAcrossB<MODE>) {
-            if (mineB) tmaLoad3dPair(sB, &tmB, col, kb * kBK, c.e, full);
-            if (mineB > kBlockBytes) tmaLoad3dPair(sB + kBlockBytes, &tmB, col + 64, kb * kBK, c.e, full);
+            if (mineB) tmaLoad3dPair(sB, &tmB, col, x, c.e, full);
+            if (mineB > kBlockBytes) tmaLoad3dPair(sB + kBlockBytes, &tmB, col + 64, x, c.e, full);
           } else if (mineB) {
-            tmaLoad3dPair(sB, mapB, kb * kBK, col, c.e, full);
+            if (bn == 256) tmaLoad3dPair(sB, &tmB, x, col, c.e, full);
+            else tmaLoad3dPair(sB, &tmBNarrow, x, col, c.e, full);
           }
-          armed = max(armed, s + 1);
-          if (++s == kPairStages) { s = 0; phase ^= 1; }
+          sA += kStageBytes;
+          bar += 8;
+          if (sA == ringEnd) { sA = ring; bar = bars; phase ^= 1; whole = true; }
         }
       }
       if (*abortFlag) {
-        // copies already issued (by either CTA) still write into shared memory: wait for them (bounded). Stages in front of s were loaded in this round
-        for (int i = 0; i < armed; ++i) {
-          if (tails >> i & 1) mbarWait(smemAddr(&tailBar[i]), (tailPhase >> i & 1) ^ 1, 1u << 20);
-          else if (leader) mbarWait(smemAddr(&fullBar[i]), i < s ? phase : phase ^ 1, 1u << 20);
+        // copies already issued (by either CTA) still write into shared memory: wait for them (bounded). Stages in front of the next one were loaded in this round
+        for (int i = 0; i < kPairStages; ++i) {
+          const uint32_t at = bars + i * 8;
+          if (!whole && at >= bar) break;
+          if (tails >> i & 1) mbarWait(at + toTail, (tailPhase >> i & 1) ^ 1, 1u << 20);
+          else if (leader) mbarWait(at, at < bar ? phase : phase ^ 1, 1u << 20);
         }
       }
     }
@@ -543,13 +580,13 @@ expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         const Tile c = tiles.at(t);
         if (c.steps == 0) continue;   // nothing to add up: the epilogue writes zeros
         const int buf = it & 1;
-        if (!mbarWait(smemAddr(&accEmpty[buf]), ((it >> 1) & 1) ^ 1)) { fail(2000 + buf); break; }
+        if (!waitOr(smemAddr(&accEmpty[buf]), ((it >> 1) & 1) ^ 1, abortFlag)) { fail(2000 + buf); break; }
         ++it;
         tcFenceAfter();
         const uint32_t dT = tmemBase + buf * kAccCols;
         const int last = (tiles.length(c) - (c.steps - 1) * kBK + kUmmaK - 1) / kUmmaK;   // sixteens in the last step
         for (int kb = 0; kb < c.steps; ++kb) {
-          if (!mbarWait(smemAddr(&fullBar[s]), phase)) { fail(3000 + s); bad = true; break; }
+          if (!waitOr(smemAddr(&fullBar[s]), phase, abortFlag)) { fail(3000 + s); bad = true; break; }
           tcFenceAfter();
           const uint32_t sA = ring + s * kStageBytes;
           const uint64_t da = descOf<kAcrossA<MODE>>(sA), db = descOf<kAcrossB<MODE>>(sA + kHalfBytes);
@@ -572,11 +609,11 @@ expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       const Tile c = tiles.at(t);
       const int buf = it & 1;
       if (c.steps) {
-        if (!__all_sync(~0u, mbarWait(smemAddr(&accFull[buf]), (it >> 1) & 1))) { if (lane == 0) fail(4000 + buf); break; }
+        if (!warpWaitOr(smemAddr(&accFull[buf]), (it >> 1) & 1, abortFlag, lane)) { if (lane == 0) fail(4000 + buf); break; }
         ++it;
         tcFenceAfter();
       }
-      storeTile<MODE>(a, tiles, c, c.row0 + (int)cr * 128 + q * 32, halfCols, tmemBase + ((uint32_t)(q * 32) << 16) + buf * kAccCols, wbuf, half, lane);
+      storeTile<MODE>(a, tiles, c, c.row0 + (int)cr * 128 + q * 32, tmemBase + ((uint32_t)(q * 32) << 16) + buf * kAccCols, wbuf, half, lane);
       if (c.steps) {
         tcFenceBefore();
         __syncwarp();

@@ -168,12 +168,12 @@ static int pairsAtOnce(ncclEpGroup* g) {
 // rows an expert may have, not how many it has: where a tile of 128 holds them all, single CTAs take a tile each, else pairs tiles of 256.
 static ncclResult_t launchExpertGemm(ncclEpGroup* g, int mode, const void* A, int innerA, int rowsA, const void* B, int innerB, int rowsB, ExpertGemmArgs* a, cudaStream_t stream) {
   const bool pair = mode == EXPERT_DW || a->cap > kExpertOneCtaRows;
-  a->boxRows = pair ? 128 : (a->cap + 7) / 8 * 8;
+  a->boxRows = pair ? 128 : std::min(32, (a->cap + 7) / 8 * 8);
   a->status = g->comm->devStatusDev;
   CUtensorMap maps[3];
   NCCLCHECK(makeMap(&maps[0], A, innerA, rowsA, a->experts, mode == EXPERT_DW ? 64 : a->boxRows));
   NCCLCHECK(makeMap(&maps[1], B, innerB, rowsB, a->experts, mode == EXPERT_FORWARD ? 128 : 64));
-  if (mode == EXPERT_FORWARD) NCCLCHECK(makeMap(&maps[2], B, innerB, rowsB, a->experts, pair ? 64 : 32));
+  if (mode == EXPERT_FORWARD) NCCLCHECK(makeMap(&maps[2], B, innerB, rowsB, a->experts, pair || a->gated ? 64 : 32));
   else maps[2] = maps[1];
   void* args[4] = {&maps[0], &maps[1], &maps[2], a};
   // no more CTAs than the narrowest tiles of all rows
