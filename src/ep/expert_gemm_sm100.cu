@@ -33,14 +33,14 @@ constexpr int kBK = 64, kUmmaK = 16, kMaxBN = 256;
 constexpr int kEpiWarps = 8, kFirstEpiWarp = 2, kFixWarp = kFirstEpiWarp + kEpiWarps;
 constexpr int kThreads = kFixWarp * 32, kPairThreads = kThreads + 32;
 constexpr uint32_t kTmemCols = 512, kAccCols = 256;
-constexpr uint32_t kRingBytes = 192 << 10;
-constexpr int kMaxStages = 12, kPairStages = 6;
+constexpr uint32_t kRingBytes = 224 << 10;
+constexpr int kMaxStages = 12, kMaxPairStages = 7;
 constexpr uint32_t kHalfBytes = 128 * kBK * 2;   // 128 rows (or columns) of an operand, 64 steps
 constexpr uint32_t kBlockBytes = 64 * kBK * 2;   // a box of 64 x 64
-constexpr size_t kEpiBytes = kEpiWarps * 4096, kCtrlBytes = 512, kTableBytes = (kExpertMax + 1) * 4 + 12;
-constexpr size_t kSmemBytes = 1024 + kRingBytes + kEpiBytes + kCtrlBytes + kTableBytes;
-static_assert((2 * kMaxStages + 4) * 8 + 8 <= kCtrlBytes && (4 * kPairStages + 4) * 8 + 8 <= kCtrlBytes, "control block too small");
-static_assert(kPairStages * 2 * kHalfBytes <= kRingBytes && kSmemBytes <= 227 * 1024, "shared memory");
+constexpr size_t kCtrlBytes = 512, kTableBytes = (kExpertMax + 1) * 4 + 12;
+constexpr size_t kSmemBytes = 1024 + kRingBytes + kCtrlBytes + kTableBytes;
+static_assert((2 * kMaxStages + 4) * 8 + 8 <= kCtrlBytes && (4 * kMaxPairStages + 4) * 8 + 8 <= kCtrlBytes, "control block too small");
+static_assert(kMaxPairStages * 2 * kHalfBytes <= kRingBytes && 6 * 2 * kHalfBytes + kEpiWarps * 4096 <= kRingBytes && kSmemBytes <= 227 * 1024, "shared memory");
 
 __device__ __forceinline__ void tmaLoad3d(uint32_t dstSmem, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
   asm volatile(
@@ -194,100 +194,101 @@ __device__ __forceinline__ void reportTimeout(const ExpertGemmArgs& a, uint32_t 
   }
 }
 
-// Epilogue of one warp for its 32 rows, `row` the first of them, and every other 64 columns of the tile: tBase is the tensor-memory address of the
-// warp's first lane and the tile's first column. A lane has a row of the accumulator; 64 columns at a time pass through 4 KiB of shared memory (16-byte chunks
-// XOR-swizzled by row), so that memory sees 128 contiguous bytes of a row.
-template <int MODE, typename T>
-__device__ __forceinline__ void storeTile(const ExpertGemmArgs& a, const T& tiles, const Tile& c, int row, uint32_t tBase, uint8_t* wbuf, int half, int lane) {
-  const int parts = tiles.parts, outCols = tiles.outCols, left = tiles.rowLimit(c) - row;   // rows from here on
-  const size_t first = (size_t)c.e * (MODE == EXPERT_DW ? a.outRows : a.cap) + row;
-  for (int cc = half * 64; cc < outCols && c.col0 + cc < a.cols && left > 0; cc += 128) {
-    const int col = c.col0 + cc, width = min(min(64, outCols - cc), a.cols - col);   // a multiple of 8
-    auto chunk = [&](int r, int j) { return (uint4*)(wbuf + r * 128 + ((j ^ (r & 7)) * 16)); };
-    auto store = [&](__nv_bfloat16* to, size_t ld) {
-      __syncwarp();
+// 32 neighbouring bf16 of one row, `n` of them (a multiple of 8) inside the matrix: 32 bytes per access where rows allow it.
+__device__ __forceinline__ void storeRow32(__nv_bfloat16* to, const float (&v)[32], int n, bool wide) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int r = k * 4 + (lane >> 3), j = lane & 7;
-        if (r < left && j * 8 < width) *(uint4*)(to + (size_t)r * ld + j * 8) = *chunk(r, j);
-      }
-      __syncwarp();
-    };
-    auto sums = [&](int part, int h, float (&v)[32]) {
+  for (int j = 0; j < 32; j += 16) {
+    const uint4 lo = packBf16x8(v + j), hi = packBf16x8(v + j + 8);
+    if (wide) {
+      if (j < n) asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + j), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
+    } else {
+      if (j < n) *(uint4*)(to + j) = lo;
+      if (j + 8 < n) *(uint4*)(to + j + 8) = hi;
+    }
+  }
+}
+__device__ __forceinline__ void addRow32(const __nv_bfloat16* from, float (&v)[32], int n) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 8) {
+    if (j >= n) break;
+    float f[8];
+    unpackBf16x8(*(const uint4*)(from + j), f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[j + i] += f[i];
+  }
+}
+
+// Epilogue of one warp for its 32 rows, `row` the first of them, and every other 64 columns of the tile: tBase is the tensor-memory address of the
+// warp's first lane and the tile's first column. A lane has a row of the accumulator and stores 32 of its columns at a time, whole sectors straight from
+// registers: shared memory is busy with the operands, and its room makes a seventh stage (32 experts of 64 rows, 4096 x 7168: 295 us through shared memory, 284 so).
+template <int MODE, typename T>
+__device__ __forceinline__ void storeTile(const ExpertGemmArgs& a, const T& tiles, const Tile& c, int row, uint32_t tBase, int half, int lane) {
+  const int parts = tiles.parts, outCols = tiles.outCols;
+  const bool mine = row + lane < c.rows;
+  if (row >= c.rows) return;
+  const size_t at = (size_t)c.e * a.cap + row + lane;
+  for (int cc = half * 32; cc < outCols && c.col0 + cc < a.cols; cc += 64) {
+    const int col = c.col0 + cc, n = a.cols - col;   // a multiple of 8
+    auto sums = [&](int part, float (&v)[32]) {
       uint32_t r[32];
-      tmemLd32(tBase + part * outCols + cc + h * 32, r);
+      tmemLd32(tBase + part * outCols + cc, r);
       tmemLdWait32(r);
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-      if (MODE == EXPERT_FORWARD && a.bias) {
-        const __nv_bfloat16* b = (const __nv_bfloat16*)a.bias + ((size_t)c.e * parts + part) * a.cols + col + h * 32;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (h * 32 + j * 8 >= width) break;
-          float f[8];
-          unpackBf16x8(__ldg((const uint4*)b + j), f);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[j * 8 + i] += f[i];
-        }
-      }
+      if (MODE == EXPERT_FORWARD && a.bias) addRow32((const __nv_bfloat16*)a.bias + ((size_t)c.e * parts + part) * a.cols + col, v, n);
+      if (MODE == EXPERT_FORWARD && a.pre && mine) storeRow32((__nv_bfloat16*)a.pre + (at * parts + part) * a.cols + col, v, n, a.wide);
     };
-    if (MODE == EXPERT_FORWARD && a.pre) {
-      for (int p = 0; p < parts; ++p) {
+    float v[32];
+    sums(0, v);
+    if (MODE == EXPERT_FORWARD) {
+      if (parts == 2) {
+        float u[32];
+        sums(1, u);
+        const int base = a.act == ACT_SWIGLU ? ACT_SILU : ACT_GELU;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (h * 32 >= width) break;
-          float v[32];
-          sums(p, h, v);
+        for (int i = 0; i < 32; ++i) v[i] = activation(base, v[i]) * u[i];
+      } else if (a.act != ACT_NONE) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) *chunk(lane, h * 4 + j) = packBf16x8(v + j * 8);
-        }
-        store((__nv_bfloat16*)a.pre + (first * parts + p) * a.cols + col, (size_t)parts * a.cols);
+        for (int i = 0; i < 32; ++i) v[i] = activation(a.act, v[i]);
       }
+      if (a.residual && mine) addRow32((const __nv_bfloat16*)a.residual + at * a.cols + col, v, n);
     }
-    if (MODE == EXPERT_FORWARD && a.residual) {
-      const __nv_bfloat16* from = (const __nv_bfloat16*)a.residual + first * a.cols + col;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int r = k * 4 + (lane >> 3), j = lane & 7;
-        *chunk(r, j) = r < left && j * 8 < width ? *(const uint4*)(from + (size_t)r * a.cols + j * 8) : make_uint4(0, 0, 0, 0);
-      }
-      __syncwarp();
-    }
+    if (mine) storeRow32((__nv_bfloat16*)a.out + at * a.cols + col, v, n, a.wide);
+  }
+}
+
+// Epilogue of DW, where the results are the traffic: 64 columns of 32 rows at a time pass through 4 KiB of shared memory (16-byte chunks XOR-swizzled by row),
+// so that memory sees 128 contiguous bytes of a row. 32 experts of 64 rows, 4096 x 7168: 431 us (4.4 TB/s written; the framework's fill of the same memory
+// 474), with the stores of storeTile 501, with bulk copies from shared memory 609. Experts of 512 rows, 28672 x 4096: 802, 845 and 805.
+__device__ __forceinline__ void storeTileLines(const ExpertGemmArgs& a, const Tile& c, int row, int outCols, uint32_t tBase, uint8_t* wbuf, int half, int lane) {
+  const int left = a.outRows - row;   // rows from here on
+  for (int cc = half * 64; cc < outCols && c.col0 + cc < a.cols && left > 0; cc += 128) {
+    const int col = c.col0 + cc, width = min(min(64, outCols - cc), a.cols - col);   // a multiple of 8
+    auto chunk = [&](int r, int j) { return (uint4*)(wbuf + r * 128 + ((j ^ (r & 7)) * 16)); };
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      if (h * 32 >= width) break;
-      float v[32];
-      if (MODE == EXPERT_DW && c.steps == 0) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+      uint32_t r[32];
+      if (c.steps) {
+        tmemLd32(tBase + cc + h * 32, r);
+        tmemLdWait32(r);
       } else {
-        sums(0, h, v);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) r[i] = 0;
       }
-      if (MODE == EXPERT_FORWARD) {
-        if (parts == 2) {
-          float u[32];
-          sums(1, h, u);
-          const int base = a.act == ACT_SWIGLU ? ACT_SILU : ACT_GELU;
+      float v[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = activation(base, v[i]) * u[i];
-        } else if (a.act != ACT_NONE) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = activation(a.act, v[i]);
-        }
-        if (a.residual) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float f[8];
-            unpackBf16x8(*chunk(lane, h * 4 + j), f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[j * 8 + i] += f[i];
-          }
-        }
-      }
+      for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) *chunk(lane, h * 4 + j) = packBf16x8(v + j * 8);
     }
-    store((__nv_bfloat16*)a.out + first * a.cols + col, (size_t)a.cols);
+    __syncwarp();
+    __nv_bfloat16* to = (__nv_bfloat16*)a.out + ((size_t)c.e * a.outRows + row) * a.cols + col;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int r = k * 4 + (lane >> 3), j = lane & 7;
+      if (r < left && j * 8 < width) *(uint4*)(to + (size_t)r * a.cols + j * 8) = *chunk(r, j);
+    }
+    __syncwarp();
   }
 }
 
@@ -303,8 +304,7 @@ expertGemmKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   static_assert(MODE != EXPERT_DW, "DW runs on pairs");
   extern __shared__ uint8_t smemRaw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smemRaw + 1023) & ~(uintptr_t)1023);
-  uint8_t* epiBuf = smem + kRingBytes;
-  uint8_t* ctrl = epiBuf + kEpiBytes;
+  uint8_t* ctrl = smem + kRingBytes;
   uint64_t* fullBar = (uint64_t*)ctrl;              // [kMaxStages]
   uint64_t* emptyBar = fullBar + kMaxStages;        // [kMaxStages]
   uint64_t* accFull = emptyBar + kMaxStages;        // [2]
@@ -416,14 +416,13 @@ expertGemmKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     __syncwarp();
   } else {
     const int q = warp & 3, half = (warp - kFirstEpiWarp) >> 2;   // TMEM lanes [32q, 32q+32) belong to the warps with warp % 4 == q
-    uint8_t* wbuf = epiBuf + (size_t)(warp - kFirstEpiWarp) * 4096;
     int it = 0;
     for (int t = blockIdx.x; t < tiles.count && !__any_sync(~0u, *abortFlag); t += gridDim.x, ++it) {
       const Tile c = tiles.at(t);
       const int buf = it & 1;
       if (!warpWaitOr(smemAddr(&accFull[buf]), (it >> 1) & 1, abortFlag, lane)) { if (lane == 0) fail(4000 + buf); break; }
       tcFenceAfter();
-      storeTile<MODE>(a, tiles, c, q * 32, tmemBase + ((uint32_t)(q * 32) << 16) + buf * kAccCols, wbuf, half, lane);
+      storeTile<MODE>(a, tiles, c, q * 32, tmemBase + ((uint32_t)(q * 32) << 16) + buf * kAccCols, half, lane);
       tcFenceBefore();
       __syncwarp();
       if (lane == 0) mbarArrive(smemAddr(&accEmpty[buf]));
@@ -452,10 +451,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmBNarrow,
                      const __grid_constant__ ExpertGemmArgs a) {
   constexpr uint32_t kStageBytes = 2 * kHalfBytes;
+  constexpr int kPairStages = MODE == EXPERT_DW ? 6 : 7;   // DW's epilogue takes the room of the seventh
   extern __shared__ uint8_t smemRaw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smemRaw + 1023) & ~(uintptr_t)1023);
-  uint8_t* epiBuf = smem + kRingBytes;
-  uint8_t* ctrl = epiBuf + kEpiBytes;
+  uint8_t* ctrl = smem + kRingBytes;
   uint64_t* fullBar = (uint64_t*)ctrl;              // [kPairStages]
   uint64_t* emptyBar = fullBar + kPairStages;       // [kPairStages]
   uint64_t* tailBar = emptyBar + kPairStages;       // [kPairStages]
@@ -603,7 +602,6 @@ expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     __syncwarp();
   } else if (warp < kFixWarp) {
     const int q = warp & 3, half = (warp - kFirstEpiWarp) >> 2;   // TMEM lanes [32q, 32q+32) belong to the warps with warp % 4 == q
-    uint8_t* wbuf = epiBuf + (size_t)(warp - kFirstEpiWarp) * 4096;
     int it = 0;
     for (int t = pair; t < tiles.count && !__any_sync(~0u, *abortFlag); t += pairs) {
       const Tile c = tiles.at(t);
@@ -613,7 +611,10 @@ expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         ++it;
         tcFenceAfter();
       }
-      storeTile<MODE>(a, tiles, c, c.row0 + (int)cr * 128 + q * 32, tmemBase + ((uint32_t)(q * 32) << 16) + buf * kAccCols, wbuf, half, lane);
+      const int row = c.row0 + (int)cr * 128 + q * 32;
+      const uint32_t tBase = tmemBase + ((uint32_t)(q * 32) << 16) + buf * kAccCols;
+      if constexpr (MODE == EXPERT_DW) storeTileLines(a, c, row, tiles.outCols, tBase, smem + 6 * kStageBytes + (warp - kFirstEpiWarp) * 4096, half, lane);
+      else storeTile<MODE>(a, tiles, c, row, tBase, half, lane);
       if (c.steps) {
         tcFenceBefore();
         __syncwarp();

@@ -169,6 +169,7 @@ static int pairsAtOnce(ncclEpGroup* g) {
 static ncclResult_t launchExpertGemm(ncclEpGroup* g, int mode, const void* A, int innerA, int rowsA, const void* B, int innerB, int rowsB, ExpertGemmArgs* a, cudaStream_t stream) {
   const bool pair = mode == EXPERT_DW || a->cap > kExpertOneCtaRows;
   a->boxRows = pair ? 128 : std::min(32, (a->cap + 7) / 8 * 8);
+  a->wide = a->cols % 16 == 0 && aligned({a->out, a->pre}, 32);
   a->status = g->comm->devStatusDev;
   CUtensorMap maps[3];
   NCCLCHECK(makeMap(&maps[0], A, innerA, rowsA, a->experts, mode == EXPERT_DW ? 64 : a->boxRows));

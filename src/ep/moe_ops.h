@@ -45,6 +45,7 @@ struct ExpertGemmArgs {
   int cols;                   // columns of the result
   int depth;                  // length of the sums (DW: cap; the rows in use count)
   int boxRows;                // rows of a box of the first operand (the kernel on single CTAs)
+  int wide;                   // rows of out and pre may be stored in packs of 32 bytes
   int gated, act;             // forward: gate rows of W, then up rows, `cols` of each
   const void* bias;           // bf16 [experts][cols, twice when gated] or null
   const void* residual;       // bf16, laid out like out, or null
