@@ -207,35 +207,55 @@ __device__ __forceinline__ void storeRow32(__nv_bfloat16* to, const float (&v)[3
     }
   }
 }
-__device__ __forceinline__ void addRow32(const __nv_bfloat16* from, float (&v)[32], int n) {
+// 32 neighbouring bf16, as storeRow32 takes them: fetched early, added when the sums are there.
+struct Row32 {
+  uint4 q[4];
+  __device__ __forceinline__ void load(const __nv_bfloat16* from, int n) {
 #pragma unroll
-  for (int j = 0; j < 32; j += 8) {
-    if (j >= n) break;
-    float f[8];
-    unpackBf16x8(*(const uint4*)(from + j), f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[j + i] += f[i];
+    for (int j = 0; j < 4; ++j) q[j] = j * 8 < n ? *(const uint4*)(from + j * 8) : make_uint4(0, 0, 0, 0);
   }
-}
+  __device__ __forceinline__ void addTo(float (&v)[32]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float f[8];
+      unpackBf16x8(q[j], f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[j * 8 + i] += f[i];
+    }
+  }
+};
 
-// Epilogue of one warp for its 32 rows, `row` the first of them, and every other 64 columns of the tile: tBase is the tensor-memory address of the
+// Epilogue of one warp for its 32 rows, `row` the first of them, and every other 32 columns of the tile: tBase is the tensor-memory address of the
 // warp's first lane and the tile's first column. A lane has a row of the accumulator and stores 32 of its columns at a time, whole sectors straight from
 // registers: shared memory is busy with the operands, and its room makes a seventh stage (32 experts of 64 rows, 4096 x 7168: 295 us through shared memory, 284 so).
-template <int MODE, typename T>
-__device__ __forceinline__ void storeTile(const ExpertGemmArgs& a, const T& tiles, const Tile& c, int row, uint32_t tBase, int half, int lane) {
+// What is added (bias, residual) is on its way while the sums are not complete (`ready` waits for them), and while the columns before are stored.
+template <int MODE, typename T, typename Ready>
+__device__ __forceinline__ bool storeTile(const ExpertGemmArgs& a, const T& tiles, const Tile& c, int row, uint32_t tBase, int half, int lane, Ready ready) {
   const int parts = tiles.parts, outCols = tiles.outCols;
   const bool mine = row + lane < c.rows;
-  if (row >= c.rows) return;
   const size_t at = (size_t)c.e * a.cap + row + lane;
-  for (int cc = half * 32; cc < outCols && c.col0 + cc < a.cols; cc += 64) {
+  const int end = row < c.rows ? min(outCols, a.cols - c.col0) : 0;
+  Row32 bias[2], residual;
+  auto fetch = [&](int cc) {
     const int col = c.col0 + cc, n = a.cols - col;   // a multiple of 8
+    if (MODE == EXPERT_FORWARD && a.bias && cc < end) {
+      const __nv_bfloat16* b = (const __nv_bfloat16*)a.bias + (size_t)c.e * parts * a.cols + col;
+      bias[0].load(b, n);
+      if (parts == 2) bias[1].load(b + a.cols, n);
+    }
+    if (MODE == EXPERT_FORWARD && a.residual && mine && cc < end) residual.load((const __nv_bfloat16*)a.residual + at * a.cols + col, n);
+  };
+  fetch(half * 32);
+  if (!ready()) return false;
+  for (int cc = half * 32; cc < end; cc += 64) {
+    const int col = c.col0 + cc, n = a.cols - col;
     auto sums = [&](int part, float (&v)[32]) {
       uint32_t r[32];
       tmemLd32(tBase + part * outCols + cc, r);
       tmemLdWait32(r);
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-      if (MODE == EXPERT_FORWARD && a.bias) addRow32((const __nv_bfloat16*)a.bias + ((size_t)c.e * parts + part) * a.cols + col, v, n);
+      if (MODE == EXPERT_FORWARD && a.bias) bias[part].addTo(v);
       if (MODE == EXPERT_FORWARD && a.pre && mine) storeRow32((__nv_bfloat16*)a.pre + (at * parts + part) * a.cols + col, v, n, a.wide);
     };
     float v[32];
@@ -251,10 +271,12 @@ __device__ __forceinline__ void storeTile(const ExpertGemmArgs& a, const T& tile
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = activation(a.act, v[i]);
       }
-      if (a.residual && mine) addRow32((const __nv_bfloat16*)a.residual + at * a.cols + col, v, n);
+      if (a.residual) residual.addTo(v);
     }
+    fetch(cc + 64);
     if (mine) storeRow32((__nv_bfloat16*)a.out + at * a.cols + col, v, n, a.wide);
   }
+  return true;
 }
 
 // Epilogue of DW, where the results are the traffic: 64 columns of 32 rows at a time pass through 4 KiB of shared memory (16-byte chunks XOR-swizzled by row),
@@ -420,9 +442,12 @@ expertGemmKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     for (int t = blockIdx.x; t < tiles.count && !__any_sync(~0u, *abortFlag); t += gridDim.x, ++it) {
       const Tile c = tiles.at(t);
       const int buf = it & 1;
-      if (!warpWaitOr(smemAddr(&accFull[buf]), (it >> 1) & 1, abortFlag, lane)) { if (lane == 0) fail(4000 + buf); break; }
-      tcFenceAfter();
-      storeTile<MODE>(a, tiles, c, q * 32, tmemBase + ((uint32_t)(q * 32) << 16) + buf * kAccCols, half, lane);
+      auto ready = [&] {
+        const bool ok = warpWaitOr(smemAddr(&accFull[buf]), (it >> 1) & 1, abortFlag, lane);
+        tcFenceAfter();
+        return ok;
+      };
+      if (!storeTile<MODE>(a, tiles, c, q * 32, tmemBase + ((uint32_t)(q * 32) << 16) + buf * kAccCols, half, lane, ready)) { if (lane == 0) fail(4000 + buf); break; }
       tcFenceBefore();
       __syncwarp();
       if (lane == 0) mbarArrive(smemAddr(&accEmpty[buf]));
@@ -606,16 +631,23 @@ expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     for (int t = pair; t < tiles.count && !__any_sync(~0u, *abortFlag); t += pairs) {
       const Tile c = tiles.at(t);
       const int buf = it & 1;
-      if (c.steps) {
-        if (!warpWaitOr(smemAddr(&accFull[buf]), (it >> 1) & 1, abortFlag, lane)) { if (lane == 0) fail(4000 + buf); break; }
-        ++it;
-        tcFenceAfter();
-      }
       const int row = c.row0 + (int)cr * 128 + q * 32;
       const uint32_t tBase = tmemBase + ((uint32_t)(q * 32) << 16) + buf * kAccCols;
-      if constexpr (MODE == EXPERT_DW) storeTileLines(a, c, row, tiles.outCols, tBase, smem + 6 * kStageBytes + (warp - kFirstEpiWarp) * 4096, half, lane);
-      else storeTile<MODE>(a, tiles, c, row, tBase, half, lane);
+      auto ready = [&] {   // (nothing to wait for where there was nothing to add up)
+        const bool ok = c.steps == 0 || warpWaitOr(smemAddr(&accFull[buf]), (it >> 1) & 1, abortFlag, lane);
+        tcFenceAfter();
+        return ok;
+      };
+      bool ok;
+      if constexpr (MODE == EXPERT_DW) {
+        ok = ready();
+        if (ok) storeTileLines(a, c, row, tiles.outCols, tBase, smem + 6 * kStageBytes + (warp - kFirstEpiWarp) * 4096, half, lane);
+      } else {
+        ok = storeTile<MODE>(a, tiles, c, row, tBase, half, lane, ready);
+      }
+      if (!ok) { if (lane == 0) fail(4000 + buf); break; }
       if (c.steps) {
+        ++it;
         tcFenceBefore();
         __syncwarp();
         if (lane == 0) mbarArriveRelaxed(mapaShared(smemAddr(&accEmpty[buf]), 0));
