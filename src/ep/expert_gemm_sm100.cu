@@ -261,16 +261,9 @@ __device__ __forceinline__ bool storeTile(const ExpertGemmArgs& a, const T& tile
     float v[32];
     sums(0, v);
     if (MODE == EXPERT_FORWARD) {
-      if (parts == 2) {
-        float u[32];
-        sums(1, u);
-        const int base = a.act == ACT_SWIGLU ? ACT_SILU : ACT_GELU;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = activation(base, v[i]) * u[i];
-      } else if (a.act != ACT_NONE) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = activation(a.act, v[i]);
-      }
+      float u[32];
+      if (parts == 2) sums(1, u);
+      activate32(a.act, v, u);
       if (a.residual) residual.addTo(v);
     }
     fetch(cc + 64);
@@ -279,39 +272,98 @@ __device__ __forceinline__ bool storeTile(const ExpertGemmArgs& a, const T& tile
   return true;
 }
 
-// Epilogue of DW, where the results are the traffic: 64 columns of 32 rows at a time pass through 4 KiB of shared memory (16-byte chunks XOR-swizzled by row),
-// so that memory sees 128 contiguous bytes of a row. 32 experts of 64 rows, 4096 x 7168: 431 us (4.4 TB/s written; the framework's fill of the same memory
-// 474), with the stores of storeTile 501, with bulk copies from shared memory 609. Experts of 512 rows, 28672 x 4096: 802, 845 and 805.
-__device__ __forceinline__ void storeTileLines(const ExpertGemmArgs& a, const Tile& c, int row, int outCols, uint32_t tBase, uint8_t* wbuf, int half, int lane) {
-  const int left = a.outRows - row;   // rows from here on
-  for (int cc = half * 64; cc < outCols && c.col0 + cc < a.cols && left > 0; cc += 128) {
-    const int col = c.col0 + cc, width = min(min(64, outCols - cc), a.cols - col);   // a multiple of 8
-    auto chunk = [&](int r, int j) { return (uint4*)(wbuf + r * 128 + ((j ^ (r & 7)) * 16)); };
+// The same through shared memory: 64 columns of 32 rows at a time pass 4 KiB (16-byte chunks XOR-swizzled by row), so that memory sees 128 contiguous bytes of a
+// row. For DW, whose results are the traffic: 32 experts of 64 rows, 4096 x 7168, 410 us (4.6 TB/s written; the framework's fill of the same memory
+// 474), with the stores above 501, with bulk copies from shared memory 609. And where a lane's own row would be touched 16 bytes at a time, 32 lines by an
+// instruction (residual, rows that are not whole packs of 32 bytes): 64 experts of about 140 rows, 2056 x 1400 with a residual, 153 and 145 us. With `pre` it computes
+// the sums twice: five experts of 310 rows, 2200 x 1000 with both, there and back, 94 us by the stores above, 112 so.
+template <int MODE, typename T, typename Ready>
+__device__ __forceinline__ bool storeTileStaged(const ExpertGemmArgs& a, const T& tiles, const Tile& c, int row, uint32_t tBase, uint8_t* wbuf, int half, int lane, Ready ready) {
+  const int parts = tiles.parts, outCols = tiles.outCols, left = tiles.rowLimit(c) - row;   // rows from here on
+  const size_t first = (size_t)c.e * (MODE == EXPERT_DW ? a.outRows : a.cap) + row;
+  const int end = left > 0 ? min(outCols, a.cols - c.col0) : 0;
+  auto chunk = [&](int r, int j) { return (uint4*)(wbuf + r * 128 + ((j ^ (r & 7)) * 16)); };
+  const int mine = lane >> 3, j0 = lane & 7;   // of four rows, and of a row's eight chunks
+  uint4 residual[8];
+  auto fetch = [&](int cc) {
+    if (MODE != EXPERT_FORWARD || !a.residual) return;
+    const __nv_bfloat16* from = (const __nv_bfloat16*)a.residual + first * a.cols + c.col0 + cc;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int k = 0; k < 8; ++k) residual[k] = cc + j0 * 8 < end && k * 4 + mine < left ? *(const uint4*)(from + (size_t)(k * 4 + mine) * a.cols + j0 * 8) : make_uint4(0, 0, 0, 0);
+  };
+  fetch(half * 64);
+  if (!ready()) return false;
+  for (int cc = half * 64; cc < end; cc += 128) {
+    const int col = c.col0 + cc, width = min(64, end - cc);   // a multiple of 8
+    auto store = [&](__nv_bfloat16* to, size_t ld) {
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int r = k * 4 + mine;
+        if (r < left && j0 * 8 < width) *(uint4*)(to + (size_t)r * ld + j0 * 8) = *chunk(r, j0);
+      }
+      __syncwarp();
+    };
+    auto sums = [&](int part, int h, float (&v)[32]) {
+      Row32 bias;
+      const bool biased = MODE == EXPERT_FORWARD && a.bias;
+      if (biased) bias.load((const __nv_bfloat16*)a.bias + ((size_t)c.e * parts + part) * a.cols + col + h * 32, a.cols - col - h * 32);
       uint32_t r[32];
-      if (c.steps) {
-        tmemLd32(tBase + cc + h * 32, r);
+      if (MODE != EXPERT_DW || c.steps) {
+        tmemLd32(tBase + part * outCols + cc + h * 32, r);
         tmemLdWait32(r);
       } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) r[i] = 0;
       }
-      float v[32];
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+      if (biased) bias.addTo(v);
+    };
+    if (MODE == EXPERT_FORWARD && a.pre) {
+      for (int p = 0; p < parts; ++p) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h * 32 >= width) break;
+          float v[32];
+          sums(p, h, v);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) *chunk(lane, h * 4 + j) = packBf16x8(v + j * 8);
+        }
+        store((__nv_bfloat16*)a.pre + (first * parts + p) * a.cols + col, (size_t)parts * a.cols);
+      }
+    }
+    if (MODE == EXPERT_FORWARD && a.residual) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) *chunk(k * 4 + mine, j0) = residual[k];
+      __syncwarp();
+      fetch(cc + 128);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (h * 32 >= width) break;
+      float v[32];
+      sums(0, h, v);
+      if (MODE == EXPERT_FORWARD) {
+        float u[32];
+        if (parts == 2) sums(1, h, u);
+        activate32(a.act, v, u);
+        if (a.residual) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float f[8];
+            unpackBf16x8(*chunk(lane, h * 4 + j), f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[j * 8 + i] += f[i];
+          }
+        }
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) *chunk(lane, h * 4 + j) = packBf16x8(v + j * 8);
     }
-    __syncwarp();
-    __nv_bfloat16* to = (__nv_bfloat16*)a.out + ((size_t)c.e * a.outRows + row) * a.cols + col;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int r = k * 4 + (lane >> 3), j = lane & 7;
-      if (r < left && j * 8 < width) *(uint4*)(to + (size_t)r * a.cols + j * 8) = *chunk(r, j);
-    }
-    __syncwarp();
+    store((__nv_bfloat16*)a.out + first * a.cols + col, (size_t)a.cols);
   }
+  return true;
 }
 
 }  // namespace
@@ -355,7 +407,7 @@ expertGemmKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   tcFenceAfter();
   const uint32_t tmemBase = *tmemSlot;
   // us of a step, where the weights come as fast as they are used. Wide tiles: 32 experts of 16 rows, 4096 x 7168 gated, 256 columns 299 us, 128 373; two
-  // experts of one row, 28672 x 4096 80 and 126. Narrow ones where they would leave SMs idle: 4096 x 14336 87, 79 and (64) NARROW_US
+  // experts of one row, 28672 x 4096 80 and 126. Narrow ones where they would leave SMs idle: 4096 x 14336 87, 79 and (64) 52 us
   const Tiles<MODE, 128> tiles(a, table, gridDim.x, MODE != EXPERT_FORWARD ? 64 : a.gated ? 128 : 32,
                                [](int w) { return w == 256 ? 0.33f : w == 128 ? 0.27f : w == 64 ? 0.23f : 0.2f; });
   const int bn = tiles.bn, parts = tiles.parts, outCols = tiles.outCols;
@@ -471,12 +523,12 @@ expertGemmKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 //   tailBar[s]   DW, in each CTA: the bytes of its own loads of a stage whose last rows are to be zeroed;
 //   fixBar[s]    (the first CTA's copy) the other CTA has written its zeros; the first CTA's warp for that arrives at fullBar then, in the
 //                producer's place. (An arrival of both producers in every step, so that fullBar could count two, took half of DW's rate.)
-template <int MODE>
+template <int MODE, bool STAGED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmBNarrow,
                      const __grid_constant__ ExpertGemmArgs a) {
   constexpr uint32_t kStageBytes = 2 * kHalfBytes;
-  constexpr int kPairStages = MODE == EXPERT_DW ? 6 : 7;   // DW's epilogue takes the room of the seventh
+  constexpr int kPairStages = STAGED ? 6 : 7;   // an epilogue through shared memory takes the room of the seventh
   extern __shared__ uint8_t smemRaw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smemRaw + 1023) & ~(uintptr_t)1023);
   uint8_t* ctrl = smem + kRingBytes;
@@ -639,12 +691,8 @@ expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         return ok;
       };
       bool ok;
-      if constexpr (MODE == EXPERT_DW) {
-        ok = ready();
-        if (ok) storeTileLines(a, c, row, tiles.outCols, tBase, smem + 6 * kStageBytes + (warp - kFirstEpiWarp) * 4096, half, lane);
-      } else {
-        ok = storeTile<MODE>(a, tiles, c, row, tBase, half, lane, ready);
-      }
+      if constexpr (STAGED) ok = storeTileStaged<MODE>(a, tiles, c, row, tBase, smem + 6 * kStageBytes + (warp - kFirstEpiWarp) * 4096, half, lane, ready);
+      else ok = storeTile<MODE>(a, tiles, c, row, tBase, half, lane, ready);
       if (!ok) { if (lane == 0) fail(4000 + buf); break; }
       if (c.steps) {
         ++it;
@@ -694,9 +742,10 @@ expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
 }
 
 const void* expertGemmKernelFn(int mode) { return mode == EXPERT_DX ? (const void*)expertGemmKernel<EXPERT_DX> : (const void*)expertGemmKernel<EXPERT_FORWARD>; }
-const void* expertGemmPairKernelFn(int mode) {
-  return mode == EXPERT_DW ? (const void*)expertGemmPairKernel<EXPERT_DW>
-         : mode == EXPERT_DX ? (const void*)expertGemmPairKernel<EXPERT_DX> : (const void*)expertGemmPairKernel<EXPERT_FORWARD>;
+const void* expertGemmPairKernelFn(int mode, bool staged) {
+  if (mode == EXPERT_DW) return (const void*)expertGemmPairKernel<EXPERT_DW, true>;
+  if (mode == EXPERT_DX) return staged ? (const void*)expertGemmPairKernel<EXPERT_DX, true> : (const void*)expertGemmPairKernel<EXPERT_DX, false>;
+  return staged ? (const void*)expertGemmPairKernel<EXPERT_FORWARD, true> : (const void*)expertGemmPairKernel<EXPERT_FORWARD, false>;
 }
 size_t expertGemmSmemBytes() { return kSmemBytes; }
 int expertGemmThreads(bool pair) { return pair ? kPairThreads : kThreads; }

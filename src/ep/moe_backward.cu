@@ -39,6 +39,7 @@ __global__ void __launch_bounds__(kActThreads) expertActKernel(const __grid_cons
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[p][i] = 0.0f;
   if (inside) {
+#pragma unroll 2
     for (int row = slice * kRows + ty; row < rows; row += a.slices * kRows) {
       float g[8], z[kParts][8];
       unpackBf16x8(*(const uint4*)(dout + (size_t)row * a.cols), g);
@@ -93,6 +94,7 @@ __global__ void __launch_bounds__(kActThreads) expertBiasKernel(const __grid_con
   const size_t n = (size_t)a.experts * a.cols * (a.act == ACT_SWIGLU || a.act == ACT_GEGLU ? 2 : 1);
   for (size_t i = (size_t)blockIdx.x * kActThreads + threadIdx.x; i < n; i += (size_t)gridDim.x * kActThreads) {
     float s = 0.0f;
+#pragma unroll 8
     for (int k = 0; k < a.slices; ++k) s += a.partial[k * n + i];
     ((__nv_bfloat16*)a.dbias)[i] = __float2bfloat16_rn(s);
   }

@@ -147,8 +147,8 @@ static int pairsAtOnce(ncclEpGroup* g) {
   int n = g->expertPairs.load(std::memory_order_relaxed);
   if (n >= 0) return n;
   n = g->smCount / 2;
-  for (int mode : {EXPERT_FORWARD, EXPERT_DX, EXPERT_DW}) {
-    const void* fn = expertGemmPairKernelFn(mode);
+  for (int form = 0; form < 5; ++form) {
+    const void* fn = expertGemmPairKernelFn(form % 3, form >= 3);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(g->smCount & ~1);
     cfg.blockDim = dim3(expertGemmThreads(true));
@@ -181,16 +181,16 @@ static ncclResult_t launchExpertGemm(ncclEpGroup* g, int mode, const void* A, in
   const double rows = mode == EXPERT_DW ? a->outRows : a->cap, tilesN = (a->cols + 31) / 32;
   if (pair) {
     const int pairs = (int)std::min<double>(pairsAtOnce(g), (double)a->experts * (int)((rows + 255) / 256) * tilesN);
-    return launchMoe(g, expertGemmPairKernelFn(mode), dim3(2 * pairs), expertGemmThreads(true), expertGemmSmemBytes(), args, stream);
+    return launchMoe(g, expertGemmPairKernelFn(mode, (a->residual || !a->wide) && !a->pre), dim3(2 * pairs), expertGemmThreads(true), expertGemmSmemBytes(), args, stream);
   }
   const int ctas = (int)std::min<double>(g->smCount, (double)a->experts * tilesN);
   return launchMoe(g, expertGemmKernelFn(mode), dim3(ctas), expertGemmThreads(false), expertGemmSmemBytes(), args, stream);
 }
 
-// Slices of rows that the activation's backward works on at a time: enough CTAs to fill the chip eight times over.
+// Slices of rows that the activation's backward works on at a time: enough CTAs to fill the chip four times over.
 static int actSlices(const ncclEpGroup* g, int experts, int rows, int cols) {
   const long long perSlice = (long long)experts * ((cols + kActCols - 1) / kActCols);
-  const long long want = ((long long)g->smCount * 8 + perSlice - 1) / perSlice, most = (rows + 7) / 8;
+  const long long want = ((long long)g->smCount * 4 + perSlice - 1) / perSlice, most = (rows + 7) / 8;
   return (int)std::max<long long>(1, std::min<long long>({want, most, 64}));
 }
 
