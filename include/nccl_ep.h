@@ -122,7 +122,7 @@ typedef enum { NCCL_EP_SCORE_SOFTMAX = 0, NCCL_EP_SCORE_SIGMOID = 1 } ncclEpScor
 typedef enum { NCCL_EP_GROUP_SCORE_MAX = 0, NCCL_EP_GROUP_SCORE_TOP2 = 1 } ncclEpGroupScore_t;
 typedef struct { unsigned int size; unsigned int magic; ncclEpScore_t score; int groups; int keep_groups; ncclEpGroupScore_t group_score; int renormalize; float scale; } ncclEpRouteConfig_t;
 ncclResult_t ncclEpRoute(ncclEpGroup_t ep_group, const void* logits, ncclDataType_t type, const float* bias, int64_t* topk_idx, float* topk_weights, int num_tokens, int num_experts, int num_topk, const ncclEpRouteConfig_t* config, cudaStream_t stream);
-/* d(logits) (type of the logits, all of it written) from d(topk_weights); of the configuration score, renormalize and scale count. */
+/* d(logits) (type of the logits, all of it written; it may take the logits' place) from d(topk_weights); of the configuration score, renormalize and scale count. */
 ncclResult_t ncclEpRouteBackward(ncclEpGroup_t ep_group, const float* d_weights, const void* logits, ncclDataType_t type, const int64_t* topk_idx, void* d_logits, int num_tokens, int num_experts, int num_topk, const ncclEpRouteConfig_t* config, cudaStream_t stream);
 
 /* The experts' products over rows packed as dispatch packs them (expert-major): for every expert e and its first counts[e] rows
@@ -130,7 +130,8 @@ ncclResult_t ncclEpRouteBackward(ncclEpGroup_t ep_group, const float* d_weights,
  * x [experts, rows, k], w [experts, n, k], bias [experts, n], out and residual [experts, rows, n], all bf16; n and k are multiples of 8.
  * The gated activations take w as [gate rows | up rows] (n a multiple of 16) and give silu(gate) * up or gelu(gate) * up: out and residual have n / 2
  * columns. counts: int32 on the device, null: all rows. Rows behind an expert's last are neither read into a result nor written.
- * bias, residual and pre may be null; pre [experts, rows, n] gets x w^T + bias for the backward pass. residual may be out. At most 256 experts. */
+ * bias, residual and pre may be null; pre [experts, rows, n] gets x w^T + bias for the backward pass. residual may be out. At most 256 experts,
+ * and 2^24 rows, n and k. */
 typedef enum { NCCL_EP_ACT_NONE = 0, NCCL_EP_ACT_RELU = 1, NCCL_EP_ACT_GELU = 2, NCCL_EP_ACT_SILU = 3, NCCL_EP_ACT_SWIGLU = 4, NCCL_EP_ACT_GEGLU = 5 } ncclEpActivation_t;
 ncclResult_t ncclEpExpertLinear(ncclEpGroup_t ep_group, const void* x, const void* w, const int* counts, const void* bias, const void* residual, void* out, void* pre, int num_experts, int num_rows, int n, int k, ncclEpActivation_t activation, cudaStream_t stream);
 /* Gradients: d_x [experts, rows, k] (the rows in use), d_w [experts, n, k] and d_bias [experts, n] (of every expert, zeros where it has no
@@ -142,7 +143,7 @@ ncclResult_t ncclEpExpertLinearBackward(ncclEpGroup_t ep_group, const void* d_ou
  * rank, expert-major; the routing of that dispatch must still be in place. */
 ncclResult_t ncclEpDispatchRows(ncclEpHandle_t handle, int* rows, cudaStream_t stream);
 /* Gradients of combine: d_y[rows[t,k]] = weights[t,k] * d_out[t], d_weights[t,k] = <d_out[t], y[rows[t,k]]> (0 without a row). d_out [tokens, hidden], y and d_y
- * [num_rows, hidden] bf16, hidden a multiple of 8; rows of d_y that no entry names are not written. */
+ * [num_rows, hidden] bf16, hidden a multiple of 8; rows of d_y that no entry names are not written, and d_y may be y where every row is named once. */
 ncclResult_t ncclEpCombineBackward(ncclEpGroup_t ep_group, const void* d_out, const void* y, const float* weights, const int* rows, void* d_y, float* d_weights, int num_tokens, int num_topk, int hidden, int num_rows, cudaStream_t stream);
 /* Gradient of dispatch: d_x[t] = sum over k of d_tokens[rows[t,k]], bf16 [tokens, hidden]. */
 ncclResult_t ncclEpDispatchBackward(ncclEpGroup_t ep_group, const void* d_tokens, const int* rows, void* d_x, int num_tokens, int num_topk, int hidden, int num_rows, cudaStream_t stream);

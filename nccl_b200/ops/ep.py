@@ -298,7 +298,7 @@ class ExpertParallel:
 
     def _logits(self, logits):
         code, shape = self._logit_codes.get(logits.dtype), logits.shape
-        if code is None or len(shape) != 2 or shape[1] != self.E:
+        if code is None or len(shape) != 2 or shape[1] != self.E or shape[0] >= 1 << 31:
             raise ValueError("logits must be an fp32, fp16 or bf16 tensor [tokens, %d], not %s %s" % (self.E, str(logits.dtype).replace("torch.", ""), list(shape)))
         self._need("logits", logits, logits.dtype, shape)
         return code
@@ -322,7 +322,8 @@ class ExpertParallel:
         return idx, weights
 
     def route_backward(self, dweights, logits, idx, score="softmax", renormalize=True, scale=1.0, out=None):
-        """Gradient of the logits (their type) from that of the weights; ``idx`` and the rule as ``route`` had them. The choice has no gradient."""
+        """Gradient of the logits (their type) from that of the weights; ``idx`` and the rule as ``route`` had them. The choice has no gradient.
+        ``out`` may be the logits."""
         code = self._logits(logits)
         T, topk = idx.shape
         self._need("dweights", dweights, self.torch.float32, (T, topk))
@@ -342,8 +343,8 @@ class ExpertParallel:
         E, rows, k = x.shape
         n = w.shape[1]
         gated = activation in ("swiglu", "geglu")
-        if n % (16 if gated else 8) or k % 8 or not 0 < E <= 256:
-            raise ValueError("%d experts (at most 256), n = %d must be a multiple of %d and k = %d of 8" % (E, n, 16 if gated else 8, k))
+        if n % (16 if gated else 8) or k % 8 or not 0 < E <= 256 or max(rows, n, k) > 1 << 24 or not n or not k:
+            raise ValueError("%d experts (at most 256) of %d rows, n = %d must be a multiple of %d and k = %d of 8, none above 2^24" % (E, rows, n, 16 if gated else 8, k))
         self._need("x", x, torch.bfloat16, (E, rows, k))
         self._need("w", w, torch.bfloat16, (E, n, k))
         if counts is not None:
@@ -407,15 +408,15 @@ class ExpertParallel:
         if dout.dim() != 2 or y.dim() < 2 or weights.dim() != 2:
             raise ValueError("dout must be [tokens, hidden], y [..., hidden], weights [tokens, topk], not %s, %s, %s" % (list(dout.shape), list(y.shape), list(weights.shape)))
         (T, H), K, bf16 = dout.shape, weights.shape[1], torch.bfloat16
-        if H % 8 or not 0 < K <= 16:
-            raise ValueError("hidden = %d must be a multiple of 8, topk = %d at most 16" % (H, K))
+        if H == 0 or H % 8 or not 0 < K <= 16 or y.numel() // H >= 1 << 31 or T >= 1 << 31:
+            raise ValueError("hidden = %d must be a multiple of 8, topk = %d at most 16, rows and tokens below 2^31" % (H, K))
         self._need("dout", dout, bf16, (T, H))
         self._need("y", y, bf16, (*y.shape[:-1], H))
         self._need("weights", weights, torch.float32, (T, K))
         self._need("rows", rows, torch.int32, (T, K))
-        dy, dweights = self._result("dy", dy, bf16, y.shape), self._result("dweights", dweights, torch.float32, (T, K))
+        dy, dweights = torch.empty_like(y) if dy is None else self._result("dy", dy, bf16, y.shape), self._result("dweights", dweights, torch.float32, (T, K))
         self._moe_call("ncclEpCombineBackward", self.group, dout.data_ptr(), y.data_ptr(), weights.data_ptr(), rows.data_ptr(), dy.data_ptr(), dweights.data_ptr(), T, K, H,
-                       y.numel() // H if H else 0)
+                       y.numel() // H)
         return dy, dweights
 
     def dispatch_backward(self, dtoks, rows, out=None):
@@ -424,8 +425,8 @@ class ExpertParallel:
         if dtoks.dim() < 2 or rows.dim() != 2:
             raise ValueError("dtoks must be [..., hidden] and rows [tokens, topk], not %s and %s" % (list(dtoks.shape), list(rows.shape)))
         (T, K), H = rows.shape, dtoks.shape[-1]
-        if H == 0 or H % 8 or not 0 < K <= 16:
-            raise ValueError("hidden = %d must be a multiple of 8, topk = %d at most 16" % (H, K))
+        if H == 0 or H % 8 or not 0 < K <= 16 or dtoks.numel() // H >= 1 << 31 or T >= 1 << 31:
+            raise ValueError("hidden = %d must be a multiple of 8, topk = %d at most 16, rows and tokens below 2^31" % (H, K))
         self._need("dtoks", dtoks, torch.bfloat16, dtoks.shape)
         self._need("rows", rows, torch.int32, (T, K))
         out = self._result("out", out, torch.bfloat16, (T, H))

@@ -133,9 +133,10 @@ static ncclResult_t checkLinear(const ncclEpGroup* g, const char* what, int expe
     WARN("%s: %d experts (at most %d), %d rows, n=%d must be a multiple of %d, k=%d of 8", what, experts, kExpertMax, rows, n, unit, k);
     return ncclInvalidArgument;
   }
-  // a tile is numbered with 31 bits, whatever its width; rows in use and their places too
+  // sums of more steps would outlast the kernels' waits; and a tile is numbered with 31 bits, whatever its width
+  const int longest = 1 << 24;
   const double tilesN = (n + 31) / 32, tilesK = (k + 31) / 32, most = 1 << 30;
-  if ((double)experts * ((rows + 127) / 128) * std::max(tilesN, tilesK) > most || (double)experts * ((n + 127) / 128) * tilesK > most || rows > (1 << 30) || (double)experts * rows > 2.0 * most - 1) {
+  if ((double)experts * ((rows + 127) / 128) * std::max(tilesN, tilesK) > most || (double)experts * ((n + 127) / 128) * tilesK > most || rows > longest || n > longest || k > longest) {
     WARN("%s: %d experts x %d rows x n=%d, k=%d are too many tiles", what, experts, rows, n, k);
     return ncclInvalidArgument;
   }
@@ -214,6 +215,11 @@ ncclResult_t ncclEpRoute(ncclEpGroup_t g, const void* logits, ncclDataType_t typ
   if (tokens == 0) return ncclSuccess;
   if (!logits || !idx || !weights) return ncclInvalidArgument;
   if (!aligned({logits}, kind == ROUTE_F32 ? 4 : 2) || !aligned({bias, weights}, 4) || !aligned({idx}, 8)) { WARN("ncclEpRoute: misaligned tensors"); return ncclInvalidArgument; }
+  const size_t entries = (size_t)tokens * topk, logitBytes = (size_t)tokens * experts * (kind == ROUTE_F32 ? 4 : 2);
+  if (overlap({{idx, entries * 8}, {weights, entries * 4}}, {{logits, logitBytes}, {bias, (size_t)experts * 4}}) || overlap({{idx, entries * 8}}, {{weights, entries * 4}})) {
+    WARN("ncclEpRoute: an output shares memory with another tensor");
+    return ncclInvalidArgument;
+  }
   a.logits = logits;
   a.bias = bias;
   a.idx = idx;
@@ -240,6 +246,12 @@ ncclResult_t ncclEpRouteBackward(ncclEpGroup_t g, const float* dweights, const v
   if (tokens == 0) return ncclSuccess;
   if (!dweights || !logits || !idx || !dlogits) return ncclInvalidArgument;
   if (!aligned({logits, dlogits}, kind == ROUTE_F32 ? 4 : 2) || !aligned({dweights}, 4) || !aligned({idx}, 8)) { WARN("ncclEpRouteBackward: misaligned tensors"); return ncclInvalidArgument; }
+  const size_t entries = (size_t)tokens * topk, logitBytes = (size_t)tokens * experts * (kind == ROUTE_F32 ? 4 : 2);
+  // a token's row is read before its gradient is written: the one may take the other's place
+  if (overlap({{dlogits, logitBytes}}, {{logits == dlogits ? nullptr : logits, logitBytes}, {dweights, entries * 4}, {idx, entries * 8}})) {
+    WARN("ncclEpRouteBackward: the output shares memory with an input (it may take the logits' place)");
+    return ncclInvalidArgument;
+  }
   a.logits = logits;
   a.idx = (int64_t*)idx;
   a.dweights = dweights;

@@ -144,6 +144,7 @@ def test_rows_of_one_expert(ep, counts):
 @pytest.mark.parametrize("act", [None, "relu", "gelu", "silu", "swiglu", "geglu"])
 @pytest.mark.parametrize("E,cap,n,k,counts", [
     (3, 40, 16, 8, [0, 40, 7]),                          # the smallest sizes
+    (2, 200, 16, 8, [200, 3]),                           # and on pairs
     (5, 70, 272, 72, [70, 0, 0, 33, 1]),                 # tiles that hang over on every side
     (4, 300, 528, 392, [299, 128, 0, 200]),
     (2, 1, 512, 256, [1, 0]),                            # a single token
@@ -152,6 +153,42 @@ def test_rows_of_one_expert(ep, counts):
 ])
 def test_activations_and_sizes(ep, act, E, cap, n, k, counts):
     check(ep, E, cap, n, k, act, counts, bias=True, residual=act in (None, "swiglu"))
+
+
+def test_smallest_ungated(ep):
+    check(ep, 2, 5, 8, 8, None, [5, 1], bias=True, residual=True)
+    check(ep, 2, 150, 8, 8, "gelu", [150, 1], bias=True)
+
+
+def test_captured_as_a_process_first_calls():
+    """Kernels that have not been loaded yet, in a graph."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from nccl_b200 import Communicator, get_unique_id
+from nccl_b200.ops.ep import ExpertParallel
+torch.cuda.set_device(0)
+c = Communicator(1, 0, get_unique_id())
+ep = ExpertParallel(c, 4, 1, 128)
+x, w, d = (torch.randn(4, *s, device="cuda").bfloat16() for s in ((200, 64), (96, 64), (200, 96)))
+n, l = torch.tensor([3, 200, 0, 50], dtype=torch.int32, device="cuda"), torch.randn(9, 4, device="cuda")
+def step():
+    idx, g = ep.route(l, 2, score="sigmoid")
+    return ep.expert_linear(x, w, n), ep.expert_linear_backward(d, x, w, n)[1], ep.route_backward(g, l, idx, score="sigmoid")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+want = step()
+torch.cuda.synchronize()
+assert torch.equal(got[0][1], want[0][1]) and torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+print("same")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "same" in out.stdout, out.stderr[-2000:]
 
 
 def test_many_experts_few_of_them_used(ep):
@@ -264,6 +301,8 @@ def test_no_rows_and_refusals(ep):
                      ((x, w, c), dict(bias=torch.zeros(2, 47, **bf))), ((x, w, c), dict(residual=d.float())), ((x, w, c), dict(out=d[:, :8])), ((x, w, c), dict(pre=x))):
         with pytest.raises(ValueError):
             ep.expert_linear(*args, **kw)
+    with pytest.raises(ValueError):
+        ep.expert_linear(torch.empty(2, 16, 0, **bf), torch.empty(2, 48, 0, **bf), c)
     for args, kw in (((d[:, :, :40].contiguous(), x, w, c), {}), ((d, x, w, c), dict(activation="gelu")), ((d, x, w, c), dict(activation="gelu", pre=x)),
                      ((d, x, w, c), dict(dx=d)), ((d, x, w, c), dict(need_dbias=True, dbias=d))):
         with pytest.raises(ValueError):

@@ -272,7 +272,15 @@ def test_no_tokens_and_refusals(group):
                  dict(bias=torch.zeros(16)), dict(idx=torch.zeros(5, 4, device="cuda", dtype=torch.int32)), dict(weights=torch.zeros(4, 5, device="cuda"))):
         with pytest.raises(ValueError):
             ep.route(l, 4, **args)
+    raw = torch.zeros(5 * 16 + 40, device="cuda")
+    for kw in (dict(weights=raw[:20].view(5, 4)), dict(idx=raw[10:50].view(torch.int64).view(5, 4))):
+        with pytest.raises(NcclError):   # over the logits
+            ep.route(raw[:80].view(5, 16), 4, **kw)
     idx, w = ep.route(l, 4)
+    place = l.clone()
+    assert torch.equal(ep.route_backward(w, place, idx, renormalize=False, out=place), ep.route_backward(w, l, idx, renormalize=False)) and not torch.equal(place, l)
+    with pytest.raises(NcclError):
+        ep.route_backward(raw[70:90].view(5, 4), l, idx, out=raw[:80].view(5, 16))
     for dw, i in ((w.double(), idx), (w[:, :3], idx), (w, idx[:4])):
         with pytest.raises(ValueError):
             ep.route_backward(dw, l, i)
