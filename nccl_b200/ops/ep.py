@@ -386,7 +386,7 @@ class ExpertParallel:
         dw = self._result("dw", dw, bf16, (E, n, k)) if need_dw else None
         dbias = self._result("dbias", dbias, bf16, (E, n)) if need_dbias else None
         size = self.lib.ncclEpExpertLinearBackwardWork(self.group, E, rows, n, act, int(need_dbias))
-        work = torch.empty(size, dtype=torch.uint8, device=self._device) if size else None
+        work = torch.empty(size, dtype=torch.uint8, device=self._place) if size else None
         self._moe_call("ncclEpExpertLinearBackward", self.group, dout.data_ptr(), x.data_ptr(), w.data_ptr(), ptr(counts), ptr(pre) if act else None, ptr(dx), ptr(dw),
                        ptr(dbias), ptr(work), E, rows, n, k, act)
         return dx, dw, dbias
