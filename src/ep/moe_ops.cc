@@ -181,8 +181,13 @@ static ncclResult_t launchExpertGemm(ncclEpGroup* g, int mode, const void* A, in
   // no more CTAs than the narrowest tiles of all rows
   const double rows = mode == EXPERT_DW ? a->outRows : a->cap, tilesN = (a->cols + 31) / 32;
   if (pair) {
-    const int pairs = (int)std::min<double>(pairsAtOnce(g), (double)a->experts * (int)((rows + 255) / 256) * tilesN);
-    return launchMoe(g, expertGemmPairKernelFn(mode, (a->residual || !a->wide) && !a->pre), dim3(2 * pairs), expertGemmThreads(true), expertGemmSmemBytes(), args, stream);
+    const double tiles = (double)a->experts * (int)((rows + 255) / 256) * tilesN;
+    const int pairs = (int)std::min<double>(pairsAtOnce(g), tiles);
+    // Through shared memory go results that a lane would touch 16 bytes at a time (a residual, rows that are not whole packs of 32 bytes). With `pre` that makes the
+    // sums twice, which pays where there may be many tiles (of 256 columns, eight for each pair): 16 experts of 1800 rows, 4696 x 328, there and back 668 us straight from registers,
+    // 517 so; five of 310 rows, 2200 x 1000, 86 and 100.
+    const bool staged = (a->residual || !a->wide) && (!a->pre || tiles / 8 > 8.0 * pairs);
+    return launchMoe(g, expertGemmPairKernelFn(mode, staged), dim3(2 * pairs), expertGemmThreads(true), expertGemmSmemBytes(), args, stream);
   }
   const int ctas = (int)std::min<double>(g->smCount, (double)a->experts * tilesN);
   return launchMoe(g, expertGemmKernelFn(mode), dim3(ctas), expertGemmThreads(false), expertGemmSmemBytes(), args, stream);

@@ -201,9 +201,30 @@ def test_many_experts_few_of_them_used(ep):
 @pytest.mark.parametrize("E,cap,n,k,act,counts", [
     (2, 2100, 768, 512, None, [2049, 1111]),              # several panels of row tiles
     (8, 700, 4096, 512, "swiglu", [700, 650, 3, 0, 129, 256, 511, 512]),
+    (64, 300, 2008, 64, "gelu", [(37 * e) % 301 for e in range(64)]),      # many tiles of rows that are no whole packs of 32 bytes
+    (64, 300, 4016, 64, "geglu", [(53 * e) % 301 for e in range(64)]),
 ])
 def test_large(ep, E, cap, n, k, act, counts):
-    check(ep, E, cap, n, k, act, counts, bias=act is None)
+    check(ep, E, cap, n, k, act, counts, bias=act is None or E == 64, residual=E == 64)
+
+
+@pytest.mark.parametrize("act", [None, "relu", "gelu", "silu", "swiglu", "geglu"])
+@pytest.mark.parametrize("n,residual", [(272, False), (272, True), (528, True), (560, False), (2064, True)])
+def test_results_do_not_depend_on_what_else_is_kept(ep, act, n, residual):
+    """With and without the pre-activations kept, results take different ways to memory."""
+    counts = [200, 0, 131, 77, 256]
+    x, w, b, r, _, c = make(5, 256, n, 136, act, n, True, residual, counts)
+    pre = torch.empty(5, 256, n, dtype=torch.bfloat16, device="cuda")
+    lone, kept = ep.expert_linear(x, w, c, bias=b, activation=act, residual=r), ep.expert_linear(x, w, c, bias=b, activation=act, residual=r, pre=pre)
+    place = None
+    if residual:
+        place = r.clone()
+        ep.expert_linear(x, w, c, bias=b, activation=act, residual=place, out=place)
+    for e, m in enumerate(counts):
+        v, bound, _, _ = forward(act, x[e, :m].double(), w[e].double(), b[e].double(), None if r is None else r[e, :m].double())
+        assert within(lone[e, :m], v, bound) and torch.equal(lone[e, :m], kept[e, :m])
+        if residual:
+            assert torch.equal(place[e, :m], lone[e, :m]) and torch.equal(place[e, m:], r[e, m:])
 
 
 # The second CTA of a pair has neither a row nor a column of such tiles, and many steps in which to fall behind
