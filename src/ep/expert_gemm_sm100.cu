@@ -116,6 +116,9 @@ struct Tile {
   int e, rows, row0, col0, steps;   // expert, its rows in use, first row and column of the result, 64-wide steps of the sum
 };
 
+// ceil(2^32 / n): the quotient of numbers below 2^26 by 2 .. 8 is the high word of the product.
+__constant__ uint32_t kInverse[9] = {0, 0, 0x80000000u, 0x55555556u, 0x40000000u, 0x33333334u, 0x2aaaaaabu, 0x24924925u, 0x20000000u};
+
 // The tiles of all experts and their order.
 template <int MODE, int BM>
 struct Tiles {
@@ -162,21 +165,31 @@ struct Tiles {
     count = rowTiles * tilesN;
   }
 
-  // Panels of 8 row tiles: those in flight share both operands.
-  __device__ __forceinline__ Tile at(int t) const {
+  // Panels of 8 row tiles: those in flight share both operands. No search where the expert stays, and no division: with both DW over 32 experts of 64 rows, whose
+  // tiles are short, took 415 us, without 332. `from`: an expert at or before t's, as that of the tile before.
+  __device__ __forceinline__ Tile at(int t, int from) const {
     Tile r;
-    int lo = 0, hi = a.experts;
-    while (hi - lo > 1) {   // the last expert whose tiles begin at or before t
-      const int mid = (lo + hi) / 2;
-      if (start[mid] * tilesN <= t) lo = mid;
-      else hi = mid;
+    int lo = from;
+    if (start[lo + 1] * tilesN <= t) {   // the last expert whose tiles begin at or before t
+      int hi = a.experts;
+      ++lo;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (start[mid] * tilesN <= t) lo = mid;
+        else hi = mid;
+      }
     }
     r.e = lo;
     r.rows = rowsOf(a, lo);
-    const int j = t - start[lo] * tilesN, mine = start[lo + 1] - start[lo];
-    const int panel = j / (8 * tilesN), width = min(8, mine - panel * 8), k = j - panel * 8 * tilesN;
-    r.row0 = (panel * 8 + k % width) * BM;
-    r.col0 = k / width * outCols;
+    const int first = start[lo], mine = start[lo + 1] - first;
+    int k = t - first * tilesN, panel = 0;
+    if (mine > 8) {
+      panel = k / (8 * tilesN);
+      k -= panel * 8 * tilesN;
+    }
+    const int width = min(8, mine - panel * 8), col = width == 1 ? k : (int)__umulhi((uint32_t)k, kInverse[width]);   // k / width
+    r.row0 = (panel * 8 + k - col * width) * BM;
+    r.col0 = col * outCols;
     r.steps = ((MODE == EXPERT_DW ? r.rows : a.depth) + kBK - 1) / kBK;
     return r;
   }
@@ -194,141 +207,183 @@ __device__ __forceinline__ void reportTimeout(const ExpertGemmArgs& a, uint32_t 
   }
 }
 
-// 32 neighbouring bf16 of one row, `n` of them (a multiple of 8) inside the matrix: 32 bytes per access where rows allow it.
-__device__ __forceinline__ void storeRow32(__nv_bfloat16* to, const float (&v)[32], int n, bool wide) {
+// 32 lanes x 8 or 16 columns of an accumulator, and the wait for them.
+__device__ __forceinline__ void tmemLd(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmemLd(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                 "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmemLd(uint32_t taddr, uint32_t (&r)[32]) { tmemLd32(taddr, r); }
+template <int N>
+__device__ __forceinline__ void tmemLdReady(uint32_t (&r)[N]) {   // nothing that uses them moves in front
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int j = 0; j < 32; j += 16) {
-    const uint4 lo = packBf16x8(v + j), hi = packBf16x8(v + j + 8);
-    if (wide) {
-      if (j < n) asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + j), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
-    } else {
-      if (j < n) *(uint4*)(to + j) = lo;
-      if (j + 8 < n) *(uint4*)(to + j + 8) = hi;
-    }
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i])::"memory");
+}
+template <int N>
+__device__ __forceinline__ void asFloat(const uint32_t (&r)[N], float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = __uint_as_float(r[i]);
+}
+// v += N neighbouring bf16.
+template <int N>
+__device__ __forceinline__ void addBf16(const uint4 (&q)[N / 8], float (&v)[N]) {
+#pragma unroll
+  for (int j = 0; j < N / 8; ++j) {
+    float f[8];
+    unpackBf16x8(q[j], f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[j * 8 + i] += f[i];
   }
 }
-// 32 neighbouring bf16, as storeRow32 takes them: fetched early, added when the sums are there.
-struct Row32 {
-  uint4 q[4];
-  __device__ __forceinline__ void load(const __nv_bfloat16* from, int n) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) q[j] = j * 8 < n ? *(const uint4*)(from + j * 8) : make_uint4(0, 0, 0, 0);
-  }
-  __device__ __forceinline__ void addTo(float (&v)[32]) const {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float f[8];
-      unpackBf16x8(q[j], f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[j * 8 + i] += f[i];
+// A tile's bias, eight columns to a lane, fetched before the sums are complete: from memory (or level 2) for every step it took longer than the step. All lanes
+// ask for the same columns.
+struct TileBias {
+  uint4 q[2];
+  __device__ __forceinline__ void load(const __nv_bfloat16* bias, int cols, int parts, int end, int lane) {
+    q[0] = q[1] = make_uint4(0, 0, 0, 0);
+    if (lane * 8 < end) {
+      q[0] = *(const uint4*)(bias + lane * 8);
+      if (parts == 2) q[1] = *(const uint4*)(bias + cols + lane * 8);
     }
   }
+  __device__ __forceinline__ uint4 at(int part, int col) const {
+    const uint4 m = part ? q[1] : q[0];
+    const int from = col / 8;
+    return make_uint4(__shfl_sync(~0u, m.x, from), __shfl_sync(~0u, m.y, from), __shfl_sync(~0u, m.z, from), __shfl_sync(~0u, m.w, from));
+  }
 };
+// 16 neighbouring columns of one row, 8 or 16 of them inside the matrix.
+__device__ __forceinline__ void storeRow16(__nv_bfloat16* to, const float (&v)[16], bool both, bool wide) {
+  const uint4 lo = packBf16x8(v), hi = packBf16x8(v + 8);
+  if (wide) {
+    st32(to, Pack32{lo, hi});
+  } else {
+    *(uint4*)to = lo;
+    if (both) *(uint4*)(to + 8) = hi;
+  }
+}
+
+// Epilogues take an accumulator in small steps in a loop that is not unrolled: each warp passes this code once per tile, and straight through 32 or 64
+// columns it did so at the pace at which instructions can be fetched (64 experts of 50 rows, 5000 x 184 with bias and residual: 186 us unrolled, 168 so; 64 of 200, 6656 x
+// 432, geglu and bias: 222 and 207).
 
 // Epilogue of one warp for its 32 rows, `row` the first of them, and every other 32 columns of the tile: tBase is the tensor-memory address of the
-// warp's first lane and the tile's first column. A lane has a row of the accumulator and stores 32 of its columns at a time, whole sectors straight from
+// warp's first lane and the tile's first column. A lane has a row of the accumulator and stores 16 of its columns at a time, whole sectors straight from
 // registers: shared memory is busy with the operands, and its room makes a seventh stage (32 experts of 64 rows, 4096 x 7168: 295 us through shared memory, 284 so).
-// What is added (bias, residual) is on its way while the sums are not complete (`ready` waits for them), and while the columns before are stored.
 template <int MODE, typename T, typename Ready>
 __device__ __forceinline__ bool storeTile(const ExpertGemmArgs& a, const T& tiles, const Tile& c, int row, uint32_t tBase, int half, int lane, Ready ready) {
   const int parts = tiles.parts, outCols = tiles.outCols;
   const bool mine = row + lane < c.rows;
-  const size_t at = (size_t)c.e * a.cap + row + lane;
+  const size_t at = ((size_t)c.e * a.cap + row + lane) * a.cols + c.col0;
   const int end = row < c.rows ? min(outCols, a.cols - c.col0) : 0;
-  Row32 bias[2], residual;
-  auto fetch = [&](int cc) {
-    const int col = c.col0 + cc, n = a.cols - col;   // a multiple of 8
-    if (MODE == EXPERT_FORWARD && a.bias && cc < end) {
-      const __nv_bfloat16* b = (const __nv_bfloat16*)a.bias + (size_t)c.e * parts * a.cols + col;
-      bias[0].load(b, n);
-      if (parts == 2) bias[1].load(b + a.cols, n);
-    }
-    if (MODE == EXPERT_FORWARD && a.residual && mine && cc < end) residual.load((const __nv_bfloat16*)a.residual + at * a.cols + col, n);
-  };
-  fetch(half * 32);
+  TileBias bias;
+  if (MODE == EXPERT_FORWARD && a.bias) bias.load((const __nv_bfloat16*)a.bias + (size_t)c.e * parts * a.cols + c.col0, a.cols, parts, end, lane);
   if (!ready()) return false;
-  for (int cc = half * 32; cc < end; cc += 64) {
-    const int col = c.col0 + cc, n = a.cols - col;
-    auto sums = [&](int part, float (&v)[32]) {
+  if (MODE != EXPERT_FORWARD || (a.act == ACT_NONE && !a.bias && !a.pre && !a.residual)) {
+    // the sums as they are: 32 at a time (64 experts of 50 rows, 4992 x 184: 55 us, 63 by the loop below)
+#pragma unroll 1
+    for (int cc = half * 32; cc < end; cc += 64) {
       uint32_t r[32];
-      tmemLd32(tBase + part * outCols + cc, r);
-      tmemLdWait32(r);
+      tmemLd(tBase + cc, r);
+      tmemLdReady(r);
+      if (!mine) continue;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-      if (MODE == EXPERT_FORWARD && a.bias) bias[part].addTo(v);
-      if (MODE == EXPERT_FORWARD && a.pre && mine) storeRow32((__nv_bfloat16*)a.pre + (at * parts + part) * a.cols + col, v, n, a.wide);
+      for (int j = 0; j < 32; j += 16) {
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[j + i]);
+        if (cc + j < end) storeRow16((__nv_bfloat16*)a.out + at + cc + j, v, cc + j + 8 < end, a.wide);
+      }
+    }
+    return true;
+  }
+#pragma unroll 1
+  for (int cc = half * 32; cc < end; cc += cc & 16 ? 48 : 16) {
+    const bool both = cc + 8 < end;   // (columns come in eights)
+    uint32_t r[16];
+    float v[16], u[16];
+    auto sums = [&](int part, float (&to)[16]) {
+      tmemLd(tBase + part * outCols + cc, r);
+      tmemLdReady(r);
+      asFloat(r, to);
+      if (MODE == EXPERT_FORWARD && a.bias) {
+        const uint4 add[2] = {bias.at(part, cc), bias.at(part, cc + 8)};
+        addBf16<16>(add, to);
+      }
+      if (MODE == EXPERT_FORWARD && a.pre && mine) storeRow16((__nv_bfloat16*)a.pre + (at - c.col0) * parts + part * a.cols + c.col0 + cc, to, both, a.wide);
     };
-    float v[32];
     sums(0, v);
     if (MODE == EXPERT_FORWARD) {
-      float u[32];
       if (parts == 2) sums(1, u);
-      activate32(a.act, v, u);
-      if (a.residual) residual.addTo(v);
+      activateAll<16>(a.act, v, u);
+      if (a.residual && mine) {
+        const uint4* from = (const uint4*)((const __nv_bfloat16*)a.residual + at + cc);
+        const uint4 add[2] = {*from, both ? from[1] : make_uint4(0, 0, 0, 0)};
+        addBf16<16>(add, v);
+      }
     }
-    fetch(cc + 64);
-    if (mine) storeRow32((__nv_bfloat16*)a.out + at * a.cols + col, v, n, a.wide);
+    if (mine) storeRow16((__nv_bfloat16*)a.out + at + cc, v, both, a.wide);
   }
   return true;
 }
 
 // The same through shared memory: 64 columns of 32 rows at a time pass 4 KiB (16-byte chunks XOR-swizzled by row), so that memory sees 128 contiguous bytes of a
-// row. For DW, whose results are the traffic: 32 experts of 64 rows, 4096 x 7168, 410 us (4.6 TB/s written; the framework's fill of the same memory
-// 474), with the stores above 501, with bulk copies from shared memory 609. And where a lane's own row would be touched 16 bytes at a time, 32 lines by an
-// instruction (residual, rows that are not whole packs of 32 bytes): 64 experts of about 140 rows, 2056 x 1400 with a residual, 153 and 145 us. With `pre` it computes
-// the sums twice: five experts of 310 rows, 2200 x 1000 with both, there and back, 94 us by the stores above, 112 so.
+// row. For DW, whose results are the traffic: 32 experts of 64 rows, 4096 x 7168, 431 us, with the stores above 501, with bulk copies from shared memory
+// 609 (332 us since, 5.7 TB/s written; the framework's fill of the same memory takes 474). And where a lane's own row would be touched 16 bytes at a time, 32 lines by an
+// instruction (residual, rows that are not whole packs of 32 bytes): 64 experts of about 140 rows, 2056 x 1400 with a residual, 153 and 145 us.
 template <int MODE, typename T, typename Ready>
 __device__ __forceinline__ bool storeTileStaged(const ExpertGemmArgs& a, const T& tiles, const Tile& c, int row, uint32_t tBase, uint8_t* wbuf, int half, int lane, Ready ready) {
   const int parts = tiles.parts, outCols = tiles.outCols, left = tiles.rowLimit(c) - row;   // rows from here on
   const size_t first = (size_t)c.e * (MODE == EXPERT_DW ? a.outRows : a.cap) + row;
   const int end = left > 0 ? min(outCols, a.cols - c.col0) : 0;
+  TileBias bias;
+  if (MODE == EXPERT_FORWARD && a.bias) bias.load((const __nv_bfloat16*)a.bias + (size_t)c.e * parts * a.cols + c.col0, a.cols, parts, end, lane);
   auto chunk = [&](int r, int j) { return (uint4*)(wbuf + r * 128 + ((j ^ (r & 7)) * 16)); };
   const int mine = lane >> 3, j0 = lane & 7;   // of four rows, and of a row's eight chunks
   uint4 residual[8];
   auto fetch = [&](int cc) {
     if (MODE != EXPERT_FORWARD || !a.residual) return;
-    const __nv_bfloat16* from = (const __nv_bfloat16*)a.residual + first * a.cols + c.col0 + cc;
+    const __nv_bfloat16* from = (const __nv_bfloat16*)a.residual + (first + mine) * a.cols + c.col0 + cc + j0 * 8;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) residual[k] = cc + j0 * 8 < end && k * 4 + mine < left ? *(const uint4*)(from + (size_t)(k * 4 + mine) * a.cols + j0 * 8) : make_uint4(0, 0, 0, 0);
+    for (int k = 0; k < 8; ++k) residual[k] = cc + j0 * 8 < end && k * 4 + mine < left ? *(const uint4*)(from + (size_t)(k * 4) * a.cols) : make_uint4(0, 0, 0, 0);
   };
   fetch(half * 64);
   if (!ready()) return false;
+#pragma unroll 1
   for (int cc = half * 64; cc < end; cc += 128) {
-    const int col = c.col0 + cc, width = min(64, end - cc);   // a multiple of 8
+    const int width = min(64, end - cc), col = c.col0 + cc;   // a multiple of 8
     auto store = [&](__nv_bfloat16* to, size_t ld) {
       __syncwarp();
+      to += mine * ld + j0 * 8;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int r = k * 4 + mine;
-        if (r < left && j0 * 8 < width) *(uint4*)(to + (size_t)r * ld + j0 * 8) = *chunk(r, j0);
-      }
+      for (int k = 0; k < 8; ++k, to += 4 * ld)
+        if (k * 4 + mine < left && j0 * 8 < width) *(uint4*)to = *chunk(k * 4 + mine, j0);
       __syncwarp();
     };
-    auto sums = [&](int part, int h, float (&v)[32]) {
-      Row32 bias;
-      const bool biased = MODE == EXPERT_FORWARD && a.bias;
-      if (biased) bias.load((const __nv_bfloat16*)a.bias + ((size_t)c.e * parts + part) * a.cols + col + h * 32, a.cols - col - h * 32);
-      uint32_t r[32];
-      if (MODE != EXPERT_DW || c.steps) {
-        tmemLd32(tBase + part * outCols + cc + h * 32, r);
-        tmemLdWait32(r);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) r[i] = 0;
+    auto sums = [&](int part, int at, float (&v)[8]) {
+      uint32_t r[8];
+      tmemLd(tBase + part * outCols + cc + at, r);
+      tmemLdReady(r);
+      asFloat(r, v);
+      if (a.bias) {
+        const uint4 add[1] = {bias.at(part, cc + at)};
+        addBf16<8>(add, v);
       }
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-      if (biased) bias.addTo(v);
     };
     if (MODE == EXPERT_FORWARD && a.pre) {
+#pragma unroll 1
       for (int p = 0; p < parts; ++p) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (h * 32 >= width) break;
-          float v[32];
-          sums(p, h, v);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) *chunk(lane, h * 4 + j) = packBf16x8(v + j * 8);
+#pragma unroll 1
+        for (int at = 0; at < width; at += 8) {
+          float v[8];
+          sums(p, at, v);
+          *chunk(lane, at / 8) = packBf16x8(v);
         }
         store((__nv_bfloat16*)a.pre + (first * parts + p) * a.cols + col, (size_t)parts * a.cols);
       }
@@ -339,27 +394,33 @@ __device__ __forceinline__ bool storeTileStaged(const ExpertGemmArgs& a, const T
       __syncwarp();
       fetch(cc + 128);
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (h * 32 >= width) break;
-      float v[32];
-      sums(0, h, v);
-      if (MODE == EXPERT_FORWARD) {
-        float u[32];
-        if (parts == 2) sums(1, h, u);
-        activate32(a.act, v, u);
+    if (MODE == EXPERT_FORWARD) {
+#pragma unroll 1
+      for (int at = 0; at < width; at += 8) {
+        float v[8], u[8];
+        sums(0, at, v);
+        if (parts == 2) sums(1, at, u);
+        activateAll<8>(a.act, v, u);
         if (a.residual) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float f[8];
-            unpackBf16x8(*chunk(lane, h * 4 + j), f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[j * 8 + i] += f[i];
-          }
+          const uint4 add[1] = {*chunk(lane, at / 8)};
+          addBf16<8>(add, v);
         }
+        *chunk(lane, at / 8) = packBf16x8(v);
       }
+    } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) *chunk(lane, h * 4 + j) = packBf16x8(v + j * 8);
+      for (int at = 0; at < 64; at += 32) {
+        if (at >= width) break;
+        uint32_t r[32] = {};
+        if (MODE != EXPERT_DW || c.steps) {
+          tmemLd(tBase + cc + at, r);
+          tmemLdReady(r);
+        }
+        float v[32];
+        asFloat(r, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *chunk(lane, at / 8 + j) = packBf16x8(v + j * 8);
+      }
     }
     store((__nv_bfloat16*)a.out + first * a.cols + col, (size_t)a.cols);
   }
@@ -428,8 +489,10 @@ expertGemmKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       uint32_t phase = 0, sA = ring, bar = bars;
       const uint32_t ringEnd = ring + stages * stageBytes;
       bool whole = false;   // every stage was loaded once
+      int at = 0;   // expert of the tile before
       for (int t = blockIdx.x; t < tiles.count && !*abortFlag; t += gridDim.x) {
-        const Tile c = tiles.at(t);
+        const Tile c = tiles.at(t, at);
+        at = c.e;
         const int second = c.col0 + (parts == 2 ? a.cols : boxRows);   // row of W in a tile's second box
         const int aBoxes = (c.rows + 31) / 32, end = c.steps * kBK;
         const uint32_t bytes = (uint32_t)(aBoxes * a.boxRows + bn) * 128;
@@ -467,8 +530,10 @@ expertGemmKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       int s = 0, it = 0;
       uint32_t phase = 0;
       bool bad = false;
+      int at = 0;   // expert of the tile before
       for (int t = blockIdx.x; t < tiles.count && !bad && !*abortFlag; t += gridDim.x, ++it) {
-        const Tile c = tiles.at(t);
+        const Tile c = tiles.at(t, at);
+        at = c.e;
         const int buf = it & 1;
         if (!waitOr(smemAddr(&accEmpty[buf]), ((it >> 1) & 1) ^ 1, abortFlag)) { fail(2000 + buf); break; }
         tcFenceAfter();
@@ -491,8 +556,10 @@ expertGemmKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   } else {
     const int q = warp & 3, half = (warp - kFirstEpiWarp) >> 2;   // TMEM lanes [32q, 32q+32) belong to the warps with warp % 4 == q
     int it = 0;
+    int at = 0;   // expert of the tile before
     for (int t = blockIdx.x; t < tiles.count && !__any_sync(~0u, *abortFlag); t += gridDim.x, ++it) {
-      const Tile c = tiles.at(t);
+      const Tile c = tiles.at(t, at);
+      at = c.e;
       const int buf = it & 1;
       auto ready = [&] {
         const bool ok = warpWaitOr(smemAddr(&accFull[buf]), (it >> 1) & 1, abortFlag, lane);
@@ -599,8 +666,10 @@ expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       const uint32_t ringEnd = ring + kPairStages * kStageBytes;
       uint32_t phase = 0, sA = ring, bar = bars, tails = 0, tailPhase = 0;   // bit s: the last load of stage s counts on tailBar, and the phase of that
       bool whole = false;                                                    // every stage was loaded once
+      int at = 0;   // expert of the tile before
       for (int t = pair; t < tiles.count && !*abortFlag; t += pairs) {
-        const Tile c = tiles.at(t);
+        const Tile c = tiles.at(t, at);
+        at = c.e;
         const uint32_t mineA = bytesA(c, cr), mineB = bytesB(c, cr), both = bytesA(c, 0) + bytesA(c, 1) + bytesB(c, 0) + bytesB(c, 1);
         const int row = c.row0 + (int)cr * 128, col = firstB(c), end = c.steps * kBK;
         const int tailAt = MODE == EXPERT_DW && c.rows % kUmmaK != 0 ? end - kBK : -1;
@@ -652,8 +721,10 @@ expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       int s = 0, it = 0;
       uint32_t phase = 0;
       bool bad = false;
+      int at = 0;   // expert of the tile before
       for (int t = pair; t < tiles.count && !bad && !*abortFlag; t += pairs) {
-        const Tile c = tiles.at(t);
+        const Tile c = tiles.at(t, at);
+        at = c.e;
         if (c.steps == 0) continue;   // nothing to add up: the epilogue writes zeros
         const int buf = it & 1;
         if (!waitOr(smemAddr(&accEmpty[buf]), ((it >> 1) & 1) ^ 1, abortFlag)) { fail(2000 + buf); break; }
@@ -680,8 +751,10 @@ expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   } else if (warp < kFixWarp) {
     const int q = warp & 3, half = (warp - kFirstEpiWarp) >> 2;   // TMEM lanes [32q, 32q+32) belong to the warps with warp % 4 == q
     int it = 0;
+    int at = 0;   // expert of the tile before
     for (int t = pair; t < tiles.count && !__any_sync(~0u, *abortFlag); t += pairs) {
-      const Tile c = tiles.at(t);
+      const Tile c = tiles.at(t, at);
+      at = c.e;
       const int buf = it & 1;
       const int row = c.row0 + (int)cr * 128 + q * 32;
       const uint32_t tBase = tmemBase + ((uint32_t)(q * 32) << 16) + buf * kAccCols;
@@ -703,13 +776,15 @@ expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     }
   } else if (MODE == EXPERT_DW) {
     // rows behind the expert's last are somebody's old values: zeros up to the next sixteen, so that they add nothing (a row is 128 bytes of every box)
-    int at = 0;   // steps of the tiles before
+    int done = 0;   // steps of the tiles before
     uint32_t phases = 0;
+    int at = 0;   // expert of the tile before
     for (int t = pair; t < tiles.count && !__any_sync(~0u, *abortFlag); t += pairs) {
-      const Tile c = tiles.at(t);
+      const Tile c = tiles.at(t, at);
+      at = c.e;
       if (c.steps == 0) continue;
-      const int s = (at + c.steps - 1) % kPairStages, rows = (kUmmaK - c.rows % kUmmaK) % kUmmaK;
-      at = (at + c.steps) % kPairStages;
+      const int s = (done + c.steps - 1) % kPairStages, rows = (kUmmaK - c.rows % kUmmaK) % kUmmaK;
+      done = (done + c.steps) % kPairStages;
       if (rows == 0) continue;
       const uint32_t parity = phases >> s & 1;
       phases ^= 1u << s;

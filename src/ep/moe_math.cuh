@@ -53,28 +53,29 @@ __device__ __forceinline__ float activation(float v) {
   if (ACT == ACT_GELU) return v * normalCdf(v);
   return ACT == ACT_RELU && v < 0.0f ? 0.0f : v;   // (a NaN stays one)
 }
-// Of 32 values, times `up` of a gated layer (u): decided once, not for every value.
-__device__ __forceinline__ void activate32(int act, float (&v)[32], const float* u) {
+// Of N values, times `up` of a gated layer (u): decided once, not for every value.
+template <int N>
+__device__ __forceinline__ void activateAll(int act, float (&v)[N], const float (&u)[N]) {
   switch (act) {
     case ACT_RELU:
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = activation<ACT_RELU>(v[i]);
+      for (int i = 0; i < N; ++i) v[i] = activation<ACT_RELU>(v[i]);
       break;
     case ACT_GELU:
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = activation<ACT_GELU>(v[i]);
+      for (int i = 0; i < N; ++i) v[i] = activation<ACT_GELU>(v[i]);
       break;
     case ACT_SILU:
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = activation<ACT_SILU>(v[i]);
+      for (int i = 0; i < N; ++i) v[i] = activation<ACT_SILU>(v[i]);
       break;
     case ACT_SWIGLU:
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = activation<ACT_SILU>(v[i]) * u[i];
+      for (int i = 0; i < N; ++i) v[i] = activation<ACT_SILU>(v[i]) * u[i];
       break;
     case ACT_GEGLU:
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = activation<ACT_GELU>(v[i]) * u[i];
+      for (int i = 0; i < N; ++i) v[i] = activation<ACT_GELU>(v[i]) * u[i];
       break;
     default: break;
   }
