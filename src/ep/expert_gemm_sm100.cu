@@ -9,12 +9,12 @@
 // Two kernels. expertGemmPairKernel: CTA pairs (clusters of two, tcgen05 cta_group::2) on tiles of 256 rows x up to 256 columns; each CTA stages
 // its 128 rows of the first operand and its half of the second per 64 steps of the sum, and keeps the results of its rows. A CTA alone
 // would need 48 KiB where one of a pair needs 32, more than level 2 delivers while the tensor cores work on them (4 x 2048 rows, 4096 x 4096:
-// 1142 TFLOP/s). expertGemmKernel: one CTA per tile of 128 rows, where no expert can have more: there the weights are the traffic.
+// 1142 TFLOP/s; pairs 1530 to 1560). expertGemmKernel: one CTA per tile of 128 rows, where no expert can have more: there the weights are the traffic.
 //
 // Persistent CTAs, one per SM, in roles:
 //   warp 0      TMA producer: operand tiles (128-byte swizzle) through a ring in shared memory
 //   warp 1      MMA issuer (of a pair: the first CTA's) into one of two accumulators in tensor memory
-//   warps 2-9   epilogue, two warps to 32 rows: bias, activation, residual, rounding, stores of whole 128-byte lines
+//   warps 2-9   epilogue, two warps to 32 rows: bias, activation, residual, rounding, stores
 //   warp 10     DW: the last step of a sum may hold rows behind the expert's last; zeros are written over them in shared memory
 // Rows of the first operand that were not fetched, or lie behind the last, are whatever shared memory held: they reach only results that nobody stores.
 // Every wait is bounded; on expiry the kernel records a status, waits for its copies in flight, frees its tensor memory and returns.
@@ -275,7 +275,7 @@ __device__ __forceinline__ void storeRow16(__nv_bfloat16* to, const float (&v)[1
 
 // Epilogue of one warp for its 32 rows, `row` the first of them, and every other 32 columns of the tile: tBase is the tensor-memory address of the
 // warp's first lane and the tile's first column. A lane has a row of the accumulator and stores 16 of its columns at a time, whole sectors straight from
-// registers: shared memory is busy with the operands, and its room makes a seventh stage (32 experts of 64 rows, 4096 x 7168: 295 us through shared memory, 284 so).
+// registers: shared memory is busy with the operands, and its room makes a seventh stage (32 experts of 64 rows, 4096 x 7168: 295 us through shared memory, 285 so).
 template <int MODE, typename T, typename Ready>
 __device__ __forceinline__ bool storeTile(const ExpertGemmArgs& a, const T& tiles, const Tile& c, int row, uint32_t tBase, int half, int lane, Ready ready) {
   const int parts = tiles.parts, outCols = tiles.outCols;
@@ -292,14 +292,14 @@ __device__ __forceinline__ bool storeTile(const ExpertGemmArgs& a, const T& tile
       uint32_t r[32];
       tmemLd(tBase + cc, r);
       tmemLdReady(r);
-      if (!mine) continue;
 #pragma unroll
       for (int j = 0; j < 32; j += 16) {
         float v[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[j + i]);
-        if (cc + j < end) storeRow16((__nv_bfloat16*)a.out + at + cc + j, v, cc + j + 8 < end, a.wide);
+        if (mine && cc + j < end) storeRow16((__nv_bfloat16*)a.out + at + cc + j, v, cc + j + 8 < end, a.wide);
       }
+      __syncwarp();   // together again for the next load from tensor memory
     }
     return true;
   }
@@ -316,7 +316,10 @@ __device__ __forceinline__ bool storeTile(const ExpertGemmArgs& a, const T& tile
         const uint4 add[2] = {bias.at(part, cc), bias.at(part, cc + 8)};
         addBf16<16>(add, to);
       }
-      if (MODE == EXPERT_FORWARD && a.pre && mine) storeRow16((__nv_bfloat16*)a.pre + (at - c.col0) * parts + part * a.cols + c.col0 + cc, to, both, a.wide);
+      if (MODE == EXPERT_FORWARD && a.pre) {
+        if (mine) storeRow16((__nv_bfloat16*)a.pre + (at - c.col0) * parts + part * a.cols + c.col0 + cc, to, both, a.wide);
+        __syncwarp();
+      }
     };
     sums(0, v);
     if (MODE == EXPERT_FORWARD) {
@@ -329,6 +332,7 @@ __device__ __forceinline__ bool storeTile(const ExpertGemmArgs& a, const T& tile
       }
     }
     if (mine) storeRow16((__nv_bfloat16*)a.out + at + cc, v, both, a.wide);
+    __syncwarp();
   }
   return true;
 }

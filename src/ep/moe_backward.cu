@@ -18,7 +18,11 @@ __device__ __forceinline__ int rowsInUse(const int* counts, int e, int cap) { re
 
 // dz = dout * act'(z) for the rows in use of every expert; gated: d(gate) = dout * up * act'(gate) and d(up) = dout * act(gate). CTA (c, e, s) takes
 // columns [c * kActCols, ...) of expert e, a thread 8 neighbouring ones, and of each gridDim.z * 8 rows the 8 of slice s. The sums over a slice's rows stay
-// in registers and are joined in a fixed order: the bias gradient has the same bits every time.
+// in registers and are joined in a fixed order: the bias gradient has the same bits every time. Memory bounds it: 8 x 512 rows, 28672 columns, swiglu, 102 us
+// (5.7 TB/s).
+// Two roundings to bf16: z, as the forward call kept it (fp32 would double the largest tensor that a layer keeps), and dz, which the products
+// that follow take as a bf16 operand. With the rounding of their results the gradients are off by 0.0024 to 0.003 of their norm, with neither by 0.0017;
+// the bias gradient adds dz before its rounding where there is an activation.
 template <int ACT>
 __global__ void __launch_bounds__(kActThreads) expertActKernel(const __grid_constant__ ExpertActArgs a) {
   pdlEnter();
@@ -88,7 +92,7 @@ __global__ void __launch_bounds__(kActThreads) expertActKernel(const __grid_cons
   }
 }
 
-// dbias = bf16(the slices' sums, in order).
+// dbias = bf16(the slices' sums, in order). Short: 5 experts of 2200 columns 6 us under a profiler, most of them a launch's.
 __global__ void __launch_bounds__(kActThreads) expertBiasKernel(const __grid_constant__ ExpertActArgs a) {
   pdlEnter();
   const size_t n = (size_t)a.experts * a.cols * (a.act == ACT_SWIGLU || a.act == ACT_GEGLU ? 2 : 1);
@@ -115,7 +119,7 @@ const void* expertBiasKernelFn() { return (const void*)expertBiasKernel; }
 // ---------------------------------------------------------------------------------------------- combine's gradient
 // combine is out[t] = sum_k w[t,k] * y[row(t,k)], so dy[row] = w * dout[t] and dw[t,k] = <dout[t], y[row]>. One CTA per token: its
 // gradient is read once for all of the token's rows, KR rows are on their way together. The products' sums are joined lane by lane and warp by
-// warp, in the same order every time.
+// warp, in the same order every time. Memory bounds it: 4096 tokens of 8 rows of 7168, 168 us (5.9 TB/s).
 template <int KR>
 __global__ void __launch_bounds__(kMoeRowThreads) combineBackwardKernel(const __grid_constant__ MoeRowsArgs a) {
   pdlEnter();
@@ -184,7 +188,8 @@ const void* combineBackwardKernelFn(int topk) {
 }
 
 // ---------------------------------------------------------------------------------------------- dispatch's gradient
-// dispatch copies a token to a row of each of its experts, so dx[t] = sum_k dtoks[row(t,k)], in fp32 and in the order of the entries.
+// dispatch copies a token to a row of each of its experts, so dx[t] = sum_k dtoks[row(t,k)], in fp32 and in the order of the entries. Memory bounds it: 4096
+// tokens of 8 rows of 7168, 89 us (5.9 TB/s).
 __global__ void __launch_bounds__(kMoeRowThreads) dispatchBackwardKernel(const __grid_constant__ MoeRowsArgs a) {
   pdlEnter();
   constexpr int KR = 8;
