@@ -280,7 +280,7 @@ class ExpertParallel:
         return t
 
     def _route_cfg(self, *rule):
-        """Address of the configuration; the group keeps it."""
+        """The configuration, kept for the next call. Whoever hands its address on holds it until then: another thread may clear the store."""
         cfg = self._route_cfgs.get(rule)
         if cfg is None:
             score, groups, keep, group_score, renormalize, scale = rule
@@ -288,13 +288,15 @@ class ExpertParallel:
                 raise ValueError("score must be one of %s, not %r" % (", ".join(map(repr, self.SCORES)), score))
             if group_score not in self.GROUP_SCORES:
                 raise ValueError("group_score must be one of %s, not %r" % (", ".join(map(repr, self.GROUP_SCORES)), group_score))
+            if max(abs(groups), abs(keep)) >> 31:
+                raise ValueError("%r groups, %r kept" % (groups, keep))   # (the library refuses what 32 bits can say)
             cfg = _hdr(RouteCfg())
             cfg.score, cfg.groups, cfg.keep_groups, cfg.group_score = self.SCORES[score], groups, keep, self.GROUP_SCORES[group_score]
             cfg.renormalize, cfg.scale = int(bool(renormalize)), scale
             if len(self._route_cfgs) >= 64:
                 self._route_cfgs.clear()
             self._route_cfgs[rule] = cfg
-        return ctypes.addressof(cfg)
+        return cfg
 
     def _logits(self, logits):
         code, shape = self._logit_codes.get(logits.dtype), logits.shape
@@ -318,7 +320,7 @@ class ExpertParallel:
             self._need("bias", bias, f32, (self.E,))
         cfg = self._route_cfg(score, groups, groups if keep_groups is None else keep_groups, group_score, renormalize, scale)
         idx, weights = self._result("idx", idx, i64, (T, topk)), self._result("weights", weights, f32, (T, topk))
-        self._moe_call("ncclEpRoute", self.group, logits.data_ptr(), code, None if bias is None else bias.data_ptr(), idx.data_ptr(), weights.data_ptr(), T, self.E, topk, cfg)
+        self._moe_call("ncclEpRoute", self.group, logits.data_ptr(), code, None if bias is None else bias.data_ptr(), idx.data_ptr(), weights.data_ptr(), T, self.E, topk, ctypes.addressof(cfg))
         return idx, weights
 
     def route_backward(self, dweights, logits, idx, score="softmax", renormalize=True, scale=1.0, out=None):
@@ -330,7 +332,7 @@ class ExpertParallel:
         self._need("idx", idx, self.torch.int64, (logits.shape[0], topk))
         cfg = self._route_cfg(score, 1, 1, "max", renormalize, scale)
         out = self._result("out", out, logits.dtype, logits.shape)
-        self._moe_call("ncclEpRouteBackward", self.group, dweights.data_ptr(), logits.data_ptr(), code, idx.data_ptr(), out.data_ptr(), T, self.E, topk, cfg)
+        self._moe_call("ncclEpRouteBackward", self.group, dweights.data_ptr(), logits.data_ptr(), code, idx.data_ptr(), out.data_ptr(), T, self.E, topk, ctypes.addressof(cfg))
         return out
 
     def _linear(self, x, w, counts, activation):

@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kMoeRowThreads) combineBackwardKernel(const __
   constexpr int kWarps = kMoeRowThreads / 32;
   __shared__ float sums[kWarps][KR];
   const int packs = a.hidden / 8, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+  for (unsigned t = blockIdx.x; t < (unsigned)a.tokens; t += gridDim.x) {   // (signed, the last step may pass 2^31)
     const uint4* g4 = (const uint4*)a.dout + (size_t)t * packs;
     for (int k0 = 0; k0 < a.topk; k0 += KR) {
       int row[KR];
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kMoeRowThreads) dispatchBackwardKernel(const _
   pdlEnter();
   constexpr int KR = 8;
   const int packs = a.hidden / 8;
-  for (int t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+  for (unsigned t = blockIdx.x; t < (unsigned)a.tokens; t += gridDim.x) {   // (signed, the last step may pass 2^31)
     for (int p = threadIdx.x; p < packs; p += kMoeRowThreads) {
       float acc[8];
 #pragma unroll
@@ -228,13 +228,13 @@ const void* dispatchBackwardKernelFn() { return (const void*)dispatchBackwardKer
 // wrote none (unused entries, rows beyond the capacity): a word counts when its row is in use and names this entry as its source.
 __global__ void __launch_bounds__(kMoeRowThreads) dispatchRowsKernel(const __grid_constant__ DispatchRowsArgs a) {
   pdlEnter();
-  for (int i = blockIdx.x * kMoeRowThreads + threadIdx.x; i < a.entries; i += gridDim.x * kMoeRowThreads) {
+  for (size_t i = (size_t)blockIdx.x * kMoeRowThreads + threadIdx.x; i < a.entries; i += (size_t)gridDim.x * kMoeRowThreads) {
     const int64_t e = a.idx[i];
     const int row = a.rowOf[i];
     int got = -1;
     if (e >= 0 && e < a.experts && row / a.cap == (int)e && row - (int)e * a.cap < a.counts[e]) {
       const int2 from = a.srcInfo[row];
-      if (from.x == a.rank && from.y == i) got = row;
+      if (from.x == a.rank && from.y == (int)i) got = row;
     }
     a.rows[i] = got;
   }

@@ -93,7 +93,7 @@ static void dealLanes(RouteArgs* a, int kind, std::initializer_list<const void*>
 
 static ncclResult_t launchRoute(ncclEpGroup* g, const void* fn, RouteArgs* a, cudaStream_t stream) {
   void* args[1] = {a};
-  return launchMoe(g, fn, dim3((a->tokens + routeWarps() - 1) / routeWarps()), routeWarps() * 32, 0, args, stream);
+  return launchMoe(g, fn, dim3(((unsigned)a->tokens + routeWarps() - 1) / routeWarps()), routeWarps() * 32, 0, args, stream);
 }
 
 // ---------------------------------------------------------------- the experts' products
@@ -384,12 +384,12 @@ ncclResult_t ncclEpDispatchRows(ncclEpHandle_t h, int* rows, cudaStream_t stream
   a.srcInfo = h->srcInfo;
   a.counts = h->expertCount;
   a.rows = rows;
-  a.entries = h->T * h->K;
+  a.entries = (size_t)h->T * h->K;
   a.experts = g->E;
   a.cap = g->maxTokens;
   a.rank = g->comm->rank;
   void* args[1] = {&a};
-  return launchMoe(g, dispatchRowsKernelFn(), dim3(std::min((a.entries + kMoeRowThreads - 1) / kMoeRowThreads, g->smCount * 4)), kMoeRowThreads, 0, args, stream);
+  return launchMoe(g, dispatchRowsKernelFn(), dim3((unsigned)std::min<size_t>((a.entries + kMoeRowThreads - 1) / kMoeRowThreads, (size_t)g->smCount * 4)), kMoeRowThreads, 0, args, stream);
 }
 
 static ncclResult_t checkRows(const char* what, int tokens, int topk, int hidden, int numRows) {

@@ -94,7 +94,8 @@ struct DispatchRowsArgs {
   const int2* srcInfo;
   const int* counts;
   int* rows;
-  int entries, experts, cap, rank;
+  size_t entries;
+  int experts, cap, rank;
 };
 const void* dispatchRowsKernelFn();
 

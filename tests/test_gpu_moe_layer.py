@@ -202,6 +202,38 @@ def test_captured_layer(comm):
     other.destroy()
 
 
+def test_as_many_tokens_as_31_bits_count(comm):
+    """The last token and its neighbours, where steps of 32-bit counters pass their end."""
+    from nccl_b200.ops.ep import ExpertParallel
+    if torch.cuda.mem_get_info()[0] < 90 << 30:
+        pytest.skip("needs 90 GB")
+    ep, T = ExpertParallel(comm, 1, 4, 128), (1 << 31) - 1
+    ends = [0, 1, T // 2, T - 5000, T - 2, T - 1]
+    y = torch.arange(1, 33, device="cuda", dtype=torch.float32).bfloat16().view(4, 8)
+    rows = torch.full((T, 1), -1, device="cuda", dtype=torch.int32)
+    for i, t in enumerate(ends):
+        rows[t] = i % 4
+    dx = torch.ones(T, 8, device="cuda", dtype=torch.bfloat16)
+    ep.dispatch_backward(y, rows, out=dx)
+    for i, t in enumerate(ends):
+        assert torch.equal(dx[t], y[i % 4]), t
+        if 0 < t < T - 1:
+            assert not dx[t + 2 - (t == T - 2) * 4].any()
+    rows.fill_(-1)
+    rows[T - 1] = 2
+    weights, dweights, dy = torch.full((T, 1), 0.5, device="cuda"), torch.ones(T, 1, device="cuda"), torch.zeros_like(y)
+    ep.combine_backward(dx, y, weights, rows, dy=dy, dweights=dweights)
+    assert torch.equal(dy[2], dx[T - 1] / 2) and not dy[[0, 1, 3]].any()
+    assert dweights[T - 1].item() == (dx[T - 1].float() * y[2].float()).sum().item() and not dweights[[0, 1, T - 5000, T - 2]].any()
+    del dx, rows, weights, dweights
+    logits = torch.zeros(T, 1, device="cuda", dtype=torch.bfloat16)
+    logits[T - 2] = -math.inf
+    idx, w = ep.route(logits, 1)
+    assert idx[[0, T - 3, T - 2, T - 1], 0].tolist() == [0, 0, -1, 0] and w[[0, T - 3, T - 2, T - 1], 0].tolist() == [1, 1, 0, 1]
+    grad = ep.route_backward(w, logits, idx, score="sigmoid", renormalize=False, out=logits)
+    assert grad[[0, T - 3, T - 2, T - 1], 0].tolist() == [0.25, 0.25, 0.0, 0.25]
+
+
 def test_refusals(comm):
     from nccl_b200._lib import NcclError
     from nccl_b200.ops.ep import ExpertParallel

@@ -72,6 +72,32 @@ def test_route_refuses(ep):
     assert len(ep.calls) == 1
 
 
+def test_a_rule_in_use_outlives_the_store(ep):
+    """Another thread may clear the store of rules between a call's look into it and its launch."""
+    import weakref
+    result, kept = ep._result, []
+
+    def clearing(*args):
+        kept.extend(weakref.ref(c) for c in ep._route_cfgs.values())
+        ep._route_cfgs.clear()
+        return result(*args)
+
+    ep._result = clearing
+    alive = []
+    for name in ("ncclEpRoute", "ncclEpRouteBackward"):
+        ep._moe[name] = lambda *args: alive.append(kept[-1]() is not None) or 0
+    logits = torch.randn(5, 16)
+    idx, w = ep.route(logits, 3, scale=1.25)
+    ep.route_backward(w, logits, idx, scale=1.5)
+    assert alive == [True, True] and len(kept) == 2
+
+
+@pytest.mark.parametrize("kw", [dict(groups=1 + (1 << 32)), dict(groups=4, keep_groups=2 + (1 << 32)), dict(groups=1 - (1 << 32))])
+def test_numbers_of_groups_beyond_32_bits(ep, kw):
+    with pytest.raises(ValueError):
+        ep.route(torch.randn(5, 16), 2, **kw)
+
+
 def test_expert_linear_hands_over_and_refuses(ep):
     bf = dict(dtype=torch.bfloat16)
     x, w, c = torch.randn(2, 16, 32).bfloat16(), torch.randn(2, 48, 32).bfloat16(), torch.tensor([16, 3], dtype=torch.int32)
