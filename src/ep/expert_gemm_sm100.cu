@@ -13,7 +13,7 @@
 //
 // Persistent CTAs, one per SM, in roles:
 //   warp 0      TMA producer: operand tiles (128-byte swizzle) through a ring in shared memory
-//   warp 1      MMA issuer (of a pair: the first CTA's) into one of two accumulators in tensor memory
+//   warp 1      MMA issuer (of a pair: the first CTA's) into one of two accumulators in tensor memory; a pair's second: the bias's gradient from the slices' sums
 //   warps 2-9   epilogue, two warps to 32 rows: bias, activation, residual, rounding, stores
 //   warp 10     DW: the last step of a sum may hold rows behind the expert's last; zeros are written over them in shared memory
 // Rows of the first operand that were not fetched, or lie behind the last, are whatever shared memory held: they reach only results that nobody stores.
@@ -720,6 +720,7 @@ expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     }
     __syncwarp();
   } else if (warp == 1) {
+    if (MODE != EXPERT_FORWARD && !leader && a.partial) biasFromSlices(a.partial, (__nv_bfloat16*)a.dbias, a.sums, a.slices, (size_t)pair * 32 + lane, (size_t)pairs * 32);
     if (leader && electOne()) {
       const uint32_t idesc = umInstrBf16(256, bn) | (kAcrossA<MODE> ? 1u << 15 : 0u) | (kAcrossB<MODE> ? 1u << 16 : 0u);
       int s = 0, it = 0;

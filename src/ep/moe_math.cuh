@@ -101,4 +101,21 @@ __device__ __forceinline__ void activationAndSlope(float v, float* value, float*
   }
 }
 
+// dbias[i] = bf16(sum of partial[k][i] over the slices, in order): thread `at` of `threads`, four neighbouring sums at a time (n is a multiple of 8).
+__device__ __forceinline__ void biasFromSlices(const float* partial, __nv_bfloat16* dbias, size_t n, int slices, size_t at, size_t threads) {
+  for (size_t i = at * 4; i < n; i += threads * 4) {
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+    for (int k = 0; k < slices; ++k) {
+      const float4 v = *(const float4*)(partial + k * n + i);
+      s.x += v.x;
+      s.y += v.y;
+      s.z += v.z;
+      s.w += v.w;
+    }
+    __nv_bfloat162 out[2] = {__floats2bfloat162_rn(s.x, s.y), __floats2bfloat162_rn(s.z, s.w)};
+    *(uint2*)(dbias + i) = *(uint2*)out;
+  }
+}
+
 }  // namespace b200

@@ -51,6 +51,10 @@ struct ExpertGemmArgs {
   const void* residual;       // bf16, laid out like out, or null
   void* out;                  // bf16 [experts][cap or outRows][cols]
   void* pre;                  // bf16 [experts][cap][cols, twice when gated]: what the activation is applied to, or null
+  const float* partial;       // backward, on pairs: sums for the bias's gradient, [slices][sums], that a warp without other work adds up, or null
+  void* dbias;                // bf16 [sums]
+  size_t sums;                // a multiple of 8
+  int slices;
   uint32_t* status;           // {code, kind, what, CTA} of the communicator, written when a wait runs out
 };
 

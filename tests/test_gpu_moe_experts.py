@@ -263,6 +263,24 @@ def test_wanted_gradients_alone(ep):
     assert torch.equal(got[2], db)
 
 
+@pytest.mark.parametrize("E,cap,n,k,act,counts", [(3, 50, 72, 128, "silu", [50, 0, 20]), (3, 300, 2200, 8, "gelu", [300, 0, 129]), (2, 129, 16, 64, "swiglu", [1, 129]),
+                                                  (256, 20, 8, 8, None, [20, 0] * 128)])
+def test_bias_gradient_is_the_same_whatever_else_is_wanted(ep, E, cap, n, k, act, counts):
+    """A kernel of its own adds the slices up, or a warp of a product that follows: the same sums in the same order."""
+    x, w, b, _, dout, c = make(E, cap, n, k, act, 3, True, False, counts)
+    pre = torch.empty(E, cap, n, dtype=torch.bfloat16, device="cuda")
+    ep.expert_linear(x, w, c, bias=b, activation=act, pre=pre)
+    alone = ep.expert_linear_backward(dout, x, w, c, pre=pre, activation=act, need_dx=False, need_dw=False, need_dbias=True)[2]
+    for dx, dw in ((True, False), (False, True), (True, True)):
+        got = ep.expert_linear_backward(dout, x, w, c, pre=pre, activation=act, need_dx=dx, need_dw=dw, need_dbias=True, dbias=torch.full_like(alone, math.nan))
+        assert torch.equal(got[2], alone), (dx, dw)
+    bound, mass = 2.0 ** -8, 2.0 ** -24 * cap   # one rounding of the result; an addition a row, in fp32
+    if act is None:
+        for e, m in enumerate(counts):
+            rows = dout[e, :m].double()
+            assert within(alone[e], rows.sum(0), bound * rows.sum(0).abs() + mass * rows.abs().sum(0) * (1 + bound))
+
+
 def test_values_that_are_not_finite_stay_with_their_row(ep):
     x, w, _, _, _, c = make(2, 40, 64, 64, None, 1, False, False, [40, 40])
     want = ep.expert_linear(x, w, c)
