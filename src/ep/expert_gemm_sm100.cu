@@ -350,6 +350,7 @@ __device__ __forceinline__ bool storeTileStaged(const ExpertGemmArgs& a, const T
   if (MODE == EXPERT_FORWARD && a.bias) bias.load((const __nv_bfloat16*)a.bias + (size_t)c.e * parts * a.cols + c.col0, a.cols, parts, end, lane);
   auto chunk = [&](int r, int j) { return (uint4*)(wbuf + r * 128 + ((j ^ (r & 7)) * 16)); };
   const int mine = lane >> 3, j0 = lane & 7;   // of four rows, and of a row's eight chunks
+  const bool plain = a.act == ACT_NONE && !a.bias && !a.residual;
   uint4 residual[8];
   auto fetch = [&](int cc) {
     if (MODE != EXPERT_FORWARD || !a.residual) return;
@@ -398,7 +399,7 @@ __device__ __forceinline__ bool storeTileStaged(const ExpertGemmArgs& a, const T
       __syncwarp();
       fetch(cc + 128);
     }
-    if (MODE == EXPERT_FORWARD) {
+    if (MODE == EXPERT_FORWARD && !plain) {
 #pragma unroll 1
       for (int at = 0; at < width; at += 8) {
         float v[8], u[8];
@@ -411,7 +412,7 @@ __device__ __forceinline__ bool storeTileStaged(const ExpertGemmArgs& a, const T
         }
         *chunk(lane, at / 8) = packBf16x8(v);
       }
-    } else {
+    } else {   // the sums as they are: 32 at a time
 #pragma unroll
       for (int at = 0; at < 64; at += 32) {
         if (at >= width) break;
