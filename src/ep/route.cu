@@ -9,7 +9,7 @@
 // One warp per token. Its lanes are dealt out to the groups (as many to each, a power of two), and a lane holds up to V neighbouring experts of its group in
 // registers: the lowest lane of equal ones has the lowest index, and a group's score is a butterfly over its lanes. A pass of the selection is a
 // maximum over the lane's values as ordered words, one redux over the warp's and a ballot. Its instructions bound it (8192 tokens of 256 experts: 6.6 us by
-// bf16 logits alone, 12.4 with a bias, 14.5 in 8 groups too, 1100 instructions of a warp for each, of which the bytes would take 0.8; occupancies from 24 to 64 warps per SM made no difference).
+// bf16 logits alone, 12.4 with a bias, 14.5 in 8 groups too, 1100 instructions of a warp for each token; the bytes would take 0.8; occupancies from 24 to 64 warps per SM made no difference).
 //
 // What is chosen is what the formulas say in exact arithmetic, not what fp32 makes of them: without a bias experts are ranked by their
 // logits, which order them as the scores do; where rounded values decide (bias, sums of two scores) and two that matter are nearer
