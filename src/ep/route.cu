@@ -189,9 +189,10 @@ struct Heads<Key, V, UNIQUE, false> {
 
 // Whether the order of two rank values (or sums of two) may be another one than that of the exact values. The short exponential is off by
 // (2 + 1.2 |x|) 2^-23 of itself and the division by 2^-22: of a sigmoid that is s (1 - s) (2 + 1.2 |l|) 2^-23 + 2^-22 s < 2^-21, of a softmax share, e^x / sum with
-// e^x (2 + 1.2 |x|) <= 2 and a sum that is as exact, about as much. Differences of two of them, or of sums of two, are off by 2^-19; half a unit of
-// rounding to the value itself is added where the bias is large.
-__device__ __forceinline__ bool near(float above, float below) { return above - below <= 0x1p-19f + 0x1p-21f * fabsf(above); }
+// e^x (2 + 1.2 |x|) <= 2 and a sum that is as exact, about as much. Differences of two of them, or of sums of two, are off by 2^-19. Adding the bias and the second
+// value rounds by half a unit each: 2^-21 of `size`, the largest sum of magnitudes on either side, holds all of it. (Not of the value itself: two that cancel leave little of it, and all of their
+// rounding.)
+__device__ __forceinline__ bool near(float above, float below, float size) { return above - below <= 0x1p-19f + 0x1p-21f * size; }
 
 // The token's experts (entry k in lane k, -1 = none). R = float: *sure says whether rounding may have decided.
 template <typename R, typename T, int V>
@@ -270,9 +271,10 @@ __device__ __forceinline__ int chooseExperts(const RouteArgs& a, const T* row, c
     mine = group < a.groups && ahead < a.keep;
     if (!kExact && scores) {
       const bool real = group < a.groups;
-      const float last = (float)__shfl_sync(kAll, score, __ffs(__ballot_sync(kAll, real && ahead == a.keep - 1)) - 1);
-      const float next = (float)__shfl_sync(kAll, score, __ffs(__ballot_sync(kAll, real && ahead == a.keep)) - 1);
-      if (near(last, next)) *sure = false;
+      const int lastLane = __ffs(__ballot_sync(kAll, real && ahead == a.keep - 1)) - 1, nextLane = __ffs(__ballot_sync(kAll, real && ahead == a.keep)) - 1;
+      const float last = (float)__shfl_sync(kAll, score, lastLane), next = (float)__shfl_sync(kAll, score, nextLane);
+      const float size = !(one > (R)-INFINITY) ? 0.0f : fabsf((float)one) + (sums && two > (R)-INFINITY ? fabsf((float)two) : 0.0f);   // (0: no expert)
+      if (near(last, next, fmaxf(__shfl_sync(kAll, size, lastLane), __shfl_sync(kAll, size, nextLane)))) *sure = false;
     }
   }
   if constexpr (sizeof(T) == 2 && !kExact) {
@@ -319,7 +321,7 @@ __device__ __forceinline__ int chooseExperts(const RouteArgs& a, const T* row, c
     // two next to each other that are too near; equal logits and biases have equal values in exact arithmetic too, and the lower index came first
     const float own = fromOrdered((uint32_t)value), above = __shfl_up_sync(kAll, own, 1);
     const int other = __shfl_up_sync(kAll, taken, 1);
-    const bool doubt = lane > 0 && taken >= 0 && near(above, own) && !(cleanLogit(toFloat<T>(row[taken])) == cleanLogit(toFloat<T>(row[other])) && a.bias[taken] == a.bias[other]);
+    const bool doubt = lane > 0 && taken >= 0 && near(above, own, fabsf(above)) && !(cleanLogit(toFloat<T>(row[taken])) == cleanLogit(toFloat<T>(row[other])) && a.bias[taken] == a.bias[other]);
     if (__any_sync(kAll, doubt)) *sure = false;
     if (lane >= a.topk) taken = -1;
   }
