@@ -191,8 +191,8 @@ struct Heads<Key, V, UNIQUE, false> {
 // (2 + 1.2 |x|) 2^-23 of itself and the division by 2^-22: of a sigmoid that is s (1 - s) (2 + 1.2 |l|) 2^-23 + 2^-22 s < 2^-21, of a softmax share, e^x / sum with
 // e^x (2 + 1.2 |x|) <= 2 and a sum that is as exact, about as much. Differences of two of them, or of sums of two, are off by 2^-19. Adding the bias and the second
 // value rounds by half a unit each: 2^-21 of `size`, the largest sum of magnitudes on either side, holds all of it. (Not of the value itself: two that cancel leave little of it, and all of their
-// rounding.)
-__device__ __forceinline__ bool near(float above, float below, float size) { return above - below <= 0x1p-19f + 0x1p-21f * size; }
+// rounding.) Infinite values, as sums beyond fp32 are, and a size beyond fp32 are near to everything.
+__device__ __forceinline__ bool near(float above, float below, float size) { return !(above - below > 0x1p-19f + 0x1p-21f * size); }
 
 // The token's experts (entry k in lane k, -1 = none). R = float: *sure says whether rounding may have decided.
 template <typename R, typename T, int V>
@@ -274,7 +274,8 @@ __device__ __forceinline__ int chooseExperts(const RouteArgs& a, const T* row, c
       const int lastLane = __ffs(__ballot_sync(kAll, real && ahead == a.keep - 1)) - 1, nextLane = __ffs(__ballot_sync(kAll, real && ahead == a.keep)) - 1;
       const float last = (float)__shfl_sync(kAll, score, lastLane), next = (float)__shfl_sync(kAll, score, nextLane);
       const float size = !(one > (R)-INFINITY) ? 0.0f : fabsf((float)one) + (sums && two > (R)-INFINITY ? fabsf((float)two) : 0.0f);   // (0: no expert)
-      if (near(last, next, fmaxf(__shfl_sync(kAll, size, lastLane), __shfl_sync(kAll, size, nextLane)))) *sure = false;
+      const float larger = fmaxf(__shfl_sync(kAll, size, lastLane), __shfl_sync(kAll, size, nextLane));
+      if (near(last, next, larger) && (last > -INFINITY || larger > 0.0f)) *sure = false;   // (of groups without experts the lower ones stay)
     }
   }
   if constexpr (sizeof(T) == 2 && !kExact) {

@@ -111,3 +111,17 @@ def test_groups_next_to_each_other(group, E, groups, size, score, top2):
     topk = 2 if per > 1 else 1
     want = chosen(logits, bias, score, groups, 1, top2, topk)
     same(group(E), logits, bias, want, topk, score=score, groups=groups, keep_groups=1, group_score="top2" if top2 else "max")
+
+
+def test_sums_beyond_fp32(group):
+    """Two groups whose sums fp32 has no numbers for, above and below; a group without experts is behind both, however low they are."""
+    ep = group(4)
+    logits = torch.zeros(2, 4)
+    rule = dict(score="sigmoid", groups=2, keep_groups=1, group_score="top2")
+    same(ep, logits, torch.tensor([3.0e38, 2.0e38, 3.1e38, 3.0e38]), torch.tensor([[2, 3]] * 2), 2, **rule)
+    same(ep, logits, torch.tensor([3.1e38, 3.0e38, 3.0e38, 2.0e38]), torch.tensor([[0, 1]] * 2), 2, **rule)
+    same(ep, logits, torch.tensor([-3.1e38, -3.0e38, -3.0e38, -2.0e38]), torch.tensor([[3, 2]] * 2), 2, **rule)
+    logits[0, :2] = -math.inf      # token 0 has no expert in group 0, token 1 none at all
+    logits[1] = -math.inf
+    same(ep, logits, torch.tensor([-3.1e38, -3.0e38, -3.0e38, -2.0e38]), torch.tensor([[3, 2], [-1, -1]]), 2, **rule)
+    same(ep, logits, torch.tensor([1.0, 1.0, -3.0e38, -2.0e38]), torch.tensor([[3, 2], [-1, -1]]), 2, **rule)
