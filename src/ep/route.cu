@@ -69,6 +69,12 @@ __device__ __forceinline__ void loadLogits(const T* row, const Share& my, bool w
   }
 }
 
+// The sum of a lane's values as a tree: six additions in a row for 64 of them, where one after the other would round 63 times.
+template <int FROM, int N, typename R, int V>
+__device__ __forceinline__ R treeSum(const R (&v)[V]) {
+  if constexpr (N == 1) return v[FROM];
+  else return treeSum<FROM, N / 2>(v) + treeSum<FROM + N / 2, N / 2>(v);
+}
 __device__ __forceinline__ float warpSum(float v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
@@ -187,9 +193,11 @@ struct Heads<Key, V, UNIQUE, false> {
   }
 };
 
-// Whether the order of two rank values (or sums of two) may be another one than that of the exact values. The short exponential is off by
-// (2 + 1.2 |x|) 2^-23 of itself and the division by 2^-22: of a sigmoid that is s (1 - s) (2 + 1.2 |l|) 2^-23 + 2^-22 s < 2^-21, of a softmax share, e^x / sum with
-// e^x (2 + 1.2 |x|) <= 2 and a sum that is as exact, about as much. Differences of two of them, or of sums of two, are off by 2^-19. Adding the bias and the second
+// Whether the order of two rank values (or sums of two) may be another one than that of the exact values. In units of u = 2^-23 the short exponential of x is off by
+// 2 + 1.2 |x| of itself, its argument's rounding adds 0.5 |x|, the division 2. Of a sigmoid that is s (1 - s) (2 + 1.2 |l|) + 2 s < 4. Of softmax shares p = e^x / sum, of
+// which up to four are compared: sum of p (2 + 1.7 |x|) < 3 for themselves, as much and the same over all other experts (at most 1.7 * 1.9, where those have half of the sum) for the
+// denominator's terms, 5.5 for adding it up (trees of six additions in a lane and five over the warp) and 2 for the division, less than 14 in all. So differences of two values, or of sums
+// of two, are off by less than 16 u = 2^-19. Adding the bias and the second
 // value rounds by half a unit each: 2^-21 of `size`, the largest sum of magnitudes on either side, holds all of it. (Not of the value itself: two that cancel leave little of it, and all of their
 // rounding.) Infinite values, as sums beyond fp32 are, and a size beyond fp32 are near to everything.
 __device__ __forceinline__ bool near(float above, float below, float size) { return !(above - below > 0x1p-19f + 0x1p-21f * size); }
@@ -214,13 +222,9 @@ __device__ __forceinline__ int chooseExperts(const RouteArgs& a, const T* row, c
 #pragma unroll
       for (int j = 1; j < V; ++j) top = (R)l[j] > top ? (R)l[j] : top;
       top = warpMax(top);
-      R sum = 0;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        v[j] = l[j] > -INFINITY ? rankExp((R)l[j] - top) : (R)0;
-        sum += v[j];
-      }
-      sum = warpSum(sum);
+      for (int j = 0; j < V; ++j) v[j] = l[j] > -INFINITY ? rankExp((R)l[j] - top) : (R)0;
+      const R sum = warpSum(treeSum<0, V>(v));
 #pragma unroll
       for (int j = 0; j < V; ++j) v[j] = rankDivide(v[j], sum);   // (a token without experts: taken out below)
     }

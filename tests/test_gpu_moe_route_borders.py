@@ -125,3 +125,28 @@ def test_sums_beyond_fp32(group):
     logits[1] = -math.inf
     same(ep, logits, torch.tensor([-3.1e38, -3.0e38, -3.0e38, -2.0e38]), torch.tensor([[3, 2], [-1, -1]]), 2, **rule)
     same(ep, logits, torch.tensor([1.0, 1.0, -3.0e38, -2.0e38]), torch.tensor([[3, 2], [-1, -1]]), 2, **rule)
+
+
+@pytest.mark.parametrize("E,groups,keep", [(1020, 17, 16), (1020, 1, 1), (240, 1, 1), (32, 1, 1)])
+def test_shares_of_many_experts(group, E, groups, keep):
+    """One large share and many that fp32 loses one by one beside it: the large one's rank value is next to another's."""
+    T = 800
+    g = torch.Generator().manual_seed(E)
+    logits = torch.full((T, E), -16.7, dtype=torch.float64)
+    bias = (-0.5 - torch.arange(E) // (E // groups) / 128).double()   # groups and experts further apart than what is looked at
+    bias[0], bias[E - 1] = 0.0, float(torch.tensor(1 - 5.6e-8 * E, dtype=torch.float32))
+    delta = 4e-6 * (2 * torch.rand(T, generator=g).double() - 1)
+
+    def difference(l):
+        v = torch.softmax(l, 1) + bias
+        return v[:, 0] - v[:, E - 1] - delta
+
+    # (the share itself moves by no more than 1: where that does not reach, the two are as near as it gets)
+    logits = solve(logits, 0, difference, -3.0, 3.0).double()
+    want = chosen(logits, bias, "softmax", groups, keep, False, 3)[:, :2]
+    idx, _ = group(E).route(logits.float().cuda(), 2, score="softmax", bias=bias.float().cuda(), groups=groups, keep_groups=keep)
+    v = torch.softmax(logits, 1) + bias
+    apart = (v[:, 0] - v[:, E - 1]).abs()
+    assert ((apart < 1e-5) & (apart > 0)).sum() > T // 2
+    far = (idx.cpu() != want).any(1)
+    assert not far.any(), (int(far.sum()), float(apart[far].max()))
