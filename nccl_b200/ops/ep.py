@@ -396,7 +396,7 @@ class ExpertParallel:
     def dispatch_rows(self, rows=None):
         """int32 [tokens, topk]: the row of the dispatched tensor (as [experts * capacity, hidden]) that holds each entry of the last ``dispatch``, -1
         for entries without an expert. Groups of one rank with the expert-major layout; the next dispatch moves the rows."""
-        if self.handle is None:
+        if self.handle is None or self._keep is None:
             raise ValueError("nothing has been dispatched yet")
         idx = self._keep[1]
         rows = self._result("rows", rows, self.torch.int32, tuple(idx.shape))

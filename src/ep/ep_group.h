@@ -37,6 +37,10 @@ struct ncclEpHandle {
   int outSlots = 0;                   // flat layout: rows of the last dispatch's outputs
   const int64_t* topkIdx = nullptr;
   const float* topkW = nullptr;
+  // routing of the last dispatch that was carried out (the two above may be those of one that was refused, or not made yet); null: none, or
+  // its rows were given up half-way
+  const int64_t* sentIdx = nullptr;
+  int sentT = 0;
   int2* srcInfo = nullptr;
   int* rowOf = nullptr;               // one-rank groups, expert-major: where (token, k) went
   int* expertCount = nullptr;

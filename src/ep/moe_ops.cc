@@ -385,17 +385,17 @@ ncclResult_t ncclEpDispatchRows(ncclEpHandle_t h, int* rows, cudaStream_t stream
   if (!h) return ncclInvalidArgument;
   ncclEpGroup* g = h->g;
   if (!h->rowOf) { WARN("ncclEpDispatchRows: needs a group of one rank and the expert-major layout"); return ncclInvalidUsage; }
-  if (!h->topkIdx || h->pending) { WARN("ncclEpDispatchRows: no dispatch has been completed on this handle"); return ncclInvalidUsage; }
-  if (h->T == 0) return ncclSuccess;
+  if (!h->sentIdx || h->pending) { WARN("ncclEpDispatchRows: no dispatch has been completed on this handle"); return ncclInvalidUsage; }
+  if (h->sentT == 0) return ncclSuccess;
   if (!rows || !aligned({rows}, 4)) return ncclInvalidArgument;
   B200_ON_DEVICE(g);
   DispatchRowsArgs a;
-  a.idx = h->topkIdx;
+  a.idx = h->sentIdx;
   a.rowOf = h->rowOf;
   a.srcInfo = h->srcInfo;
   a.counts = h->expertCount;
   a.rows = rows;
-  a.entries = (size_t)h->T * h->K;
+  a.entries = (size_t)h->sentT * h->K;
   a.experts = g->E;
   a.cap = g->maxTokens;
   a.rank = g->comm->rank;

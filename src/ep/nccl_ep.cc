@@ -371,6 +371,8 @@ ncclResult_t ncclEpDispatch(ncclEpHandle_t h, const ncclEpDispatchInputs_t* in, 
   const bool sendOnly = config && config->send_only;
   if (sendOnly) a.phases = 1;
   void* counters = (li && li->expert_counters && li->expert_counters->data) ? li->expert_counters->data : nullptr;
+  h->sentIdx = nullptr;   // whatever happens from here on, the rows of the dispatch before are gone
+  h->sentT = h->T;
   const size_t T = (size_t)h->T, K = (size_t)h->K, rows = a.layout == EP_EXPERT_MAJOR ? g->El * cap : cap;
   if (localForm(g, a.layout, sendOnly) && (uintptr_t)in->tokens->data % 16 == 0 &&   // the general kernel quantises from 8-byte loads
       (!counters || onThisGpu(counters, g->comm->cudaDev)) &&
@@ -379,7 +381,9 @@ ncclResult_t ncclEpDispatch(ncclEpHandle_t h, const ncclEpDispatchInputs_t* in, 
                {{a.x[me], T * g->H * 2}, {a.topkIdx[me], T * K * sizeof(int64_t)}, {a.topkW[me], T * K * sizeof(float)}})) {
     a.userCount = (int*)counters;
     const bool wide = !(((uintptr_t)a.x[me] | (uintptr_t)a.outTokens[me]) & 31);   // rows are whole multiples of 128 bytes
-    return launchEpLocal(g, epDispatchLocalKernelFn(fp8, wide), &a, std::max(h->T, a.layout == EP_RANK_MAJOR ? (g->maxTokens + kEpLocalThreads - 1) / kEpLocalThreads : 1), stream);
+    NCCLCHECK(launchEpLocal(g, epDispatchLocalKernelFn(fp8, wide), &a, std::max(h->T, a.layout == EP_RANK_MAJOR ? (g->maxTokens + kEpLocalThreads - 1) / kEpLocalThreads : 1), stream));
+    h->sentIdx = h->topkIdx;
+    return ncclSuccess;
   }
   // the per-rank layouts count the tokens of every local expert with atomics while they unpack: start from zero
   if (a.layout != EP_EXPERT_MAJOR && !sendOnly) CUDACHECK(cudaMemsetAsync(h->expertCount, 0, (size_t)g->El * sizeof(int), stream));
@@ -393,9 +397,11 @@ ncclResult_t ncclEpDispatch(ncclEpHandle_t h, const ncclEpDispatchInputs_t* in, 
     h->pendingCtas = ctas;
     h->pendingSmem = dispatchSmem(g->H, fp8, a.bulkStages);
     h->pendingCounters = counters;
+    h->sentIdx = h->topkIdx;
     return ncclSuccess;
   }
   if (counters) CUDACHECK(cudaMemcpyAsync(counters, h->expertCount, (size_t)g->El * sizeof(int), cudaMemcpyDeviceToDevice, stream));
+  h->sentIdx = h->topkIdx;
   return ncclSuccess;
 }
 
