@@ -385,7 +385,8 @@ ncclResult_t ncclEpDispatchRows(ncclEpHandle_t h, int* rows, cudaStream_t stream
   if (!h) return ncclInvalidArgument;
   ncclEpGroup* g = h->g;
   if (!h->rowOf) { WARN("ncclEpDispatchRows: needs a group of one rank and the expert-major layout"); return ncclInvalidUsage; }
-  if (!h->sentIdx || h->pending) { WARN("ncclEpDispatchRows: no dispatch has been completed on this handle"); return ncclInvalidUsage; }
+  // (a combine that waits for its other half does not touch the rows)
+  if (!h->sentIdx || h->pending == 1) { WARN("ncclEpDispatchRows: no dispatch has been completed on this handle"); return ncclInvalidUsage; }
   if (h->sentT == 0) return ncclSuccess;
   if (!rows || !aligned({rows}, 4)) return ncclInvalidArgument;
   B200_ON_DEVICE(g);

@@ -58,3 +58,16 @@ def test_no_rows_after_nothing_but_a_refusal(ep):
     assert (rows == 77).all()
     toks, _, _ = ep.dispatch(x, idx, w, fp8=False)
     assert good(ep.dispatch_rows(), toks, x, idx)
+
+
+def test_rows_while_a_combine_is_on_its_way(ep):
+    x, idx, w = inputs(5)
+    toks, _, _ = ep.dispatch(x, idx, w, fp8=False)
+    before = ep.dispatch_rows()
+    out = ep.combine(toks.clone(), send_only=True)
+    rows = ep.dispatch_rows()
+    ep.complete()
+    assert torch.equal(rows, before) and good(rows, toks, x, idx)
+    # the token itself times the sum of its weights: three roundings of fp32 and one to bf16
+    want = x.double() * w.double().sum(1, keepdim=True)
+    assert ((out.double() - want).abs() <= (2.0 ** -8 + 4 * 2.0 ** -24) * want.abs()).all()
