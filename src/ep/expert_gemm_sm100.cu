@@ -54,10 +54,11 @@ __device__ __forceinline__ void tmaLoad3dPair(uint32_t dstSmem, const CUtensorMa
       ::"r"(dstSmem), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(barCluster) : "memory");
 }
 
-// Waits of the roles: they end early when another role has given up. The flag is looked at where there is something to wait for, not in every step.
-__device__ __forceinline__ bool waitOr(uint32_t bar, uint32_t parity, volatile uint32_t* abortFlag) {
+// Waits of the roles: they end early when another role has given up. The flag is looked at where there is something to wait for, not in every step. `waits`: how
+// many waits of the other roles this one may span.
+__device__ __forceinline__ bool waitOr(uint32_t bar, uint32_t parity, volatile uint32_t* abortFlag, uint32_t waits = 1) {
   if (mbarTry(bar, parity)) return true;
-  for (uint32_t i = 0; i < (1u << 24) && !*abortFlag; ++i)
+  for (uint64_t i = 0; i < (uint64_t)waits << 24 && !*abortFlag; ++i)
     if (mbarTry(bar, parity)) return true;
   return false;
 }
@@ -81,9 +82,9 @@ __device__ __forceinline__ bool warpWaitOr(uint32_t bar, uint32_t parity, volati
 __device__ __forceinline__ void mbarArriveRelaxed(uint32_t clusterAddr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(clusterAddr) : "memory");
 }
-// As mbarWait, for what the other CTA of the pair wrote before it arrived.
-__device__ __forceinline__ bool mbarWaitCluster(uint32_t bar, uint32_t parity, uint32_t limit = 1u << 24) {
-  for (uint32_t i = 0; i < limit; ++i) {
+// As waitOr, for what the other CTA of the pair wrote before it arrived.
+__device__ __forceinline__ bool waitClusterOr(uint32_t bar, uint32_t parity, volatile uint32_t* abortFlag) {
+  for (uint32_t i = 0; i < 1u << 24; ++i) {
     uint32_t ok;
     asm volatile(
         "{\n.reg .pred p;\n"
@@ -91,6 +92,7 @@ __device__ __forceinline__ bool mbarWaitCluster(uint32_t bar, uint32_t parity, u
         "selp.u32 %0, 1, 0, p;\n}"
         : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     if (ok) return true;
+    if (*abortFlag) break;
   }
   return false;
 }
@@ -783,7 +785,7 @@ expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   } else if (MODE == EXPERT_DW) {
     // rows behind the expert's last are somebody's old values: zeros up to the next sixteen, so that they add nothing (a row is 128 bytes of every box)
     int done = 0;   // steps of the tiles before
-    uint32_t phases = 0;
+    uint32_t phases = 0, since = 1;   // tiles since the last one that had such rows
     int at = 0;   // expert of the tile before
     for (int t = pair; t < tiles.count && !__any_sync(~0u, *abortFlag); t += pairs) {
       const Tile c = tiles.at(t, at);
@@ -791,10 +793,15 @@ expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       if (c.steps == 0) continue;
       const int s = (done + c.steps - 1) % kPairStages, rows = (kUmmaK - c.rows % kUmmaK) % kUmmaK;
       done = (done + c.steps) % kPairStages;
-      if (rows == 0) continue;
+      if (rows == 0) {
+        ++since;
+        continue;
+      }
       const uint32_t parity = phases >> s & 1;
       phases ^= 1u << s;
-      if (!__all_sync(~0u, mbarWait(smemAddr(&tailBar[s]), parity))) { if (lane == 0) fail(5000 + s); break; }
+      // (all lanes ask: a step waits for this warp, and one lane that tells the others costs 32 experts of 61 rows, 4096 x 7168, 4 %)
+      if (!__all_sync(~0u, waitOr(smemAddr(&tailBar[s]), parity, abortFlag, since))) { if (lane == 0) fail(5000 + s); break; }
+      since = 1;
       const int from = c.rows - (c.steps - 1) * kBK;
       for (int i = lane; i < 4 * rows * 8; i += 32) {
         const int box = i / (rows * 8), r = i / 8 % rows;
@@ -805,7 +812,7 @@ expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       if (!leader) {
         if (lane == 0) mbarArriveCluster(mapaShared(smemAddr(&fixBar[s]), 0));
       } else {
-        if (!__all_sync(~0u, mbarWaitCluster(smemAddr(&fixBar[s]), parity))) { if (lane == 0) fail(6000 + s); break; }
+        if (!__all_sync(~0u, waitClusterOr(smemAddr(&fixBar[s]), parity, abortFlag))) { if (lane == 0) fail(6000 + s); break; }
         if (lane == 0) mbarArrive(smemAddr(&fullBar[s]));
       }
     }
