@@ -43,3 +43,23 @@ def test_weight_gradients_of_experts_of_which_few_end_inside_a_step(ep, counts):
         d, xe = dout[e, :m].double(), x[e, :m].double()
         ref, far = d.T @ xe, m * U32 * (d.abs().T @ xe.abs())
         assert ((dw[e].double() - ref).abs() <= far + HALF * (ref.abs() + far)).all(), e
+
+
+# columns that end at every eight of a lane's steps and of the tiles, on single CTAs and on pairs (with `pre` and few tiles results go straight from registers)
+@pytest.mark.parametrize("n", [8, 16, 24, 40, 64, 72, 88, 104, 136, 248, 264, 296])
+@pytest.mark.parametrize("cap,counts", [(70, [70, 3, 33]), (300, [300, 129, 1])])
+def test_residual_in_the_results_place(ep, n, cap, counts):
+    E, k = len(counts), 72
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn(E, cap, k, device="cuda", generator=g).bfloat16()
+    w = (torch.randn(E, n, k, device="cuda", generator=g) / math.sqrt(k)).bfloat16()
+    r = torch.randn(E, cap, n, device="cuda", generator=g).bfloat16()
+    c = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    for e, m in enumerate(counts):
+        r[e, m:] = 77.0
+    out, pre = r.clone(), torch.empty_like(r)
+    assert ep.expert_linear(x, w, c, residual=out, out=out, pre=pre) is out
+    for e, m in enumerate(counts):
+        z, far = x[e, :m].double() @ w[e].double().T, k * U32 * (x[e, :m].double().abs() @ w[e].double().abs().T)
+        v = z + r[e, :m].double()
+        assert ((out[e, :m].double() - v).abs() <= far + U32 * v.abs() + HALF * (v.abs() + far)).all() and (out[e, m:] == 77.0).all()
