@@ -97,6 +97,13 @@ __device__ __forceinline__ bool waitClusterOr(uint32_t bar, uint32_t parity, vol
   return false;
 }
 
+// After one of the roles has given up: copies that count on a barrier of the other CTA, and products whose end nobody waited for, may still be on
+// their way into memory that this CTA is about to leave. No barrier here shows their end, so they get a millisecond, hundreds of times what they take.
+__device__ __noinline__ void letThemLand() {
+  const uint64_t from = globalTimerNs();
+  for (int i = 0; i < 1 << 16 && globalTimerNs() - from < 1000000; ++i) __nanosleep(1000);
+}
+
 // An operand that lies across the sum, in boxes of 64 values x 64 steps with 128-byte swizzle: the next 64 values are a box further, the
 // next 8 steps 1024 bytes.
 __device__ __forceinline__ uint64_t descAcross(uint32_t smemByteAddr) {
@@ -592,6 +599,7 @@ expertGemmKernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 
   tcFenceBefore();
   __syncthreads();
+  if (*abortFlag) letThemLand();
   if (warp == 1) {
     tcFenceAfter();
     tmemDealloc(tmemBase, kTmemCols);
@@ -831,6 +839,7 @@ expertGemmPairKernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   // the pair meets: nobody touches the partner's shared or tensor memory afterwards
   tcFenceBefore();
   __syncthreads();
+  if (*abortFlag) letThemLand();
   __syncwarp();
   clusterSync();
   if (warp == 1) {
