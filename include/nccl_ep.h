@@ -130,12 +130,13 @@ ncclResult_t ncclEpRouteBackward(ncclEpGroup_t ep_group, const float* d_weights,
  * x [experts, rows, k], w [experts, n, k], bias [experts, n], out and residual [experts, rows, n], all bf16; n and k are multiples of 8.
  * The gated activations take w as [gate rows | up rows] (n a multiple of 16) and give silu(gate) * up or gelu(gate) * up: out and residual have n / 2
  * columns. counts: int32 on the device, null: all rows. Rows behind an expert's last are neither read into a result nor written.
- * bias, residual and pre may be null; pre [experts, rows, n] gets x w^T + bias for the backward pass. residual may be out. At most 256 experts,
- * and 2^24 rows, n and k. */
-typedef enum { NCCL_EP_ACT_NONE = 0, NCCL_EP_ACT_RELU = 1, NCCL_EP_ACT_GELU = 2, NCCL_EP_ACT_SILU = 3, NCCL_EP_ACT_SWIGLU = 4, NCCL_EP_ACT_GEGLU = 5 } ncclEpActivation_t;
+ * bias, residual and pre may be null; pre [experts, rows, n] gets x w^T + bias for the backward pass, in bf16, or in fp32 where
+ * NCCL_EP_ACT_PRE_FP32 is added to the activation (gradients are then as exact as one rounding of the activation's gradient to bf16 leaves them).
+ * residual may be out. At most 256 experts, and 2^24 rows, n and k. */
+typedef enum { NCCL_EP_ACT_NONE = 0, NCCL_EP_ACT_RELU = 1, NCCL_EP_ACT_GELU = 2, NCCL_EP_ACT_SILU = 3, NCCL_EP_ACT_SWIGLU = 4, NCCL_EP_ACT_GEGLU = 5, NCCL_EP_ACT_PRE_FP32 = 256 } ncclEpActivation_t;
 ncclResult_t ncclEpExpertLinear(ncclEpGroup_t ep_group, const void* x, const void* w, const int* counts, const void* bias, const void* residual, void* out, void* pre, int num_experts, int num_rows, int n, int k, ncclEpActivation_t activation, cudaStream_t stream);
 /* Gradients: d_x [experts, rows, k] (the rows in use), d_w [experts, n, k] and d_bias [experts, n] (of every expert, zeros where it has no
- * rows), each unless null, all bf16. pre: as the forward call gave it (null without an activation). work: ncclEpExpertLinearBackwardWork bytes. */
+ * rows), each unless null, all bf16. pre: as the forward call gave it, with the same activation (null without one). work: ncclEpExpertLinearBackwardWork bytes. */
 size_t ncclEpExpertLinearBackwardWork(ncclEpGroup_t ep_group, int num_experts, int num_rows, int n, ncclEpActivation_t activation, int with_bias);
 ncclResult_t ncclEpExpertLinearBackward(ncclEpGroup_t ep_group, const void* d_out, const void* x, const void* w, const int* counts, const void* pre, void* d_x, void* d_w, void* d_bias, void* work, int num_experts, int num_rows, int n, int k, ncclEpActivation_t activation, cudaStream_t stream);
 

@@ -16,7 +16,7 @@ The rest of a mixture-of-experts layer, forward and backward, on the rows of the
 
     idx, weights = ep.route(logits, topk, score="sigmoid", bias=balance, groups=8, keep_groups=4, group_score="top2", scale=2.5)
     toks, _, counts = ep.dispatch(x, idx, weights, fp8=False)
-    pre = torch.empty(ep.El, ep.cap, 2 * ffn, dtype=torch.bfloat16, device="cuda")
+    pre = torch.empty(ep.El, ep.cap, 2 * ffn, dtype=torch.float32, device="cuda")       # (or bf16: half the memory, less exact gradients)
     act = ep.expert_linear(toks, w_gate_up, counts, activation="swiglu", pre=pre)       # w_gate_up [El, 2 * ffn, hidden]
     y = ep.expert_linear(act, w_down, counts)                                           # w_down [El, hidden, ffn]
     out = ep.combine(y)
@@ -106,6 +106,7 @@ class ExpertParallel:
     LAYOUTS = {"expert_major": 1, "rank_major": 2, "flat": 3}
     SCORES = {"softmax": 0, "sigmoid": 1}
     GROUP_SCORES = {"max": 0, "top2": 1}
+    PRE_FP32 = 256   # beside the activation's code
     ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "silu": 3, "swiglu": 4, "geglu": 5}
 
     def __init__(self, comm, num_experts, max_tokens, hidden, max_sms=0, timeout_ms=0, enable_mask=False, layout="expert_major"):
@@ -353,13 +354,20 @@ class ExpertParallel:
             self._need("counts", counts, torch.int32, (E,))
         return E, rows, n, k, n // 2 if gated else n, self.ACTIVATIONS[activation]
 
+    def _pre(self, pre, shape):
+        """What the type of the kept pre-activations adds to the activation's code."""
+        fp32 = pre.dtype is self.torch.float32
+        self._need("pre", pre, self.torch.float32 if fp32 else self.torch.bfloat16, shape)
+        return self.PRE_FP32 if fp32 else 0
+
     def expert_linear(self, x, w, counts, bias=None, activation=None, residual=None, out=None, pre=None):
         """act(x w^T + bias) + residual for every expert over its rows in use, as ``dispatch`` packs and counts them; bf16 with fp32 sums.
 
         x [experts, rows, k], w [experts, n, k], counts int32 [experts] (None: all rows), bias [experts, n], residual and the result [experts, rows, n].
         activation: None, "relu", "gelu" (by erf), "silu", or gated, "swiglu" and "geglu": w is then gate rows and up rows one after the other, and
         the result, silu(gate) * up or gelu(gate) * up, has n / 2 columns. n and k are multiples of 8 (gated: n of 16). ``pre``
-        [experts, rows, n] gets x w^T + bias for the backward pass. Rows behind an expert's last are not written; ``residual`` may be ``out``."""
+        [experts, rows, n], bf16 or fp32, gets x w^T + bias for the backward pass: fp32 for gradients as exact as bf16 products make them, bf16
+        for half the memory. Rows behind an expert's last are not written; ``residual`` may be ``out``."""
         torch = self.torch
         E, rows, n, k, cols, act = self._linear(x, w, counts, activation)
         bf16, ptr = torch.bfloat16, lambda t: None if t is None else t.data_ptr()   # noqa: E731
@@ -368,7 +376,7 @@ class ExpertParallel:
         if residual is not None:
             self._need("residual", residual, bf16, (E, rows, cols))
         if pre is not None:
-            self._need("pre", pre, bf16, (E, rows, n))
+            act |= self._pre(pre, (E, rows, n))
         out = self._result("out", out, bf16, (E, rows, cols))
         self._moe_call("ncclEpExpertLinear", self.group, x.data_ptr(), w.data_ptr(), ptr(counts), ptr(bias), ptr(residual), out.data_ptr(), ptr(pre), E, rows, n, k, act)
         return out
@@ -383,7 +391,7 @@ class ExpertParallel:
         if act:
             if pre is None:
                 raise ValueError("the gradient of an activation needs what it was applied to: give expert_linear and this call the same `pre`")
-            self._need("pre", pre, bf16, (E, rows, n))
+            act |= self._pre(pre, (E, rows, n))
         dx = self._result("dx", dx, bf16, (E, rows, k)) if need_dx else None
         dw = self._result("dw", dw, bf16, (E, n, k)) if need_dw else None
         dbias = self._result("dbias", dbias, bf16, (E, n)) if need_dbias else None

@@ -278,6 +278,24 @@ __device__ __forceinline__ void storeRow16(__nv_bfloat16* to, const float (&v)[1
   }
 }
 
+// The same in fp32.
+__device__ __forceinline__ void storeRow16(float* to, const float (&v)[16], bool both, bool wide) {
+  uint4 q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+  if (wide) {
+    st32(to, Pack32{q[0], q[1]});
+    st32(to + 8, Pack32{q[2], q[3]});
+  } else {
+    ((uint4*)to)[0] = q[0];
+    ((uint4*)to)[1] = q[1];
+    if (both) {
+      ((uint4*)to)[2] = q[2];
+      ((uint4*)to)[3] = q[3];
+    }
+  }
+}
+
 // Epilogues take an accumulator in small steps in a loop that is not unrolled: each warp passes this code once per tile, and straight through 32 or 64
 // columns it did so at the pace at which instructions can be fetched (64 experts of 50 rows, 5000 x 184 with bias and residual: 186 us unrolled, 168 so; 64 of 200, 6656 x
 // 432, geglu and bias: 222 and 207).
@@ -337,7 +355,9 @@ __device__ __forceinline__ bool storeTile(const ExpertGemmArgs& a, const T& tile
         addBf16<16>(add, to);
       }
       if (MODE == EXPERT_FORWARD && a.pre) {
-        if (mine) storeRow16((__nv_bfloat16*)a.pre + (at - c.col0) * parts + part * a.cols + c.col0 + cc, to, both, a.wide);
+        const size_t o = (at - c.col0) * parts + part * a.cols + c.col0 + cc;
+        if (mine && a.preFp32) storeRow16((float*)a.pre + o, to, both, a.wide);
+        if (mine && !a.preFp32) storeRow16((__nv_bfloat16*)a.pre + o, to, both, a.wide);
         __syncwarp();
       }
     };
@@ -382,12 +402,13 @@ __device__ __forceinline__ bool storeTileStaged(const ExpertGemmArgs& a, const T
 #pragma unroll 1
   for (int cc = half * 64; cc < end; cc += 128) {
     const int width = min(64, end - cc), col = c.col0 + cc;   // a multiple of 8
-    auto store = [&](__nv_bfloat16* to, size_t ld) {
+    auto store = [&](auto* to, size_t ld, int columns) {
+      constexpr int kPer = 16 / sizeof(*to);   // of a chunk
       __syncwarp();
-      to += mine * ld + j0 * 8;
+      to += mine * ld + j0 * kPer;
 #pragma unroll
       for (int k = 0; k < 8; ++k, to += 4 * ld)
-        if (k * 4 + mine < left && j0 * 8 < width) *(uint4*)to = *chunk(k * 4 + mine, j0);
+        if (k * 4 + mine < left && j0 * kPer < columns) *(uint4*)to = *chunk(k * 4 + mine, j0);
       __syncwarp();
     };
     auto sums = [&](int part, int at, float (&v)[8]) {
@@ -403,13 +424,21 @@ __device__ __forceinline__ bool storeTileStaged(const ExpertGemmArgs& a, const T
     if (MODE == EXPERT_FORWARD && a.pre) {
 #pragma unroll 1
       for (int p = 0; p < parts; ++p) {
+        const size_t o = (first * parts + p) * a.cols + col;
 #pragma unroll 1
         for (int at = 0; at < width; at += 8) {
           float v[8];
           sums(p, at, v);
-          *chunk(lane, at / 8) = packBf16x8(v);
+          if (!a.preFp32) {
+            *chunk(lane, at / 8) = packBf16x8(v);
+          } else {   // 32 columns fill a row
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              *chunk(lane, at / 4 % 8 + i) = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+            if (at % 32 == 24 || at + 8 == width) store((float*)a.pre + o + at / 32 * 32, (size_t)parts * a.cols, at % 32 + 8);
+          }
         }
-        store((__nv_bfloat16*)a.pre + (first * parts + p) * a.cols + col, (size_t)parts * a.cols);
+        if (!a.preFp32) store((__nv_bfloat16*)a.pre + o, (size_t)parts * a.cols, width);
       }
     }
     if (MODE == EXPERT_FORWARD && a.residual) {
@@ -446,7 +475,7 @@ __device__ __forceinline__ bool storeTileStaged(const ExpertGemmArgs& a, const T
         for (int j = 0; j < 4; ++j) *chunk(lane, at / 8 + j) = packBf16x8(v + j * 8);
       }
     }
-    store((__nv_bfloat16*)a.out + first * a.cols + col, (size_t)a.cols);
+    store((__nv_bfloat16*)a.out + first * a.cols + col, (size_t)a.cols, width);
   }
   return true;
 }

@@ -12,19 +12,24 @@ namespace b200 {
 
 namespace {
 
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float* f) { unpackBf16x8(*(const uint4*)p, f); }
+__device__ __forceinline__ void load8(const float* p, float* f) {
+  *(float4*)f = *(const float4*)p;
+  *(float4*)(f + 4) = *(const float4*)(p + 4);
+}
 __device__ __forceinline__ int rowsInUse(const int* counts, int e, int cap) { return counts ? min(max(counts[e], 0), cap) : cap; }
 
 }  // namespace
 
 // dz = dout * act'(z) for the rows in use of every expert; gated: d(gate) = dout * up * act'(gate) and d(up) = dout * act(gate). CTA (c, e, s) takes
 // columns [c * kActCols, ...) of expert e, a thread 8 neighbouring ones, and of each gridDim.z * 8 rows the 8 of slice s. The sums over a slice's rows stay
-// in registers and are joined in a fixed order: the bias gradient has the same bits every time. Memory bounds it: 8 x 512 rows, 28672 columns, swiglu, 102 us
-// (5.7 TB/s).
-// Two roundings to bf16: z, as the forward call kept it (fp32 would double the largest tensor that a layer keeps), and dz, which the products
-// that follow take as a bf16 operand. With the rounding of their results the gradients are off by 0.0024 to 0.003 of their norm, with neither by 0.0017;
-// the bias gradient adds dz before its rounding where there is an activation.
-template <int ACT>
-__global__ void __launch_bounds__(kActThreads) expertActKernel(const __grid_constant__ ExpertActArgs a) {
+// in registers and are joined in a fixed order: the bias gradient has the same bits every time. Memory bounds it: 8 x 512 rows, 28672 columns, swiglu, 97 us
+// (6.0 TB/s), with z in fp32 121 us, where four CTAs fit an SM (with the three that the compiler chose, 154).
+// dz is rounded to bf16: the products that follow take it as a bf16 operand. z comes as the forward call kept it (Z), in fp32, or rounded to bf16 where the caller prefers half
+// the memory in the largest tensor that a layer keeps. With the rounding of their results the gradients are off by 0.00235 of their norm with z in fp32, by 0.0024 (gelu, silu) and 0.003 (gated) with it in
+// bf16, without either by 0.0017; the bias gradient adds dz before its rounding where there is an activation.
+template <int ACT, typename Z>
+__global__ void __launch_bounds__(kActThreads, 4) expertActKernel(const __grid_constant__ ExpertActArgs a) {
   pdlEnter();
   constexpr bool kGated = ACT == ACT_SWIGLU || ACT == ACT_GEGLU;
   constexpr int kParts = kGated ? 2 : 1, kRows = kActThreads * 8 / kActCols;   // rows of a CTA at a time
@@ -48,10 +53,10 @@ __global__ void __launch_bounds__(kActThreads) expertActKernel(const __grid_cons
       float g[8], z[kParts][8];
       unpackBf16x8(*(const uint4*)(dout + (size_t)row * a.cols), g);
       if (ACT != ACT_NONE) {
-        const __nv_bfloat16* pre = (const __nv_bfloat16*)a.pre + base + (size_t)row * ld;
+        const Z* pre = (const Z*)a.pre + base + (size_t)row * ld;
         __nv_bfloat16* dz = (__nv_bfloat16*)a.dz + base + (size_t)row * ld;
 #pragma unroll
-        for (int p = 0; p < kParts; ++p) unpackBf16x8(*(const uint4*)(pre + p * a.cols), z[p]);
+        for (int p = 0; p < kParts; ++p) load8(pre + p * a.cols, z[p]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           float value, slope;
@@ -100,15 +105,20 @@ __global__ void __launch_bounds__(kActThreads) expertBiasKernel(const __grid_con
   biasFromSlices(a.partial, (__nv_bfloat16*)a.dbias, n, a.slices, (size_t)blockIdx.x * kActThreads + threadIdx.x, (size_t)gridDim.x * kActThreads);
 }
 
-const void* expertActKernelFn(int act) {
+template <typename Z>
+static const void* actKernelFn(int act) {
   switch (act) {
-    case ACT_RELU: return (const void*)expertActKernel<ACT_RELU>;
-    case ACT_GELU: return (const void*)expertActKernel<ACT_GELU>;
-    case ACT_SILU: return (const void*)expertActKernel<ACT_SILU>;
-    case ACT_SWIGLU: return (const void*)expertActKernel<ACT_SWIGLU>;
-    case ACT_GEGLU: return (const void*)expertActKernel<ACT_GEGLU>;
-    default: return (const void*)expertActKernel<ACT_NONE>;
+    case ACT_RELU: return (const void*)expertActKernel<ACT_RELU, Z>;
+    case ACT_GELU: return (const void*)expertActKernel<ACT_GELU, Z>;
+    case ACT_SILU: return (const void*)expertActKernel<ACT_SILU, Z>;
+    case ACT_SWIGLU: return (const void*)expertActKernel<ACT_SWIGLU, Z>;
+    case ACT_GEGLU: return (const void*)expertActKernel<ACT_GEGLU, Z>;
+    default: return nullptr;
   }
+}
+const void* expertActKernelFn(int act, bool preFp32) {
+  if (act == ACT_NONE) return (const void*)expertActKernel<ACT_NONE, __nv_bfloat16>;   // (reads no z)
+  return preFp32 ? actKernelFn<float>(act) : actKernelFn<__nv_bfloat16>(act);
 }
 const void* expertBiasKernelFn() { return (const void*)expertBiasKernel; }
 

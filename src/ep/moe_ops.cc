@@ -125,6 +125,10 @@ static ncclResult_t makeMap(CUtensorMap* map, const void* base, int inner, int r
   return ncclSuccess;
 }
 
+// The activation without the flag beside it.
+static int actOf(ncclEpActivation_t a) { return (int)a & ~(int)NCCL_EP_ACT_PRE_FP32; }
+static bool preInFp32(ncclEpActivation_t a) { return ((int)a & (int)NCCL_EP_ACT_PRE_FP32) != 0; }
+
 static ncclResult_t checkLinear(const ncclEpGroup* g, const char* what, int experts, int rows, int n, int k, int act) {
   if (g->comm->compCap < 100) { WARN("%s needs compute capability 10.0 (found %d)", what, g->comm->compCap); return ncclInvalidUsage; }
   if (act < ACT_NONE || act > ACT_GEGLU) { WARN("%s: unknown activation %d", what, act); return ncclInvalidArgument; }
@@ -267,13 +271,14 @@ ncclResult_t ncclEpRouteBackward(ncclEpGroup_t g, const float* dweights, const v
 }
 
 ncclResult_t ncclEpExpertLinear(ncclEpGroup_t g, const void* x, const void* w, const int* counts, const void* bias, const void* residual, void* out, void* pre, int experts,
-                                int rows, int n, int k, ncclEpActivation_t act, cudaStream_t stream) {
+                                int rows, int n, int k, ncclEpActivation_t activation, cudaStream_t stream) {
   if (!g) return ncclInvalidArgument;
+  const int act = actOf(activation);
   NCCLCHECK(checkLinear(g, "ncclEpExpertLinear", experts, rows, n, k, act));
   if (rows == 0) return ncclSuccess;
   if (!x || !w || !out) return ncclInvalidArgument;
   if (!aligned({x, w, bias, residual, out, pre}, 16) || !aligned({counts}, 4)) { WARN("ncclEpExpertLinear: tensors must be 16-byte aligned"); return ncclInvalidArgument; }
-  const size_t er = (size_t)experts * rows, outBytes = er * (actGated(act) ? n / 2 : n) * 2, preBytes = er * n * 2;
+  const size_t er = (size_t)experts * rows, outBytes = er * (actGated(act) ? n / 2 : n) * 2, preBytes = er * n * (preInFp32(activation) ? 4 : 2);
   if (overlap({{out, outBytes}, {pre, preBytes}}, {{x, er * k * 2}, {w, (size_t)experts * n * k * 2}, {counts, (size_t)experts * 4}, {bias, (size_t)experts * n * 2},
                                                    {residual == out ? nullptr : residual, outBytes}}) ||
       overlap({{pre, preBytes}}, {{out, outBytes}, {residual, outBytes}})) {
@@ -295,28 +300,31 @@ ncclResult_t ncclEpExpertLinear(ncclEpGroup_t g, const void* x, const void* w, c
   a.residual = residual;
   a.out = out;
   a.pre = pre;
+  a.preFp32 = preInFp32(activation);
   return launchExpertGemm(g, EXPERT_FORWARD, x, k, rows, w, k, n, &a, stream);
 }
 
-size_t ncclEpExpertLinearBackwardWork(ncclEpGroup_t g, int experts, int rows, int n, ncclEpActivation_t act, int withBias) {
+size_t ncclEpExpertLinearBackwardWork(ncclEpGroup_t g, int experts, int rows, int n, ncclEpActivation_t activation, int withBias) {
   if (!g || experts <= 0 || experts > kExpertMax || rows <= 0 || n <= 0) return 0;
+  const int act = actOf(activation);
   const int cols = actGated(act) ? n / 2 : n;
   return dzBytes(experts, rows, n, act) + (withBias ? (size_t)actSlices(g, experts, rows, cols) * experts * n * sizeof(float) : 0);
 }
 
 ncclResult_t ncclEpExpertLinearBackward(ncclEpGroup_t g, const void* dout, const void* x, const void* w, const int* counts, const void* pre, void* dx, void* dw, void* dbias,
-                                        void* work, int experts, int rows, int n, int k, ncclEpActivation_t act, cudaStream_t stream) {
+                                        void* work, int experts, int rows, int n, int k, ncclEpActivation_t activation, cudaStream_t stream) {
   if (!g) return ncclInvalidArgument;
+  const int act = actOf(activation);
   NCCLCHECK(checkLinear(g, "ncclEpExpertLinearBackward", experts, rows, n, k, act));
-  const bool needDz = act != NCCL_EP_ACT_NONE;
+  const bool needDz = act != ACT_NONE;
   if (!aligned({dout, x, w, pre, dx, dw, dbias, work}, 16) || !aligned({counts}, 4)) { WARN("ncclEpExpertLinearBackward: tensors must be 16-byte aligned"); return ncclInvalidArgument; }
   if (rows > 0 && (!dout || (needDz && !pre) || (dx && !w) || (dw && !x) || ((needDz || dbias) && !work))) {
     WARN("ncclEpExpertLinearBackward: a tensor that the wanted gradients need is missing");
     return ncclInvalidArgument;
   }
   const size_t er = (size_t)experts * rows, weights = (size_t)experts * n * k * 2, biases = (size_t)experts * n * 2;
-  const Span given[] = {{dout, er * (actGated(act) ? n / 2 : n) * 2}, {x, er * k * 2}, {w, weights}, {counts, (size_t)experts * 4}, {pre, er * n * 2}};
-  const Span made[] = {{dx, er * k * 2}, {dw, weights}, {dbias, biases}, {work, ncclEpExpertLinearBackwardWork(g, experts, rows, n, act, dbias != nullptr)}};
+  const Span given[] = {{dout, er * (actGated(act) ? n / 2 : n) * 2}, {x, er * k * 2}, {w, weights}, {counts, (size_t)experts * 4}, {pre, er * n * (preInFp32(activation) ? 4 : 2)}};
+  const Span made[] = {{dx, er * k * 2}, {dw, weights}, {dbias, biases}, {work, ncclEpExpertLinearBackwardWork(g, experts, rows, n, activation, dbias != nullptr)}};
   for (const Span& o : made) {
     for (const Span& i : given)
       if (overlap({o}, {i})) { WARN("ncclEpExpertLinearBackward: an output shares memory with an input"); return ncclInvalidArgument; }
@@ -350,7 +358,7 @@ ncclResult_t ncclEpExpertLinearBackward(ncclEpGroup_t g, const void* dout, const
     e.partial = dbias ? (float*)((char*)work + dzBytes(experts, rows, n, act)) : nullptr;
     e.dbias = dbias;
     void* args[1] = {&e};
-    NCCLCHECK(launchMoe(g, expertActKernelFn(act), dim3((cols + kActCols - 1) / kActCols, experts, e.slices), kActThreads, 0, args, stream));
+    NCCLCHECK(launchMoe(g, expertActKernelFn(act, preInFp32(activation)), dim3((cols + kActCols - 1) / kActCols, experts, e.slices), kActThreads, 0, args, stream));
     if (dbias && !biasAside)
       NCCLCHECK(launchMoe(g, expertBiasKernelFn(), dim3((unsigned)std::min<size_t>(((size_t)experts * n / 4 + kActThreads - 1) / kActThreads, (size_t)g->smCount * 8)), kActThreads, 0, args, stream));
   }

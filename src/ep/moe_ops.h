@@ -50,7 +50,8 @@ struct ExpertGemmArgs {
   const void* bias;           // bf16 [experts][cols, twice when gated] or null
   const void* residual;       // bf16, laid out like out, or null
   void* out;                  // bf16 [experts][cap or outRows][cols]
-  void* pre;                  // bf16 [experts][cap][cols, twice when gated]: what the activation is applied to, or null
+  void* pre;                  // bf16 or fp32 [experts][cap][cols, twice when gated]: what the activation is applied to, or null
+  int preFp32;
   const float* partial;       // backward, on pairs: sums for the bias's gradient, [slices][sums], that a warp without other work adds up, or null
   void* dbias;                // bf16 [sums]
   size_t sums;                // a multiple of 8
@@ -68,13 +69,13 @@ int expertGemmThreads(bool pair);
 struct ExpertActArgs {
   const int* counts;
   const void* dout;           // bf16 [experts][cap][cols]
-  const void* pre;            // bf16 [experts][cap][cols, twice when gated]; not read without an activation
-  void* dz;                   // as pre; null without an activation
+  const void* pre;            // bf16 or fp32 [experts][cap][cols, twice when gated]; not read without an activation
+  void* dz;                   // bf16, laid out like pre; null without an activation
   float* partial;             // [slices][experts][cols, twice when gated] sums of dz over the rows of a slice, or null
   void* dbias;                // bf16 [experts][cols, twice when gated] or null
   int experts, cap, cols, act, slices;
 };
-const void* expertActKernelFn(int act);
+const void* expertActKernelFn(int act, bool preFp32);
 const void* expertBiasKernelFn();
 constexpr int kActCols = 256, kActThreads = 256;   // columns and threads of a CTA
 
