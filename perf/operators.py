@@ -173,7 +173,7 @@ def prepare(case, seed):
         out = c["n"] // 2 if c["activation"] in GATED else c["n"]
         s["out"] = torch.zeros(c["experts"], c["tokens"], out, dtype=torch.bfloat16, device="cuda")
         if c["train"]:
-            s["pre"] = torch.zeros(c["experts"], c["tokens"], c["n"], dtype=torch.bfloat16, device="cuda")
+            s["pre"] = torch.zeros(c["experts"], c["tokens"], c["n"], dtype=torch.float32, device="cuda")
             s["dx"] = torch.zeros_like(s["x"])
     else:
         s["dout"], s["y"], s["weights"], s["rows"], s["dtoks"] = _combine_inputs(c, seed)
