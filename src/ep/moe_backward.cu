@@ -124,7 +124,7 @@ const void* expertBiasKernelFn() { return (const void*)expertBiasKernel; }
 
 // ---------------------------------------------------------------------------------------------- combine's gradient
 // combine is out[t] = sum_k w[t,k] * y[row(t,k)], so dy[row] = w * dout[t] and dw[t,k] = <dout[t], y[row]>. One CTA per token: its
-// gradient is read once for all of the token's rows, KR rows are on their way together. The products' sums are joined lane by lane and warp by
+// gradient is read once for up to KR of the token's rows (eight at most), which are on their way together. The products' sums are joined lane by lane and warp by
 // warp, in the same order every time. Memory bounds it: 4096 tokens of 8 rows of 7168, 168 us (5.9 TB/s).
 template <int KR>
 __global__ void __launch_bounds__(kMoeRowThreads) combineBackwardKernel(const __grid_constant__ MoeRowsArgs a) {

@@ -24,8 +24,8 @@ __device__ __forceinline__ uint4 packBf16x8(const float* f) {
   return q;
 }
 
-// 1 / (1 + exp(-v)). The short exponential and division are off by a few units of 2^-22 where the result is rounded to bf16 (2^-9 at
-// most): the epilogue computes one per element. For v below -87 the divisor is huge and the result 0, as it should be.
+// 1 / (1 + exp(-v)). The short exponential and division are off by a few units of 2^-22 where the result is rounded to bf16 (2^-8 at
+// most): the epilogue computes one per element. Where the divisor passes 2^126, for v below -87.3, the short division gives 0: silu, less than 1.1e-36 there, is flushed.
 __device__ __forceinline__ float sigmoidOf(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
 
 // The normal distribution function at v, 0.5 erfc(-v / sqrt 2), from a Chebyshev fit of erfc with a relative error of 1.2e-7 everywhere (W. H. Press et al.,

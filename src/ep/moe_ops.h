@@ -60,7 +60,7 @@ struct ExpertGemmArgs {
 };
 
 constexpr int kExpertOneCtaRows = 128;   // an expert with more rows takes the kernel on CTA pairs
-const void* expertGemmKernelFn(int mode);       // FORWARD, DX; tensor maps of A, B and B in boxes of 32 rows
+const void* expertGemmKernelFn(int mode);       // FORWARD, DX; tensor maps of A, B and B in boxes of 32 rows (gated: 64)
 const void* expertGemmPairKernelFn(int mode, bool staged);   // tensor maps of A, B and B in boxes of 64 rows; clusters of two. staged: results go through shared memory (DW: always)
 size_t expertGemmSmemBytes();
 int expertGemmThreads(bool pair);
