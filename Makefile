@@ -19,9 +19,9 @@ LDSAN     := -fsanitize=$(SAN)
 endif
 
 HOST_SRCS := $(wildcard src/core/*.cc src/host/*.cc src/comm/*.cc src/mem/*.cc src/sched/*.cc \
-               src/topo/*.cc src/transport/*.cc src/plugin/*.cc src/ras/*.cc src/ep/*.cc src/tp/*.cc \
+               src/topo/*.cc src/transport/*.cc src/plugin/*.cc src/ras/*.cc src/ep/*.cc src/tp/*.cc src/cp/*.cc \
                src/contrib/*.cc)
-CU_SRCS   := $(wildcard src/kernels/*.cu src/ep/*.cu src/tp/*.cu src/contrib/*.cu)
+CU_SRCS   := $(wildcard src/kernels/*.cu src/ep/*.cu src/tp/*.cu src/cp/*.cu src/contrib/*.cu)
 HOST_OBJS := $(HOST_SRCS:%.cc=$(BUILD)/%.o)
 CU_OBJS   := $(CU_SRCS:%.cu=$(BUILD)/%.cu.o)
 

@@ -1,0 +1,653 @@
+// Attention for sm_100a, the backward pass, which computes the probabilities again: with p_ij = exp(s_ij - lse_i), s_ij = scale q_i.k_j,
+//   dv_j = sum_i p_ij do_i      ds_ij = p_ij (do_i.v_j - <do_i, o_i>)      dq_i = scale sum_j ds_ij k_j      dk_j = scale sum_i ds_ij q_i
+// over the pairs that see each other; the sums for dk and dv run over the heads that share them as well.
+//
+// Two kernels, each with the sums of its tile in tensor memory from the first product to the last: one owns a tile of keys and walks the queries (dk, dv), one
+// owns a tile of queries and walks the keys (dq). Together they make seven products of a tile where five would do, if the tiles of dq were added up
+// in memory by whoever has a part of them: then the order of the additions, and the result, would change from run to run, or CTAs would have to wait for one another.
+//
+// Roles as in the forward pass: warps 0-7 have a row of the tile each and, in two groups, a half of its columns; warp 8 feeds the ring, warp 9 issues products. Probabilities
+// and ds go back into tensor memory in 16 bits, each over the half it was computed from, and are the first operand of the next products from there.
+// fp16: probabilities are held times 2^15, ds times a power of two that brings the largest that it could be (by the longest rows of do and v) to 2^15; the sums are in
+// fp32 and are multiplied back.
+#include "attention.cuh"
+
+namespace b200 {
+
+using namespace attn;
+
+namespace {
+
+constexpr uint32_t kTmemCols = 512;
+
+template <int DP> struct BackwardShape {
+  static constexpr uint32_t kTileBytes = DP / 64 * kHalfTile;
+  static constexpr int kStages = DP == 64 ? 8 : 5;
+  static constexpr uint32_t kRing = 2 * kTileBytes, kStats = kRing + kStages * kTileBytes, kCtrl = kStats + 2048;
+  static constexpr size_t kBytes = kCtrl + 1024;   // (dynamic shared memory, all that these kernels have, begins on a multiple of 1024 bytes)
+  static_assert(kBytes <= 227 * 1024, "shared memory");
+};
+
+// The power of two that ds is multiplied by, in fp16: |ds| <= p (|do.v| + |do.o|) <= 2 |do| |v|.
+template <typename T>
+__device__ __forceinline__ float gradScale(const AttnArgs& a, int b, int kvHead) {
+  if (Pack<T>::kBackwardBias == 0.0f) return 1.0f;
+  const uint32_t* at = a.bounds + ((size_t)b * a.kvHeads + kvHead) * 2;
+  const float most = 2.0f * sqrtf(__uint_as_float(at[0])) * sqrtf(__uint_as_float(at[1]));
+  if (!(most > 0.0f) || most > 3.0e38f) return 1.0f;   // nothing to do, or nothing to save
+  int e;
+  frexpf(most, &e);                                     // most < 2^e
+  return exp2f((float)max(-100, min(100, 15 - e)));
+}
+
+struct BackwardBars {
+  uint64_t *full, *empty, *own, *first, *second, *firstDone, *secondDone, *outBar, *fix, *drain;
+  uint32_t* tmemSlot;
+  volatile uint32_t* abortFlag;
+};
+
+template <int DP>
+__device__ __forceinline__ BackwardBars backwardSetUp(uint8_t* smem, int warp) {
+  BackwardBars s;
+  s.full = (uint64_t*)(smem + BackwardShape<DP>::kCtrl);
+  s.empty = s.full + BackwardShape<DP>::kStages;
+  s.own = s.empty + BackwardShape<DP>::kStages;
+  s.first = s.own + 1;           // [2] scores
+  s.second = s.first + 2;        // do.v
+  s.firstDone = s.second + 1;    // probabilities are in tensor memory
+  s.secondDone = s.firstDone + 1;
+  s.outBar = s.secondDone + 1;
+  s.fix = s.outBar + 1;          // [2]
+  s.drain = s.fix + 2;
+  s.tmemSlot = (uint32_t*)(s.drain + 1);
+  s.abortFlag = s.tmemSlot + 1;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2 * BackwardShape<DP>::kStages; ++i) mbarInit(smemAddr(&s.full[i]), 1);
+    mbarInit(smemAddr(s.own), 1);
+    mbarInit(smemAddr(&s.first[0]), 1);
+    mbarInit(smemAddr(&s.first[1]), 1);
+    mbarInit(smemAddr(s.second), 1);
+    mbarInit(smemAddr(s.firstDone), kComputeWarps);
+    mbarInit(smemAddr(s.secondDone), kComputeWarps);
+    mbarInit(smemAddr(s.outBar), 1);
+    mbarInit(smemAddr(&s.fix[0]), 1);
+    mbarInit(smemAddr(&s.fix[1]), 1);
+    mbarInit(smemAddr(s.drain), 1);
+    *s.abortFlag = 0;
+    mbarInitFence();
+  }
+  if (warp == kMmaWarp) {
+    tmemAlloc(smemAddr(s.tmemSlot), kTmemCols);
+    tmemRelinquish();
+  }
+  return s;
+}
+
+// Rows of sums [128][DP] in tensor memory, times `factor` (and plus what is there already), become a gradient's rows; `to` names the row of this thread, null for none.
+template <typename T, int DP>
+__device__ __forceinline__ void storeGradient(const AttnArgs& a, uint32_t tmem, bool some, float factor, bool exists, bool valid, size_t row, void* grad, const float* add) {
+#pragma unroll
+  for (int k = 0; k < DP / 32; ++k) {
+    uint32_t o[32];
+    float f[32];
+    if (some) {
+      tmemLd32(tmem + k * 32, o);
+      tmemLdWait32(o);
+    }
+    if (!exists) continue;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) f[e] = some && valid ? __uint_as_float(o[e]) * factor : 0.0f;
+    if (add && valid) {
+#pragma unroll
+      for (int e = 0; e < 32; e += 4) {
+        if (k * 32 + e >= a.dim) break;
+        const float4 v = *(const float4*)(add + row * a.dim + k * 32 + e);
+        f[e] += v.x; f[e + 1] += v.y; f[e + 2] += v.z; f[e + 3] += v.w;
+      }
+    }
+    if (a.gradFp32) {
+      float* to = (float*)grad + row * a.dim;
+#pragma unroll
+      for (int e = 0; e < 32; e += 4)
+        if (k * 32 + e < a.dim) *(float4*)(to + k * 32 + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+    } else {
+      uint16_t* to = (uint16_t*)grad + row * a.dim;
+#pragma unroll
+      for (int e = 0; e < 32; e += 8)
+        if (k * 32 + e < a.dim)
+          *(uint4*)(to + k * 32 + e) = make_uint4(Pack<T>::two(f[e], f[e + 1]), Pack<T>::two(f[e + 2], f[e + 3]), Pack<T>::two(f[e + 4], f[e + 5]), Pack<T>::two(f[e + 6], f[e + 7]));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- dk and dv
+// Tensor memory: scores [keys x queries] (then probabilities) at 0, do.v (then ds) at 128, dv at 256, dk at 384. Products of tile j: dv += P do as soon as the
+// probabilities are there, with the next tile's scores behind it; dk += dS q as soon as ds is, with the next do.v behind it. So the tensor cores work on one pair while
+// the other's elements are computed.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDo, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                     const __grid_constant__ AttnArgs a) {
+  using Shape = BackwardShape<DP>;
+  constexpr int kStages = Shape::kStages;
+  constexpr uint32_t kTileBytes = Shape::kTileBytes;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const BackwardBars s = backwardSetUp<DP>(smem, warp);
+  volatile uint32_t* abortFlag = s.abortFlag;
+  const int rows = a.tileTokens * a.group;
+  if (warp < kComputeWarps && rows < 128) {
+    // rows of a tile that no copy writes are operands of sums over the rows: zero, for good
+    const int each = (128 - rows) * 8;
+    for (int i = threadIdx.x; i < kStages * (DP / 64) * each; i += kComputeWarps * 32)
+      *(uint4*)(smem + Shape::kRing + i / each * kHalfTile + rows * 128 + i % each * 16) = make_uint4(0, 0, 0, 0);
+    fenceProxyAsync();
+  }
+  tcFenceBefore();
+  __syncthreads();
+  tcFenceAfter();
+  const uint32_t tmem = *s.tmemSlot;
+  pdlEnter();
+
+  const unsigned owners = a.batch * a.kvHeads, owner = blockIdx.x % owners;
+  const int kvHead = owner % a.kvHeads, b = owner / a.kvHeads, key0 = blockIdx.x / owners * 128;   // (the first keys are seen most)
+  const Sequence seq = sequenceOf(a, b);
+  // tiles of queries: from the first that sees a key of this tile to the last
+  const int all = (seq.q + a.tileTokens - 1) / a.tileTokens;
+  const long long firstTok = a.causal ? max(0ll, (long long)key0 - seq.offset) : 0;
+  const int begin = (int)min((long long)all, firstTok / a.tileTokens);
+  const int n = key0 < seq.kv ? all - begin : 0;
+  const int fixRows = seq.q < a.q ? seq.q % a.tileTokens * a.group : 0;   // of the last tile, behind which rows may hold anything
+  const uint32_t smem0 = smemAddr(smem);
+  auto fail = [&](uint32_t what) {
+    *abortFlag = 1;
+    reportTimeout(a.status, what);
+  };
+
+  if (warp == kProducerWarp) {
+    uint32_t armed = 0;
+    int place = 0;
+    bool ok = !*abortFlag, ownArmed = false;
+    auto next = [&](const CUtensorMap* map, int tile, const float* stats) {
+      const int at = place % kStages;
+      const uint32_t ph = (place / kStages) & 1;
+      ok = ok && warpWaitOr(smemAddr(&s.empty[at]), ph ^ 1, abortFlag);
+      if (!ok) {
+        if (lane == 0) fail(1000 + at);
+        return;
+      }
+      if (lane == 0) {
+        const uint32_t bar = smemAddr(&s.full[at]);
+        mbarExpectTx(bar, DP / 64 * rows * 128 + (stats ? 1024 : 0));
+        loadTile<DP>(smem0 + Shape::kRing + at * kTileBytes, map, (begin + tile) * a.tileTokens, kvHead * a.group, b, bar);
+        if (stats) bulkLoad(smem0 + Shape::kStats + (tile & 1) * 1024, stats, 1024, bar);
+      }
+      armed |= 1u << at;
+      ++place;
+    };
+    if (n > 0) {
+      if (ok && lane == 0) {
+        mbarExpectTx(smemAddr(s.own), 2 * kTileBytes);
+        loadTile<DP>(smem0, &tmK, key0, kvHead, b, smemAddr(s.own));
+        loadTile<DP>(smem0 + kTileBytes, &tmV, key0, kvHead, b, smemAddr(s.own));
+      }
+      ownArmed = ok;
+      // stats of a tile arrive with its do: the buffer was last read for the tile before the last, whose q has left its stage by then
+      const float* stats = a.stats + (((size_t)b * a.kvHeads + kvHead) * a.tiles + begin) * 256;
+      for (int i = 0; i < n && ok; ++i) {
+        next(&tmQ, i, nullptr);
+        if (ok && i >= 2) {
+          const int was = 2 * (i - 2);   // place of that q
+          ok = warpWaitOr(smemAddr(&s.empty[was % kStages]), (was / kStages) & 1, abortFlag);
+          if (!ok && lane == 0) fail(1050);
+        }
+        if (ok) next(&tmDo, i, stats + (size_t)i * 256);
+      }
+      if (ok && fixRows) {
+        for (int k = 0; k < 2 && ok; ++k) {
+          const int at = place - 2 + k;
+          ok = warpWaitOr(smemAddr(&s.full[at % kStages]), (at / kStages) & 1, abortFlag);
+          if (ok) {
+            clearRows<DP>(smem + Shape::kRing + at % kStages * kTileBytes, fixRows, lane);
+            if (lane == 0) mbarArrive(smemAddr(&s.fix[k]));
+          } else if (lane == 0) {
+            fail(1100);
+          }
+        }
+      }
+      if (__any_sync(~0u, *abortFlag)) {
+        for (int at = 0; at < kStages; ++at)
+          if (armed >> at & 1) mbarWait(smemAddr(&s.full[at]), (uint32_t)((place - 1 - (place - 1 - at + kStages) % kStages) / kStages) & 1, 1u << 20);
+        if (ownArmed) mbarWait(smemAddr(s.own), 0, 1u << 20);
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    if (n > 0 && electOne()) {
+      bool ok = true;
+      auto need = [&](bool got, uint32_t what) {
+        if (ok && !got) fail(what);
+        ok = ok && got;
+        return ok;
+      };
+      auto full = [&](int place) { return need(waitOr(smemAddr(&s.full[place % kStages]), (place / kStages) & 1, abortFlag), 2000 + place % kStages); };
+      auto tileAt = [&](int place) { return smem0 + Shape::kRing + (place % kStages) * kTileBytes; };
+      auto scores = [&](int i) {
+        if (!full(2 * i)) return;
+        if (fixRows && i == n - 1 && !need(waitOr(smemAddr(&s.fix[0]), 0, abortFlag), 2200)) return;
+        tcFenceAfter();
+        productOfTiles<T, DP>(tmem, smem0, tileAt(2 * i));
+        ummaCommit(smemAddr(&s.first[0]));
+      };
+      auto doV = [&](int i) {
+        if (!full(2 * i + 1)) return;
+        if (fixRows && i == n - 1 && !need(waitOr(smemAddr(&s.fix[1]), 0, abortFlag), 2201)) return;
+        tcFenceAfter();
+        productOfTiles<T, DP>(tmem + 128, smem0 + kTileBytes, tileAt(2 * i + 1));
+        ummaCommit(smemAddr(s.second));
+      };
+      if (need(waitOr(smemAddr(s.own), 0, abortFlag), 2100)) scores(0);
+      if (ok) doV(0);
+      for (int i = 0; i < n && ok; ++i) {
+        if (!need(waitOr(smemAddr(s.firstDone), i & 1, abortFlag), 2300)) break;
+        tcFenceAfter();
+        productWithTmem<T, DP>(tmem + 256, tmem, tmem + 64, tileAt(2 * i + 1), i != 0);
+        ummaCommit(smemAddr(&s.empty[(2 * i + 1) % kStages]));   // (its do.v was issued in front of this)
+        if (i + 1 < n) scores(i + 1);
+        if (!ok || !need(waitOr(smemAddr(s.secondDone), i & 1, abortFlag), 2400)) break;
+        tcFenceAfter();
+        productWithTmem<T, DP>(tmem + 384, tmem + 128, tmem + 192, tileAt(2 * i), i != 0);
+        ummaCommit(smemAddr(&s.empty[2 * i % kStages]));
+        if (i + 1 < n) doV(i + 1);
+        else ummaCommit(smemAddr(s.outBar));
+      }
+      if (!ok) {
+        ummaCommit(smemAddr(s.drain));
+        mbarWait(smemAddr(s.drain), 0, 1u << 20);
+      }
+    }
+  } else {
+    const int half = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, key = key0 + row;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tS = tmem + lanes + half * 64, tDp = tS + 128;
+    const float c = a.scale * kLog2e, up = n > 0 ? gradScale<T>(a, b, kvHead) : 1.0f, down = up * exp2f(-Pack<T>::kBackwardBias);
+    const bool valid = key < seq.kv;
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+      const float* stats = (const float*)(smem + Shape::kStats + (i & 1) * 1024);   // lse [128], <do, o> [128]
+      ok = warpWaitOr(smemAddr(&s.full[(2 * i + 1) % kStages]), ((2 * i + 1) / kStages) & 1, abortFlag) && warpWaitOr(smemAddr(&s.first[0]), i & 1, abortFlag);
+      if (!ok) {
+        if (lane == 0) fail(3000);
+        break;
+      }
+      tcFenceAfter();
+      const int tok0 = (begin + i) * a.tileTokens;
+      uint32_t x[2][32];
+      float p[64];
+      tmemLd32(tS, x[0]);
+      tmemLd32(tS + 32, x[1]);
+      tmemLdWait32(x[0]);
+      tmemLdWait32(x[1]);
+#pragma unroll
+      for (int k = 0; k < 64; k += 4) {
+        const float4 lse = *(const float4*)(stats + half * 64 + k);
+        p[k] = exp2Fast(fmaf(__uint_as_float(x[k / 32][k % 32]), c, -lse.x));
+        p[k + 1] = exp2Fast(fmaf(__uint_as_float(x[k / 32][k % 32 + 1]), c, -lse.y));
+        p[k + 2] = exp2Fast(fmaf(__uint_as_float(x[k / 32][k % 32 + 2]), c, -lse.z));
+        p[k + 3] = exp2Fast(fmaf(__uint_as_float(x[k / 32][k % 32 + 3]), c, -lse.w));
+      }
+      // the first token that sees this key
+      if (a.causal && tok0 + seq.offset < key0 + 127) {
+        const int seen = key - seq.offset - tok0;   // token of the tile
+        const int from = seen <= 0 ? 0 : min(seen, 128) * a.group;
+#pragma unroll
+        for (int k = 0; k < 64; ++k)
+          if (half * 64 + k < from) p[k] = 0.0f;
+      }
+      uint32_t packed[32];
+#pragma unroll
+      for (int k = 0; k < 32; ++k) packed[k] = Pack<T>::two(p[2 * k], p[2 * k + 1]);
+      tmemSt32(tS, packed);
+      tmemStWait();
+      tcFenceBefore();
+      __syncwarp();
+      if (lane == 0) mbarArrive(smemAddr(s.firstDone));
+      ok = warpWaitOr(smemAddr(s.second), i & 1, abortFlag);
+      if (!ok) {
+        if (lane == 0) fail(3001);
+        break;
+      }
+      tcFenceAfter();
+      tmemLd32(tDp, x[0]);
+      tmemLd32(tDp + 32, x[1]);
+      tmemLdWait32(x[0]);
+      tmemLdWait32(x[1]);
+#pragma unroll
+      for (int k = 0; k < 64; k += 4) {
+        const float4 delta = *(const float4*)(stats + 128 + half * 64 + k);
+        const float d[4] = {delta.x, delta.y, delta.z, delta.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float dp = __uint_as_float(x[(k + e) / 32][(k + e) % 32]);
+          p[k + e] *= (dp - d[e]) * down;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 32; ++k) packed[k] = Pack<T>::two(p[2 * k], p[2 * k + 1]);
+      tmemSt32(tDp, packed);
+      tmemStWait();
+      tcFenceBefore();
+      __syncwarp();
+      if (lane == 0) mbarArrive(smemAddr(s.secondDone));
+    }
+    if (ok && n > 0) {
+      ok = warpWaitOr(smemAddr(s.outBar), 0, abortFlag);
+      if (!ok && lane == 0) fail(3100);
+      tcFenceAfter();
+    }
+    if (!__any_sync(~0u, *abortFlag)) {
+      const size_t at = ((size_t)b * a.kv + key) * a.kvHeads + kvHead;
+      if (half == 0) storeGradient<T, DP>(a, tmem + lanes + 256, n > 0, exp2f(-Pack<T>::kBackwardBias), key < a.kv, valid, at, a.dv, a.addDv);
+      else storeGradient<T, DP>(a, tmem + lanes + 384, n > 0, a.scale / up, key < a.kv, valid, at, a.dk, a.addDk);
+    }
+  }
+
+  tcFenceBefore();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tcFenceAfter();
+    tmemDealloc(tmem, kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- dq
+// Tensor memory: scores [queries x keys] of two tiles at 0 and 128, do.v (then ds) at 256, dq at 384. Scores are two tiles ahead, so that exponentials are
+// computed while the tensor cores work on the tile before.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDo, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                    const __grid_constant__ AttnArgs a) {
+  using Shape = BackwardShape<DP>;
+  constexpr int kStages = Shape::kStages;
+  constexpr uint32_t kTileBytes = Shape::kTileBytes;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const BackwardBars s = backwardSetUp<DP>(smem, warp);
+  volatile uint32_t* abortFlag = s.abortFlag;
+  tcFenceBefore();
+  __syncthreads();
+  tcFenceAfter();
+  const uint32_t tmem = *s.tmemSlot;
+  pdlEnter();
+
+  const int rows = a.tileTokens * a.group;
+  const unsigned owners = a.batch * a.kvHeads, owner = blockIdx.x % owners;
+  const int kvHead = owner % a.kvHeads, b = owner / a.kvHeads, qTile = a.tiles - 1 - (int)(blockIdx.x / owners), tok0 = qTile * a.tileTokens;
+  const Sequence seq = sequenceOf(a, b);
+  const int last = min(tok0 + a.tileTokens, seq.q) - 1;
+  const int n = last < tok0 ? 0 : (visibleOf(a, seq, last) + 127) / 128;
+  const int fixRows = seq.kv < a.kv ? seq.kv % 128 : 0, fixTile = fixRows ? seq.kv / 128 : -1;   // keys and values behind the last may be anything
+  const uint32_t smem0 = smemAddr(smem);
+  auto fail = [&](uint32_t what) {
+    *abortFlag = 1;
+    reportTimeout(a.status, what);
+  };
+
+  if (warp == kProducerWarp) {
+    uint32_t armed = 0;
+    int place = 0;
+    bool ok = !*abortFlag, ownArmed = false;
+    auto next = [&](const CUtensorMap* map, int tile) {
+      const int at = place % kStages;
+      const uint32_t ph = (place / kStages) & 1;
+      ok = ok && warpWaitOr(smemAddr(&s.empty[at]), ph ^ 1, abortFlag);
+      if (!ok) {
+        if (lane == 0) fail(1000 + at);
+        return;
+      }
+      if (lane == 0) {
+        const uint32_t bar = smemAddr(&s.full[at]);
+        mbarExpectTx(bar, kTileBytes);
+        loadTile<DP>(smem0 + Shape::kRing + at * kTileBytes, map, tile * 128, kvHead, b, bar);
+      }
+      armed |= 1u << at;
+      ++place;
+    };
+    if (n > 0) {
+      if (ok && lane == 0) {
+        mbarExpectTx(smemAddr(s.own), 2 * (DP / 64) * rows * 128);
+        loadTile<DP>(smem0, &tmQ, tok0, kvHead * a.group, b, smemAddr(s.own));
+        loadTile<DP>(smem0 + kTileBytes, &tmDo, tok0, kvHead * a.group, b, smemAddr(s.own));
+      }
+      ownArmed = ok;
+      for (int i = 0; i < n && ok; ++i) {
+        next(&tmK, i);
+        if (ok) next(&tmV, i);
+      }
+      if (ok && fixTile >= 0 && fixTile == n - 1) {
+        for (int k = 0; k < 2 && ok; ++k) {
+          const int at = place - 2 + k;
+          ok = warpWaitOr(smemAddr(&s.full[at % kStages]), (at / kStages) & 1, abortFlag);
+          if (ok) {
+            clearRows<DP>(smem + Shape::kRing + at % kStages * kTileBytes, fixRows, lane);
+            if (lane == 0) mbarArrive(smemAddr(&s.fix[k]));
+          } else if (lane == 0) {
+            fail(1100);
+          }
+        }
+      }
+      if (__any_sync(~0u, *abortFlag)) {
+        for (int at = 0; at < kStages; ++at)
+          if (armed >> at & 1) mbarWait(smemAddr(&s.full[at]), (uint32_t)((place - 1 - (place - 1 - at + kStages) % kStages) / kStages) & 1, 1u << 20);
+        if (ownArmed) mbarWait(smemAddr(s.own), 0, 1u << 20);
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    if (n > 0 && electOne()) {
+      bool ok = true;
+      auto need = [&](bool got, uint32_t what) {
+        if (ok && !got) fail(what);
+        ok = ok && got;
+        return ok;
+      };
+      auto full = [&](int place) { return need(waitOr(smemAddr(&s.full[place % kStages]), (place / kStages) & 1, abortFlag), 2000 + place % kStages); };
+      auto tileAt = [&](int place) { return smem0 + Shape::kRing + (place % kStages) * kTileBytes; };
+      const bool fixed = fixTile == n - 1;
+      auto scores = [&](int i) {
+        if (!full(2 * i)) return;
+        if (fixed && i == n - 1 && !need(waitOr(smemAddr(&s.fix[0]), 0, abortFlag), 2200)) return;
+        tcFenceAfter();
+        productOfTiles<T, DP>(tmem + (i & 1) * 128, smem0, tileAt(2 * i));
+        ummaCommit(smemAddr(&s.first[i & 1]));
+      };
+      auto doV = [&](int i) {
+        if (!full(2 * i + 1)) return;
+        if (fixed && i == n - 1 && !need(waitOr(smemAddr(&s.fix[1]), 0, abortFlag), 2201)) return;
+        tcFenceAfter();
+        productOfTiles<T, DP>(tmem + 256, smem0 + kTileBytes, tileAt(2 * i + 1));
+        ummaCommit(smemAddr(s.second));
+        ummaCommit(smemAddr(&s.empty[(2 * i + 1) % kStages]));
+      };
+      if (need(waitOr(smemAddr(s.own), 0, abortFlag), 2100)) scores(0);
+      if (ok) doV(0);
+      if (ok && n > 1) scores(1);
+      for (int i = 0; i < n && ok; ++i) {
+        if (!need(waitOr(smemAddr(s.secondDone), i & 1, abortFlag), 2300)) break;
+        tcFenceAfter();
+        productWithTmem<T, DP>(tmem + 384, tmem + 256, tmem + 320, tileAt(2 * i), i != 0);
+        ummaCommit(smemAddr(&s.empty[2 * i % kStages]));
+        if (i + 1 < n) doV(i + 1);
+        else ummaCommit(smemAddr(s.outBar));
+        if (ok && i + 2 < n) scores(i + 2);   // over scores that were read before ds was there
+      }
+      if (!ok) {
+        ummaCommit(smemAddr(s.drain));
+        mbarWait(smemAddr(s.drain), 0, 1u << 20);
+      }
+    }
+  } else {
+    const int half = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tDp = tmem + lanes + 256 + half * 64;
+    const int tok = tok0 + row / a.group, head = kvHead * a.group + row % a.group;
+    const bool valid = row < rows && tok < seq.q, exists = row < rows && tok < a.q;
+    const int limit = valid ? visibleOf(a, seq, tok) : 0;
+    const float c = a.scale * kLog2e, up = n > 0 ? gradScale<T>(a, b, kvHead) : 1.0f, down = up * exp2f(-Pack<T>::kBackwardBias);
+    float lse = 0.0f, delta = 0.0f;
+    if (n > 0) {
+      const float* stats = a.stats + (((size_t)b * a.kvHeads + kvHead) * a.tiles + qTile) * 256;
+      lse = stats[row];
+      delta = stats[128 + row];
+    }
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+      ok = warpWaitOr(smemAddr(&s.first[i & 1]), (i >> 1) & 1, abortFlag);
+      if (!ok) {
+        if (lane == 0) fail(3000);
+        break;
+      }
+      tcFenceAfter();
+      const uint32_t tS = tmem + lanes + (i & 1) * 128 + half * 64;
+      uint32_t x[2][32];
+      float p[64];
+      tmemLd32(tS, x[0]);
+      tmemLd32(tS + 32, x[1]);
+      tmemLdWait32(x[0]);
+      tmemLdWait32(x[1]);
+#pragma unroll
+      for (int k = 0; k < 64; ++k) p[k] = exp2Fast(fmaf(__uint_as_float(x[k / 32][k % 32]), c, -lse));
+      const int k0 = i * 128 + half * 64;
+      const bool hide = __any_sync(~0u, limit < k0 + 64);
+      ok = warpWaitOr(smemAddr(s.second), i & 1, abortFlag);
+      if (!ok) {
+        if (lane == 0) fail(3001);
+        break;
+      }
+      tcFenceAfter();
+      tmemLd32(tDp, x[0]);
+      tmemLd32(tDp + 32, x[1]);
+      tmemLdWait32(x[0]);
+      tmemLdWait32(x[1]);
+#pragma unroll
+      for (int k = 0; k < 64; ++k) p[k] *= (__uint_as_float(x[k / 32][k % 32]) - delta) * down;
+      if (hide) {
+#pragma unroll
+        for (int k = 0; k < 64; ++k)
+          if (k0 + k >= limit) p[k] = 0.0f;
+      }
+      uint32_t packed[32];
+#pragma unroll
+      for (int k = 0; k < 32; ++k) packed[k] = Pack<T>::two(p[2 * k], p[2 * k + 1]);
+      tmemSt32(tDp, packed);
+      tmemStWait();
+      tcFenceBefore();
+      __syncwarp();
+      if (lane == 0) mbarArrive(smemAddr(s.secondDone));
+    }
+    if (ok && n > 0) {
+      ok = warpWaitOr(smemAddr(s.outBar), 0, abortFlag);
+      if (!ok && lane == 0) fail(3100);
+      tcFenceAfter();
+    }
+    if (!__any_sync(~0u, *abortFlag) && half == 0) {
+      const size_t at = ((size_t)b * a.q + tok) * a.heads + head;
+      storeGradient<T, DP>(a, tmem + lanes + 384, n > 0, a.scale / up, exists, valid, at, a.dq, a.addDq);
+    }
+  }
+
+  tcFenceBefore();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tcFenceAfter();
+    tmemDealloc(tmem, kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- what both need of each row of queries
+// A warp per row: <do, o> (unless it is given), and the log-sum-exp in units of log 2, laid out as the tiles are. Rows that nobody has, and rows that
+// see no key, get an infinite log-sum-exp: their probabilities are zero. fp16: the longest row of do, and by the CTAs behind the tiles of v. A maximum does not go
+// by the order, and the bits of floats that are not negative are ordered as they are (NaN on top).
+template <typename T>
+__global__ void __launch_bounds__(256) attnStatsKernel(const __grid_constant__ AttnStatsArgs a) {
+  pdlEnter();
+  const int lane = threadIdx.x & 31, packs = a.dim / 8;
+  const size_t tileRows = (size_t)a.batch * a.kvHeads * a.tiles * 128;
+  size_t w = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  auto load = [&](const void* x, const long long* stride, int b, int tok, int head, float* f) {
+    const uint4 v = *(const uint4*)((const uint16_t*)x + (b * stride[0] + tok * stride[1] + head * stride[2] + lane * 8));
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 p = Pack<T>::both(u[i]);
+      f[2 * i] = p.x;
+      f[2 * i + 1] = p.y;
+    }
+  };
+  auto sum = [&](float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    return v;
+  };
+  if (w >= tileRows) {   // a row of v
+    w -= tileRows;
+    if (!a.bounds || w >= (size_t)a.batch * a.kv * a.kvHeads) return;
+    const int head = (int)(w % a.kvHeads), tok = (int)(w / a.kvHeads % a.kv), b = (int)(w / a.kvHeads / a.kv);
+    if (tok >= (a.kvLengths ? a.kvLengths[b] : a.kv)) return;
+    float f[8], ss = 0.0f;
+    if (lane < packs) {
+      load(a.v, a.vStride, b, tok, head, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss += f[i] * f[i];
+    }
+    ss = sum(ss);
+    if (lane == 0) atomicMax(a.bounds + ((size_t)b * a.kvHeads + head) * 2 + 1, __float_as_uint(ss) & 0x7fffffffu);
+    return;
+  }
+  const int row = (int)(w % 128), tile = (int)(w / 128 % a.tiles), kvHead = (int)(w / 128 / a.tiles % a.kvHeads), b = (int)(w / 128 / a.tiles / a.kvHeads);
+  const int tok = tile * a.tileTokens + row / a.group, head = kvHead * a.group + row % a.group;
+  const int used = a.qLengths ? min(a.qLengths[b], a.q) : a.q;
+  const bool valid = row < a.tileTokens * a.group && tok < used;
+  float lse = INFINITY, delta = 0.0f;
+  if (valid) {
+    const size_t at = ((size_t)b * a.heads + head) * a.q + tok;
+    if (a.delta) delta = a.delta[at];
+    if (!a.delta || a.bounds) {
+      float f[8], g[8], ss = 0.0f, dot = 0.0f;
+      if (lane < packs) {
+        load(a.dout, a.doutStride, b, tok, head, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss += f[i] * f[i];
+        if (!a.delta) {
+          load(a.out, a.outStride, b, tok, head, g);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dot += f[i] * g[i];
+        }
+      }
+      if (!a.delta) delta = sum(dot);
+      if (a.bounds) {
+        ss = sum(ss);
+        if (lane == 0) atomicMax(a.bounds + ((size_t)b * a.kvHeads + kvHead) * 2, __float_as_uint(ss) & 0x7fffffffu);
+      }
+    }
+    if (a.stats) {
+      lse = a.lse[at];
+      lse = lse == -INFINITY ? INFINITY : fmaf(lse, kLog2e, -Pack<T>::kBackwardBias);
+    }
+    if (a.deltaOut && lane == 0) a.deltaOut[at] = delta;
+  } else if (a.deltaOut && lane == 0 && row < a.tileTokens * a.group && tok < a.q) {
+    a.deltaOut[((size_t)b * a.heads + head) * a.q + tok] = 0.0f;
+  }
+  if (a.stats && lane == 0) {
+    float* to = a.stats + (w / 128) * 256 + row;
+    to[0] = lse;
+    to[128] = delta;
+  }
+}
+
+}  // namespace
+
+template <typename T> static const void* kvFn(int dim) { return dim <= 64 ? (const void*)attnBackwardKvKernel<T, 64> : (const void*)attnBackwardKvKernel<T, 128>; }
+template <typename T> static const void* qFn(int dim) { return dim <= 64 ? (const void*)attnBackwardQKernel<T, 64> : (const void*)attnBackwardQKernel<T, 128>; }
+const void* attnBackwardKvKernelFn(int type, int dim) { return type == ATTN_F16 ? kvFn<__half>(dim) : kvFn<__nv_bfloat16>(dim); }
+const void* attnBackwardQKernelFn(int type, int dim) { return type == ATTN_F16 ? qFn<__half>(dim) : qFn<__nv_bfloat16>(dim); }
+size_t attnBackwardSmemBytes(int dim) { return dim <= 64 ? BackwardShape<64>::kBytes : BackwardShape<128>::kBytes; }
+const void* attnStatsKernelFn(int type) { return type == ATTN_F16 ? (const void*)attnStatsKernel<__half> : (const void*)attnStatsKernel<__nv_bfloat16>; }
+
+}  // namespace b200

@@ -1,0 +1,454 @@
+// Attention for sm_100a, the forward pass: o_i = sum_j p_ij v_j / l_i over the keys j that query i sees, p_ij = exp(scale q_i.k_j - m_i), l_i their sum, and
+// lse_i = m_i + ln l_i. One pass over the keys with a running maximum: probabilities never reach memory.
+//
+// One CTA per SM, in roles:
+//   warps 0-7   two groups of four; a thread holds a row of 128 scores: maximum, exponentials, their sum, and the probabilities in 16 bits back into
+//               tensor memory, over the scores. The maximum is only raised (and the sums so far multiplied) where a score passes it by 2^8: the largest
+//               probability is then 2^8 instead of 1, which costs nothing in a floating-point type.
+//   warp 8      TMA producer: tiles of queries once, keys and values through a ring in shared memory
+//   warp 9      MMA issuer: S = Q K^T from shared memory, O += P V with P from tensor memory
+// While one group works on its scores the tensor cores work for the other. In the form for many rows ("pairs") the groups have a tile of 128 rows of
+// queries each; in the form for few rows they share one and take the tiles of keys in turn, and their results are joined at the end. There the keys may also be cut into
+// parts for several CTAs, whose results a second kernel joins.
+// Rows behind a tile's last are whatever shared memory held: they reach only results that nobody stores. Values behind a sequence's last key may be
+// anything (0 * NaN is NaN): zeros are written over them in shared memory.
+// Every wait is bounded; on expiry the kernel records a status, waits for its copies and products in flight, frees its tensor memory and returns.
+#include "attention.cuh"
+
+namespace b200 {
+
+using namespace attn;
+
+namespace {
+
+constexpr uint32_t kTmemCols = 512;
+constexpr float kLag = 8.0f;   // by how many powers of two a score may pass the running maximum
+
+template <int DP, bool PAIRS> struct ForwardShape {
+  static constexpr uint32_t kTileBytes = DP / 64 * kHalfTile;
+  static constexpr int kQTiles = PAIRS ? 2 : 1;
+  static constexpr int kStages = (PAIRS ? 4 : 6) * (DP == 64 ? 2 : 1) - (!PAIRS && DP == 64 ? 1 : 0);
+  static constexpr uint32_t kRing = kQTiles * kTileBytes, kCtrl = kRing + kStages * kTileBytes;
+  static constexpr size_t kBytes = 1024 + kCtrl + 1024;
+  static_assert(kBytes <= 227 * 1024, "shared memory");
+  // the joined form hands 128 rows of DP fp32 sums, their maxima and sums over
+  static_assert(PAIRS || (DP * 128 * 4 + 1024 <= kStages * kTileBytes), "shared memory");
+};
+
+// The order in which tiles of keys and values go through the ring: K0 V0 K1 V1 ... where one tile serves both groups, K0 K1 V0 K2 V1 K3 ... where the groups take turns.
+template <bool PAIRS> __device__ __forceinline__ int placeOfK(int i) { return PAIRS ? 2 * i : i < 2 ? i : 2 * i - 1; }
+template <bool PAIRS> __device__ __forceinline__ int placeOfV(int i, int n) { return PAIRS ? 2 * i + 1 : min(i + 2, n) + i; }
+
+template <typename T, int DP, bool PAIRS>
+__global__ void __launch_bounds__(kThreads, 1)
+attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnArgs a) {
+  using Shape = ForwardShape<DP, PAIRS>;
+  constexpr int kStages = Shape::kStages;
+  constexpr uint32_t kTileBytes = Shape::kTileBytes;
+  extern __shared__ uint8_t smemRaw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smemRaw + 1023) & ~(uintptr_t)1023);
+  uint64_t* fullBar = (uint64_t*)(smem + Shape::kCtrl);   // [kStages]
+  uint64_t* emptyBar = fullBar + kStages;                 // [kStages]
+  uint64_t* qBar = emptyBar + kStages;                    // [2]
+  uint64_t* scoreBar = qBar + 2;                          // [2] scores of a group are there
+  uint64_t* probBar = scoreBar + 2;                       // [2] its probabilities are
+  uint64_t* outBar = probBar + 2;                         // [2] its sums are complete
+  uint64_t* fixBar = outBar + 2;                          // the last values have zeros behind them
+  uint64_t* drainBar = fixBar + 1;
+  uint32_t* tmemSlot = (uint32_t*)(drainBar + 1);
+  volatile uint32_t* abortFlag = tmemSlot + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) { mbarInit(smemAddr(&fullBar[s]), 1); mbarInit(smemAddr(&emptyBar[s]), 1); }
+    for (int t = 0; t < 2; ++t) { mbarInit(smemAddr(&qBar[t]), 1); mbarInit(smemAddr(&scoreBar[t]), 1); mbarInit(smemAddr(&probBar[t]), 4); mbarInit(smemAddr(&outBar[t]), 1); }
+    mbarInit(smemAddr(fixBar), 1);
+    mbarInit(smemAddr(drainBar), 1);
+    *abortFlag = 0;
+    mbarInitFence();
+  }
+  if (warp == kMmaWarp) {
+    tmemAlloc(smemAddr(tmemSlot), kTmemCols);
+    tmemRelinquish();
+  }
+  tcFenceBefore();
+  __syncthreads();
+  tcFenceAfter();
+  const uint32_t tmem = *tmemSlot;
+  pdlEnter();   // the set-up above overlaps the end of the kernel before
+
+  // ---- this CTA's share: the tiles of queries with the most visible keys come first
+  const unsigned owners = a.batch * a.kvHeads, owner = blockIdx.x % owners, share = blockIdx.x / owners;
+  const int kvHead = owner % a.kvHeads, b = owner / a.kvHeads, part = PAIRS ? 0 : share % a.splits;
+  const int tile0 = (int)(gridDim.x / owners - 1 - share) / (PAIRS ? 1 : a.splits) * Shape::kQTiles;
+  const Sequence seq = sequenceOf(a, b);
+  int begin = 0, n = 0, count[2];   // tiles of keys: the first of this part, how many for both groups, and for each
+  int tok0[2];
+  if (PAIRS) {
+    for (int t = 0; t < 2; ++t) {
+      tok0[t] = (tile0 + t) * a.tileTokens;
+      const int last = min(tok0[t] + a.tileTokens, seq.q) - 1;
+      count[t] = last < tok0[t] ? 0 : (visibleOf(a, seq, last) + 127) / 128;
+      n = max(n, count[t]);
+    }
+  } else {
+    tok0[0] = tok0[1] = tile0 * a.tileTokens;
+    const int last = min(tok0[0] + a.tileTokens, seq.q) - 1;
+    const int all = last < tok0[0] ? 0 : (visibleOf(a, seq, last) + 127) / 128;
+    const int each = (all + a.splits - 1) / a.splits;
+    begin = min(all, part * each);
+    n = min(all, begin + each) - begin;
+    count[0] = (n + 1) / 2;
+    count[1] = n / 2;
+  }
+  // values behind the sequence's last: the tensor map gives zeros behind the tensor's last
+  const int fixTile = seq.kv < a.kv && seq.kv % 128 ? seq.kv / 128 - begin : -1;
+  const uint32_t smem0 = smemAddr(smem);
+  auto fail = [&](uint32_t what) {
+    *abortFlag = 1;
+    reportTimeout(a.status, what);
+  };
+
+  if (warp == kProducerWarp) {
+    uint32_t armed = 0, qArmed = 0;   // bits: stages and tiles of queries on their way
+    int place = 0;
+    bool ok = true;
+    auto next = [&](const CUtensorMap* map, int tile) {
+      const int s = place % kStages;
+      const uint32_t ph = (place / kStages) & 1;
+      ok = ok && warpWaitOr(smemAddr(&emptyBar[s]), ph ^ 1, abortFlag);
+      if (!ok) {
+        if (lane == 0) fail(1000 + s);
+        return;
+      }
+      if (lane == 0) {
+        const uint32_t bar = smemAddr(&fullBar[s]);
+        mbarExpectTx(bar, kTileBytes);
+        loadTile<DP>(smem0 + Shape::kRing + s * kTileBytes, map, (begin + tile) * 128, kvHead, b, bar);
+      }
+      armed |= 1u << s;
+      ++place;
+    };
+    if (n > 0) {
+      if (lane == 0)
+        for (int t = 0; t < Shape::kQTiles; ++t) {
+          if (!count[t]) continue;
+          mbarExpectTx(smemAddr(&qBar[t]), DP / 64 * a.tileTokens * a.group * 128);
+          loadTile<DP>(smem0 + t * kTileBytes, &tmQ, tok0[t], kvHead * a.group, b, smemAddr(&qBar[t]));
+        }
+      for (int t = 0; t < Shape::kQTiles; ++t) qArmed |= count[t] ? 1u << t : 0u;
+      if (PAIRS) {
+        for (int i = 0; i < n && ok; ++i) {
+          next(&tmK, i);
+          if (ok) next(&tmV, i);
+        }
+      } else {
+        for (int i = 0; i < min(n, 2) && ok; ++i) next(&tmK, i);
+        for (int i = 0; i < n && ok; ++i) {
+          next(&tmV, i);
+          if (ok && i + 2 < n) next(&tmK, i + 2);
+        }
+      }
+      if (ok && fixTile >= 0 && fixTile < n) {
+        const int at = placeOfV<PAIRS>(fixTile, n), s = at % kStages;   // the last tile: its stage is not used again
+        ok = warpWaitOr(smemAddr(&fullBar[s]), (at / kStages) & 1, abortFlag);
+        if (ok) {
+          clearRows<DP>(smem + Shape::kRing + s * kTileBytes, seq.kv % 128, lane);
+          if (lane == 0) mbarArrive(smemAddr(fixBar));
+        } else if (lane == 0) {
+          fail(1100);
+        }
+      }
+      if (__any_sync(~0u, *abortFlag)) {
+        // copies already issued still write into this CTA's shared memory: wait for them (bounded)
+        for (int s = 0; s < kStages; ++s)
+          if (armed >> s & 1) mbarWait(smemAddr(&fullBar[s]), (uint32_t)((place - 1 - (place - 1 - s + kStages) % kStages) / kStages) & 1, 1u << 20);
+        for (int t = 0; t < 2; ++t)
+          if (qArmed >> t & 1) mbarWait(smemAddr(&qBar[t]), 0, 1u << 20);
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    if (n > 0 && electOne()) {
+      bool ok = true;
+      auto need = [&](bool got, uint32_t what) {
+        if (ok && !got) fail(what);
+        ok = ok && got;
+        return ok;
+      };
+      auto full = [&](int place) { return need(waitOr(smemAddr(&fullBar[place % kStages]), (place / kStages) & 1, abortFlag), 2000 + place % kStages); };
+      auto tileAt = [&](int place) { return smem0 + Shape::kRing + (place % kStages) * kTileBytes; };
+      auto scores = [&](int t, int tile) {   // S of group t
+        const int at = placeOfK<PAIRS>(tile);
+        if (!full(at)) return;
+        tcFenceAfter();
+        productOfTiles<T, DP>(tmem + t * 128, smem0 + (PAIRS ? t : 0) * kTileBytes, tileAt(at));
+        ummaCommit(smemAddr(&scoreBar[t]));
+        if (!PAIRS) ummaCommit(smemAddr(&emptyBar[at % kStages]));
+      };
+      for (int t = 0; t < 2 && ok; ++t) {
+        if (!count[t]) continue;
+        if ((PAIRS || t == 0) && !need(waitOr(smemAddr(&qBar[t]), 0, abortFlag), 2100)) break;
+        scores(t, PAIRS ? 0 : t);
+      }
+      if (PAIRS && ok) ummaCommit(smemAddr(&emptyBar[0]));
+      for (int i = 0; i < (PAIRS ? n : count[0]) && ok; ++i) {
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (i >= count[t]) continue;
+          const int tile = PAIRS ? i : 2 * i + t, at = placeOfV<PAIRS>(tile, n);
+          if (!full(at)) break;
+          if (tile == fixTile && !need(waitOr(smemAddr(fixBar), 0, abortFlag), 2200)) break;
+          if (!need(waitOr(smemAddr(&probBar[t]), i & 1, abortFlag), 2300 + t)) break;
+          tcFenceAfter();
+          productWithTmem<T, DP>(tmem + 256 + t * 128, tmem + t * 128, tmem + t * 128 + 32, tileAt(at), i != 0);
+          if (!PAIRS) ummaCommit(smemAddr(&emptyBar[at % kStages]));
+          if (i + 1 == count[t]) ummaCommit(smemAddr(&outBar[t]));
+          else scores(t, PAIRS ? i + 1 : tile + 2);   // over the probabilities: products are carried out in order
+        }
+        if (PAIRS && ok) {
+          ummaCommit(smemAddr(&emptyBar[placeOfV<true>(i, n) % kStages]));
+          if (i + 1 < n) ummaCommit(smemAddr(&emptyBar[placeOfK<true>(i + 1) % kStages]));
+        }
+      }
+      if (!ok) {   // products in flight still read shared memory and write tensor memory
+        ummaCommit(smemAddr(drainBar));
+        mbarWait(smemAddr(drainBar), 0, 1u << 20);
+      }
+    }
+  } else {
+    const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t tS = tmem + lanes + t * 128, tO = tmem + lanes + 256 + t * 128;
+    const int rows = a.tileTokens * a.group;
+    const bool working = quarter * 32 < rows;   // a warp without rows only keeps step
+    const int tok = tok0[t] + row / a.group, head = kvHead * a.group + row % a.group;
+    const bool valid = row < rows && tok < seq.q, exists = row < rows && tok < a.q;
+    const int limit = valid ? visibleOf(a, seq, tok) : 0x7fffffff;   // (rows that nobody stores are not masked)
+    const float c = a.scale * kLog2e;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int i = 0; i < count[t]; ++i) {
+      ok = warpWaitOr(smemAddr(&scoreBar[t]), i & 1, abortFlag);
+      if (!ok) {
+        if (lane == 0) fail(3000 + t);
+        break;
+      }
+      tcFenceAfter();
+      if (working) {
+        uint32_t s[4][32];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tmemLd32(tS + k * 32, s[k]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tmemLdWait32(s[k]);
+        const int k0 = (begin + (PAIRS ? i : 2 * i + t)) * 128;
+        if (__any_sync(~0u, limit < k0 + 128)) {
+#pragma unroll
+          for (int k = 0; k < 128; ++k)
+            if (k0 + k >= limit) s[k / 32][k % 32] = __float_as_uint(-INFINITY);
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) top[u] = fmaxf(top[u], __uint_as_float(s[u][k]));
+        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        const bool raise = (mx - m) * c > kLag;   // (nothing seen so far and nothing now: NaN, no)
+        if (__any_sync(~0u, raise)) {
+          const float to = raise ? mx : m, factor = raise ? exp2Fast((m - to) * c) : 1.0f;
+          m = to;
+          l *= factor;
+          if (i > 0) {
+            // the products that wrote these sums were issued, and finished, in front of the scores
+#pragma unroll
+            for (int k = 0; k < DP / 32; ++k) {
+              uint32_t o[32];
+              tmemLd32(tO + k * 32, o);
+              tmemLdWait32(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+              tmemSt32(tO + k * 32, o);
+            }
+          }
+        }
+        const float shift = Pack<T>::kForwardBias - (m == -INFINITY ? 0.0f : m * c);
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t p[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            const float x = exp2Fast(fmaf(__uint_as_float(s[half * 2 + k / 16][k % 16 * 2]), c, shift));
+            const float y = exp2Fast(fmaf(__uint_as_float(s[half * 2 + k / 16][k % 16 * 2 + 1]), c, shift));
+            sum[k % 2 * 2] += x;
+            sum[k % 2 * 2 + 1] += y;
+            p[k] = Pack<T>::two(x, y);
+          }
+          tmemSt32(tS + half * 32, p);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmemStWait();
+      }
+      tcFenceBefore();
+      __syncwarp();
+      if (lane == 0) mbarArrive(smemAddr(&probBar[t]));
+    }
+    if (ok && count[t]) {
+      ok = warpWaitOr(smemAddr(&outBar[t]), 0, abortFlag);
+      if (!ok && lane == 0) fail(3100 + t);
+      tcFenceAfter();
+    }
+    float weight = 1.0f;   // of this group's sums
+    if (!PAIRS) {
+      // the second group hands its sums over: [channel][row], behind every copy and product of the CTA
+      float* sums = (float*)(smem + Shape::kRing);
+      float* ml = sums + DP * 128;
+      if (t == 1 && count[1] && ok) {
+        ok = warpWaitOr(smemAddr(&outBar[0]), 0, abortFlag);
+        if (!ok && lane == 0) fail(3200);
+      }
+      if (t == 1 && count[1] && ok && working) {
+#pragma unroll
+        for (int k = 0; k < DP / 32; ++k) {
+          uint32_t o[32];
+          tmemLd32(tO + k * 32, o);
+          tmemLdWait32(o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) sums[(k * 32 + e) * 128 + row] = __uint_as_float(o[e]);
+        }
+        ml[row] = m;
+        ml[128 + row] = l;
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (t == 0 && count[1]) {
+        const float m1 = ml[row], l1 = ml[128 + row], to = fmaxf(m, m1);
+        weight = m == to ? 1.0f : exp2Fast((m - to) * c);
+        const float other = m1 == to ? 1.0f : exp2Fast((m1 - to) * c);
+        l = l * weight + l1 * other;
+        m = to;
+        if (working)
+          for (int k = 0; k < DP; ++k) sums[k * 128 + row] *= other;
+      }
+    }
+    if ((PAIRS || t == 0) && !__any_sync(~0u, *abortFlag) && working) {
+      const float* sums = (const float*)(smem + Shape::kRing);
+      const bool empty = !valid || l == 0.0f;
+      const float inv = empty ? 0.0f : 1.0f / l;
+      const size_t at = ((size_t)b * a.q + tok) * a.heads + head;   // row of out
+      const size_t atLse = ((size_t)b * a.heads + head) * a.q + tok;
+      float lse = empty ? -INFINITY : fmaf(m, a.scale, logf(l) - Pack<T>::kForwardBias * kLn2);
+      float mine = inv, theirs = 0.0f;
+      const float* from = nullptr;
+      if (a.splits > 1) {
+        if (exists) a.partLse[(size_t)part * a.batch * a.q * a.heads + at] = lse;
+      } else {
+        if (a.joinOut && valid) {
+          const float other = a.joinLse[atLse], top = fmaxf(lse, other);
+          if (top != -INFINITY) {
+            const float x = expf(lse - top), y = expf(other - top), both = x + y;
+            lse = top + logf(both);
+            mine = inv * x / both;
+            theirs = y / both;
+            from = a.joinOut + at * a.dim;
+          }
+        }
+        if (exists) a.lse[atLse] = lse;
+      }
+#pragma unroll
+      for (int k = 0; k < DP / 32; ++k) {
+        uint32_t o[32];
+        float f[32];
+        if (count[0] || (PAIRS && count[t])) {
+          if (count[t]) {
+            tmemLd32(tO + k * 32, o);
+            tmemLdWait32(o);
+          }
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            f[e] = count[t] ? __uint_as_float(o[e]) * weight : 0.0f;
+            if (!PAIRS && count[1]) f[e] += sums[(k * 32 + e) * 128 + row];
+          }
+        }
+        if (!exists) continue;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) f[e] = empty || !count[t] ? 0.0f : f[e] * mine;
+        if (from) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            if (k * 32 + e >= a.dim) break;
+            const float4 v = *(const float4*)(from + k * 32 + e);
+            f[e] += theirs * v.x; f[e + 1] += theirs * v.y; f[e + 2] += theirs * v.z; f[e + 3] += theirs * v.w;
+          }
+        }
+        if (a.splits > 1 || a.outFp32) {
+          float* to = a.splits > 1 ? a.partOut + ((size_t)part * a.batch * a.q * a.heads + at) * a.dim : (float*)a.out + at * a.dim;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            if (k * 32 + e < a.dim) *(float4*)(to + k * 32 + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+        } else {
+          uint16_t* to = (uint16_t*)a.out + at * a.dim;
+#pragma unroll
+          for (int e = 0; e < 32; e += 8)
+            if (k * 32 + e < a.dim)
+              *(uint4*)(to + k * 32 + e) = make_uint4(Pack<T>::two(f[e], f[e + 1]), Pack<T>::two(f[e + 2], f[e + 3]), Pack<T>::two(f[e + 4], f[e + 5]), Pack<T>::two(f[e + 6], f[e + 7]));
+        }
+      }
+    }
+  }
+
+  // ---- teardown
+  tcFenceBefore();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tcFenceAfter();
+    tmemDealloc(tmem, kTmemCols);
+  }
+}
+
+// Joins the parts of the keys: out = sum_s exp(lse_s - L) out_s with L = ln sum_s exp(lse_s); what `join` names is one more part. A thread has four channels of a row.
+template <typename T>
+__global__ void __launch_bounds__(256) attnJoinKernel(const __grid_constant__ AttnArgs a) {
+  pdlEnter();
+  const int quads = a.dim / 4;
+  const size_t rows = (size_t)a.batch * a.q * a.heads, i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  const size_t row = i / quads;
+  const int d = (int)(i % quads) * 4;
+  if (row >= rows) return;
+  const int head = (int)(row % a.heads);
+  const size_t token = row / a.heads;   // of the batch
+  const int b = (int)(token / a.q), tok = (int)(token % a.q);
+  const size_t atLse = ((size_t)b * a.heads + head) * a.q + tok;
+  const bool join = a.joinOut && tok < (a.qLengths ? a.qLengths[b] : a.q);
+  float top = join ? a.joinLse[atLse] : -INFINITY, total = 0.0f;
+  const float other = top;
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.partLse[(size_t)s * rows + row]);
+  const float base = top == -INFINITY ? 0.0f : top;
+  float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int s = 0; s <= a.splits; ++s) {
+    if (s == a.splits && !join) break;
+    const float w = expf((s < a.splits ? a.partLse[(size_t)s * rows + row] : other) - base);
+    total += w;
+    if (w == 0.0f) continue;   // (a part that saw no key holds zeros)
+    const float4 v = *(const float4*)((s < a.splits ? a.partOut + ((size_t)s * rows + row) * a.dim : a.joinOut + row * a.dim) + d);
+    f.x += w * v.x; f.y += w * v.y; f.z += w * v.z; f.w += w * v.w;
+  }
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  f.x *= inv; f.y *= inv; f.z *= inv; f.w *= inv;
+  if (d == 0) a.lse[atLse] = total == 0.0f ? -INFINITY : base + logf(total);
+  if (a.outFp32) *(float4*)((float*)a.out + row * a.dim + d) = f;
+  else *(uint2*)((uint16_t*)a.out + row * a.dim + d) = make_uint2(Pack<T>::two(f.x, f.y), Pack<T>::two(f.z, f.w));
+}
+
+}  // namespace
+
+template <typename T> static const void* forwardFn(int dim, bool pairs) {
+  if (dim <= 64) return pairs ? (const void*)attnForwardKernel<T, 64, true> : (const void*)attnForwardKernel<T, 64, false>;
+  return pairs ? (const void*)attnForwardKernel<T, 128, true> : (const void*)attnForwardKernel<T, 128, false>;
+}
+const void* attnForwardKernelFn(int type, int dim, bool pairs) { return type == ATTN_F16 ? forwardFn<__half>(dim, pairs) : forwardFn<__nv_bfloat16>(dim, pairs); }
+size_t attnForwardSmemBytes(int dim, bool pairs) {
+  if (dim <= 64) return pairs ? ForwardShape<64, true>::kBytes : ForwardShape<64, false>::kBytes;
+  return pairs ? ForwardShape<128, true>::kBytes : ForwardShape<128, false>::kBytes;
+}
+const void* attnJoinKernelFn(int type) { return type == ATTN_F16 ? (const void*)attnJoinKernel<__half> : (const void*)attnJoinKernel<__nv_bfloat16>; }
+int attnThreads() { return kThreads; }
+
+}  // namespace b200

@@ -1,0 +1,493 @@
+// Host side of the context-parallel operators: checks of arguments, plans, tensor maps and launches. See include/nccl_cp.h for the API; the kernels are in
+// attention_forward.cu, attention_backward.cu and rotary.cu.
+#include "cp.h"
+
+#include <cuda.h>
+
+#include <algorithm>
+#include <cmath>
+#include <initializer_list>
+#include <new>
+
+#include "../comm/device_plane.h"
+#include "nccl_cp.h"
+
+using namespace b200;
+
+struct ncclCpContext {
+  ncclComm* comm = nullptr;
+  int smCount = 0;
+};
+
+// The context's GPU is the current one while this lives.
+namespace {
+struct OnDevice {
+  int before = -1, dev;
+  cudaError_t rc;
+  explicit OnDevice(int d) : dev(d) {
+    rc = cudaGetDevice(&before);
+    if (rc == cudaSuccess && before != dev) rc = cudaSetDevice(dev);
+  }
+  ~OnDevice() { if (before >= 0 && before != dev) cudaSetDevice(before); }
+};
+}  // namespace
+#define B200_ON_DEVICE(cp)               \
+  OnDevice onDevice((cp)->comm->cudaDev); \
+  CUDACHECK(onDevice.rc)
+
+static bool aligned(std::initializer_list<const void*> ps, size_t to) {
+  uintptr_t all = 0;
+  for (const void* p : ps) all |= (uintptr_t)p;
+  return all % to == 0;
+}
+
+static ncclResult_t launchCp(ncclCpContext* cp, const void* fn, unsigned grid, unsigned gridY, int threads, size_t smem, void** args, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr;
+  cfg.gridDim = dim3(grid, gridY);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  if (devPlanePdl()) {
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+  }
+  if (smem > 40000) CUDACHECK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const cudaError_t e = cudaLaunchKernelExC(&cfg, fn, args);
+  if (e != cudaSuccess) {
+    WARN("context-parallel kernel launch failed: %s", cudaGetErrorString(e));
+    (void)cudaGetLastError();
+    return ncclUnhandledCudaError;
+  }
+  if (cp->comm->devPlane) cp->comm->devPlane->launches++;
+  return ncclSuccess;
+}
+
+// ---------------------------------------------------------------- memory that tensors span
+namespace {
+struct Span {
+  const void* p;
+  size_t bytes;
+};
+}  // namespace
+static bool meets(const Span& a, const Span& b) {
+  return a.p && b.p && a.bytes && b.bytes && (uintptr_t)a.p < (uintptr_t)b.p + b.bytes && (uintptr_t)b.p < (uintptr_t)a.p + a.bytes;
+}
+static bool overlap(std::initializer_list<Span> outs, std::initializer_list<Span> ins) {
+  for (const Span* a = outs.begin(); a != outs.end(); ++a) {
+    for (const Span& b : ins)
+      if (meets(*a, b)) return true;
+    for (const Span* b = a + 1; b != outs.end(); ++b)
+      if (meets(*a, *b)) return true;
+  }
+  return false;
+}
+// [batch][tokens][heads][dim] with strides of the first three in elements.
+static Span spanOf(const void* p, int batch, int tokens, int heads, int dim, const long long* stride, size_t size) {
+  if (!p || batch <= 0 || tokens <= 0 || heads <= 0) return {p, 0};
+  return {p, ((size_t)(batch - 1) * stride[0] + (size_t)(tokens - 1) * stride[1] + (size_t)(heads - 1) * stride[2] + dim) * size};
+}
+
+// ---------------------------------------------------------------- attention
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiledFn encodeFn() {
+  static const EncodeTiledFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess) return (EncodeTiledFn)p;
+    (void)cudaGetLastError();
+    return (EncodeTiledFn) nullptr;
+  }();
+  return fn;
+}
+
+static bool isFp16(const ncclCpAttention_t* c) { return c->type == ncclFloat16; }
+
+// [batch][tokens][heads][dim], boxes of `boxTokens` tokens x `boxHeads` heads x 64 channels with 128-byte swizzle. A tensor without tokens is never read: its map names one.
+static ncclResult_t makeMap(CUtensorMap* map, const ncclCpAttention_t* c, const void* base, int tokens, int heads, const long long* stride, int boxTokens, int boxHeads) {
+  EncodeTiledFn enc = encodeFn();
+  if (!enc) { WARN("cuTensorMapEncodeTiled is not available"); return ncclUnhandledCudaError; }
+  const int sizes[3] = {heads, std::max(tokens, 1), c->batch};
+  cuuint64_t dims[4] = {(cuuint64_t)c->head_dim, (cuuint64_t)sizes[0], (cuuint64_t)sizes[1], (cuuint64_t)sizes[2]};
+  cuuint64_t strides[3];
+  for (int i = 0; i < 3; ++i) strides[i] = sizes[i] > 1 ? (cuuint64_t)stride[2 - i] * 2 : (cuuint64_t)c->head_dim * 2;   // (of one there is no next)
+  cuuint32_t box[4] = {64, (cuuint32_t)boxHeads, (cuuint32_t)boxTokens, 1}, estr[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, isFp16(c) ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) { WARN("cuTensorMapEncodeTiled failed (%d)", (int)r); return ncclUnhandledCudaError; }
+  return ncclSuccess;
+}
+
+static ncclResult_t checkShape(const char* what, const ncclCpAttention_t* c) {
+  if (!c || c->magic != NCCL_CP_MAGIC || c->size != sizeof(*c)) { WARN("%s: shape was not initialised", what); return ncclInvalidArgument; }
+  if (c->type != ncclFloat16 && c->type != ncclBfloat16) { WARN("%s: q, k and v must be fp16 or bf16", what); return ncclInvalidArgument; }
+  if (c->result_type != c->type && c->result_type != ncclFloat32) { WARN("%s: results must be of the inputs' type or fp32", what); return ncclInvalidArgument; }
+  if (c->batch < 0 || c->q_tokens < 0 || c->kv_tokens < 0 || c->heads <= 0 || c->kv_heads <= 0 || c->heads % c->kv_heads || c->heads / c->kv_heads > kAttnRows || c->head_dim <= 0 ||
+      c->head_dim % 8 || c->head_dim > kAttnMaxDim || c->q_tokens > kAttnMaxTokens || c->kv_tokens > kAttnMaxTokens) {
+    WARN("%s: batch %d, %d queries and %d keys (at most %d), %d heads over %d (at most %d to one), head_dim %d (a multiple of 8, at most %d)", what, c->batch, c->q_tokens, c->kv_tokens,
+         kAttnMaxTokens, c->heads, c->kv_heads, kAttnRows, c->head_dim, kAttnMaxDim);
+    return ncclInvalidArgument;
+  }
+  if (c->mask != NCCL_CP_FULL && c->mask != NCCL_CP_CAUSAL && c->mask != NCCL_CP_CAUSAL_END) { WARN("%s: unknown mask %d", what, (int)c->mask); return ncclInvalidArgument; }
+  if (!(c->scale > 0.0f) || !std::isfinite(c->scale)) { WARN("%s: scale must be positive and finite", what); return ncclInvalidArgument; }
+  // CTAs are counted with 31 bits, rows of a result with 40
+  const double tiles = (double)c->batch * c->kv_heads * ((double)c->q_tokens * (c->heads / c->kv_heads) + c->kv_tokens) / 64 + 1;
+  if (tiles * kAttnMaxSplits > 2147483647.0) { WARN("%s: too many tiles", what); return ncclInvalidArgument; }
+  return ncclSuccess;
+}
+
+// An operand as the tensor maps take it.
+static ncclResult_t checkOperand(const char* what, const char* name, const void* p, int batch, int tokens, int heads, const long long* stride) {
+  const int sizes[3] = {batch, tokens, heads};
+  bool ok = p && aligned({p}, 16);
+  for (int i = 0; i < 3; ++i)
+    if (sizes[i] > 1) ok = ok && stride[i] > 0 && stride[i] % 8 == 0 && stride[i] < 1ll << 38;
+  if (!ok) { WARN("%s: %s must be there, at 16 bytes, with positive strides of multiples of 8 elements", what, name); return ncclInvalidArgument; }
+  return ncclSuccess;
+}
+
+static void fillAttention(const ncclCpAttention_t* c, const int* qLengths, const int* kvLengths, AttnArgs* a) {
+  memset(a, 0, sizeof(*a));
+  a->batch = c->batch;
+  a->q = c->q_tokens;
+  a->kv = c->kv_tokens;
+  a->heads = c->heads;
+  a->kvHeads = c->kv_heads;
+  a->dim = c->head_dim;
+  a->group = c->heads / c->kv_heads;
+  a->tileTokens = std::min(kAttnRows / a->group, std::max(c->q_tokens, 1));
+  a->tiles = (c->q_tokens + a->tileTokens - 1) / a->tileTokens;
+  a->causal = (int)c->mask;
+  a->offset = (int)std::max<long long>(-(long long)c->q_tokens, std::min<long long>(c->offset, c->kv_tokens));   // further out nothing changes any more
+  a->scale = c->scale;
+  a->qLengths = qLengths;
+  a->kvLengths = kvLengths;
+  a->splits = 1;
+}
+
+// How a forward call is cut up.
+struct ForwardPlan {
+  bool pairs;
+  int splits;
+};
+static ForwardPlan forwardPlan(const ncclCpContext* cp, const ncclCpAttention_t* c) {
+  AttnArgs a;
+  fillAttention(c, nullptr, nullptr, &a);
+  const long long owners = (long long)c->batch * c->kv_heads, ctas = owners * a.tiles, kvTiles = (c->kv_tokens + 127) / 128;
+  ForwardPlan p;
+  p.pairs = (a.tiles + 1) / 2 * owners >= cp->smCount && a.tiles > 1;
+  p.splits = p.pairs || ctas >= cp->smCount || !ctas ? 1 : (int)std::max<long long>(1, std::min<long long>({cp->smCount / ctas, kvTiles / 2, kAttnMaxSplits}));
+  return p;
+}
+static size_t forwardWork(const ncclCpAttention_t* c, const ForwardPlan& p) {
+  return p.splits == 1 ? 0 : (size_t)p.splits * c->batch * c->q_tokens * c->heads * (c->head_dim + 1) * 4;
+}
+
+static size_t statsBytes(const AttnArgs& a) { return (size_t)a.batch * a.kvHeads * a.tiles * 256 * 4; }
+static size_t boundsBytes(const ncclCpAttention_t* c) { return isFp16(c) ? (size_t)c->batch * c->kv_heads * 8 : 0; }
+
+static ncclResult_t needsGpu(const ncclCpContext* cp, const char* what) {
+  if (cp->comm->compCap < 100) { WARN("%s needs compute capability 10.0 (found %d)", what, cp->comm->compCap); return ncclInvalidUsage; }
+  return ncclSuccess;
+}
+
+static ncclResult_t launchStats(ncclCpContext* cp, const ncclCpAttention_t* c, AttnStatsArgs* a, cudaStream_t stream) {
+  const size_t rows = (size_t)a->batch * a->kvHeads * a->tiles * kAttnRows + (a->bounds ? (size_t)a->batch * a->kv * a->kvHeads : 0);
+  if (!rows) return ncclSuccess;
+  void* args[1] = {a};
+  return launchCp(cp, attnStatsKernelFn(isFp16(c) ? ATTN_F16 : ATTN_BF16), (unsigned)((rows + 7) / 8), 1, 256, 0, args, stream);
+}
+
+static void fillStats(const ncclCpAttention_t* c, const AttnArgs& a, AttnStatsArgs* s) {
+  memset(s, 0, sizeof(*s));
+  s->batch = a.batch;
+  s->q = a.q;
+  s->kv = a.kv;
+  s->heads = a.heads;
+  s->kvHeads = a.kvHeads;
+  s->dim = a.dim;
+  s->group = a.group;
+  s->tileTokens = a.tileTokens;
+  s->tiles = a.tiles;
+  s->qLengths = a.qLengths;
+  s->kvLengths = a.kvLengths;
+  memcpy(s->doutStride, c->dout_stride, sizeof(s->doutStride));
+  memcpy(s->outStride, c->out_stride, sizeof(s->outStride));
+  memcpy(s->vStride, c->v_stride, sizeof(s->vStride));
+}
+
+extern "C" {
+
+ncclResult_t ncclCpCreate(ncclComm_t comm, ncclCp_t* out) {
+  if (!out) return ncclInvalidArgument;
+  *out = nullptr;
+  if (!commValid(comm) || comm->hostOnly) { WARN("ncclCpCreate needs a GPU communicator"); return ncclInvalidArgument; }
+  NCCLCHECK(commEnsureReady(comm));
+  int sms = 0;
+  CUDACHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, comm->cudaDev));
+  ncclCpContext* cp = new (std::nothrow) ncclCpContext;
+  if (!cp) return ncclSystemError;
+  cp->comm = comm;
+  cp->smCount = std::max(sms, 1);
+  *out = cp;
+  return ncclSuccess;
+}
+
+ncclResult_t ncclCpDestroy(ncclCp_t cp) {
+  delete cp;
+  return ncclSuccess;
+}
+
+size_t ncclCpAttentionWork(ncclCp_t cp, const ncclCpAttention_t* c) {
+  if (!cp || checkShape("ncclCpAttentionWork", c) != ncclSuccess) return 0;
+  return forwardWork(c, forwardPlan(cp, c));
+}
+
+ncclResult_t ncclCpAttention(ncclCp_t cp, const ncclCpAttention_t* c, const void* q, const void* k, const void* v, const int* qLengths, const int* kvLengths, const float* joinOut,
+                             const float* joinLse, void* out, float* lse, void* work, cudaStream_t stream) {
+  const char* what = "ncclCpAttention";
+  if (!cp) return ncclInvalidArgument;
+  NCCLCHECK(checkShape(what, c));
+  NCCLCHECK(needsGpu(cp, what));
+  if (!c->batch || !c->q_tokens) return ncclSuccess;
+  NCCLCHECK(checkOperand(what, "q", q, c->batch, c->q_tokens, c->heads, c->q_stride));
+  if (c->kv_tokens) {
+    NCCLCHECK(checkOperand(what, "k", k, c->batch, c->kv_tokens, c->kv_heads, c->k_stride));
+    NCCLCHECK(checkOperand(what, "v", v, c->batch, c->kv_tokens, c->kv_heads, c->v_stride));
+  } else {
+    k = v = q;   // not read
+  }
+  const ForwardPlan plan = forwardPlan(cp, c);
+  const size_t rows = (size_t)c->batch * c->q_tokens * c->heads, workBytes = forwardWork(c, plan), lengthBytes = (size_t)c->batch * 4;
+  if (!out || !lse || (workBytes && !work) || !joinOut != !joinLse || !aligned({out, joinOut}, 16) || !aligned({lse, joinLse, qLengths, kvLengths}, 4) || !aligned({work}, 256)) {
+    WARN("%s: out, lse and (for %zu bytes) work must be there and aligned, join_out and join_lse come as a pair", what, workBytes);
+    return ncclInvalidArgument;
+  }
+  const size_t outBytes = rows * c->head_dim * (c->result_type == ncclFloat32 ? 4 : 2);
+  const Span joined = {(const void*)joinOut == out && c->result_type == ncclFloat32 ? nullptr : joinOut, rows * c->head_dim * 4};   // a row is read before it is written, by the same thread
+  if (overlap({{out, outBytes}, {lse, rows * 4}, {workBytes ? work : nullptr, workBytes}},
+              {spanOf(q, c->batch, c->q_tokens, c->heads, c->head_dim, c->q_stride, 2), c->kv_tokens ? spanOf(k, c->batch, c->kv_tokens, c->kv_heads, c->head_dim, c->k_stride, 2) : Span{nullptr, 0},
+               c->kv_tokens ? spanOf(v, c->batch, c->kv_tokens, c->kv_heads, c->head_dim, c->v_stride, 2) : Span{nullptr, 0}, joined, {joinLse == lse ? nullptr : joinLse, rows * 4},
+               {qLengths, lengthBytes}, {kvLengths, lengthBytes}})) {
+    WARN("%s: an output shares memory with another tensor", what);
+    return ncclInvalidArgument;
+  }
+  AttnArgs a;
+  fillAttention(c, qLengths, kvLengths, &a);
+  a.out = out;
+  a.outFp32 = c->result_type == ncclFloat32;
+  a.lse = lse;
+  a.joinOut = joinOut;
+  a.joinLse = joinLse;
+  a.splits = plan.splits;
+  a.partOut = (float*)work;
+  a.partLse = (float*)work + (size_t)plan.splits * rows * c->head_dim;
+  a.status = cp->comm->devStatusDev;
+  const int type = isFp16(c) ? ATTN_F16 : ATTN_BF16;
+  B200_ON_DEVICE(cp);
+  CUtensorMap maps[3];
+  NCCLCHECK(makeMap(&maps[0], c, q, c->q_tokens, c->heads, c->q_stride, a.tileTokens, a.group));
+  NCCLCHECK(makeMap(&maps[1], c, k, c->kv_tokens, c->kv_heads, c->k_stride, kAttnRows, 1));
+  NCCLCHECK(makeMap(&maps[2], c, v, c->kv_tokens, c->kv_heads, c->v_stride, kAttnRows, 1));
+  void* args[4] = {&maps[0], &maps[1], &maps[2], &a};
+  const unsigned grid = (unsigned)c->batch * c->kv_heads * (plan.pairs ? (a.tiles + 1) / 2 : a.tiles) * plan.splits;
+  NCCLCHECK(launchCp(cp, attnForwardKernelFn(type, c->head_dim, plan.pairs), grid, 1, attnThreads(), attnForwardSmemBytes(c->head_dim, plan.pairs), args, stream));
+  if (plan.splits == 1) return ncclSuccess;
+  void* join[1] = {&a};
+  return launchCp(cp, attnJoinKernelFn(type), (unsigned)((rows * (c->head_dim / 4) + 255) / 256), 1, 256, 0, join, stream);
+}
+
+size_t ncclCpAttentionBackwardWork(ncclCp_t cp, const ncclCpAttention_t* c) {
+  if (!cp || checkShape("ncclCpAttentionBackwardWork", c) != ncclSuccess) return 0;
+  AttnArgs a;
+  fillAttention(c, nullptr, nullptr, &a);
+  return statsBytes(a) + boundsBytes(c);
+}
+
+ncclResult_t ncclCpAttentionBackward(ncclCp_t cp, const ncclCpAttention_t* c, const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
+                                     const float* delta, const int* qLengths, const int* kvLengths, const float* addDq, const float* addDk, const float* addDv, void* dq, void* dk,
+                                     void* dv, void* work, cudaStream_t stream) {
+  const char* what = "ncclCpAttentionBackward";
+  if (!cp) return ncclInvalidArgument;
+  NCCLCHECK(checkShape(what, c));
+  NCCLCHECK(needsGpu(cp, what));
+  if (!c->batch || (!c->q_tokens && !c->kv_tokens)) return ncclSuccess;
+  const bool some = c->q_tokens && c->kv_tokens;
+  const size_t rows = (size_t)c->batch * c->q_tokens * c->heads, cols = (size_t)c->batch * c->kv_tokens * c->kv_heads, lengthBytes = (size_t)c->batch * 4;
+  const size_t size = c->result_type == ncclFloat32 ? 4 : 2, D = c->head_dim;
+  AttnArgs a;
+  fillAttention(c, qLengths, kvLengths, &a);
+  const size_t workBytes = statsBytes(a) + boundsBytes(c);
+  if (c->q_tokens) {
+    NCCLCHECK(checkOperand(what, "q", q, c->batch, c->q_tokens, c->heads, c->q_stride));
+    NCCLCHECK(checkOperand(what, "d_out", dout, c->batch, c->q_tokens, c->heads, c->dout_stride));
+    if (!delta || out) NCCLCHECK(checkOperand(what, "out", out, c->batch, c->q_tokens, c->heads, c->out_stride));
+  }
+  if (c->kv_tokens) {
+    NCCLCHECK(checkOperand(what, "k", k, c->batch, c->kv_tokens, c->kv_heads, c->k_stride));
+    NCCLCHECK(checkOperand(what, "v", v, c->batch, c->kv_tokens, c->kv_heads, c->v_stride));
+  }
+  const bool adds = addDq || addDk || addDv;
+  if ((c->q_tokens && (!lse || !dq)) || (c->kv_tokens && (!dk || !dv)) || (workBytes && !work) || (adds && ((c->q_tokens && !addDq) || (c->kv_tokens && (!addDk || !addDv)))) ||
+      !aligned({dq, dk, dv, addDq, addDk, addDv}, 16) || !aligned({lse, delta, qLengths, kvLengths}, 4) || !aligned({work}, 256)) {
+    WARN("%s: lse, d_q, d_k, d_v and work must be there and aligned, add_dq, add_dk and add_dv come together", what);
+    return ncclInvalidArgument;
+  }
+  // a gradient's row is read before it is written, by the same thread
+  const auto added = [&](const float* p, const void* to, size_t n) { return Span{(const void*)p == to && size == 4 ? nullptr : p, n * D * 4}; };
+  const auto operand = [&](const void* p, int tokens, int heads, const long long* stride) { return tokens ? spanOf(p, c->batch, tokens, heads, c->head_dim, stride, 2) : Span{nullptr, 0}; };
+  if (overlap({{dq, rows * D * size}, {dk, cols * D * size}, {dv, cols * D * size}, {workBytes ? work : nullptr, workBytes}},
+              {operand(q, c->q_tokens, c->heads, c->q_stride), operand(dout, c->q_tokens, c->heads, c->dout_stride), operand(out, c->q_tokens, c->heads, c->out_stride),
+               operand(k, c->kv_tokens, c->kv_heads, c->k_stride), operand(v, c->kv_tokens, c->kv_heads, c->v_stride), {lse, rows * 4}, {delta, rows * 4}, {qLengths, lengthBytes},
+               {kvLengths, lengthBytes}, added(addDq, dq, rows), added(addDk, dk, cols), added(addDv, dv, cols)})) {
+    WARN("%s: an output shares memory with another tensor", what);
+    return ncclInvalidArgument;
+  }
+  const int type = isFp16(c) ? ATTN_F16 : ATTN_BF16;
+  a.gradFp32 = size == 4;
+  a.dq = dq;
+  a.dk = dk;
+  a.dv = dv;
+  a.addDq = addDq;
+  a.addDk = addDk;
+  a.addDv = addDv;
+  a.stats = (const float*)work;
+  a.bounds = isFp16(c) ? (const uint32_t*)((const char*)work + statsBytes(a)) : nullptr;
+  a.status = cp->comm->devStatusDev;
+  B200_ON_DEVICE(cp);
+  if (some) {
+    AttnStatsArgs s;
+    fillStats(c, a, &s);
+    s.dout = dout;
+    s.out = out;
+    s.v = v;
+    s.lse = lse;
+    s.delta = delta;
+    s.stats = (float*)work;
+    s.bounds = (uint32_t*)a.bounds;
+    if (s.bounds) CUDACHECK(cudaMemsetAsync(s.bounds, 0, boundsBytes(c), stream));
+    NCCLCHECK(launchStats(cp, c, &s, stream));
+  }
+  if (!c->q_tokens) q = dout = k;   // not read
+  if (!c->kv_tokens) k = v = q;
+  CUtensorMap maps[6];
+  NCCLCHECK(makeMap(&maps[0], c, q, c->q_tokens, c->heads, c->q_stride, a.tileTokens, a.group));
+  NCCLCHECK(makeMap(&maps[1], c, dout, c->q_tokens, c->heads, c->dout_stride, a.tileTokens, a.group));
+  NCCLCHECK(makeMap(&maps[2], c, k, c->kv_tokens, c->kv_heads, c->k_stride, kAttnRows, 1));
+  NCCLCHECK(makeMap(&maps[3], c, v, c->kv_tokens, c->kv_heads, c->v_stride, kAttnRows, 1));
+  void* args[5] = {&maps[0], &maps[1], &maps[2], &maps[3], &a};
+  const unsigned owners = (unsigned)c->batch * c->kv_heads, keyTiles = (c->kv_tokens + kAttnRows - 1) / kAttnRows;
+  if (c->kv_tokens) NCCLCHECK(launchCp(cp, attnBackwardKvKernelFn(type, c->head_dim), owners * keyTiles, 1, attnThreads(), attnBackwardSmemBytes(c->head_dim), args, stream));
+  if (c->q_tokens) NCCLCHECK(launchCp(cp, attnBackwardQKernelFn(type, c->head_dim), owners * a.tiles, 1, attnThreads(), attnBackwardSmemBytes(c->head_dim), args, stream));
+  return ncclSuccess;
+}
+
+ncclResult_t ncclCpAttentionDelta(ncclCp_t cp, const ncclCpAttention_t* c, const void* dout, const void* out, const int* qLengths, float* delta, cudaStream_t stream) {
+  const char* what = "ncclCpAttentionDelta";
+  if (!cp) return ncclInvalidArgument;
+  NCCLCHECK(checkShape(what, c));
+  if (!c->batch || !c->q_tokens) return ncclSuccess;
+  NCCLCHECK(checkOperand(what, "d_out", dout, c->batch, c->q_tokens, c->heads, c->dout_stride));
+  NCCLCHECK(checkOperand(what, "out", out, c->batch, c->q_tokens, c->heads, c->out_stride));
+  if (!delta || !aligned({delta, qLengths}, 4)) return ncclInvalidArgument;
+  if (overlap({{delta, (size_t)c->batch * c->q_tokens * c->heads * 4}}, {spanOf(dout, c->batch, c->q_tokens, c->heads, c->head_dim, c->dout_stride, 2),
+                                                                          spanOf(out, c->batch, c->q_tokens, c->heads, c->head_dim, c->out_stride, 2), {qLengths, (size_t)c->batch * 4}})) {
+    WARN("%s: delta shares memory with another tensor", what);
+    return ncclInvalidArgument;
+  }
+  AttnArgs a;
+  fillAttention(c, qLengths, nullptr, &a);
+  AttnStatsArgs s;
+  fillStats(c, a, &s);
+  s.dout = dout;
+  s.out = out;
+  s.deltaOut = delta;
+  B200_ON_DEVICE(cp);
+  return launchStats(cp, c, &s, stream);
+}
+
+// ---------------------------------------------------------------- rotary positions
+ncclResult_t ncclCpRotary(ncclCp_t cp, const ncclCpRotary_t* c, const void* x0, const void* x1, void* y0, void* y1, const void* positions, const double* turns, cudaStream_t stream) {
+  const char* what = "ncclCpRotary";
+  if (!cp) return ncclInvalidArgument;
+  if (!c || c->magic != NCCL_CP_MAGIC || c->size != sizeof(*c)) { WARN("%s: shape was not initialised", what); return ncclInvalidArgument; }
+  const int type = c->type == ncclFloat16 ? ATTN_F16 : c->type == ncclBfloat16 ? ATTN_BF16 : c->type == ncclFloat32 ? ATTN_F32 : -1;
+  if (type < 0) { WARN("%s: tensors must be fp16, bf16 or fp32", what); return ncclInvalidArgument; }
+  const int size = type == ATTN_F32 ? 4 : 2, E = 16 / size;
+  if (c->batch < 0 || c->tokens < 0 || c->head_dim <= 0 || c->half <= 0 || c->half > 512 || 2 * c->half > c->head_dim || c->heads[0] <= 0 || c->heads[1] < 0 || c->head_dim > 1 << 20 ||
+      (long long)c->batch * c->tokens > 0x7fffffff || ((long long)c->heads[0] + c->heads[1]) * c->head_dim > 1 << 30) {
+    WARN("%s: batch %d, %d tokens (2^31 together), %d and %d heads of %d channels, %d pairs (at most 512)", what, c->batch, c->tokens, c->heads[0], c->heads[1], c->head_dim, c->half);
+    return ncclInvalidArgument;
+  }
+  if (!std::isfinite(c->amplitude)) { WARN("%s: amplitude must be finite", what); return ncclInvalidArgument; }
+  if (!c->batch || !c->tokens) return ncclSuccess;
+  if (!x0 || !y0 || (c->heads[1] && (!x1 || !y1)) || !turns || !aligned({turns}, 8) || !aligned({positions}, c->positions64 ? 8 : 4) || !aligned({x0, y0, c->heads[1] ? x1 : nullptr, c->heads[1] ? y1 : nullptr}, size)) {
+    WARN("%s: tensors must be there and aligned to their elements", what);
+    return ncclInvalidArgument;
+  }
+  RotaryArgs a;
+  memset(&a, 0, sizeof(a));
+  Span in[2] = {}, out[2] = {};
+  bool inPlace[2] = {};
+  a.wide = c->head_dim % E == 0 && (c->interleaved ? 2 * c->half : c->half) % E == 0;
+  const int tensors = c->heads[1] ? 2 : 1;
+  for (int t = 0; t < tensors; ++t) {
+    a.x[t] = t ? x1 : x0;
+    a.y[t] = t ? y1 : y0;
+    a.heads[t] = c->heads[t];
+    const int sizes[3] = {c->batch, c->tokens, c->heads[t]};
+    inPlace[t] = a.x[t] == a.y[t];
+    for (int i = 0; i < 3; ++i) {
+      const long long xs = c->x_stride[t][i], ys = c->y_stride[t][i];
+      if (sizes[i] > 1) {
+        if (xs < 0 || xs >= 1ll << 40 || ys < c->head_dim || ys >= 1ll << 40) { WARN("%s: strides must not be negative, and rows of a result not overlap", what); return ncclInvalidArgument; }
+        a.wide = a.wide && xs % E == 0 && ys % E == 0;
+        inPlace[t] = inPlace[t] && xs == ys;
+      }
+      a.inStride[t][i] = sizes[i] > 1 ? xs : 0;
+      a.outStride[t][i] = sizes[i] > 1 ? ys : 0;
+    }
+    a.wide = a.wide && aligned({a.x[t], a.y[t]}, 16);
+    in[t] = spanOf(a.x[t], c->batch, c->tokens, c->heads[t], c->head_dim, a.inStride[t], size);
+    out[t] = spanOf(a.y[t], c->batch, c->tokens, c->heads[t], c->head_dim, a.outStride[t], size);
+  }
+  const Span other[2] = {{positions, (size_t)0}, {turns, (size_t)c->half * 8}};
+  for (int t = 0; t < tensors; ++t) {
+    bool bad = meets(out[t], other[1]);
+    if (positions) {
+      const long long s0 = c->batch > 1 ? c->position_stride[0] : 0, s1 = c->tokens > 1 ? c->position_stride[1] : 0;
+      if (s0 < 0 || s1 < 0 || s0 >= 1ll << 40 || s1 >= 1ll << 40) { WARN("%s: strides must not be negative", what); return ncclInvalidArgument; }
+      bad = bad || meets(out[t], {positions, ((size_t)(c->batch - 1) * s0 + (size_t)(c->tokens - 1) * s1 + 1) * (c->positions64 ? 8 : 4)});
+    }
+    // a tensor that is turned in place may lie between another's rows (one projection's queries and keys)
+    for (int u = 0; u < tensors; ++u) {
+      if (!inPlace[t]) bad = bad || meets(out[t], in[u]);
+      if (u != t && !(inPlace[t] && inPlace[u])) bad = bad || meets(out[t], out[u]);
+    }
+    if (bad) { WARN("%s: an output shares memory with another tensor", what); return ncclInvalidArgument; }
+  }
+  a.batch = c->batch;
+  a.tokens = c->tokens;
+  a.dim = c->head_dim;
+  a.half = c->half;
+  a.positions = positions;
+  a.positionStride[0] = c->position_stride[0];
+  a.positionStride[1] = c->position_stride[1];
+  a.positions64 = c->positions64;
+  a.offset = c->offset;
+  a.turns = turns;
+  a.amplitude = c->amplitude;
+  a.interleaved = c->interleaved != 0;
+  a.inverse = c->inverse != 0;
+  B200_ON_DEVICE(cp);
+  const int tokens = c->batch * c->tokens, items = (c->heads[0] + c->heads[1]) * (c->head_dim / (a.wide ? E : 1));
+  const int shares = std::max(1, std::min({cp->smCount / tokens, (items + 255) / 256, 64}));   // of a token, where tokens are few
+  void* args[1] = {&a};
+  return launchCp(cp, rotaryKernelFn(type), (unsigned)std::min(tokens, 1 << 20), (unsigned)shares, 256, 0, args, stream);
+}
+
+}  // extern "C"

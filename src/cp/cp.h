@@ -1,0 +1,83 @@
+// Internal interface between the host code of the context-parallel operators (cp.cc) and their kernels.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace b200 {
+
+constexpr int kAttnRows = 128;       // rows of a tile: (token, head of a group) pairs of queries, or keys
+constexpr int kAttnMaxDim = 128;     // channels of a head
+constexpr int kAttnMaxTokens = 1 << 30;
+constexpr int kAttnMaxSplits = 64;   // parts of the keys that CTAs work on at the same time
+
+// Rows of queries are packed: the heads that share keys and values lie next to each other, so that a tile holds `tileTokens` tokens of the `group` heads
+// of one key head, row = token * group + head. tileTokens * group <= 128; rows behind that are nobody's.
+struct AttnArgs {
+  int batch, q, kv, heads, kvHeads, dim;
+  int group, tileTokens;
+  int causal;                 // 0: no, 1: key j is visible to query i where j <= i + offset, 2: the same with offset = kv length - q length of the sequence
+  int offset;
+  float scale;
+  const int* qLengths;        // [batch] or null
+  const int* kvLengths;
+  // forward
+  void* out;                  // [batch][q][heads][dim], of the inputs' type or fp32
+  int outFp32;
+  float* lse;                 // [batch][heads][q]
+  const float* joinOut;       // what other keys gave, or null
+  const float* joinLse;
+  int splits;                 // above 1: fp32 results of each part of the keys go to partOut [splits][batch * q * heads][dim], partLse [splits][rows]
+  float* partOut;
+  float* partLse;
+  // backward
+  const float* stats;         // [batch][kvHeads][tiles][2][128]: log-sum-exp in units of log 2 and <d(out), out> of each row
+  int tiles;                  // of the queries of a key head
+  const uint32_t* bounds;     // fp16: [batch][kvHeads][2] squared norms of the longest rows of d(out) and v, as bits
+  void *dq, *dk, *dv;         // contiguous, of the inputs' type or fp32
+  int gradFp32;
+  const float *addDq, *addDk, *addDv;
+  uint32_t* status;           // {code, kind, what, CTA} of the communicator, written when a wait runs out
+};
+
+struct AttnStatsArgs {
+  const void *dout, *out, *v;
+  long long doutStride[3], outStride[3], vStride[3];   // batch, token, head
+  const float* lse;
+  const float* delta;         // [batch][heads][q], or null: computed here
+  float* deltaOut;            // only that, or null
+  float* stats;
+  uint32_t* bounds;           // fp16, else null
+  int batch, q, kv, heads, kvHeads, dim, group, tileTokens, tiles;
+  const int* qLengths;
+  const int* kvLengths;
+};
+
+struct RotaryArgs {
+  const void* x[2];           // [batch][tokens][heads][dim]
+  void* y[2];
+  long long inStride[2][3], outStride[2][3];           // batch, token, head
+  int heads[2];
+  const void* positions;      // [batch][tokens] of 32 or 64 bits, or null: offset + token
+  long long positionStride[2];
+  int positions64;
+  long long offset;
+  const double* turns;        // [half] turns of one step
+  float amplitude;
+  int batch, tokens, dim, half;
+  int interleaved, inverse;
+  int wide;                   // channels of a pack (16 bytes) may be moved together
+};
+
+enum AttnType : int { ATTN_F16 = 0, ATTN_BF16 = 1, ATTN_F32 = 2 };
+// dim <= 64 or <= 128. `pairs`: two tiles of queries for each CTA; else one, whose keys its two halves share.
+const void* attnForwardKernelFn(int type, int dim, bool pairs);
+size_t attnForwardSmemBytes(int dim, bool pairs);
+const void* attnJoinKernelFn(int type);
+const void* attnBackwardKvKernelFn(int type, int dim);
+const void* attnBackwardQKernelFn(int type, int dim);
+size_t attnBackwardSmemBytes(int dim);
+int attnThreads();
+const void* attnStatsKernelFn(int type);
+const void* rotaryKernelFn(int type);
+
+}  // namespace b200
