@@ -12,7 +12,14 @@ namespace attn {
 
 using namespace sm100;
 
-constexpr int kComputeWarps = 8, kProducerWarp = 8, kMmaWarp = 9, kThreads = 320;
+// Warps of a CTA: those that hold rows, then the producer, the issuer of products and two without a role (registers are dealt out to groups of four warps: they move
+// from the last group to those that hold rows).
+template <int COMPUTE, int LAUNCH, int FEW, int MANY> struct Warps {
+  static constexpr int kCompute = COMPUTE, kProducer = COMPUTE, kMma = COMPUTE + 1, kThreads = (COMPUTE + 4) * 32, kLaunchRegs = LAUNCH, kFewRegs = FEW, kManyRegs = MANY;
+  static_assert(COMPUTE % 4 == 0 && COMPUTE * MANY + 4 * FEW <= (COMPUTE + 4) * LAUNCH && (COMPUTE + 4) * 32 * LAUNCH <= 65536, "registers");
+};
+using ForwardWarps = Warps<8, 168, 80, 208>;
+using BackwardWarps = Warps<8, 168, 80, 208>;
 constexpr uint32_t kHalfTile = 128 * 128;          // bytes of 128 rows x 64 channels
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -38,42 +45,48 @@ template <typename T> constexpr uint32_t instr(int N, bool acrossB) {
   return (1u << 4) | (Pack<T>::kFormat << 7) | (Pack<T>::kFormat << 10) | ((acrossB ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
 }
 
-// A tile of 128 rows lies in boxes of 128 rows x 64 channels with 128-byte swizzle. As an operand whose sum runs over the channels it is umDescK128; as one whose
-// sum runs over the rows: the next 64 channels are a box further, the next 8 rows 1024 bytes.
-__device__ __forceinline__ uint64_t descAcross(uint32_t addr) {
-  uint64_t d = 0;
-  d |= (uint64_t)((addr & 0x3FFFF) >> 4);
-  d |= (uint64_t)(kHalfTile >> 4) << 16;
-  d |= (uint64_t)(1024 >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
-}
-__device__ __forceinline__ void mmaSS(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) { ummaBf16(d, a, b, idesc, accumulate); }   // (the type is in idesc)
-__device__ __forceinline__ void mmaTS(uint32_t d, uint32_t aTmem, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// A tile of 128 rows lies in boxes of 128 rows x 64 channels with 128-byte swizzle. As an operand whose sum runs over the channels: rows of 128 bytes, the next 8 of them 1024
+// bytes on. As one whose sum runs over the rows: the next 64 channels are a box further, the next 8 rows 1024 bytes. The lower word of a descriptor has the address in units of
+// 16 bytes (and the leading offset above it), so that steps along the sum add a constant to it; the upper word is the same for all.
+constexpr uint32_t kDescHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t descAlong(uint32_t addr) { return (addr & 0x3FFFF) >> 4 | 1u << 16; }
+__device__ __forceinline__ uint32_t descAcross(uint32_t addr) { return (addr & 0x3FFFF) >> 4 | (kHalfTile >> 4) << 16; }
+
+// The first step of a sum says at run time whether it is added to what is there, the others add.
+template <bool FIRST>
+__device__ __forceinline__ void mmaSS(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
   asm volatile(
-      "{\n.reg .pred p;\n"
-      "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
-      ::"r"(d), "r"(aTmem), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+      "{\n.reg .pred p;\n.reg .b64 x, y;\n"
+      "setp.ne.b32 p, %5, 0;\n"
+      "mov.b64 x, {%1, %4};\n"
+      "mov.b64 y, {%2, %4};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(kDescHigh), "n"(FIRST ? 0 : 1) : "memory");
 }
-// D[128 x 128] = A B^T over DP channels of two tiles in shared memory.
-template <typename T, int DP>
+__device__ __forceinline__ void mmaTS(uint32_t d, uint32_t aTmem, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\n.reg .b64 y;\n"
+      "setp.ne.b32 p, %5, 0;\n"
+      "mov.b64 y, {%2, %4};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}"
+      ::"r"(d), "r"(aTmem), "r"(b), "r"(idesc), "r"(kDescHigh), "r"(accumulate) : "memory");
+}
+// D[128 x N] = A B^T over DP channels of two tiles in shared memory, from the lower words of their descriptors (descAlong).
+template <typename T, int DP, int N = 128>
 __device__ __forceinline__ void productOfTiles(uint32_t d, uint32_t a, uint32_t b) {
-  const uint32_t idesc = instr<T>(128, false);
+  mmaSS<true>(d, a, b, instr<T>(N, false));
 #pragma unroll
-  for (int k = 0; k < DP / 16; ++k) {
-    const uint32_t at = (k / 4) * kHalfTile + (k % 4) * 32;
-    mmaSS(d, umDescK128(a + at), umDescK128(b + at), idesc, k != 0);
+  for (int k = 1; k < DP / 16; ++k) {
+    const uint32_t at = ((k / 4) * kHalfTile + (k % 4) * 32) >> 4;
+    mmaSS<false>(d, a + at, b + at, instr<T>(N, false));
   }
 }
-// D[128 x DP] (+)= A B with A [128 x 128] in tensor memory, 16 bits a value: columns [0, 64) of the sum at `a0`, the others at `a1`; B 128 rows of DP channels.
+// D[128 x DP] (+)= A B with A [128 x 128] in tensor memory, 16 bits a value, columns [0, 64) of the sum at `a`, the others 64 columns on; B (descAcross) 128 rows of DP channels.
 template <typename T, int DP>
-__device__ __forceinline__ void productWithTmem(uint32_t d, uint32_t a0, uint32_t a1, uint32_t b, bool accumulate) {
-  const uint32_t idesc = instr<T>(DP, true);
+__device__ __forceinline__ void productWithTmem(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
+  mmaTS(d, a, b, instr<T>(DP, true), accumulate);
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    mmaTS(d, (k < 4 ? a0 : a1) + (k % 4) * 8, descAcross(b + k * 2048), idesc, accumulate || k != 0);
+  for (int k = 1; k < 8; ++k) mmaTS(d, a + k / 4 * 64 + k % 4 * 8, b + (k * 2048 >> 4), instr<T>(DP, true), 1);
 }
 
 // ---------------------------------------------------------------- copies
@@ -116,6 +129,30 @@ __device__ __forceinline__ float exp2Fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float m;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
+// Two fp32 operations in one instruction, each rounded like the single one.
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t pair(float lo, float hi) { return packF32x2(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ float lowOf(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float highOf(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
 
 // ---------------------------------------------------------------- sequences
 struct Sequence {
@@ -151,6 +188,18 @@ __device__ __forceinline__ bool waitOr(uint32_t bar, uint32_t parity, volatile u
 // The same for a whole warp, with one answer.
 __device__ __forceinline__ bool warpWaitOr(uint32_t bar, uint32_t parity, volatile uint32_t* abortFlag) {
   return __all_sync(~0u, waitOr(bar, parity, abortFlag));
+}
+
+// A barrier of N threads that tells them all whether all are well.
+template <int N> __device__ __forceinline__ bool allWell(int id, bool well) {
+  uint32_t all;
+  asm volatile(
+      "{\n.reg .pred p, q;\n"
+      "setp.ne.u32 p, %3, 0;\n"
+      "barrier.cta.red.and.pred q, %1, %2, p;\n"
+      "selp.u32 %0, 1, 0, q;\n}"
+      : "=r"(all) : "r"(id), "n"(N), "r"((uint32_t)well) : "memory");
+  return all != 0;
 }
 
 }  // namespace attn

@@ -25,7 +25,7 @@ template <int DP> struct BackwardShape {
   static constexpr int kStages = DP == 64 ? 8 : 5;
   static constexpr uint32_t kRing = 2 * kTileBytes, kStats = kRing + kStages * kTileBytes, kCtrl = kStats + 2048;
   static constexpr size_t kBytes = kCtrl + 1024;   // (dynamic shared memory, all that these kernels have, begins on a multiple of 1024 bytes)
-  static_assert(kBytes <= 227 * 1024, "shared memory");
+  static_assert(kBytes <= 227 * 1024 && (2 * kStages + 11) * 8 + 8 <= 1024, "shared memory");
 };
 
 // The power of two that ds is multiplied by, in fp16: |ds| <= p (|do.v| + |do.o|) <= 2 |do| |v|.
@@ -67,8 +67,8 @@ __device__ __forceinline__ BackwardBars backwardSetUp(uint8_t* smem, int warp) {
     mbarInit(smemAddr(&s.first[0]), 1);
     mbarInit(smemAddr(&s.first[1]), 1);
     mbarInit(smemAddr(s.second), 1);
-    mbarInit(smemAddr(s.firstDone), kComputeWarps);
-    mbarInit(smemAddr(s.secondDone), kComputeWarps);
+    mbarInit(smemAddr(s.firstDone), BackwardWarps::kCompute);
+    mbarInit(smemAddr(s.secondDone), BackwardWarps::kCompute);
     mbarInit(smemAddr(s.outBar), 1);
     mbarInit(smemAddr(&s.fix[0]), 1);
     mbarInit(smemAddr(&s.fix[1]), 1);
@@ -76,7 +76,7 @@ __device__ __forceinline__ BackwardBars backwardSetUp(uint8_t* smem, int warp) {
     *s.abortFlag = 0;
     mbarInitFence();
   }
-  if (warp == kMmaWarp) {
+  if (warp == BackwardWarps::kMma) {
     tmemAlloc(smemAddr(s.tmemSlot), kTmemCols);
     tmemRelinquish();
   }
@@ -125,7 +125,7 @@ __device__ __forceinline__ void storeGradient(const AttnArgs& a, uint32_t tmem, 
 // probabilities are there, with the next tile's scores behind it; dk += dS q as soon as ds is, with the next do.v behind it. So the tensor cores work on one pair while
 // the other's elements are computed.
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(BackwardWarps::kThreads, 1)
 attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDo, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                      const __grid_constant__ AttnArgs a) {
   using Shape = BackwardShape<DP>;
@@ -136,10 +136,10 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   const BackwardBars s = backwardSetUp<DP>(smem, warp);
   volatile uint32_t* abortFlag = s.abortFlag;
   const int rows = a.tileTokens * a.group;
-  if (warp < kComputeWarps && rows < 128) {
+  if (warp < BackwardWarps::kCompute && rows < 128) {
     // rows of a tile that no copy writes are operands of sums over the rows: zero, for good
     const int each = (128 - rows) * 8;
-    for (int i = threadIdx.x; i < kStages * (DP / 64) * each; i += kComputeWarps * 32)
+    for (int i = threadIdx.x; i < kStages * (DP / 64) * each; i += BackwardWarps::kCompute * 32)
       *(uint4*)(smem + Shape::kRing + i / each * kHalfTile + rows * 128 + i % each * 16) = make_uint4(0, 0, 0, 0);
     fenceProxyAsync();
   }
@@ -164,7 +164,8 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     reportTimeout(a.status, what);
   };
 
-  if (warp == kProducerWarp) {
+  if (warp >= BackwardWarps::kCompute) regsGive<BackwardWarps::kFewRegs>();
+  if (warp == BackwardWarps::kProducer) {
     uint32_t armed = 0;
     int place = 0;
     bool ok = !*abortFlag, ownArmed = false;
@@ -221,7 +222,7 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         if (ownArmed) mbarWait(smemAddr(s.own), 0, 1u << 20);
       }
     }
-  } else if (warp == kMmaWarp) {
+  } else if (warp == BackwardWarps::kMma) {
     if (n > 0 && electOne()) {
       bool ok = true;
       auto need = [&](bool got, uint32_t what) {
@@ -235,14 +236,14 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         if (!full(2 * i)) return;
         if (fixRows && i == n - 1 && !need(waitOr(smemAddr(&s.fix[0]), 0, abortFlag), 2200)) return;
         tcFenceAfter();
-        productOfTiles<T, DP>(tmem, smem0, tileAt(2 * i));
+        productOfTiles<T, DP>(tmem, descAlong(smem0), descAlong(tileAt(2 * i)));
         ummaCommit(smemAddr(&s.first[0]));
       };
       auto doV = [&](int i) {
         if (!full(2 * i + 1)) return;
         if (fixRows && i == n - 1 && !need(waitOr(smemAddr(&s.fix[1]), 0, abortFlag), 2201)) return;
         tcFenceAfter();
-        productOfTiles<T, DP>(tmem + 128, smem0 + kTileBytes, tileAt(2 * i + 1));
+        productOfTiles<T, DP>(tmem + 128, descAlong(smem0 + kTileBytes), descAlong(tileAt(2 * i + 1)));
         ummaCommit(smemAddr(s.second));
       };
       if (need(waitOr(smemAddr(s.own), 0, abortFlag), 2100)) scores(0);
@@ -250,12 +251,12 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       for (int i = 0; i < n && ok; ++i) {
         if (!need(waitOr(smemAddr(s.firstDone), i & 1, abortFlag), 2300)) break;
         tcFenceAfter();
-        productWithTmem<T, DP>(tmem + 256, tmem, tmem + 64, tileAt(2 * i + 1), i != 0);
+        productWithTmem<T, DP>(tmem + 256, tmem, descAcross(tileAt(2 * i + 1)), i != 0);
         ummaCommit(smemAddr(&s.empty[(2 * i + 1) % kStages]));   // (its do.v was issued in front of this)
         if (i + 1 < n) scores(i + 1);
         if (!ok || !need(waitOr(smemAddr(s.secondDone), i & 1, abortFlag), 2400)) break;
         tcFenceAfter();
-        productWithTmem<T, DP>(tmem + 384, tmem + 128, tmem + 192, tileAt(2 * i), i != 0);
+        productWithTmem<T, DP>(tmem + 384, tmem + 128, descAcross(tileAt(2 * i)), i != 0);
         ummaCommit(smemAddr(&s.empty[2 * i % kStages]));
         if (i + 1 < n) doV(i + 1);
         else ummaCommit(smemAddr(s.outBar));
@@ -265,7 +266,8 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         mbarWait(smemAddr(s.drain), 0, 1u << 20);
       }
     }
-  } else {
+  } else if (warp < BackwardWarps::kCompute) {
+    regsTake<BackwardWarps::kManyRegs>();
     const int half = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, key = key0 + row;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tS = tmem + lanes + half * 64, tDp = tS + 128;
     const float c = a.scale * kLog2e, up = n > 0 ? gradScale<T>(a, b, kvHead) : 1.0f, down = up * exp2f(-Pack<T>::kBackwardBias);
@@ -352,7 +354,7 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 
   tcFenceBefore();
   __syncthreads();
-  if (warp == kMmaWarp) {
+  if (warp == BackwardWarps::kMma) {
     tcFenceAfter();
     tmemDealloc(tmem, kTmemCols);
   }
@@ -362,7 +364,7 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 // Tensor memory: scores [queries x keys] of two tiles at 0 and 128, do.v (then ds) at 256, dq at 384. Scores are two tiles ahead, so that exponentials are
 // computed while the tensor cores work on the tile before.
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(BackwardWarps::kThreads, 1)
 attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDo, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const __grid_constant__ AttnArgs a) {
   using Shape = BackwardShape<DP>;
@@ -391,7 +393,8 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     reportTimeout(a.status, what);
   };
 
-  if (warp == kProducerWarp) {
+  if (warp >= BackwardWarps::kCompute) regsGive<BackwardWarps::kFewRegs>();
+  if (warp == BackwardWarps::kProducer) {
     uint32_t armed = 0;
     int place = 0;
     bool ok = !*abortFlag, ownArmed = false;
@@ -440,7 +443,7 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         if (ownArmed) mbarWait(smemAddr(s.own), 0, 1u << 20);
       }
     }
-  } else if (warp == kMmaWarp) {
+  } else if (warp == BackwardWarps::kMma) {
     if (n > 0 && electOne()) {
       bool ok = true;
       auto need = [&](bool got, uint32_t what) {
@@ -455,14 +458,14 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         if (!full(2 * i)) return;
         if (fixed && i == n - 1 && !need(waitOr(smemAddr(&s.fix[0]), 0, abortFlag), 2200)) return;
         tcFenceAfter();
-        productOfTiles<T, DP>(tmem + (i & 1) * 128, smem0, tileAt(2 * i));
+        productOfTiles<T, DP>(tmem + (i & 1) * 128, descAlong(smem0), descAlong(tileAt(2 * i)));
         ummaCommit(smemAddr(&s.first[i & 1]));
       };
       auto doV = [&](int i) {
         if (!full(2 * i + 1)) return;
         if (fixed && i == n - 1 && !need(waitOr(smemAddr(&s.fix[1]), 0, abortFlag), 2201)) return;
         tcFenceAfter();
-        productOfTiles<T, DP>(tmem + 256, smem0 + kTileBytes, tileAt(2 * i + 1));
+        productOfTiles<T, DP>(tmem + 256, descAlong(smem0 + kTileBytes), descAlong(tileAt(2 * i + 1)));
         ummaCommit(smemAddr(s.second));
         ummaCommit(smemAddr(&s.empty[(2 * i + 1) % kStages]));
       };
@@ -472,7 +475,7 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       for (int i = 0; i < n && ok; ++i) {
         if (!need(waitOr(smemAddr(s.secondDone), i & 1, abortFlag), 2300)) break;
         tcFenceAfter();
-        productWithTmem<T, DP>(tmem + 384, tmem + 256, tmem + 320, tileAt(2 * i), i != 0);
+        productWithTmem<T, DP>(tmem + 384, tmem + 256, descAcross(tileAt(2 * i)), i != 0);
         ummaCommit(smemAddr(&s.empty[2 * i % kStages]));
         if (i + 1 < n) doV(i + 1);
         else ummaCommit(smemAddr(s.outBar));
@@ -483,7 +486,8 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         mbarWait(smemAddr(s.drain), 0, 1u << 20);
       }
     }
-  } else {
+  } else if (warp < BackwardWarps::kCompute) {
+    regsTake<BackwardWarps::kManyRegs>();
     const int half = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tDp = tmem + lanes + 256 + half * 64;
     const int tok = tok0 + row / a.group, head = kvHead * a.group + row % a.group;
@@ -554,7 +558,7 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 
   tcFenceBefore();
   __syncthreads();
-  if (warp == kMmaWarp) {
+  if (warp == BackwardWarps::kMma) {
     tcFenceAfter();
     tmemDealloc(tmem, kTmemCols);
   }
@@ -647,6 +651,8 @@ template <typename T> static const void* kvFn(int dim) { return dim <= 64 ? (con
 template <typename T> static const void* qFn(int dim) { return dim <= 64 ? (const void*)attnBackwardQKernel<T, 64> : (const void*)attnBackwardQKernel<T, 128>; }
 const void* attnBackwardKvKernelFn(int type, int dim) { return type == ATTN_F16 ? kvFn<__half>(dim) : kvFn<__nv_bfloat16>(dim); }
 const void* attnBackwardQKernelFn(int type, int dim) { return type == ATTN_F16 ? qFn<__half>(dim) : qFn<__nv_bfloat16>(dim); }
+int attnBackwardThreads() { return BackwardWarps::kThreads; }
+int attnBackwardRegs() { return BackwardWarps::kLaunchRegs; }
 size_t attnBackwardSmemBytes(int dim) { return dim <= 64 ? BackwardShape<64>::kBytes : BackwardShape<128>::kBytes; }
 const void* attnStatsKernelFn(int type) { return type == ATTN_F16 ? (const void*)attnStatsKernel<__half> : (const void*)attnStatsKernel<__nv_bfloat16>; }
 

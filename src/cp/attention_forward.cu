@@ -29,7 +29,8 @@ template <int DP, bool PAIRS> struct ForwardShape {
   static constexpr int kQTiles = PAIRS ? 2 : 1;
   static constexpr int kStages = (PAIRS ? 4 : 6) * (DP == 64 ? 2 : 1) - (!PAIRS && DP == 64 ? 1 : 0);
   static constexpr uint32_t kRing = kQTiles * kTileBytes, kCtrl = kRing + kStages * kTileBytes;
-  static constexpr size_t kBytes = 1024 + kCtrl + 1024;
+  static_assert((2 * kStages + 10) * 8 + 8 <= 512, "control block");
+  static constexpr size_t kBytes = kCtrl + 512;            // (dynamic shared memory, all that this kernel has, begins on a multiple of 1024 bytes)
   static_assert(kBytes <= 227 * 1024, "shared memory");
   // the joined form hands 128 rows of DP fp32 sums, their maxima and sums over
   static_assert(PAIRS || (DP * 128 * 4 + 1024 <= kStages * kTileBytes), "shared memory");
@@ -40,13 +41,13 @@ template <bool PAIRS> __device__ __forceinline__ int placeOfK(int i) { return PA
 template <bool PAIRS> __device__ __forceinline__ int placeOfV(int i, int n) { return PAIRS ? 2 * i + 1 : min(i + 2, n) + i; }
 
 template <typename T, int DP, bool PAIRS>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(ForwardWarps::kThreads, 1)
 attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnArgs a) {
   using Shape = ForwardShape<DP, PAIRS>;
+  using W = ForwardWarps;
   constexpr int kStages = Shape::kStages;
   constexpr uint32_t kTileBytes = Shape::kTileBytes;
-  extern __shared__ uint8_t smemRaw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smemRaw + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* fullBar = (uint64_t*)(smem + Shape::kCtrl);   // [kStages]
   uint64_t* emptyBar = fullBar + kStages;                 // [kStages]
   uint64_t* qBar = emptyBar + kStages;                    // [2]
@@ -67,7 +68,7 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     *abortFlag = 0;
     mbarInitFence();
   }
-  if (warp == kMmaWarp) {
+  if (warp == W::kMma) {
     tmemAlloc(smemAddr(tmemSlot), kTmemCols);
     tmemRelinquish();
   }
@@ -109,7 +110,8 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     reportTimeout(a.status, what);
   };
 
-  if (warp == kProducerWarp) {
+  if (warp >= W::kCompute) regsGive<W::kFewRegs>();
+  if (warp == W::kProducer) {
     uint32_t armed = 0, qArmed = 0;   // bits: stages and tiles of queries on their way
     int place = 0;
     bool ok = true;
@@ -167,7 +169,7 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           if (qArmed >> t & 1) mbarWait(smemAddr(&qBar[t]), 0, 1u << 20);
       }
     }
-  } else if (warp == kMmaWarp) {
+  } else if (warp == W::kMma) {
     if (n > 0 && electOne()) {
       bool ok = true;
       auto need = [&](bool got, uint32_t what) {
@@ -181,7 +183,7 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const int at = placeOfK<PAIRS>(tile);
         if (!full(at)) return;
         tcFenceAfter();
-        productOfTiles<T, DP>(tmem + t * 128, smem0 + (PAIRS ? t : 0) * kTileBytes, tileAt(at));
+        productOfTiles<T, DP>(tmem + t * 128, descAlong(smem0 + (PAIRS ? t : 0) * kTileBytes), descAlong(tileAt(at)));
         ummaCommit(smemAddr(&scoreBar[t]));
         if (!PAIRS) ummaCommit(smemAddr(&emptyBar[at % kStages]));
       };
@@ -199,7 +201,7 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           if (tile == fixTile && !need(waitOr(smemAddr(fixBar), 0, abortFlag), 2200)) break;
           if (!need(waitOr(smemAddr(&probBar[t]), i & 1, abortFlag), 2300 + t)) break;
           tcFenceAfter();
-          productWithTmem<T, DP>(tmem + 256 + t * 128, tmem + t * 128, tmem + t * 128 + 32, tileAt(at), i != 0);
+          productWithTmem<T, DP>(tmem + 256 + t * 128, tmem + t * 128, descAcross(tileAt(at)), i != 0);
           if (!PAIRS) ummaCommit(smemAddr(&emptyBar[at % kStages]));
           if (i + 1 == count[t]) ummaCommit(smemAddr(&outBar[t]));
           else scores(t, PAIRS ? i + 1 : tile + 2);   // over the probabilities: products are carried out in order
@@ -214,16 +216,17 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         mbarWait(smemAddr(drainBar), 0, 1u << 20);
       }
     }
-  } else {
+  } else if (warp < W::kCompute) {
+    regsTake<W::kManyRegs>();
     const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
-    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const uint32_t tS = tmem + lanes + t * 128, tO = tmem + lanes + 256 + t * 128;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tS = tmem + lanes + t * 128, tO = tmem + lanes + 256 + t * 128;
     const int rows = a.tileTokens * a.group;
     const bool working = quarter * 32 < rows;   // a warp without rows only keeps step
     const int tok = tok0[t] + row / a.group, head = kvHead * a.group + row % a.group;
     const bool valid = row < rows && tok < seq.q, exists = row < rows && tok < a.q;
     const int limit = valid ? visibleOf(a, seq, tok) : 0x7fffffff;   // (rows that nobody stores are not masked)
     const float c = a.scale * kLog2e;
+    const uint64_t c2 = pair(c, c);
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     for (int i = 0; i < count[t]; ++i) {
@@ -245,12 +248,14 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           for (int k = 0; k < 128; ++k)
             if (k0 + k >= limit) s[k / 32][k % 32] = __float_as_uint(-INFINITY);
         }
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        float top[4];
 #pragma unroll
-        for (int k = 0; k < 32; ++k)
+        for (int u = 0; u < 4; ++u) top[u] = fmaxf(__uint_as_float(s[u][0]), __uint_as_float(s[u][1]));
 #pragma unroll
-          for (int u = 0; u < 4; ++u) top[u] = fmaxf(top[u], __uint_as_float(s[u][k]));
-        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        for (int k = 2; k < 32; k += 2)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) top[u] = max3(top[u], __uint_as_float(s[u][k]), __uint_as_float(s[u][k + 1]));
+        const float mx = max3(fmaxf(top[0], top[1]), top[2], top[3]);
         const bool raise = (mx - m) * c > kLag;   // (nothing seen so far and nothing now: NaN, no)
         if (__any_sync(~0u, raise)) {
           const float to = raise ? mx : m, factor = raise ? exp2Fast((m - to) * c) : 1.0f;
@@ -270,21 +275,22 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
         }
         const float shift = Pack<T>::kForwardBias - (m == -INFINITY ? 0.0f : m * c);
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const uint64_t shift2 = pair(shift, shift);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           uint32_t p[32];
 #pragma unroll
           for (int k = 0; k < 32; ++k) {
-            const float x = exp2Fast(fmaf(__uint_as_float(s[half * 2 + k / 16][k % 16 * 2]), c, shift));
-            const float y = exp2Fast(fmaf(__uint_as_float(s[half * 2 + k / 16][k % 16 * 2 + 1]), c, shift));
-            sum[k % 2 * 2] += x;
-            sum[k % 2 * 2 + 1] += y;
-            p[k] = Pack<T>::two(x, y);
+            uint64_t x = fma2(packF32x2(s[half * 2 + k / 16][k % 16 * 2], s[half * 2 + k / 16][k % 16 * 2 + 1]), c2, shift2);
+            x = pair(exp2Fast(lowOf(x)), exp2Fast(highOf(x)));
+            sum[k % 2] = add2(sum[k % 2], x);
+            p[k] = Pack<T>::two(lowOf(x), highOf(x));
           }
-          tmemSt32(tS + half * 32, p);
+          tmemSt32(tS + half * 64, p);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        sum[0] = add2(sum[0], sum[1]);
+        l += lowOf(sum[0]) + highOf(sum[0]);
         tmemStWait();
       }
       tcFenceBefore();
@@ -293,18 +299,14 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
     if (ok && count[t]) {
       ok = warpWaitOr(smemAddr(&outBar[t]), 0, abortFlag);
+      if (ok && t == 1 && !PAIRS) ok = warpWaitOr(smemAddr(&outBar[0]), 0, abortFlag);
       if (!ok && lane == 0) fail(3100 + t);
       tcFenceAfter();
     }
-    float weight = 1.0f;   // of this group's sums
+    const float* sums = (const float*)(smem + Shape::kRing) + row;
+    const float* ml = (const float*)(smem + Shape::kRing) + DP * 128 + row;
     if (!PAIRS) {
       // the second group hands its sums over: [channel][row], behind every copy and product of the CTA
-      float* sums = (float*)(smem + Shape::kRing);
-      float* ml = sums + DP * 128;
-      if (t == 1 && count[1] && ok) {
-        ok = warpWaitOr(smemAddr(&outBar[0]), 0, abortFlag);
-        if (!ok && lane == 0) fail(3200);
-      }
       if (t == 1 && count[1] && ok && working) {
 #pragma unroll
         for (int k = 0; k < DP / 32; ++k) {
@@ -312,30 +314,28 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           tmemLd32(tO + k * 32, o);
           tmemLdWait32(o);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) sums[(k * 32 + e) * 128 + row] = __uint_as_float(o[e]);
+          for (int e = 0; e < 32; ++e) const_cast<float*>(sums)[(k * 32 + e) * 128] = __uint_as_float(o[e]);
         }
-        ml[row] = m;
-        ml[128 + row] = l;
+        const_cast<float*>(ml)[0] = m;
+        const_cast<float*>(ml)[128] = l;
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (t == 0 && count[1]) {
-        const float m1 = ml[row], l1 = ml[128 + row], to = fmaxf(m, m1);
-        weight = m == to ? 1.0f : exp2Fast((m - to) * c);
-        const float other = m1 == to ? 1.0f : exp2Fast((m1 - to) * c);
-        l = l * weight + l1 * other;
-        m = to;
-        if (working)
-          for (int k = 0; k < DP; ++k) sums[k * 128 + row] *= other;
-      }
+      ok = allWell<W::kCompute * 32>(1, ok);
     }
-    if ((PAIRS || t == 0) && !__any_sync(~0u, *abortFlag) && working) {
-      const float* sums = (const float*)(smem + Shape::kRing);
+    if ((PAIRS || t == 0) && ok && working) {
+      float weight = 1.0f, theirs = 0.0f;   // of this group's sums, and of the second's
+      if (!PAIRS && count[1]) {
+        const float m1 = ml[0], to = fmaxf(m, m1);
+        weight = m == to ? 1.0f : exp2Fast((m - to) * c);
+        theirs = m1 == to ? 1.0f : exp2Fast((m1 - to) * c);
+        l = l * weight + ml[128] * theirs;
+        m = to;
+      }
       const bool empty = !valid || l == 0.0f;
       const float inv = empty ? 0.0f : 1.0f / l;
       const size_t at = ((size_t)b * a.q + tok) * a.heads + head;   // row of out
       const size_t atLse = ((size_t)b * a.heads + head) * a.q + tok;
       float lse = empty ? -INFINITY : fmaf(m, a.scale, logf(l) - Pack<T>::kForwardBias * kLn2);
-      float mine = inv, theirs = 0.0f;
+      float share = inv, joined = 0.0f;
       const float* from = nullptr;
       if (a.splits > 1) {
         if (exists) a.partLse[(size_t)part * a.batch * a.q * a.heads + at] = lse;
@@ -345,8 +345,8 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           if (top != -INFINITY) {
             const float x = expf(lse - top), y = expf(other - top), both = x + y;
             lse = top + logf(both);
-            mine = inv * x / both;
-            theirs = y / both;
+            share = inv * x / both;
+            joined = y / both;
             from = a.joinOut + at * a.dim;
           }
         }
@@ -356,39 +356,37 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       for (int k = 0; k < DP / 32; ++k) {
         uint32_t o[32];
         float f[32];
-        if (count[0] || (PAIRS && count[t])) {
-          if (count[t]) {
-            tmemLd32(tO + k * 32, o);
-            tmemLdWait32(o);
-          }
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            f[e] = count[t] ? __uint_as_float(o[e]) * weight : 0.0f;
-            if (!PAIRS && count[1]) f[e] += sums[(k * 32 + e) * 128 + row];
-          }
+        if (count[t]) {
+          tmemLd32(tO + k * 32, o);
+          tmemLdWait32(o);
         }
         if (!exists) continue;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) f[e] = empty || !count[t] ? 0.0f : f[e] * mine;
+        for (int e = 0; e < 32; ++e) {
+          f[e] = count[t] ? __uint_as_float(o[e]) * weight : 0.0f;
+          if (!PAIRS && count[1]) f[e] += sums[(k * 32 + e) * 128] * theirs;
+          f[e] = empty || !count[t] ? 0.0f : f[e] * share;
+        }
+        const int channel = k * 32;
         if (from) {
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
-            if (k * 32 + e >= a.dim) break;
-            const float4 v = *(const float4*)(from + k * 32 + e);
-            f[e] += theirs * v.x; f[e + 1] += theirs * v.y; f[e + 2] += theirs * v.z; f[e + 3] += theirs * v.w;
+            if (channel + e >= a.dim) break;
+            const float4 v = *(const float4*)(from + channel + e);
+            f[e] += joined * v.x; f[e + 1] += joined * v.y; f[e + 2] += joined * v.z; f[e + 3] += joined * v.w;
           }
         }
         if (a.splits > 1 || a.outFp32) {
           float* to = a.splits > 1 ? a.partOut + ((size_t)part * a.batch * a.q * a.heads + at) * a.dim : (float*)a.out + at * a.dim;
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
-            if (k * 32 + e < a.dim) *(float4*)(to + k * 32 + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+            if (channel + e < a.dim) *(float4*)(to + channel + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
         } else {
           uint16_t* to = (uint16_t*)a.out + at * a.dim;
 #pragma unroll
           for (int e = 0; e < 32; e += 8)
-            if (k * 32 + e < a.dim)
-              *(uint4*)(to + k * 32 + e) = make_uint4(Pack<T>::two(f[e], f[e + 1]), Pack<T>::two(f[e + 2], f[e + 3]), Pack<T>::two(f[e + 4], f[e + 5]), Pack<T>::two(f[e + 6], f[e + 7]));
+            if (channel + e < a.dim)
+              *(uint4*)(to + channel + e) = make_uint4(Pack<T>::two(f[e], f[e + 1]), Pack<T>::two(f[e + 2], f[e + 3]), Pack<T>::two(f[e + 4], f[e + 5]), Pack<T>::two(f[e + 6], f[e + 7]));
         }
       }
     }
@@ -397,7 +395,7 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   // ---- teardown
   tcFenceBefore();
   __syncthreads();
-  if (warp == kMmaWarp) {
+  if (warp == W::kMma) {
     tcFenceAfter();
     tmemDealloc(tmem, kTmemCols);
   }
@@ -449,6 +447,7 @@ size_t attnForwardSmemBytes(int dim, bool pairs) {
   return pairs ? ForwardShape<128, true>::kBytes : ForwardShape<128, false>::kBytes;
 }
 const void* attnJoinKernelFn(int type) { return type == ATTN_F16 ? (const void*)attnJoinKernel<__half> : (const void*)attnJoinKernel<__nv_bfloat16>; }
-int attnThreads() { return kThreads; }
+int attnForwardThreads() { return ForwardWarps::kThreads; }
+int attnForwardRegs() { return ForwardWarps::kLaunchRegs; }
 
 }  // namespace b200

@@ -41,7 +41,8 @@ static bool aligned(std::initializer_list<const void*> ps, size_t to) {
   return all % to == 0;
 }
 
-static ncclResult_t launchCp(ncclCpContext* cp, const void* fn, unsigned grid, unsigned gridY, int threads, size_t smem, void** args, cudaStream_t stream) {
+// `regs`: what a thread of a kernel that moves registers between its warps has to be launched with.
+static ncclResult_t launchCp(ncclCpContext* cp, const void* fn, unsigned grid, unsigned gridY, int threads, size_t smem, void** args, cudaStream_t stream, int regs = 0) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr;
   cfg.gridDim = dim3(grid, gridY);
@@ -54,7 +55,13 @@ static ncclResult_t launchCp(ncclCpContext* cp, const void* fn, unsigned grid, u
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs = 1;
   }
-  if (smem > 40000) CUDACHECK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (regs) {
+    // registers that nobody was launched with would be waited for without end
+    cudaFuncAttributes built;
+    CUDACHECK(cudaFuncGetAttributes(&built, fn));
+    if (built.numRegs < regs) { WARN("an attention kernel was built with %d registers instead of %d", built.numRegs, regs); return ncclInternalError; }
+    CUDACHECK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  }
   const cudaError_t e = cudaLaunchKernelExC(&cfg, fn, args);
   if (e != cudaSuccess) {
     WARN("context-parallel kernel launch failed: %s", cudaGetErrorString(e));
@@ -295,7 +302,7 @@ ncclResult_t ncclCpAttention(ncclCp_t cp, const ncclCpAttention_t* c, const void
   NCCLCHECK(makeMap(&maps[2], c, v, c->kv_tokens, c->kv_heads, c->v_stride, kAttnRows, 1));
   void* args[4] = {&maps[0], &maps[1], &maps[2], &a};
   const unsigned grid = (unsigned)c->batch * c->kv_heads * (plan.pairs ? (a.tiles + 1) / 2 : a.tiles) * plan.splits;
-  NCCLCHECK(launchCp(cp, attnForwardKernelFn(type, c->head_dim, plan.pairs), grid, 1, attnThreads(), attnForwardSmemBytes(c->head_dim, plan.pairs), args, stream));
+  NCCLCHECK(launchCp(cp, attnForwardKernelFn(type, c->head_dim, plan.pairs), grid, 1, attnForwardThreads(), attnForwardSmemBytes(c->head_dim, plan.pairs), args, stream, attnForwardRegs()));
   if (plan.splits == 1) return ncclSuccess;
   void* join[1] = {&a};
   return launchCp(cp, attnJoinKernelFn(type), (unsigned)((rows * (c->head_dim / 4) + 255) / 256), 1, 256, 0, join, stream);
@@ -381,8 +388,8 @@ ncclResult_t ncclCpAttentionBackward(ncclCp_t cp, const ncclCpAttention_t* c, co
   NCCLCHECK(makeMap(&maps[3], c, v, c->kv_tokens, c->kv_heads, c->v_stride, kAttnRows, 1));
   void* args[5] = {&maps[0], &maps[1], &maps[2], &maps[3], &a};
   const unsigned owners = (unsigned)c->batch * c->kv_heads, keyTiles = (c->kv_tokens + kAttnRows - 1) / kAttnRows;
-  if (c->kv_tokens) NCCLCHECK(launchCp(cp, attnBackwardKvKernelFn(type, c->head_dim), owners * keyTiles, 1, attnThreads(), attnBackwardSmemBytes(c->head_dim), args, stream));
-  if (c->q_tokens) NCCLCHECK(launchCp(cp, attnBackwardQKernelFn(type, c->head_dim), owners * a.tiles, 1, attnThreads(), attnBackwardSmemBytes(c->head_dim), args, stream));
+  if (c->kv_tokens) NCCLCHECK(launchCp(cp, attnBackwardKvKernelFn(type, c->head_dim), owners * keyTiles, 1, attnBackwardThreads(), attnBackwardSmemBytes(c->head_dim), args, stream, attnBackwardRegs()));
+  if (c->q_tokens) NCCLCHECK(launchCp(cp, attnBackwardQKernelFn(type, c->head_dim), owners * a.tiles, 1, attnBackwardThreads(), attnBackwardSmemBytes(c->head_dim), args, stream, attnBackwardRegs()));
   return ncclSuccess;
 }
 

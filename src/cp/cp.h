@@ -76,7 +76,10 @@ const void* attnJoinKernelFn(int type);
 const void* attnBackwardKvKernelFn(int type, int dim);
 const void* attnBackwardQKernelFn(int type, int dim);
 size_t attnBackwardSmemBytes(int dim);
-int attnThreads();
+int attnForwardThreads();
+int attnBackwardThreads();
+int attnForwardRegs();     // that a thread is launched with
+int attnBackwardRegs();
 const void* attnStatsKernelFn(int type);
 const void* rotaryKernelFn(int type);
 
