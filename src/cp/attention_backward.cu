@@ -25,7 +25,7 @@ template <int DP> struct BackwardShape {
   static constexpr int kStages = DP == 64 ? 8 : 5;
   static constexpr uint32_t kRing = 2 * kTileBytes, kStats = kRing + kStages * kTileBytes, kCtrl = kStats + 2048;
   static constexpr size_t kBytes = kCtrl + 1024;   // (dynamic shared memory, all that these kernels have, begins on a multiple of 1024 bytes)
-  static_assert(kBytes <= 227 * 1024 && (2 * kStages + 11) * 8 + 8 <= 1024, "shared memory");
+  static_assert(kBytes <= 227 * 1024 && (2 * kStages + 12) * 8 + 8 <= 1024, "shared memory");
 };
 
 // The power of two that ds is multiplied by, in fp16: |ds| <= p (|do.v| + |do.o|) <= 2 |do| |v|.
@@ -52,11 +52,11 @@ __device__ __forceinline__ BackwardBars backwardSetUp(uint8_t* smem, int warp) {
   s.full = (uint64_t*)(smem + BackwardShape<DP>::kCtrl);
   s.empty = s.full + BackwardShape<DP>::kStages;
   s.own = s.empty + BackwardShape<DP>::kStages;
-  s.first = s.own + 1;           // [2] scores
-  s.second = s.first + 2;        // do.v
-  s.firstDone = s.second + 1;    // probabilities are in tensor memory
-  s.secondDone = s.firstDone + 1;
-  s.outBar = s.secondDone + 1;
+  s.first = s.own + 1;           // scores are there
+  s.second = s.first + 1;        // [2] do.v is, in each of its places
+  s.firstDone = s.second + 2;    // scores are used up
+  s.secondDone = s.firstDone + 1;   // [2] ds is in tensor memory, in each of its places
+  s.outBar = s.secondDone + 2;
   s.fix = s.outBar + 1;          // [2]
   s.drain = s.fix + 2;
   s.tmemSlot = (uint32_t*)(s.drain + 1);
@@ -64,11 +64,12 @@ __device__ __forceinline__ BackwardBars backwardSetUp(uint8_t* smem, int warp) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * BackwardShape<DP>::kStages; ++i) mbarInit(smemAddr(&s.full[i]), 1);
     mbarInit(smemAddr(s.own), 1);
-    mbarInit(smemAddr(&s.first[0]), 1);
-    mbarInit(smemAddr(&s.first[1]), 1);
-    mbarInit(smemAddr(s.second), 1);
+    mbarInit(smemAddr(s.first), 1);
     mbarInit(smemAddr(s.firstDone), BackwardWarps::kCompute);
-    mbarInit(smemAddr(s.secondDone), BackwardWarps::kCompute);
+    for (int i = 0; i < 2; ++i) {
+      mbarInit(smemAddr(&s.second[i]), 1);
+      mbarInit(smemAddr(&s.secondDone[i]), BackwardWarps::kCompute);
+    }
     mbarInit(smemAddr(s.outBar), 1);
     mbarInit(smemAddr(&s.fix[0]), 1);
     mbarInit(smemAddr(&s.fix[1]), 1);
@@ -237,7 +238,7 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         if (fixRows && i == n - 1 && !need(waitOr(smemAddr(&s.fix[0]), 0, abortFlag), 2200)) return;
         tcFenceAfter();
         productOfTiles<T, DP>(tmem, descAlong(smem0), descAlong(tileAt(2 * i)));
-        ummaCommit(smemAddr(&s.first[0]));
+        ummaCommit(smemAddr(s.first));
       };
       auto doV = [&](int i) {
         if (!full(2 * i + 1)) return;
@@ -271,42 +272,43 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const int half = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, key = key0 + row;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tS = tmem + lanes + half * 64, tDp = tS + 128;
     const float c = a.scale * kLog2e, up = n > 0 ? gradScale<T>(a, b, kvHead) : 1.0f, down = up * exp2f(-Pack<T>::kBackwardBias);
+    const uint64_t c2 = pair(c, c), down2 = pair(down, down);
     const bool valid = key < seq.kv;
     bool ok = true;
     for (int i = 0; i < n; ++i) {
-      const float* stats = (const float*)(smem + Shape::kStats + (i & 1) * 1024);   // lse [128], <do, o> [128]
-      ok = warpWaitOr(smemAddr(&s.full[(2 * i + 1) % kStages]), ((2 * i + 1) / kStages) & 1, abortFlag) && warpWaitOr(smemAddr(&s.first[0]), i & 1, abortFlag);
+      const float* stats = (const float*)(smem + Shape::kStats + (i & 1) * 1024);   // of the tile's rows: minus the log-sum-exp [128], minus <do, o> [128]
+      ok = warpWaitOr(smemAddr(&s.full[(2 * i + 1) % kStages]), ((2 * i + 1) / kStages) & 1, abortFlag) && warpWaitOr(smemAddr(s.first), i & 1, abortFlag);
       if (!ok) {
         if (lane == 0) fail(3000);
         break;
       }
       tcFenceAfter();
       const int tok0 = (begin + i) * a.tileTokens;
-      uint32_t x[2][32];
-      float p[64];
+      const bool hide = a.causal && tok0 + seq.offset < key0 + 127;
+      const int seen = key - seq.offset - tok0;   // the first token of the tile that sees this key
+      const int from = !hide || seen <= 0 ? 0 : min(seen, 128) * a.group;
+      uint32_t x[2][32], packed[32];
+      uint64_t p[32];
       tmemLd32(tS, x[0]);
-      tmemLd32(tS + 32, x[1]);
       tmemLdWait32(x[0]);
-      tmemLdWait32(x[1]);
+      tmemLd32(tS + 32, x[1]);
 #pragma unroll
-      for (int k = 0; k < 64; k += 4) {
-        const float4 lse = *(const float4*)(stats + half * 64 + k);
-        p[k] = exp2Fast(fmaf(__uint_as_float(x[k / 32][k % 32]), c, -lse.x));
-        p[k + 1] = exp2Fast(fmaf(__uint_as_float(x[k / 32][k % 32 + 1]), c, -lse.y));
-        p[k + 2] = exp2Fast(fmaf(__uint_as_float(x[k / 32][k % 32 + 2]), c, -lse.z));
-        p[k + 3] = exp2Fast(fmaf(__uint_as_float(x[k / 32][k % 32 + 3]), c, -lse.w));
+      for (int q = 0; q < 2; ++q) {
+        if (q) tmemLdWait32(x[1]);
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          const float4 lse = *(const float4*)(stats + half * 64 + q * 32 + k);
+          const uint64_t lo = fma2(packF32x2(x[q][k], x[q][k + 1]), c2, pair(lse.x, lse.y)), hi = fma2(packF32x2(x[q][k + 2], x[q][k + 3]), c2, pair(lse.z, lse.w));
+          p[q * 16 + k / 2] = pair(exp2Fast(lowOf(lo)), exp2Fast(highOf(lo)));
+          p[q * 16 + k / 2 + 1] = pair(exp2Fast(lowOf(hi)), exp2Fast(highOf(hi)));
+        }
       }
-      // the first token that sees this key
-      if (a.causal && tok0 + seq.offset < key0 + 127) {
-        const int seen = key - seq.offset - tok0;   // token of the tile
-        const int from = seen <= 0 ? 0 : min(seen, 128) * a.group;
+      if (hide) {
 #pragma unroll
-        for (int k = 0; k < 64; ++k)
-          if (half * 64 + k < from) p[k] = 0.0f;
+        for (int k = 0; k < 32; ++k) p[k] = pair(half * 64 + 2 * k < from ? 0.0f : lowOf(p[k]), half * 64 + 2 * k + 1 < from ? 0.0f : highOf(p[k]));
       }
-      uint32_t packed[32];
 #pragma unroll
-      for (int k = 0; k < 32; ++k) packed[k] = Pack<T>::two(p[2 * k], p[2 * k + 1]);
+      for (int k = 0; k < 32; ++k) packed[k] = Pack<T>::two(lowOf(p[k]), highOf(p[k]));
       tmemSt32(tS, packed);
       tmemStWait();
       tcFenceBefore();
@@ -319,21 +321,25 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
       tcFenceAfter();
       tmemLd32(tDp, x[0]);
-      tmemLd32(tDp + 32, x[1]);
       tmemLdWait32(x[0]);
-      tmemLdWait32(x[1]);
+      tmemLd32(tDp + 32, x[1]);
 #pragma unroll
-      for (int k = 0; k < 64; k += 4) {
-        const float4 delta = *(const float4*)(stats + 128 + half * 64 + k);
-        const float d[4] = {delta.x, delta.y, delta.z, delta.w};
+      for (int q = 0; q < 2; ++q) {
+        if (q) tmemLdWait32(x[1]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float dp = __uint_as_float(x[(k + e) / 32][(k + e) % 32]);
-          p[k + e] *= (dp - d[e]) * down;
+        for (int k = 0; k < 32; k += 4) {
+          const float4 delta = *(const float4*)(stats + 128 + half * 64 + q * 32 + k);
+          uint64_t lo = add2(packF32x2(x[q][k], x[q][k + 1]), pair(delta.x, delta.y)), hi = add2(packF32x2(x[q][k + 2], x[q][k + 3]), pair(delta.z, delta.w));
+          if (Pack<T>::kBackwardBias != 0.0f) {
+            lo = mul2(lo, down2);
+            hi = mul2(hi, down2);
+          }
+          lo = mul2(p[q * 16 + k / 2], lo);
+          hi = mul2(p[q * 16 + k / 2 + 1], hi);
+          packed[q * 16 + k / 2] = Pack<T>::two(lowOf(lo), highOf(lo));
+          packed[q * 16 + k / 2 + 1] = Pack<T>::two(lowOf(hi), highOf(hi));
         }
       }
-#pragma unroll
-      for (int k = 0; k < 32; ++k) packed[k] = Pack<T>::two(p[2 * k], p[2 * k + 1]);
       tmemSt32(tDp, packed);
       tmemStWait();
       tcFenceBefore();
@@ -361,14 +367,16 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 }
 
 // ---------------------------------------------------------------------------------------------- dq
-// Tensor memory: scores [queries x keys] of two tiles at 0 and 128, do.v (then ds) at 256, dq at 384. Scores are two tiles ahead, so that exponentials are
-// computed while the tensor cores work on the tile before.
+// Tensor memory: scores [queries x keys] at 0, do.v (then ds) of two tiles at 128 and 256, dq at 384. Scores are taken into registers at once, and the next tile's are made
+// while exponentials are computed; so is its do.v, in the other place. So products and elements of a tile do not wait for one another.
 template <typename T, int DP>
 __global__ void __launch_bounds__(BackwardWarps::kThreads, 1)
 attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDo, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const __grid_constant__ AttnArgs a) {
   using Shape = BackwardShape<DP>;
-  constexpr int kStages = Shape::kStages;
+  // Keys stay until their product with ds, values only until do.v: a ring for each, so that values come in early (in one ring of five stages the next do.v waited half of the
+  // time for values that could not be asked for before the last ds was used).
+  constexpr int kStages = Shape::kStages, kKeyStages = (kStages + 1) / 2, kValueStages = kStages - kKeyStages;
   constexpr uint32_t kTileBytes = Shape::kTileBytes;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -393,15 +401,16 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     reportTimeout(a.status, what);
   };
 
+  auto stageOf = [](int values, int tile) { return values ? kKeyStages + tile % kValueStages : tile % kKeyStages; };
+  auto phaseOf = [](int values, int tile) { return (uint32_t)(tile / (values ? kValueStages : kKeyStages)) & 1; };
+
   if (warp >= BackwardWarps::kCompute) regsGive<BackwardWarps::kFewRegs>();
   if (warp == BackwardWarps::kProducer) {
-    uint32_t armed = 0;
-    int place = 0;
+    int loaded[2] = {};   // keys, values
     bool ok = !*abortFlag, ownArmed = false;
-    auto next = [&](const CUtensorMap* map, int tile) {
-      const int at = place % kStages;
-      const uint32_t ph = (place / kStages) & 1;
-      ok = ok && warpWaitOr(smemAddr(&s.empty[at]), ph ^ 1, abortFlag);
+    auto next = [&](const CUtensorMap* map, int values) {
+      const int tile = loaded[values], at = stageOf(values, tile);
+      ok = ok && warpWaitOr(smemAddr(&s.empty[at]), phaseOf(values, tile) ^ 1, abortFlag);
       if (!ok) {
         if (lane == 0) fail(1000 + at);
         return;
@@ -411,8 +420,7 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         mbarExpectTx(bar, kTileBytes);
         loadTile<DP>(smem0 + Shape::kRing + at * kTileBytes, map, tile * 128, kvHead, b, bar);
       }
-      armed |= 1u << at;
-      ++place;
+      ++loaded[values];
     };
     if (n > 0) {
       if (ok && lane == 0) {
@@ -422,15 +430,15 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       }
       ownArmed = ok;
       for (int i = 0; i < n && ok; ++i) {
-        next(&tmK, i);
-        if (ok) next(&tmV, i);
+        next(&tmK, 0);
+        if (ok) next(&tmV, 1);
       }
       if (ok && fixTile >= 0 && fixTile == n - 1) {
         for (int k = 0; k < 2 && ok; ++k) {
-          const int at = place - 2 + k;
-          ok = warpWaitOr(smemAddr(&s.full[at % kStages]), (at / kStages) & 1, abortFlag);
+          const int at = stageOf(k, n - 1);
+          ok = warpWaitOr(smemAddr(&s.full[at]), phaseOf(k, n - 1), abortFlag);
           if (ok) {
-            clearRows<DP>(smem + Shape::kRing + at % kStages * kTileBytes, fixRows, lane);
+            clearRows<DP>(smem + Shape::kRing + at * kTileBytes, fixRows, lane);
             if (lane == 0) mbarArrive(smemAddr(&s.fix[k]));
           } else if (lane == 0) {
             fail(1100);
@@ -438,8 +446,9 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         }
       }
       if (__any_sync(~0u, *abortFlag)) {
-        for (int at = 0; at < kStages; ++at)
-          if (armed >> at & 1) mbarWait(smemAddr(&s.full[at]), (uint32_t)((place - 1 - (place - 1 - at + kStages) % kStages) / kStages) & 1, 1u << 20);
+        for (int values = 0; values < 2; ++values)
+          for (int tile = max(0, loaded[values] - (values ? kValueStages : kKeyStages)); tile < loaded[values]; ++tile)
+            mbarWait(smemAddr(&s.full[stageOf(values, tile)]), phaseOf(values, tile), 1u << 20);
         if (ownArmed) mbarWait(smemAddr(s.own), 0, 1u << 20);
       }
     }
@@ -451,36 +460,38 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         ok = ok && got;
         return ok;
       };
-      auto full = [&](int place) { return need(waitOr(smemAddr(&s.full[place % kStages]), (place / kStages) & 1, abortFlag), 2000 + place % kStages); };
-      auto tileAt = [&](int place) { return smem0 + Shape::kRing + (place % kStages) * kTileBytes; };
+      auto full = [&](int values, int tile) { return need(waitOr(smemAddr(&s.full[stageOf(values, tile)]), phaseOf(values, tile), abortFlag), 2000 + stageOf(values, tile)); };
+      auto tileAt = [&](int values, int tile) { return smem0 + Shape::kRing + stageOf(values, tile) * kTileBytes; };
       const bool fixed = fixTile == n - 1;
       auto scores = [&](int i) {
-        if (!full(2 * i)) return;
+        if (!full(0, i)) return;
         if (fixed && i == n - 1 && !need(waitOr(smemAddr(&s.fix[0]), 0, abortFlag), 2200)) return;
         tcFenceAfter();
-        productOfTiles<T, DP>(tmem + (i & 1) * 128, descAlong(smem0), descAlong(tileAt(2 * i)));
-        ummaCommit(smemAddr(&s.first[i & 1]));
+        productOfTiles<T, DP>(tmem, descAlong(smem0), descAlong(tileAt(0, i)));
+        ummaCommit(smemAddr(s.first));
       };
       auto doV = [&](int i) {
-        if (!full(2 * i + 1)) return;
+        if (!full(1, i)) return;
         if (fixed && i == n - 1 && !need(waitOr(smemAddr(&s.fix[1]), 0, abortFlag), 2201)) return;
         tcFenceAfter();
-        productOfTiles<T, DP>(tmem + 256, descAlong(smem0 + kTileBytes), descAlong(tileAt(2 * i + 1)));
-        ummaCommit(smemAddr(s.second));
-        ummaCommit(smemAddr(&s.empty[(2 * i + 1) % kStages]));
+        productOfTiles<T, DP>(tmem + 128 + (i & 1) * 128, descAlong(smem0 + kTileBytes), descAlong(tileAt(1, i)));
+        ummaCommit(smemAddr(&s.second[i & 1]));
+        ummaCommit(smemAddr(&s.empty[stageOf(1, i)]));
       };
       if (need(waitOr(smemAddr(s.own), 0, abortFlag), 2100)) scores(0);
       if (ok) doV(0);
-      if (ok && n > 1) scores(1);
       for (int i = 0; i < n && ok; ++i) {
-        if (!need(waitOr(smemAddr(s.secondDone), i & 1, abortFlag), 2300)) break;
+        if (i + 1 < n) {
+          if (!need(waitOr(smemAddr(s.firstDone), i & 1, abortFlag), 2400)) break;   // scores are in registers
+          scores(i + 1);
+          if (ok) doV(i + 1);   // over ds of the tile before, whose product is in front of this
+        }
+        if (!ok || !need(waitOr(smemAddr(&s.secondDone[i & 1]), i >> 1 & 1, abortFlag), 2300)) break;
         tcFenceAfter();
-        productWithTmem<T, DP>(tmem + 384, tmem + 256, descAcross(tileAt(2 * i)), i != 0);
-        ummaCommit(smemAddr(&s.empty[2 * i % kStages]));
-        if (i + 1 < n) doV(i + 1);
-        else ummaCommit(smemAddr(s.outBar));
-        if (ok && i + 2 < n) scores(i + 2);   // over scores that were read before ds was there
+        productWithTmem<T, DP>(tmem + 384, tmem + 128 + (i & 1) * 128, descAcross(tileAt(0, i)), i != 0);
+        ummaCommit(smemAddr(&s.empty[stageOf(0, i)]));
       }
+      if (ok) ummaCommit(smemAddr(s.outBar));
       if (!ok) {
         ummaCommit(smemAddr(s.drain));
         mbarWait(smemAddr(s.drain), 0, 1u << 20);
@@ -489,61 +500,70 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   } else if (warp < BackwardWarps::kCompute) {
     regsTake<BackwardWarps::kManyRegs>();
     const int half = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
-    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tDp = tmem + lanes + 256 + half * 64;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tS = tmem + lanes + half * 64;
     const int tok = tok0 + row / a.group, head = kvHead * a.group + row % a.group;
     const bool valid = row < rows && tok < seq.q, exists = row < rows && tok < a.q;
     const int limit = valid ? visibleOf(a, seq, tok) : 0;
-    const float c = a.scale * kLog2e, up = n > 0 ? gradScale<T>(a, b, kvHead) : 1.0f, down = up * exp2f(-Pack<T>::kBackwardBias);
-    float lse = 0.0f, delta = 0.0f;
+    const float c = a.scale * kLog2e, up = n > 0 ? gradScale<T>(a, b, kvHead) : 1.0f;
+    float shift = 0.0f, delta = 0.0f;
     if (n > 0) {
       const float* stats = a.stats + (((size_t)b * a.kvHeads + kvHead) * a.tiles + qTile) * 256;
-      lse = stats[row];
+      shift = stats[row] - Pack<T>::kBackwardBias + log2f(up);   // (up is a power of two)
       delta = stats[128 + row];
     }
+    const uint64_t c2 = pair(c, c), shift2 = pair(shift, shift), delta2 = pair(delta, delta);
     bool ok = true;
     for (int i = 0; i < n; ++i) {
-      ok = warpWaitOr(smemAddr(&s.first[i & 1]), (i >> 1) & 1, abortFlag);
+      const uint32_t tDp = tS + 128 + (i & 1) * 128;
+      ok = warpWaitOr(smemAddr(s.first), i & 1, abortFlag);
       if (!ok) {
         if (lane == 0) fail(3000);
         break;
       }
       tcFenceAfter();
-      const uint32_t tS = tmem + lanes + (i & 1) * 128 + half * 64;
-      uint32_t x[2][32];
-      float p[64];
+      uint32_t x[2][32], y[32], packed[32];
       tmemLd32(tS, x[0]);
       tmemLd32(tS + 32, x[1]);
       tmemLdWait32(x[0]);
       tmemLdWait32(x[1]);
-#pragma unroll
-      for (int k = 0; k < 64; ++k) p[k] = exp2Fast(fmaf(__uint_as_float(x[k / 32][k % 32]), c, -lse));
+      tcFenceBefore();
+      __syncwarp();
+      if (lane == 0) mbarArrive(smemAddr(s.firstDone));
       const int k0 = i * 128 + half * 64;
       const bool hide = __any_sync(~0u, limit < k0 + 64);
-      ok = warpWaitOr(smemAddr(s.second), i & 1, abortFlag);
-      if (!ok) {
-        if (lane == 0) fail(3001);
-        break;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint64_t p[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const uint64_t z = fma2(packF32x2(x[q][2 * k], x[q][2 * k + 1]), c2, shift2);
+          p[k] = pair(exp2Fast(lowOf(z)), exp2Fast(highOf(z)));
+        }
+        if (q == 0) {
+          ok = warpWaitOr(smemAddr(&s.second[i & 1]), i >> 1 & 1, abortFlag);
+          if (!ok) {
+            if (lane == 0) fail(3001);
+            break;
+          }
+          tcFenceAfter();
+        }
+        tmemLd32(tDp + q * 32, y);
+        tmemLdWait32(y);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) p[k] = mul2(p[k], add2(packF32x2(y[2 * k], y[2 * k + 1]), delta2));
+        if (hide) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) p[k] = pair(k0 + q * 32 + 2 * k < limit ? lowOf(p[k]) : 0.0f, k0 + q * 32 + 2 * k + 1 < limit ? highOf(p[k]) : 0.0f);
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) packed[q * 16 + k] = Pack<T>::two(lowOf(p[k]), highOf(p[k]));
       }
-      tcFenceAfter();
-      tmemLd32(tDp, x[0]);
-      tmemLd32(tDp + 32, x[1]);
-      tmemLdWait32(x[0]);
-      tmemLdWait32(x[1]);
-#pragma unroll
-      for (int k = 0; k < 64; ++k) p[k] *= (__uint_as_float(x[k / 32][k % 32]) - delta) * down;
-      if (hide) {
-#pragma unroll
-        for (int k = 0; k < 64; ++k)
-          if (k0 + k >= limit) p[k] = 0.0f;
-      }
-      uint32_t packed[32];
-#pragma unroll
-      for (int k = 0; k < 32; ++k) packed[k] = Pack<T>::two(p[2 * k], p[2 * k + 1]);
+      if (!ok) break;
       tmemSt32(tDp, packed);
       tmemStWait();
       tcFenceBefore();
       __syncwarp();
-      if (lane == 0) mbarArrive(smemAddr(s.secondDone));
+      if (lane == 0) mbarArrive(smemAddr(&s.secondDone[i & 1]));
     }
     if (ok && n > 0) {
       ok = warpWaitOr(smemAddr(s.outBar), 0, abortFlag);
@@ -565,83 +585,77 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 }
 
 // ---------------------------------------------------------------------------------------------- what both need of each row of queries
-// A warp per row: <do, o> (unless it is given), and the log-sum-exp in units of log 2, laid out as the tiles are. Rows that nobody has, and rows that
-// see no key, get an infinite log-sum-exp: their probabilities are zero. fp16: the longest row of do, and by the CTAs behind the tiles of v. A maximum does not go
+// Minus <do, o> (unless that is given: minus what is), and minus the log-sum-exp in units of log 2, laid out as the tiles are. Rows that nobody has, and rows that
+// see no key, get an infinite log-sum-exp: their probabilities are zero. 8 or 16 lanes take a row, a pack of 16 bytes each, and a warp several rows at a time. fp16: the longest row of do, and by the CTAs behind the tiles of v. A maximum does not go
 // by the order, and the bits of floats that are not negative are ordered as they are (NaN on top).
-template <typename T>
+constexpr int kStatsTurns = 4;   // rows of a lane
+
+template <typename T, int LANES>
 __global__ void __launch_bounds__(256) attnStatsKernel(const __grid_constant__ AttnStatsArgs a) {
   pdlEnter();
-  const int lane = threadIdx.x & 31, packs = a.dim / 8;
-  const size_t tileRows = (size_t)a.batch * a.kvHeads * a.tiles * 128;
-  size_t w = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  auto load = [&](const void* x, const long long* stride, int b, int tok, int head, float* f) {
-    const uint4 v = *(const uint4*)((const uint16_t*)x + (b * stride[0] + tok * stride[1] + head * stride[2] + lane * 8));
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+  constexpr int kWarpRows = 32 / LANES;
+  const int lane = threadIdx.x % LANES, packs = a.dim / 8;
+  const size_t tileRows = (size_t)a.batch * a.kvHeads * a.tiles * 128, vRows = a.bounds ? (size_t)a.batch * a.kv * a.kvHeads : 0;
+  const size_t first = ((size_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * kWarpRows * kStatsTurns + threadIdx.x % 32 / LANES;   // (a warp's rows are all of one kind: tiles have 128)
+  auto load = [&](const void* x, const long long* stride, int b, int tok, int head) {
+    return lane < packs ? *(const uint4*)((const uint16_t*)x + (b * stride[0] + tok * stride[1] + head * stride[2] + lane * 8)) : make_uint4(0, 0, 0, 0);
+  };
+  auto dot = [&](uint4 x, uint4 y) {
+    const uint32_t u[4] = {x.x, x.y, x.z, x.w}, v[4] = {y.x, y.y, y.z, y.w};
+    float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 p = Pack<T>::both(u[i]);
-      f[2 * i] = p.x;
-      f[2 * i + 1] = p.y;
+      const float2 p = Pack<T>::both(u[i]), q = Pack<T>::both(v[i]);
+      sum += p.x * q.x + p.y * q.y;
     }
-  };
-  auto sum = [&](float v) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-    return v;
+    for (int o = LANES / 2; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    return sum;
   };
-  if (w >= tileRows) {   // a row of v
-    w -= tileRows;
-    if (!a.bounds || w >= (size_t)a.batch * a.kv * a.kvHeads) return;
-    const int head = (int)(w % a.kvHeads), tok = (int)(w / a.kvHeads % a.kv), b = (int)(w / a.kvHeads / a.kv);
-    if (tok >= (a.kvLengths ? a.kvLengths[b] : a.kv)) return;
-    float f[8], ss = 0.0f;
-    if (lane < packs) {
-      load(a.v, a.vStride, b, tok, head, f);
+  if (first >= tileRows) {   // rows of v
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += f[i] * f[i];
+    for (int n = 0; n < kStatsTurns; ++n) {
+      const size_t w = first - tileRows + n * kWarpRows;
+      const int head = (int)(w % a.kvHeads), tok = (int)(w / a.kvHeads % max(a.kv, 1)), b = (int)min(w / a.kvHeads / max(a.kv, 1), (size_t)a.batch - 1);
+      const bool valid = w < vRows && tok < (a.kvLengths ? a.kvLengths[b] : a.kv);
+      const uint4 x = valid ? load(a.v, a.vStride, b, tok, head) : make_uint4(0, 0, 0, 0);
+      const float ss = dot(x, x);
+      if (valid && lane == 0) atomicMax(a.bounds + ((size_t)b * a.kvHeads + head) * 2 + 1, __float_as_uint(ss) & 0x7fffffffu);
     }
-    ss = sum(ss);
-    if (lane == 0) atomicMax(a.bounds + ((size_t)b * a.kvHeads + head) * 2 + 1, __float_as_uint(ss) & 0x7fffffffu);
     return;
   }
-  const int row = (int)(w % 128), tile = (int)(w / 128 % a.tiles), kvHead = (int)(w / 128 / a.tiles % a.kvHeads), b = (int)(w / 128 / a.tiles / a.kvHeads);
-  const int tok = tile * a.tileTokens + row / a.group, head = kvHead * a.group + row % a.group;
+  uint4 x[kStatsTurns], y[kStatsTurns];
+  size_t at[kStatsTurns];
+  bool valid[kStatsTurns];
+  const size_t tileOf = first / 128;   // of all: kWarpRows * kStatsTurns divides 128
+  const int tile = (int)(tileOf % a.tiles), kvHead = (int)(tileOf / a.tiles % a.kvHeads), b = (int)(tileOf / a.tiles / a.kvHeads);
   const int used = a.qLengths ? min(a.qLengths[b], a.q) : a.q;
-  const bool valid = row < a.tileTokens * a.group && tok < used;
-  float lse = INFINITY, delta = 0.0f;
-  if (valid) {
-    const size_t at = ((size_t)b * a.heads + head) * a.q + tok;
-    if (a.delta) delta = a.delta[at];
-    if (!a.delta || a.bounds) {
-      float f[8], g[8], ss = 0.0f, dot = 0.0f;
-      if (lane < packs) {
-        load(a.dout, a.doutStride, b, tok, head, f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss += f[i] * f[i];
-        if (!a.delta) {
-          load(a.out, a.outStride, b, tok, head, g);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) dot += f[i] * g[i];
-        }
-      }
-      if (!a.delta) delta = sum(dot);
-      if (a.bounds) {
-        ss = sum(ss);
-        if (lane == 0) atomicMax(a.bounds + ((size_t)b * a.kvHeads + kvHead) * 2, __float_as_uint(ss) & 0x7fffffffu);
-      }
-    }
-    if (a.stats) {
-      lse = a.lse[at];
-      lse = lse == -INFINITY ? INFINITY : fmaf(lse, kLog2e, -Pack<T>::kBackwardBias);
-    }
-    if (a.deltaOut && lane == 0) a.deltaOut[at] = delta;
-  } else if (a.deltaOut && lane == 0 && row < a.tileTokens * a.group && tok < a.q) {
-    a.deltaOut[((size_t)b * a.heads + head) * a.q + tok] = 0.0f;
+  for (int n = 0; n < kStatsTurns; ++n) {
+    const int row = (int)(first % 128) + n * kWarpRows, tok = tile * a.tileTokens + row / a.group, head = kvHead * a.group + row % a.group;
+    valid[n] = row < a.tileTokens * a.group && tok < used;
+    at[n] = ((size_t)b * a.heads + head) * a.q + tok;
+    x[n] = y[n] = make_uint4(0, 0, 0, 0);
+    if (valid[n] && (!a.delta || a.bounds)) x[n] = load(a.dout, a.doutStride, b, tok, head);
+    if (valid[n] && !a.delta) y[n] = load(a.out, a.outStride, b, tok, head);
   }
-  if (a.stats && lane == 0) {
-    float* to = a.stats + (w / 128) * 256 + row;
-    to[0] = lse;
-    to[128] = delta;
+#pragma unroll
+  for (int n = 0; n < kStatsTurns; ++n) {
+    const int row = (int)(first % 128) + n * kWarpRows, tok = tile * a.tileTokens + row / a.group;
+    float delta = a.delta ? (valid[n] ? a.delta[at[n]] : 0.0f) : dot(x[n], y[n]);
+    if (a.bounds) {
+      const float ss = dot(x[n], x[n]);
+      if (valid[n] && lane == 0) atomicMax(a.bounds + ((size_t)b * a.kvHeads + kvHead) * 2, __float_as_uint(ss) & 0x7fffffffu);
+    }
+    if (lane) continue;
+    if (a.deltaOut) {
+      if (row < a.tileTokens * a.group && tok < a.q) a.deltaOut[at[n]] = delta;
+      continue;
+    }
+    const float lse = valid[n] ? a.lse[at[n]] : -INFINITY;
+    float* to = a.stats + tileOf * 256 + row;
+    to[0] = lse == -INFINITY ? -INFINITY : fmaf(lse, -kLog2e, Pack<T>::kBackwardBias);
+    to[128] = -delta;
   }
 }
 
@@ -654,6 +668,10 @@ const void* attnBackwardQKernelFn(int type, int dim) { return type == ATTN_F16 ?
 int attnBackwardThreads() { return BackwardWarps::kThreads; }
 int attnBackwardRegs() { return BackwardWarps::kLaunchRegs; }
 size_t attnBackwardSmemBytes(int dim) { return dim <= 64 ? BackwardShape<64>::kBytes : BackwardShape<128>::kBytes; }
-const void* attnStatsKernelFn(int type) { return type == ATTN_F16 ? (const void*)attnStatsKernel<__half> : (const void*)attnStatsKernel<__nv_bfloat16>; }
+const void* attnStatsKernelFn(int type, int dim) {
+  if (dim <= 64) return type == ATTN_F16 ? (const void*)attnStatsKernel<__half, 8> : (const void*)attnStatsKernel<__nv_bfloat16, 8>;
+  return type == ATTN_F16 ? (const void*)attnStatsKernel<__half, 16> : (const void*)attnStatsKernel<__nv_bfloat16, 16>;
+}
+int attnStatsRows(int dim) { return (dim <= 64 ? 4 : 2) * 8 * kStatsTurns; }
 
 }  // namespace b200

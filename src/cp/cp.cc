@@ -206,7 +206,8 @@ static ncclResult_t launchStats(ncclCpContext* cp, const ncclCpAttention_t* c, A
   const size_t rows = (size_t)a->batch * a->kvHeads * a->tiles * kAttnRows + (a->bounds ? (size_t)a->batch * a->kv * a->kvHeads : 0);
   if (!rows) return ncclSuccess;
   void* args[1] = {a};
-  return launchCp(cp, attnStatsKernelFn(isFp16(c) ? ATTN_F16 : ATTN_BF16), (unsigned)((rows + 7) / 8), 1, 256, 0, args, stream);
+  const int each = attnStatsRows(c->head_dim);
+  return launchCp(cp, attnStatsKernelFn(isFp16(c) ? ATTN_F16 : ATTN_BF16, c->head_dim), (unsigned)((rows + each - 1) / each), 1, 256, 0, args, stream);
 }
 
 static void fillStats(const ncclCpAttention_t* c, const AttnArgs& a, AttnStatsArgs* s) {

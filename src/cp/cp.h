@@ -30,7 +30,7 @@ struct AttnArgs {
   float* partOut;
   float* partLse;
   // backward
-  const float* stats;         // [batch][kvHeads][tiles][2][128]: log-sum-exp in units of log 2 and <d(out), out> of each row
+  const float* stats;         // [batch][kvHeads][tiles][2][128]: minus the log-sum-exp in units of log 2 and minus <d(out), out> of each row
   int tiles;                  // of the queries of a key head
   const uint32_t* bounds;     // fp16: [batch][kvHeads][2] squared norms of the longest rows of d(out) and v, as bits
   void *dq, *dk, *dv;         // contiguous, of the inputs' type or fp32
@@ -80,7 +80,8 @@ int attnForwardThreads();
 int attnBackwardThreads();
 int attnForwardRegs();     // that a thread is launched with
 int attnBackwardRegs();
-const void* attnStatsKernelFn(int type);
+const void* attnStatsKernelFn(int type, int dim);
+int attnStatsRows(int dim);   // of a CTA
 const void* rotaryKernelFn(int type);
 
 }  // namespace b200
