@@ -25,7 +25,7 @@ template <int DP> struct BackwardShape {
   static constexpr int kStages = DP == 64 ? 8 : 5;
   static constexpr uint32_t kRing = 2 * kTileBytes, kStats = kRing + kStages * kTileBytes, kCtrl = kStats + 2048;
   static constexpr size_t kBytes = kCtrl + 1024;   // (dynamic shared memory, all that these kernels have, begins on a multiple of 1024 bytes)
-  static_assert(kBytes <= 227 * 1024 && (2 * kStages + 12) * 8 + 8 <= 1024, "shared memory");
+  static_assert(kBytes <= 227 * 1024 && (2 * kStages + 13) * 8 + 8 <= 1024, "shared memory");
 };
 
 // The power of two that ds is multiplied by, in fp16: |ds| <= p (|do.v| + |do.o|) <= 2 |do| |v|.
@@ -41,7 +41,7 @@ __device__ __forceinline__ float gradScale(const AttnArgs& a, int b, int kvHead)
 }
 
 struct BackwardBars {
-  uint64_t *full, *empty, *own, *first, *second, *firstDone, *secondDone, *outBar, *fix, *drain;
+  uint64_t *full, *empty, *own, *first, *second, *firstDone, *secondDone, *outBar, *probDone, *fix, *drain;
   uint32_t* tmemSlot;
   volatile uint32_t* abortFlag;
 };
@@ -57,7 +57,8 @@ __device__ __forceinline__ BackwardBars backwardSetUp(uint8_t* smem, int warp) {
   s.firstDone = s.second + 2;    // scores are used up
   s.secondDone = s.firstDone + 1;   // [2] ds is in tensor memory, in each of its places
   s.outBar = s.secondDone + 2;
-  s.fix = s.outBar + 1;          // [2]
+  s.probDone = s.outBar + 1;     // probabilities are in tensor memory
+  s.fix = s.probDone + 1;        // [2]
   s.drain = s.fix + 2;
   s.tmemSlot = (uint32_t*)(s.drain + 1);
   s.abortFlag = s.tmemSlot + 1;
@@ -71,6 +72,7 @@ __device__ __forceinline__ BackwardBars backwardSetUp(uint8_t* smem, int warp) {
       mbarInit(smemAddr(&s.secondDone[i]), BackwardWarps::kCompute);
     }
     mbarInit(smemAddr(s.outBar), 1);
+    mbarInit(smemAddr(s.probDone), BackwardWarps::kCompute);
     mbarInit(smemAddr(&s.fix[0]), 1);
     mbarInit(smemAddr(&s.fix[1]), 1);
     mbarInit(smemAddr(s.drain), 1);
@@ -122,15 +124,16 @@ __device__ __forceinline__ void storeGradient(const AttnArgs& a, uint32_t tmem, 
 }
 
 // ---------------------------------------------------------------------------------------------- dk and dv
-// Tensor memory: scores [keys x queries] (then probabilities) at 0, do.v (then ds) at 128, dv at 256, dk at 384. Products of tile j: dv += P do as soon as the
-// probabilities are there, with the next tile's scores behind it; dk += dS q as soon as ds is, with the next do.v behind it. So the tensor cores work on one pair while
-// the other's elements are computed.
+// Tensor memory: scores [keys x queries] at 0, do.v at 128 (then, over the half of a warp's columns, probabilities and ds), dv at 256, dk at 384. Scores are taken into registers
+// at once, and the next tile's are made meanwhile: its exponentials are computed while the tensor cores add this tile's to dv and dk and make the next do.v. With the
+// probabilities over the scores, the next scores waited for their product: a third of the tensor cores' time.
 template <typename T, int DP>
 __global__ void __launch_bounds__(BackwardWarps::kThreads, 1)
 attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDo, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                      const __grid_constant__ AttnArgs a) {
   using Shape = BackwardShape<DP>;
-  constexpr int kStages = Shape::kStages;
+  // Queries stay until their product with ds, two steps behind their scores; do for one step less: a ring for each.
+  constexpr int kStages = Shape::kStages, kQStages = (kStages + 1) / 2, kDoStages = kStages - kQStages;
   constexpr uint32_t kTileBytes = Shape::kTileBytes;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -165,15 +168,16 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     reportTimeout(a.status, what);
   };
 
+  auto stageOf = [](int isDo, int tile) { return isDo ? kQStages + tile % kDoStages : tile % kQStages; };
+  auto phaseOf = [](int isDo, int tile) { return (uint32_t)(tile / (isDo ? kDoStages : kQStages)) & 1; };
+
   if (warp >= BackwardWarps::kCompute) regsGive<BackwardWarps::kFewRegs>();
   if (warp == BackwardWarps::kProducer) {
-    uint32_t armed = 0;
-    int place = 0;
+    int loaded[2] = {};   // queries, do
     bool ok = !*abortFlag, ownArmed = false;
-    auto next = [&](const CUtensorMap* map, int tile, const float* stats) {
-      const int at = place % kStages;
-      const uint32_t ph = (place / kStages) & 1;
-      ok = ok && warpWaitOr(smemAddr(&s.empty[at]), ph ^ 1, abortFlag);
+    auto next = [&](const CUtensorMap* map, int isDo, const float* stats) {
+      const int tile = loaded[isDo], at = stageOf(isDo, tile);
+      ok = ok && warpWaitOr(smemAddr(&s.empty[at]), phaseOf(isDo, tile) ^ 1, abortFlag);
       if (!ok) {
         if (lane == 0) fail(1000 + at);
         return;
@@ -184,8 +188,7 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         loadTile<DP>(smem0 + Shape::kRing + at * kTileBytes, map, (begin + tile) * a.tileTokens, kvHead * a.group, b, bar);
         if (stats) bulkLoad(smem0 + Shape::kStats + (tile & 1) * 1024, stats, 1024, bar);
       }
-      armed |= 1u << at;
-      ++place;
+      ++loaded[isDo];
     };
     if (n > 0) {
       if (ok && lane == 0) {
@@ -194,23 +197,23 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         loadTile<DP>(smem0 + kTileBytes, &tmV, key0, kvHead, b, smemAddr(s.own));
       }
       ownArmed = ok;
-      // stats of a tile arrive with its do: the buffer was last read for the tile before the last, whose q has left its stage by then
+      // A tile's numbers per row arrive with its do. The buffer was last read for the tile before the last, whose do has left the ring by then if the ring has room for two; else
+      // its stage is waited for.
       const float* stats = a.stats + (((size_t)b * a.kvHeads + kvHead) * a.tiles + begin) * 256;
       for (int i = 0; i < n && ok; ++i) {
-        next(&tmQ, i, nullptr);
-        if (ok && i >= 2) {
-          const int was = 2 * (i - 2);   // place of that q
-          ok = warpWaitOr(smemAddr(&s.empty[was % kStages]), (was / kStages) & 1, abortFlag);
+        next(&tmQ, 0, nullptr);
+        if (ok && kDoStages > 2 && i >= 2) {
+          ok = warpWaitOr(smemAddr(&s.empty[stageOf(1, i - 2)]), phaseOf(1, i - 2), abortFlag);
           if (!ok && lane == 0) fail(1050);
         }
-        if (ok) next(&tmDo, i, stats + (size_t)i * 256);
+        if (ok) next(&tmDo, 1, stats + (size_t)i * 256);
       }
       if (ok && fixRows) {
         for (int k = 0; k < 2 && ok; ++k) {
-          const int at = place - 2 + k;
-          ok = warpWaitOr(smemAddr(&s.full[at % kStages]), (at / kStages) & 1, abortFlag);
+          const int at = stageOf(k, n - 1);
+          ok = warpWaitOr(smemAddr(&s.full[at]), phaseOf(k, n - 1), abortFlag);
           if (ok) {
-            clearRows<DP>(smem + Shape::kRing + at % kStages * kTileBytes, fixRows, lane);
+            clearRows<DP>(smem + Shape::kRing + at * kTileBytes, fixRows, lane);
             if (lane == 0) mbarArrive(smemAddr(&s.fix[k]));
           } else if (lane == 0) {
             fail(1100);
@@ -218,8 +221,10 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         }
       }
       if (__any_sync(~0u, *abortFlag)) {
-        for (int at = 0; at < kStages; ++at)
-          if (armed >> at & 1) mbarWait(smemAddr(&s.full[at]), (uint32_t)((place - 1 - (place - 1 - at + kStages) % kStages) / kStages) & 1, 1u << 20);
+        // copies already issued still write into this CTA's shared memory: wait for them (bounded)
+        for (int isDo = 0; isDo < 2; ++isDo)
+          for (int tile = max(0, loaded[isDo] - (isDo ? kDoStages : kQStages)); tile < loaded[isDo]; ++tile)
+            mbarWait(smemAddr(&s.full[stageOf(isDo, tile)]), phaseOf(isDo, tile), 1u << 20);
         if (ownArmed) mbarWait(smemAddr(s.own), 0, 1u << 20);
       }
     }
@@ -231,35 +236,38 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         ok = ok && got;
         return ok;
       };
-      auto full = [&](int place) { return need(waitOr(smemAddr(&s.full[place % kStages]), (place / kStages) & 1, abortFlag), 2000 + place % kStages); };
-      auto tileAt = [&](int place) { return smem0 + Shape::kRing + (place % kStages) * kTileBytes; };
+      auto full = [&](int isDo, int tile) { return need(waitOr(smemAddr(&s.full[stageOf(isDo, tile)]), phaseOf(isDo, tile), abortFlag), 2000 + stageOf(isDo, tile)); };
+      auto tileAt = [&](int isDo, int tile) { return smem0 + Shape::kRing + stageOf(isDo, tile) * kTileBytes; };
       auto scores = [&](int i) {
-        if (!full(2 * i)) return;
+        if (!full(0, i)) return;
         if (fixRows && i == n - 1 && !need(waitOr(smemAddr(&s.fix[0]), 0, abortFlag), 2200)) return;
         tcFenceAfter();
-        productOfTiles<T, DP>(tmem, descAlong(smem0), descAlong(tileAt(2 * i)));
+        productOfTiles<T, DP>(tmem, descAlong(smem0), descAlong(tileAt(0, i)));
         ummaCommit(smemAddr(s.first));
       };
       auto doV = [&](int i) {
-        if (!full(2 * i + 1)) return;
+        if (!full(1, i)) return;
         if (fixRows && i == n - 1 && !need(waitOr(smemAddr(&s.fix[1]), 0, abortFlag), 2201)) return;
         tcFenceAfter();
-        productOfTiles<T, DP>(tmem + 128, descAlong(smem0 + kTileBytes), descAlong(tileAt(2 * i + 1)));
+        productOfTiles<T, DP>(tmem + 128, descAlong(smem0 + kTileBytes), descAlong(tileAt(1, i)));
         ummaCommit(smemAddr(s.second));
       };
       if (need(waitOr(smemAddr(s.own), 0, abortFlag), 2100)) scores(0);
       if (ok) doV(0);
       for (int i = 0; i < n && ok; ++i) {
-        if (!need(waitOr(smemAddr(s.firstDone), i & 1, abortFlag), 2300)) break;
+        if (i + 1 < n) {
+          if (!need(waitOr(smemAddr(s.firstDone), i & 1, abortFlag), 2300)) break;   // scores are in registers
+          scores(i + 1);
+        }
+        if (!ok || !need(waitOr(smemAddr(s.probDone), i & 1, abortFlag), 2400)) break;
         tcFenceAfter();
-        productWithTmem<T, DP>(tmem + 256, tmem, descAcross(tileAt(2 * i + 1)), i != 0);
-        ummaCommit(smemAddr(&s.empty[(2 * i + 1) % kStages]));   // (its do.v was issued in front of this)
-        if (i + 1 < n) scores(i + 1);
-        if (!ok || !need(waitOr(smemAddr(s.secondDone), i & 1, abortFlag), 2400)) break;
+        productWithTmem<T, DP>(tmem + 256, tmem + 128, descAcross(tileAt(1, i)), i != 0);
+        if (!need(waitOr(smemAddr(s.secondDone), i & 1, abortFlag), 2500)) break;
         tcFenceAfter();
-        productWithTmem<T, DP>(tmem + 384, tmem + 128, descAcross(tileAt(2 * i)), i != 0);
-        ummaCommit(smemAddr(&s.empty[2 * i % kStages]));
-        if (i + 1 < n) doV(i + 1);
+        ummaCommit(smemAddr(&s.empty[stageOf(1, i)]));   // (its do.v was issued in front of this; the row's numbers that came with it are used up)
+        productWithTmem<T, DP>(tmem + 384, tmem + 160, descAcross(tileAt(0, i)), i != 0);
+        ummaCommit(smemAddr(&s.empty[stageOf(0, i)]));
+        if (i + 1 < n) doV(i + 1);   // over probabilities and ds: products are carried out in order
         else ummaCommit(smemAddr(s.outBar));
       }
       if (!ok) {
@@ -277,7 +285,7 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     bool ok = true;
     for (int i = 0; i < n; ++i) {
       const float* stats = (const float*)(smem + Shape::kStats + (i & 1) * 1024);   // of the tile's rows: minus the log-sum-exp [128], minus <do, o> [128]
-      ok = warpWaitOr(smemAddr(&s.full[(2 * i + 1) % kStages]), ((2 * i + 1) / kStages) & 1, abortFlag) && warpWaitOr(smemAddr(s.first), i & 1, abortFlag);
+      ok = warpWaitOr(smemAddr(&s.full[stageOf(1, i)]), phaseOf(1, i), abortFlag) && warpWaitOr(smemAddr(s.first), i & 1, abortFlag);
       if (!ok) {
         if (lane == 0) fail(3000);
         break;
@@ -290,11 +298,14 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       uint32_t x[2][32], packed[32];
       uint64_t p[32];
       tmemLd32(tS, x[0]);
-      tmemLdWait32(x[0]);
       tmemLd32(tS + 32, x[1]);
+      tmemLdWait32(x[0]);
+      tmemLdWait32(x[1]);
+      tcFenceBefore();
+      __syncwarp();
+      if (lane == 0) mbarArrive(smemAddr(s.firstDone));
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        if (q) tmemLdWait32(x[1]);
 #pragma unroll
         for (int k = 0; k < 32; k += 4) {
           const float4 lse = *(const float4*)(stats + half * 64 + q * 32 + k);
@@ -309,11 +320,6 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
 #pragma unroll
       for (int k = 0; k < 32; ++k) packed[k] = Pack<T>::two(lowOf(p[k]), highOf(p[k]));
-      tmemSt32(tS, packed);
-      tmemStWait();
-      tcFenceBefore();
-      __syncwarp();
-      if (lane == 0) mbarArrive(smemAddr(s.firstDone));
       ok = warpWaitOr(smemAddr(s.second), i & 1, abortFlag);
       if (!ok) {
         if (lane == 0) fail(3001);
@@ -321,11 +327,17 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
       tcFenceAfter();
       tmemLd32(tDp, x[0]);
-      tmemLdWait32(x[0]);
       tmemLd32(tDp + 32, x[1]);
+      tmemLdWait32(x[0]);
+      tmemLdWait32(x[1]);
+      // what is added to dv does not wait for ds
+      tmemSt32(tDp, packed);
+      tmemStWait();
+      tcFenceBefore();
+      __syncwarp();
+      if (lane == 0) mbarArrive(smemAddr(s.probDone));
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        if (q) tmemLdWait32(x[1]);
 #pragma unroll
         for (int k = 0; k < 32; k += 4) {
           const float4 delta = *(const float4*)(stats + 128 + half * 64 + q * 32 + k);
@@ -340,7 +352,7 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           packed[q * 16 + k / 2 + 1] = Pack<T>::two(lowOf(hi), highOf(hi));
         }
       }
-      tmemSt32(tDp, packed);
+      tmemSt32(tDp + 32, packed);
       tmemStWait();
       tcFenceBefore();
       __syncwarp();
@@ -586,20 +598,15 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 
 // ---------------------------------------------------------------------------------------------- what both need of each row of queries
 // Minus <do, o> (unless that is given: minus what is), and minus the log-sum-exp in units of log 2, laid out as the tiles are. Rows that nobody has, and rows that
-// see no key, get an infinite log-sum-exp: their probabilities are zero. 8 or 16 lanes take a row, a pack of 16 bytes each, and a warp several rows at a time. fp16: the longest row of do, and by the CTAs behind the tiles of v. A maximum does not go
+// see no key, get an infinite log-sum-exp: their probabilities are zero. A CTA takes a tile, 8 or 16 lanes a row, a pack of 16 bytes each. fp16: the longest row of do, and by the CTAs behind the tiles of v. A maximum does not go
 // by the order, and the bits of floats that are not negative are ordered as they are (NaN on top).
-constexpr int kStatsTurns = 4;   // rows of a lane
-
 template <typename T, int LANES>
-__global__ void __launch_bounds__(256) attnStatsKernel(const __grid_constant__ AttnStatsArgs a) {
-  pdlEnter();
-  constexpr int kWarpRows = 32 / LANES;
-  const int lane = threadIdx.x % LANES, packs = a.dim / 8;
-  const size_t tileRows = (size_t)a.batch * a.kvHeads * a.tiles * 128, vRows = a.bounds ? (size_t)a.batch * a.kv * a.kvHeads : 0;
-  const size_t first = ((size_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * kWarpRows * kStatsTurns + threadIdx.x % 32 / LANES;   // (a warp's rows are all of one kind: tiles have 128)
-  auto load = [&](const void* x, const long long* stride, int b, int tok, int head) {
-    return lane < packs ? *(const uint4*)((const uint16_t*)x + (b * stride[0] + tok * stride[1] + head * stride[2] + lane * 8)) : make_uint4(0, 0, 0, 0);
-  };
+__global__ void __launch_bounds__(256, 4) attnStatsKernel(const __grid_constant__ AttnStatsArgs a) {
+  constexpr int kAtOnce = 256 / LANES, kTurns = 4;   // rows of the CTA, and of a thread with loads on their way
+  const int lane = threadIdx.x % LANES, row0 = threadIdx.x / LANES, packs = a.dim / 8;
+  const bool has = lane < packs;
+  const int channel = has ? lane * 8 : 0;
+  auto load = [&](const void* x, long long at) { return *(const uint4*)((const uint16_t*)x + at + channel); };
   auto dot = [&](uint4 x, uint4 y) {
     const uint32_t u[4] = {x.x, x.y, x.z, x.w}, v[4] = {y.x, y.y, y.z, y.w};
     float sum = 0.0f;
@@ -608,55 +615,77 @@ __global__ void __launch_bounds__(256) attnStatsKernel(const __grid_constant__ A
       const float2 p = Pack<T>::both(u[i]), q = Pack<T>::both(v[i]);
       sum += p.x * q.x + p.y * q.y;
     }
+    sum = has ? sum : 0.0f;
 #pragma unroll
     for (int o = LANES / 2; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
     return sum;
   };
-  if (first >= tileRows) {   // rows of v
+  const unsigned owners = a.batch * a.kvHeads, qTiles = owners * a.tiles;
+  const bool ofV = blockIdx.x >= qTiles;   // 128 rows of v instead of a tile
+  const unsigned block = ofV ? blockIdx.x - qTiles : blockIdx.x, owner = block % owners;
+  const int tile = block / owners, kvHead = owner % a.kvHeads, b = owner / a.kvHeads;
+  float most = 0.0f;   // (NaN stays)
+  pdlEnter();
+  if (ofV) {
+    const int used = a.kvLengths ? min(a.kvLengths[b], a.kv) : a.kv;
+    if (tile * 128 >= used) return;
+    const long long base = b * a.vStride[0] + kvHead * a.vStride[2];
+    for (int pass = 0; pass < 128; pass += kAtOnce * kTurns) {
+      uint4 x[kTurns];
 #pragma unroll
-    for (int n = 0; n < kStatsTurns; ++n) {
-      const size_t w = first - tileRows + n * kWarpRows;
-      const int head = (int)(w % a.kvHeads), tok = (int)(w / a.kvHeads % max(a.kv, 1)), b = (int)min(w / a.kvHeads / max(a.kv, 1), (size_t)a.batch - 1);
-      const bool valid = w < vRows && tok < (a.kvLengths ? a.kvLengths[b] : a.kv);
-      const uint4 x = valid ? load(a.v, a.vStride, b, tok, head) : make_uint4(0, 0, 0, 0);
-      const float ss = dot(x, x);
-      if (valid && lane == 0) atomicMax(a.bounds + ((size_t)b * a.kvHeads + head) * 2 + 1, __float_as_uint(ss) & 0x7fffffffu);
+      for (int n = 0; n < kTurns; ++n) x[n] = load(a.v, base + min(tile * 128 + pass + row0 + n * kAtOnce, used - 1) * a.vStride[1]);
+#pragma unroll
+      for (int n = 0; n < kTurns; ++n) {
+        const float ss = dot(x[n], x[n]);
+        most = ss <= most ? most : ss;
+      }
     }
+    if (lane == 0) atomicMax(a.bounds + owner * 2 + 1, __float_as_uint(most) & 0x7fffffffu);
     return;
   }
-  uint4 x[kStatsTurns], y[kStatsTurns];
-  size_t at[kStatsTurns];
-  bool valid[kStatsTurns];
-  const size_t tileOf = first / 128;   // of all: kWarpRows * kStatsTurns divides 128
-  const int tile = (int)(tileOf % a.tiles), kvHead = (int)(tileOf / a.tiles % a.kvHeads), b = (int)(tileOf / a.tiles / a.kvHeads);
-  const int used = a.qLengths ? min(a.qLengths[b], a.q) : a.q;
+  const int used = a.qLengths ? max(0, min(a.qLengths[b], a.q)) : a.q, tok0 = tile * a.tileTokens, rows = a.tileTokens * a.group;
+  const int some = min(used - tok0, a.tileTokens) * a.group;   // rows that somebody has
+  float* to = a.stats + ((size_t)owner * a.tiles + tile) * 256 + row0;
+  const size_t base = ((size_t)b * a.heads + kvHead * a.group) * a.q + tok0;   // of lse and delta
+  const bool needX = !a.delta || a.bounds;
+  for (int pass = 0; pass < 128; pass += kAtOnce * kTurns) {
+    uint4 x[kTurns] = {}, y[kTurns] = {};
+    float lse[kTurns], delta[kTurns];
+    size_t at[kTurns];
 #pragma unroll
-  for (int n = 0; n < kStatsTurns; ++n) {
-    const int row = (int)(first % 128) + n * kWarpRows, tok = tile * a.tileTokens + row / a.group, head = kvHead * a.group + row % a.group;
-    valid[n] = row < a.tileTokens * a.group && tok < used;
-    at[n] = ((size_t)b * a.heads + head) * a.q + tok;
-    x[n] = y[n] = make_uint4(0, 0, 0, 0);
-    if (valid[n] && (!a.delta || a.bounds)) x[n] = load(a.dout, a.doutStride, b, tok, head);
-    if (valid[n] && !a.delta) y[n] = load(a.out, a.outStride, b, tok, head);
-  }
+    for (int n = 0; n < kTurns; ++n) {
+      const int row = max(0, min(pass + row0 + n * kAtOnce, some - 1)), t = row / a.group, head = row - t * a.group;   // (a row behind the last stands for it)
+      at[n] = base + (size_t)head * a.q + t;
+      if (some > 0) {
+        if (needX) x[n] = load(a.dout, b * a.doutStride[0] + (tok0 + t) * a.doutStride[1] + (kvHead * a.group + head) * a.doutStride[2]);
+        if (!a.delta) y[n] = load(a.out, b * a.outStride[0] + (tok0 + t) * a.outStride[1] + (kvHead * a.group + head) * a.outStride[2]);
+        if (a.delta) delta[n] = a.delta[at[n]];
+        if (a.stats) lse[n] = a.lse[at[n]];
+      }
+    }
 #pragma unroll
-  for (int n = 0; n < kStatsTurns; ++n) {
-    const int row = (int)(first % 128) + n * kWarpRows, tok = tile * a.tileTokens + row / a.group;
-    float delta = a.delta ? (valid[n] ? a.delta[at[n]] : 0.0f) : dot(x[n], y[n]);
-    if (a.bounds) {
-      const float ss = dot(x[n], x[n]);
-      if (valid[n] && lane == 0) atomicMax(a.bounds + ((size_t)b * a.kvHeads + kvHead) * 2, __float_as_uint(ss) & 0x7fffffffu);
+    for (int n = 0; n < kTurns; ++n) {
+      const int row = pass + row0 + n * kAtOnce;
+      if (!a.delta) delta[n] = dot(x[n], y[n]);
+      if (a.bounds) {
+        const float ss = dot(x[n], x[n]);
+        most = ss <= most ? most : ss;
+      }
+      if (row >= some) {
+        delta[n] = 0.0f;
+        lse[n] = -INFINITY;
+      }
+      if (a.stats && lane == 0) {
+        to[row - row0] = lse[n] == -INFINITY ? -INFINITY : fmaf(lse[n], -kLog2e, Pack<T>::kBackwardBias);
+        to[row - row0 + 128] = -delta[n];
+      }
+      if (a.deltaOut && lane == 0 && row < rows) {
+        const int t = row / a.group;
+        if (tok0 + t < a.q) a.deltaOut[base + (size_t)(row - t * a.group) * a.q + t] = delta[n];
+      }
     }
-    if (lane) continue;
-    if (a.deltaOut) {
-      if (row < a.tileTokens * a.group && tok < a.q) a.deltaOut[at[n]] = delta;
-      continue;
-    }
-    const float lse = valid[n] ? a.lse[at[n]] : -INFINITY;
-    float* to = a.stats + tileOf * 256 + row;
-    to[0] = lse == -INFINITY ? -INFINITY : fmaf(lse, -kLog2e, Pack<T>::kBackwardBias);
-    to[128] = -delta;
   }
+  if (a.bounds && lane == 0) atomicMax(a.bounds + owner * 2, __float_as_uint(most) & 0x7fffffffu);
 }
 
 }  // namespace
@@ -672,6 +701,5 @@ const void* attnStatsKernelFn(int type, int dim) {
   if (dim <= 64) return type == ATTN_F16 ? (const void*)attnStatsKernel<__half, 8> : (const void*)attnStatsKernel<__nv_bfloat16, 8>;
   return type == ATTN_F16 ? (const void*)attnStatsKernel<__half, 16> : (const void*)attnStatsKernel<__nv_bfloat16, 16>;
 }
-int attnStatsRows(int dim) { return (dim <= 64 ? 4 : 2) * 8 * kStatsTurns; }
 
 }  // namespace b200

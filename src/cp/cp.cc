@@ -203,11 +203,10 @@ static ncclResult_t needsGpu(const ncclCpContext* cp, const char* what) {
 }
 
 static ncclResult_t launchStats(ncclCpContext* cp, const ncclCpAttention_t* c, AttnStatsArgs* a, cudaStream_t stream) {
-  const size_t rows = (size_t)a->batch * a->kvHeads * a->tiles * kAttnRows + (a->bounds ? (size_t)a->batch * a->kv * a->kvHeads : 0);
-  if (!rows) return ncclSuccess;
+  const unsigned ctas = (unsigned)a->batch * a->kvHeads * (a->tiles + (a->bounds ? (a->kv + kAttnRows - 1) / kAttnRows : 0));
+  if (!ctas) return ncclSuccess;
   void* args[1] = {a};
-  const int each = attnStatsRows(c->head_dim);
-  return launchCp(cp, attnStatsKernelFn(isFp16(c) ? ATTN_F16 : ATTN_BF16, c->head_dim), (unsigned)((rows + each - 1) / each), 1, 256, 0, args, stream);
+  return launchCp(cp, attnStatsKernelFn(isFp16(c) ? ATTN_F16 : ATTN_BF16, c->head_dim), ctas, 1, 256, 0, args, stream);
 }
 
 static void fillStats(const ncclCpAttention_t* c, const AttnArgs& a, AttnStatsArgs* s) {

@@ -81,7 +81,6 @@ int attnBackwardThreads();
 int attnForwardRegs();     // that a thread is launched with
 int attnBackwardRegs();
 const void* attnStatsKernelFn(int type, int dim);
-int attnStatsRows(int dim);   // of a CTA
 const void* rotaryKernelFn(int type);
 
 }  // namespace b200
