@@ -120,7 +120,7 @@ class ContextParallel:
             _lib.check(rc, name, self.lib)
 
     def _remember(self, key, make):
-        """What `make` gives for sizes that were seen before; whoever uses it holds it, so that another thread may clear the store."""
+        """What `make`, which checks what the key says, gives for it, from the last call with that key; whoever uses it holds it, so that another thread may clear the store."""
         got = self._shapes.get(key)
         if got is None:
             got = make()
@@ -139,20 +139,25 @@ class ContextParallel:
 
     def _result(self, name, t, dtype, shape):
         if t is None:
-            return self.torch.empty(shape, dtype=dtype, device=self._place)
+            return self.torch.empty(*shape, dtype=dtype, device=self._place)   # (sizes one by one: 0.7 us less than as a tuple)
         self._need(name, t, dtype, shape)
         return t
 
     def _operand(self, name, t, dtype, shape):
-        """Checks a tensor that may be strided: type, shape, place, and that its rows are where the kernels' copies can begin."""
-        if t.dtype is not dtype or t.shape != shape or t.get_device() != self._device:
-            raise ValueError("%s must be a %s tensor %s on cuda:%d, not %s %s on %s" % (
-                name, str(dtype).replace("torch.", ""), list(shape), self._device, str(t.dtype).replace("torch.", ""), list(t.shape), t.device))
+        """Checks what a tensor's sizes and strides say: type, shape, and that its rows are where the kernels' copies can begin. (Where it is, each call checks.)"""
+        if t.dtype is not dtype or t.shape != shape:
+            raise ValueError("%s must be a %s tensor %s, not %s %s" % (name, str(dtype).replace("torch.", ""), list(shape), str(t.dtype).replace("torch.", ""), list(t.shape)))
         st = t.stride()
-        if t.numel() and (t.data_ptr() % 16 or (st[3] != 1 and shape[3] > 1) or any(n > 1 and (s <= 0 or s % 8) for n, s in zip(shape[:3], st))):
-            raise ValueError("%s needs its channels next to each other, rows that begin at multiples of 16 bytes, and no repeated rows: strides %s at %#x; give a contiguous copy" % (
-                name, list(st), t.data_ptr()))
+        if t.numel() and ((st[3] != 1 and shape[3] > 1) or any(n > 1 and (s <= 0 or s % 8) for n, s in zip(shape[:3], st))):
+            raise ValueError("%s needs its channels next to each other, rows that begin at multiples of 16 bytes, and no repeated rows, not strides %s: give a contiguous copy" % (name, list(st)))
         return st
+
+    def _at(self, name, t):
+        """Address of an operand whose sizes are checked."""
+        p = t.data_ptr()
+        if t.get_device() != self._device or p % 16:
+            raise ValueError("%s must be on cuda:%d, at a multiple of 16 bytes, not on %s at %#x" % (name, self._device, t.device, p))
+        return p
 
     def _lengths(self, name, t, batch):
         if t is None:
@@ -184,20 +189,18 @@ class ContextParallel:
             raise ValueError("offset = %r" % (offset,))
         return (0 if not causal else 2 if offset is None else 1), (0 if offset is None else int(offset)), scale
 
-    def _shape(self, sizes, dtype, result, mask, strides, work):
-        """The library's description of a call, and the bytes of workspace that it takes."""
-        def make():
-            B, Q, K, H, G, D = sizes
-            d = _Attention(ctypes.sizeof(_Attention), MAGIC, self._codes[dtype], self._codes[result], B, Q, K, H, G, D, mask[0], mask[2], mask[1])
-            for name, st in zip(("q_stride", "k_stride", "v_stride", "dout_stride", "out_stride"), strides):
-                if st is not None:
-                    getattr(d, name)[:] = st[:3]
-            bytes_ = work(self.handle, ctypes.addressof(d)) if work else 0
-            return d, bytes_
-        return self._remember((sizes, dtype, result, mask, strides, work is None or work.__name__), make)
+    def _describe(self, sizes, dtype, result, mask, strides, work):
+        """The library's description of a call, its address, and the bytes of workspace that it takes."""
+        B, Q, K, H, G, D = sizes
+        d = _Attention(ctypes.sizeof(_Attention), MAGIC, self._codes[dtype], self._codes[result], B, Q, K, H, G, D, mask[0], mask[2], mask[1])
+        for name, st in zip(("q_stride", "k_stride", "v_stride", "dout_stride", "out_stride"), strides):
+            if st is not None:
+                getattr(d, name)[:] = st[:3]
+        at = ctypes.addressof(d)
+        return d, at, work(self.handle, at) if work else 0
 
     def _work(self, size):
-        return self.torch.empty(size, dtype=self.torch.uint8, device=self._place) if size else None
+        return self.torch.empty(size, dtype=self.torch.uint8, device=self._place)
 
     def _result_type(self, dtype, q):
         dtype = q.dtype if dtype is None else dtype
@@ -217,20 +220,25 @@ class ContextParallel:
         a log-sum-exp of -inf. ``join``: (out, lse) over other keys, fp32 (``dtype=torch.float32`` gives that): the result is over both; they may be ``out`` and ``lse``.
 
         Sums and statistics are fp32; probabilities are rounded to q's type (by at most half a step each) before they meet v."""
-        torch, ptr = self.torch, lambda t: None if t is None else t.data_ptr()   # noqa: E731
-        sizes = B, Q, K, H, G, D = self._sizes(q, k, v)
-        strides = self._operand("q", q, q.dtype, (B, Q, H, D)), self._operand("k", k, q.dtype, (B, K, G, D)), self._operand("v", v, q.dtype, (B, K, G, D))
+        torch = self.torch
+
+        def make():
+            sizes = B, Q, K, H, G, D = self._sizes(q, k, v)
+            strides = self._operand("q", q, q.dtype, (B, Q, H, D)), self._operand("k", k, q.dtype, (B, K, G, D)), self._operand("v", v, q.dtype, (B, K, G, D))
+            result = self._result_type(dtype, q)
+            return sizes, result, self._describe(sizes, q.dtype, result, self._mask(causal, offset, scale, D), strides, self.lib.ncclCpAttentionWork)
+        (B, Q, K, H, G, D), result, (d, at, size) = self._remember(
+            (q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, causal, offset, scale, dtype), make)
+        pq, pk, pv = self._at("q", q), self._at("k", k), self._at("v", v)
         nq, nk = self._lengths("q_lengths", q_lengths, B), self._lengths("kv_lengths", kv_lengths, B)
-        dtype = self._result_type(dtype, q)
         join_out = join_lse = None
         if join is not None:
-            join_out, join_lse = join
-            self._need("join[0]", join_out, torch.float32, (B, Q, H, D))
-            self._need("join[1]", join_lse, torch.float32, (B, H, Q))
-        out, lse = self._result("out", out, dtype, (B, Q, H, D)), self._result("lse", lse, torch.float32, (B, H, Q))
-        d, size = self._shape(sizes, q.dtype, dtype, self._mask(causal, offset, scale, D), strides, self.lib.ncclCpAttentionWork)
-        work = self._work(size)
-        self._call("ncclCpAttention", ctypes.addressof(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), nq, nk, ptr(join_out), ptr(join_lse), out.data_ptr(), lse.data_ptr(), ptr(work))
+            self._need("join[0]", join[0], torch.float32, (B, Q, H, D))
+            self._need("join[1]", join[1], torch.float32, (B, H, Q))
+            join_out, join_lse = join[0].data_ptr(), join[1].data_ptr()
+        out, lse = self._result("out", out, result, (B, Q, H, D)), self._result("lse", lse, torch.float32, (B, H, Q))
+        work = self._work(size) if size else None   # (held until the call is made)
+        self._call("ncclCpAttention", at, pq, pk, pv, nq, nk, join_out, join_lse, out.data_ptr(), lse.data_ptr(), work.data_ptr() if size else None)
         return out, lse
 
     def attention_delta(self, dout, out, q_lengths=None, delta=None):
@@ -238,12 +246,15 @@ class ContextParallel:
         if out.dim() != 4 or out.dtype not in (self.torch.float16, self.torch.bfloat16):
             raise ValueError("out must be an fp16 or bf16 tensor [batch, tokens, heads, channels], not %s %s" % (str(out.dtype).replace("torch.", ""), list(out.shape)))
         B, Q, H, D = out.shape
-        sizes = self._sizes(out, out, out)
-        strides = None, None, None, self._operand("dout", dout, out.dtype, (B, Q, H, D)), self._operand("out", out, out.dtype, (B, Q, H, D))
+
+        def make():
+            sizes = self._sizes(out, out, out)
+            strides = None, None, None, self._operand("dout", dout, out.dtype, (B, Q, H, D)), self._operand("out", out, out.dtype, (B, Q, H, D))
+            return self._describe(sizes, out.dtype, out.dtype, (0, 0, 1.0), strides, None)
+        d, at, _ = self._remember((out.shape, out.stride(), out.dtype, dout.shape, dout.stride(), dout.dtype), make)
         nq = self._lengths("q_lengths", q_lengths, B)
         delta = self._result("delta", delta, self.torch.float32, (B, H, Q))
-        d, _ = self._shape(sizes, out.dtype, out.dtype, (0, 0, 1.0), strides, None)
-        self._call("ncclCpAttentionDelta", ctypes.addressof(d), dout.data_ptr(), out.data_ptr(), nq, delta.data_ptr())
+        self._call("ncclCpAttentionDelta", at, self._at("dout", dout), self._at("out", out), nq, delta.data_ptr())
         return delta
 
     def attention_backward(self, dout, q, k, v, out, lse, causal=False, offset=None, scale=None, q_lengths=None, kv_lengths=None, delta=None, add=None, dtype=None, dq=None, dk=None,
@@ -253,29 +264,34 @@ class ContextParallel:
 
         ``out`` and ``lse`` are the result over all keys of the queries: where blocks were joined, the last one's. ``delta``: what ``attention_delta`` gives (out may then be
         None). ``add``: fp32 (dq, dk, dv) so far, to which these are added; they may be the results' tensors. The same call gives the same bits."""
-        torch, ptr = self.torch, lambda t: None if t is None else t.data_ptr()   # noqa: E731
-        sizes = B, Q, K, H, G, D = self._sizes(q, k, v)
-        strides = [self._operand("q", q, q.dtype, (B, Q, H, D)), self._operand("k", k, q.dtype, (B, K, G, D)), self._operand("v", v, q.dtype, (B, K, G, D)),
-                   self._operand("dout", dout, q.dtype, (B, Q, H, D)), None]
-        if out is not None:
-            strides[4] = self._operand("out", out, q.dtype, (B, Q, H, D))
-        elif delta is None:
+        torch = self.torch
+
+        def make():
+            sizes = B, Q, K, H, G, D = self._sizes(q, k, v)
+            strides = (self._operand("q", q, q.dtype, (B, Q, H, D)), self._operand("k", k, q.dtype, (B, K, G, D)), self._operand("v", v, q.dtype, (B, K, G, D)),
+                       self._operand("dout", dout, q.dtype, (B, Q, H, D)), None if out is None else self._operand("out", out, q.dtype, (B, Q, H, D)))
+            result = self._result_type(dtype, q)
+            return sizes, result, self._describe(sizes, q.dtype, result, self._mask(causal, offset, scale, D), strides, self.lib.ncclCpAttentionBackwardWork)
+        (B, Q, K, H, G, D), result, (d, at, size) = self._remember(
+            (q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, causal, offset, scale, dtype, dout.shape, dout.stride(), dout.dtype,
+             None if out is None else (out.shape, out.stride(), out.dtype)), make)
+        if out is None and delta is None:
             raise ValueError("out or delta must be given")
+        pd, pq, pk, pv, po = self._at("dout", dout), self._at("q", q), self._at("k", k), self._at("v", v), None if out is None else self._at("out", out)
         self._need("lse", lse, torch.float32, (B, H, Q))
         if delta is not None:
             self._need("delta", delta, torch.float32, (B, H, Q))
         nq, nk = self._lengths("q_lengths", q_lengths, B), self._lengths("kv_lengths", kv_lengths, B)
-        dtype = self._result_type(dtype, q)
-        shapes = (B, Q, H, D), (B, K, G, D), (B, K, G, D)
-        given = (None, None, None) if add is None else add
+        sq, sk = (B, Q, H, D), (B, K, G, D)
+        given = (None, None, None)
         if add is not None:
-            for i, name in enumerate(("add[0]", "add[1]", "add[2]")):
-                self._need(name, given[i], torch.float32, shapes[i])
-        dq, dk, dv = (self._result(name, t, dtype, shape) for name, t, shape in zip(("dq", "dk", "dv"), (dq, dk, dv), shapes))
-        d, size = self._shape(sizes, q.dtype, dtype, self._mask(causal, offset, scale, D), tuple(strides), self.lib.ncclCpAttentionBackwardWork)
-        work = self._work(size)
-        self._call("ncclCpAttentionBackward", ctypes.addressof(d), dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr(out), lse.data_ptr(), ptr(delta), nq, nk,
-                   *[ptr(t) for t in given], dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ptr(work))
+            for name, t, shape in zip(("add[0]", "add[1]", "add[2]"), add, (sq, sk, sk)):
+                self._need(name, t, torch.float32, shape)
+            given = [t.data_ptr() for t in add]
+        dq, dk, dv = self._result("dq", dq, result, sq), self._result("dk", dk, result, sk), self._result("dv", dv, result, sk)
+        work = self._work(size) if size else None   # (held until the call is made)
+        self._call("ncclCpAttentionBackward", at, pd, pq, pk, pv, po, lse.data_ptr(), None if delta is None else delta.data_ptr(), nq, nk, *given, dq.data_ptr(), dk.data_ptr(),
+                   dv.data_ptr(), work.data_ptr() if size else None)
         return dq, dk, dv
 
     # ------------------------------------------------------------------ rotary positions
@@ -295,42 +311,46 @@ class ContextParallel:
         or ``offset`` + its index: a rank that holds rows from `begin` on gives ``offset=begin``. Pairs are channels (i, i + half), with ``interleaved`` (2 i, 2 i + 1).
         ``inverse`` turns back: the gradient's way. ``out``: (q, k) tensors for the results, which may be q and k themselves. Angles are reduced to a turn in 64 bits."""
         torch = self.torch
-        if q.dim() != 4 or q.dtype not in self._codes or (k is not None and (k.dim() != 4 or k.dtype is not q.dtype or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
-            raise ValueError("q and k must be fp16, bf16 or fp32 tensors [batch, tokens, heads, channels] that differ in heads only, not %s %s and %s" % (
-                str(q.dtype).replace("torch.", ""), list(q.shape), None if k is None else [str(k.dtype).replace("torch.", ""), list(k.shape)]))
-        B, T, _, D = q.shape
-        if not isinstance(freqs, RotaryFrequencies) or 2 * freqs.half > D:
-            raise ValueError("freqs must come from rotary_frequencies, for at most %d channels" % D)
-        self._need("freqs.turns", freqs.turns, torch.float64, (freqs.half,))
-        if B * T >> 31 or abs(offset) >> 62:
-            raise ValueError("%d sequences of %d tokens, offset %r" % (B, T, offset))
-        st = (0, 0)
-        if positions is not None:
-            if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (B, T) or positions.get_device() != self._device or min(positions.stride()) < 0:
-                raise ValueError("positions must be an int32 or int64 tensor [%d, %d] on cuda:%d, not %s %s on %s" % (
-                    B, T, self._device, str(positions.dtype).replace("torch.", ""), list(positions.shape), positions.device))
-            st = positions.stride()
-        xs = [q] if k is None else [q, k]
-        ys = [None] * len(xs) if out is None else list(out)[:len(xs)]
-        for i, x in enumerate(xs):
-            if x.get_device() != self._device or not x.shape[2] or (x.stride(3) != 1 and D > 1):
-                raise ValueError("q and k must be on cuda:%d, with heads, and channels next to each other: %s, strides %s, on %s" % (self._device, list(x.shape), list(x.stride()), x.device))
-            if ys[i] is None:
-                ys[i] = torch.empty(x.shape, dtype=x.dtype, device=self._place)
-            elif ys[i].dtype is not x.dtype or ys[i].shape != x.shape or ys[i].get_device() != self._device or (ys[i].stride(3) != 1 and D > 1):
-                raise ValueError("results must be like q and k, with channels next to each other")
-        key = (tuple(x.shape for x in xs), q.dtype, freqs.half, freqs.amplitude, interleaved, inverse, offset, None if positions is None else positions.dtype, st,
-               tuple(x.stride() for x in xs), tuple(y.stride() for y in ys))
+        xs = (q,) if k is None else (q, k)
+        ys = (None, None) if out is None else out
 
         def make():
+            if q.dim() != 4 or q.dtype not in self._codes or (k is not None and (k.dim() != 4 or k.dtype is not q.dtype or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
+                raise ValueError("q and k must be fp16, bf16 or fp32 tensors [batch, tokens, heads, channels] that differ in heads only, not %s %s and %s" % (
+                    str(q.dtype).replace("torch.", ""), list(q.shape), None if k is None else [str(k.dtype).replace("torch.", ""), list(k.shape)]))
+            B, T, _, D = q.shape
+            if not isinstance(freqs, RotaryFrequencies) or 2 * freqs.half > D:
+                raise ValueError("freqs must come from rotary_frequencies, for at most %d channels" % D)
+            if B * T >> 31 or abs(offset) >> 62:
+                raise ValueError("%d sequences of %d tokens, offset %r" % (B, T, offset))
             d = _Rotary(ctypes.sizeof(_Rotary), MAGIC, self._codes[q.dtype], B, T, D, freqs.half)
-            d.interleaved, d.inverse, d.positions64, d.amplitude, d.offset = bool(interleaved), bool(inverse), positions is not None and positions.dtype is torch.int64, freqs.amplitude, offset
-            d.position_stride[:] = st
-            for i, (x, y) in enumerate(zip(xs, ys)):
+            d.interleaved, d.inverse, d.amplitude, d.offset = bool(interleaved), bool(inverse), freqs.amplitude, offset
+            if positions is not None:
+                if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (B, T) or min(positions.stride()) < 0:
+                    raise ValueError("positions must be an int32 or int64 tensor [%d, %d], not %s %s" % (B, T, str(positions.dtype).replace("torch.", ""), list(positions.shape)))
+                d.positions64, d.position_stride[:] = positions.dtype is torch.int64, positions.stride()
+            for i, x in enumerate(xs):
+                if not x.shape[2] or (x.stride(3) != 1 and D > 1):
+                    raise ValueError("q and k must have heads, and channels next to each other: %s, strides %s" % (list(x.shape), list(x.stride())))
+                y = ys[i]
+                if y is not None and (y.dtype is not x.dtype or y.shape != x.shape or (y.stride(3) != 1 and D > 1)):
+                    raise ValueError("results must be like q and k, with channels next to each other")
                 d.heads[i] = x.shape[2]
-                d.x_stride[i][:], d.y_stride[i][:] = x.stride()[:3], y.stride()[:3]
-            return d
-        d = self._remember(key, make)
-        at = lambda ts: [t.data_ptr() for t in ts] + [None] * (2 - len(ts))   # noqa: E731
-        self._call("ncclCpRotary", ctypes.addressof(d), *at(xs), *at(ys), None if positions is None else positions.data_ptr(), freqs.turns.data_ptr())
-        return ys[0], None if k is None else ys[1]
+                d.x_stride[i][:] = x.stride()[:3]
+                d.y_stride[i][:] = (x.shape[1] * x.shape[2] * D, x.shape[2] * D, D) if y is None else y.stride()[:3]
+            return d, ctypes.addressof(d)
+        d, at = self._remember((q.shape, q.stride(), q.dtype, None if k is None else (k.shape, k.stride(), k.dtype), freqs.half, freqs.amplitude, interleaved, inverse, offset,
+                                None if positions is None else (positions.shape, positions.stride(), positions.dtype),
+                                out is None or tuple(None if y is None else (y.shape, y.stride(), y.dtype) for y in ys)), make)
+        px, py, got = [None, None], [None, None], [None, None]
+        for i, x in enumerate(xs):
+            y = ys[i]
+            if y is None:
+                y = torch.empty(*x.shape, dtype=x.dtype, device=self._place)
+            if x.get_device() != self._device or y.get_device() != self._device:
+                raise ValueError("q, k and results must be on cuda:%d, not on %s and %s" % (self._device, x.device, y.device))
+            px[i], py[i], got[i] = x.data_ptr(), y.data_ptr(), y
+        if freqs.turns.get_device() != self._device or (positions is not None and positions.get_device() != self._device):
+            raise ValueError("frequencies and positions must be on cuda:%d" % self._device)
+        self._call("ncclCpRotary", at, *px, *py, None if positions is None else positions.data_ptr(), freqs.turns.data_ptr())
+        return got[0], got[1]

@@ -5,6 +5,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <initializer_list>
 #include <new>
@@ -17,6 +18,7 @@ using namespace b200;
 struct ncclCpContext {
   ncclComm* comm = nullptr;
   int smCount = 0;
+  std::atomic<const void*> ready[16] = {};   // kernels with tiles that have been set up on this GPU
 };
 
 // The context's GPU is the current one while this lives.
@@ -41,6 +43,22 @@ static bool aligned(std::initializer_list<const void*> ps, size_t to) {
   return all % to == 0;
 }
 
+// Once for each kernel that moves registers between its warps: registers that nobody was launched with would be waited for without end.
+static ncclResult_t setUp(ncclCpContext* cp, const void* fn, size_t smem, int regs) {
+  std::atomic<const void*>* place = nullptr;
+  for (auto& r : cp->ready) {
+    const void* p = r.load(std::memory_order_relaxed);
+    if (p == fn) return ncclSuccess;
+    if (!p) { place = &r; break; }
+  }
+  cudaFuncAttributes built;
+  CUDACHECK(cudaFuncGetAttributes(&built, fn));
+  if (built.numRegs < regs) { WARN("an attention kernel was built with %d registers instead of %d", built.numRegs, regs); return ncclInternalError; }
+  CUDACHECK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (place) place->store(fn, std::memory_order_relaxed);   // (two threads that come here at once do the same)
+  return ncclSuccess;
+}
+
 // `regs`: what a thread of a kernel that moves registers between its warps has to be launched with.
 static ncclResult_t launchCp(ncclCpContext* cp, const void* fn, unsigned grid, unsigned gridY, int threads, size_t smem, void** args, cudaStream_t stream, int regs = 0) {
   cudaLaunchConfig_t cfg = {};
@@ -55,13 +73,7 @@ static ncclResult_t launchCp(ncclCpContext* cp, const void* fn, unsigned grid, u
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs = 1;
   }
-  if (regs) {
-    // registers that nobody was launched with would be waited for without end
-    cudaFuncAttributes built;
-    CUDACHECK(cudaFuncGetAttributes(&built, fn));
-    if (built.numRegs < regs) { WARN("an attention kernel was built with %d registers instead of %d", built.numRegs, regs); return ncclInternalError; }
-    CUDACHECK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  }
+  if (regs) NCCLCHECK(setUp(cp, fn, smem, regs));
   const cudaError_t e = cudaLaunchKernelExC(&cfg, fn, args);
   if (e != cudaSuccess) {
     WARN("context-parallel kernel launch failed: %s", cudaGetErrorString(e));
