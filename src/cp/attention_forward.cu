@@ -67,6 +67,9 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     mbarInit(smemAddr(drainBar), 1);
     *abortFlag = 0;
     mbarInitFence();
+    prefetchTensorMap(&tmQ);
+    prefetchTensorMap(&tmK);
+    prefetchTensorMap(&tmV);
   }
   if (warp == W::kMma) {
     tmemAlloc(smemAddr(tmemSlot), kTmemCols);
@@ -401,36 +404,57 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   }
 }
 
-// Joins the parts of the keys: out = sum_s exp(lse_s - L) out_s with L = ln sum_s exp(lse_s); what `join` names is one more part. A thread has four channels of a row.
+// Joins the parts of the keys: out = sum_s exp(lse_s - L) out_s with L = ln sum_s exp(lse_s); what `join` names is one more part. quads * a.joinShares threads take a row: four
+// channels of every joinShares-th part each, all of them on their way at once, and the first of those with the same channels joins the others' (with a thread for four channels that
+// walked the parts one after the other, 16 parts of 32 rows took 8.6 us).
+constexpr int kJoinTurns = 8;
+static_assert(kAttnMaxSplits <= kJoinTurns * (256 / (kAttnMaxDim / 4)), "parts of a thread");
 template <typename T>
 __global__ void __launch_bounds__(256) attnJoinKernel(const __grid_constant__ AttnArgs a) {
+  __shared__ float4 sums[256];
+  __shared__ float2 heads[256];   // maximum and sum of the weights
+  const int quads = a.dim / 4, each = quads * a.joinShares, perCta = 256 / each;
+  const int slot = threadIdx.x / each, share = threadIdx.x % each / quads, d = threadIdx.x % quads * 4;
+  const size_t rows = (size_t)a.batch * a.q * a.heads, row = (size_t)blockIdx.x * perCta + slot;
+  const bool some = slot < perCta && row < rows;
   pdlEnter();
-  const int quads = a.dim / 4;
-  const size_t rows = (size_t)a.batch * a.q * a.heads, i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  const size_t row = i / quads;
-  const int d = (int)(i % quads) * 4;
-  if (row >= rows) return;
+  float lse[kJoinTurns], top = -INFINITY, total = 0.0f;
+  float4 v[kJoinTurns], f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+  for (int i = 0; i < kJoinTurns; ++i) {
+    const int s = share + i * a.joinShares;
+    const bool mine = some && s < a.splits;
+    lse[i] = mine ? a.partLse[s * rows + row] : -INFINITY;
+    v[i] = mine ? *(const float4*)(a.partOut + (s * rows + row) * a.dim + d) : f;   // (zeros in a part that saw no key)
+  }
   const int head = (int)(row % a.heads);
   const size_t token = row / a.heads;   // of the batch
   const int b = (int)(token / a.q), tok = (int)(token % a.q);
   const size_t atLse = ((size_t)b * a.heads + head) * a.q + tok;
-  const bool join = a.joinOut && tok < (a.qLengths ? a.qLengths[b] : a.q);
-  float top = join ? a.joinLse[atLse] : -INFINITY, total = 0.0f;
-  const float other = top;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.partLse[(size_t)s * rows + row]);
-  const float base = top == -INFINITY ? 0.0f : top;
-  float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int s = 0; s <= a.splits; ++s) {
-    if (s == a.splits && !join) break;
-    const float w = expf((s < a.splits ? a.partLse[(size_t)s * rows + row] : other) - base);
-    total += w;
-    if (w == 0.0f) continue;   // (a part that saw no key holds zeros)
-    const float4 v = *(const float4*)((s < a.splits ? a.partOut + ((size_t)s * rows + row) * a.dim : a.joinOut + row * a.dim) + d);
-    f.x += w * v.x; f.y += w * v.y; f.z += w * v.z; f.w += w * v.w;
+  const bool join = some && share == 0 && a.joinOut && tok < (a.qLengths ? a.qLengths[b] : a.q);
+  const float otherLse = join ? a.joinLse[atLse] : -INFINITY;
+  const float4 other = join ? *(const float4*)(a.joinOut + row * a.dim + d) : f;
+  // joins (to, sum, x) to what this thread has
+  auto add = [&](float to, float weight, float4 x) {
+    if (to == -INFINITY) return;
+    const float m = fmaxf(top, to), old = expf(top - m), now = expf(to - m);
+    total = total * old + weight * now;
+    f.x = f.x * old + x.x * now; f.y = f.y * old + x.y * now; f.z = f.z * old + x.z * now; f.w = f.w * old + x.w * now;
+    top = m;
+  };
+#pragma unroll
+  for (int i = 0; i < kJoinTurns; ++i) add(lse[i], 1.0f, v[i]);
+  if (share) {
+    sums[threadIdx.x] = f;
+    heads[threadIdx.x] = make_float2(top, total);
   }
+  __syncthreads();
+  if (share || !some) return;
+  for (int i = 1; i < a.joinShares; ++i) add(heads[threadIdx.x + i * quads].x, heads[threadIdx.x + i * quads].y, sums[threadIdx.x + i * quads]);
+  add(otherLse, 1.0f, other);
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   f.x *= inv; f.y *= inv; f.z *= inv; f.w *= inv;
-  if (d == 0) a.lse[atLse] = total == 0.0f ? -INFINITY : base + logf(total);
+  if (d == 0) a.lse[atLse] = total == 0.0f ? -INFINITY : top + logf(total);
   if (a.outFp32) *(float4*)((float*)a.out + row * a.dim + d) = f;
   else *(uint2*)((uint16_t*)a.out + row * a.dim + d) = make_uint2(Pack<T>::two(f.x, f.y), Pack<T>::two(f.z, f.w));
 }

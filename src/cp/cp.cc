@@ -316,8 +316,11 @@ ncclResult_t ncclCpAttention(ncclCp_t cp, const ncclCpAttention_t* c, const void
   const unsigned grid = (unsigned)c->batch * c->kv_heads * (plan.pairs ? (a.tiles + 1) / 2 : a.tiles) * plan.splits;
   NCCLCHECK(launchCp(cp, attnForwardKernelFn(type, c->head_dim, plan.pairs), grid, 1, attnForwardThreads(), attnForwardSmemBytes(c->head_dim, plan.pairs), args, stream, attnForwardRegs()));
   if (plan.splits == 1) return ncclSuccess;
+  const int quads = c->head_dim / 4;
+  a.joinShares = std::min(256 / quads, plan.splits);
+  const int perCta = 256 / (quads * a.joinShares);
   void* join[1] = {&a};
-  return launchCp(cp, attnJoinKernelFn(type), (unsigned)((rows * (c->head_dim / 4) + 255) / 256), 1, 256, 0, join, stream);
+  return launchCp(cp, attnJoinKernelFn(type), (unsigned)((rows + perCta - 1) / perCta), 1, 256, 0, join, stream);
 }
 
 size_t ncclCpAttentionBackwardWork(ncclCp_t cp, const ncclCpAttention_t* c) {
@@ -503,10 +506,15 @@ ncclResult_t ncclCpRotary(ncclCp_t cp, const ncclCpRotary_t* c, const void* x0, 
   a.interleaved = c->interleaved != 0;
   a.inverse = c->inverse != 0;
   B200_ON_DEVICE(cp);
-  const int tokens = c->batch * c->tokens, items = (c->heads[0] + c->heads[1]) * (c->head_dim / (a.wide ? E : 1));
-  const int shares = std::max(1, std::min({cp->smCount / tokens, (items + 255) / 256, 64}));   // of a token, where tokens are few
+  // A CTA takes as many tokens as it computes angles for at a time; where tokens are few, several share the heads of one.
+  const int tokens = c->batch * c->tokens, heads = c->heads[0] + c->heads[1], width = a.wide ? E : 1;
+  a.items = (a.interleaved && a.wide ? 2 * a.half : a.half) / width + (a.dim - 2 * a.half) / width;
+  const int most = std::max(1, kRotaryAngles / a.half);
+  a.tokensAtOnce = std::max(1, std::min(most, tokens / (4 * cp->smCount)));
+  const int blocks = (tokens + a.tokensAtOnce - 1) / a.tokensAtOnce;
+  const int shares = std::max(1, std::min({cp->smCount / blocks, (heads * a.items + 255) / 256, 64}));
   void* args[1] = {&a};
-  return launchCp(cp, rotaryKernelFn(type), (unsigned)std::min(tokens, 1 << 20), (unsigned)shares, 256, 0, args, stream);
+  return launchCp(cp, rotaryKernelFn(type), (unsigned)blocks, (unsigned)shares, 256, 0, args, stream);
 }
 
 }  // extern "C"

@@ -29,6 +29,7 @@ struct AttnArgs {
   int splits;                 // above 1: fp32 results of each part of the keys go to partOut [splits][batch * q * heads][dim], partLse [splits][rows]
   float* partOut;
   float* partLse;
+  int joinShares;             // threads with the same channels of a row
   // backward
   const float* stats;         // [batch][kvHeads][tiles][2][128]: minus the log-sum-exp in units of log 2 and minus <d(out), out> of each row
   int tiles;                  // of the queries of a key head
@@ -66,7 +67,10 @@ struct RotaryArgs {
   int batch, tokens, dim, half;
   int interleaved, inverse;
   int wide;                   // channels of a pack (16 bytes) may be moved together
+  int tokensAtOnce;           // of a CTA
+  int items;                  // of a head: packs (or channels) of both of a pair, and those that are copied
 };
+constexpr int kRotaryAngles = 256;   // of a CTA at a time
 
 enum AttnType : int { ATTN_F16 = 0, ATTN_BF16 = 1, ATTN_F32 = 2 };
 // dim <= 64 or <= 128. `pairs`: two tiles of queries for each CTA; else one, whose keys its two halves share.

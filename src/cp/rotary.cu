@@ -25,72 +25,86 @@ template <> __device__ __forceinline__ __nv_bfloat16 fromFloat(float v) { return
 
 template <typename T, int E> struct alignas(E * sizeof(T)) Channels { T v[E]; };
 
-// E channels at a time: 16 bytes, or one where sizes, strides or addresses do not allow more.
+// E channels at a time: 16 bytes, or one where sizes, strides or addresses do not allow more. An item is a pack of each half of the pairs, a pack of neighbours, or one that is
+// only copied; a thread steps from item to item without a division.
 template <typename T, int E>
-__device__ __forceinline__ void turnHeads(const RotaryArgs& a, int b, int tok, const float2* table) {
-  const int paired = a.interleaved && E > 1 ? 2 * a.half / E : a.half / E;   // items of a head that turn: a pack of neighbours, or one of a and one of b
-  const int items = paired + (a.dim - 2 * a.half) / E, heads = a.heads[0] + a.heads[1];
-  const int stride = gridDim.y * blockDim.x;
-  for (int i = blockIdx.y * blockDim.x + threadIdx.x; i < heads * items; i += stride) {
-    int head = i / items;
-    const int p = i - head * items, which = head >= a.heads[0];
-    if (which) head -= a.heads[0];
-    const T* x = (const T*)a.x[which] + (b * a.inStride[which][0] + tok * a.inStride[which][1] + head * a.inStride[which][2]);
-    T* y = (T*)a.y[which] + (b * a.outStride[which][0] + tok * a.outStride[which][1] + head * a.outStride[which][2]);
-    using C = Channels<T, E>;
+__device__ __forceinline__ void turnHeads(const RotaryArgs& a, int token0, int tokens, const float2* table) {
+  using C = Channels<T, E>;
+  const bool neighbours = a.interleaved && E > 1;
+  const int paired = neighbours ? 2 * a.half / E : a.half / E, heads = a.heads[0] + a.heads[1];
+  const int stride = gridDim.y * blockDim.x, first = blockIdx.y * blockDim.x + threadIdx.x;
+  const int stepRows = stride / a.items, stepP = stride % a.items, stepTokens = stepRows / heads, stepHeads = stepRows % heads;
+  int p = first % a.items, row = first / a.items, local = row / heads, head = row % heads, b = (token0 + local) / a.tokens, tok = token0 + local - b * a.tokens;
+  while (local < tokens) {
+    const int which = head >= a.heads[0];
+    const long long h = which ? head - a.heads[0] : head;
+    const T* x = (const T*)a.x[which] + (b * a.inStride[which][0] + tok * a.inStride[which][1] + h * a.inStride[which][2]);
+    T* y = (T*)a.y[which] + (b * a.outStride[which][0] + tok * a.outStride[which][1] + h * a.outStride[which][2]);
+    const float2* angles = table + local * a.half;
     if (p >= paired) {
       const int at = 2 * a.half + (p - paired) * E;
       *(C*)(y + at) = *(const C*)(x + at);
-    } else if (E > 1 && a.interleaved) {
+    } else if (neighbours) {
       C v = *(const C*)(x + p * E);
 #pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        const float2 t = table[(p * E + e) / 2];
+      for (int e = 0; e + 1 < E; e += 2) {
+        const float2 r = angles[(p * E + e) / 2];
         const float lo = toFloat(v.v[e]), hi = toFloat(v.v[(e + 1) % E]);
-        v.v[e] = fromFloat<T>(lo * t.x - hi * t.y);
-        v.v[(e + 1) % E] = fromFloat<T>(hi * t.x + lo * t.y);
+        v.v[e] = fromFloat<T>(lo * r.x - hi * r.y);
+        v.v[(e + 1) % E] = fromFloat<T>(hi * r.x + lo * r.y);
       }
       *(C*)(y + p * E) = v;
     } else {
-      const int first = a.interleaved ? 2 * p : p * E, second = a.interleaved ? first + 1 : a.half + p * E;   // (neighbours: one channel at a time)
-      C u = *(const C*)(x + first), v = *(const C*)(x + second);
+      const int one = a.interleaved ? 2 * p : p * E, two = a.interleaved ? one + 1 : a.half + one;
+      C u = *(const C*)(x + one), v = *(const C*)(x + two);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float2 t = table[p * E + e];
+        const float2 r = angles[p * E + e];
         const float lo = toFloat(u.v[e]), hi = toFloat(v.v[e]);
-        u.v[e] = fromFloat<T>(lo * t.x - hi * t.y);
-        v.v[e] = fromFloat<T>(hi * t.x + lo * t.y);
+        u.v[e] = fromFloat<T>(lo * r.x - hi * r.y);
+        v.v[e] = fromFloat<T>(hi * r.x + lo * r.y);
       }
-      *(C*)(y + first) = u;
-      *(C*)(y + second) = v;
+      *(C*)(y + one) = u;
+      *(C*)(y + two) = v;
     }
+    p += stepP;
+    int more = stepTokens;
+    head += stepHeads;
+    if (p >= a.items) {
+      p -= a.items;
+      ++head;
+    }
+    if (head >= heads) {
+      head -= heads;
+      ++more;
+    }
+    local += more;
+    for (tok += more; tok >= a.tokens; tok -= a.tokens) ++b;
   }
 }
 
-// A CTA (of gridDim.y, where tokens are few) has a token.
+// A CTA has `tokensAtOnce` tokens; where tokens are few, gridDim.y CTAs share the heads of the same ones.
 template <typename T>
-__global__ void __launch_bounds__(256) rotaryKernel(const __grid_constant__ RotaryArgs a) {
+__global__ void __launch_bounds__(256, 6) rotaryKernel(const __grid_constant__ RotaryArgs a) {
   __shared__ float2 table[kMaxHalf];
+  const int token0 = blockIdx.x * a.tokensAtOnce, tokens = min(a.tokensAtOnce, a.batch * a.tokens - token0);
   pdlEnter();
-  for (int token = blockIdx.x; token < a.batch * a.tokens; token += gridDim.x) {
-    const int b = token / a.tokens, tok = token - b * a.tokens;
+  for (int i = threadIdx.x; i < tokens * a.half; i += blockDim.x) {
+    const int local = i / a.half, pair = i - local * a.half, b = (token0 + local) / a.tokens, tok = token0 + local - b * a.tokens;
     long long at = a.offset + tok;
     if (a.positions) {
-      const long long i = b * a.positionStride[0] + tok * a.positionStride[1];
-      at = a.positions64 ? ((const long long*)a.positions)[i] : (long long)((const int*)a.positions)[i];
+      const long long n = b * a.positionStride[0] + tok * a.positionStride[1];
+      at = a.positions64 ? ((const long long*)a.positions)[n] : (long long)((const int*)a.positions)[n];
     }
-    for (int i = threadIdx.x; i < a.half; i += blockDim.x) {
-      double t = (double)at * a.turns[i];
-      t -= rint(t);
-      float s, c;
-      sincospif((float)(2.0 * t), &s, &c);
-      table[i] = make_float2(a.amplitude * c, a.inverse ? -a.amplitude * s : a.amplitude * s);
-    }
-    __syncthreads();
-    if (a.wide) turnHeads<T, 16 / sizeof(T)>(a, b, tok, table);
-    else turnHeads<T, 1>(a, b, tok, table);
-    __syncthreads();
+    double t = (double)at * a.turns[pair];
+    t -= rint(t);
+    float s, c;
+    sincospif((float)(2.0 * t), &s, &c);
+    table[i] = make_float2(a.amplitude * c, a.inverse ? -a.amplitude * s : a.amplitude * s);
   }
+  __syncthreads();
+  if (a.wide) turnHeads<T, 16 / sizeof(T)>(a, token0, tokens, table);
+  else turnHeads<T, 1>(a, token0, tokens, table);
 }
 
 }  // namespace
