@@ -30,10 +30,9 @@ template <int DP, bool PAIRS> struct ForwardShape {
   static constexpr int kStages = (PAIRS ? 4 : 6) * (DP == 64 ? 2 : 1) - (!PAIRS && DP == 64 ? 1 : 0);
   static constexpr uint32_t kRing = kQTiles * kTileBytes, kCtrl = kRing + kStages * kTileBytes;
   static_assert((2 * kStages + 10) * 8 + 8 <= 512, "control block");
-  static constexpr size_t kBytes = kCtrl + 512;            // (dynamic shared memory, all that this kernel has, begins on a multiple of 1024 bytes)
+  static constexpr uint32_t kExchange = kCtrl + 512;       // maxima and sums of the second group's rows, where it has the first one's
+  static constexpr size_t kBytes = kExchange + (PAIRS ? 0 : 1024);   // (dynamic shared memory, all that this kernel has, begins on a multiple of 1024 bytes)
   static_assert(kBytes <= 227 * 1024, "shared memory");
-  // the joined form hands 128 rows of DP fp32 sums, their maxima and sums over
-  static_assert(PAIRS || (DP * 128 * 4 + 1024 <= kStages * kTileBytes), "shared memory");
 };
 
 // The order in which tiles of keys and values go through the ring: K0 V0 K1 V1 ... where one tile serves both groups, K0 K1 V0 K2 V1 K3 ... where the groups take turns.
@@ -302,25 +301,16 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
     if (ok && count[t]) {
       ok = warpWaitOr(smemAddr(&outBar[t]), 0, abortFlag);
-      if (ok && t == 1 && !PAIRS) ok = warpWaitOr(smemAddr(&outBar[0]), 0, abortFlag);
+      if (ok && !PAIRS && t == 0 && count[1]) ok = warpWaitOr(smemAddr(&outBar[1]), 0, abortFlag);
       if (!ok && lane == 0) fail(3100 + t);
       tcFenceAfter();
     }
-    const float* sums = (const float*)(smem + Shape::kRing) + row;
-    const float* ml = (const float*)(smem + Shape::kRing) + DP * 128 + row;
+    float* const ml = (float*)(smem + Shape::kExchange) + row;
     if (!PAIRS) {
-      // the second group hands its sums over: [channel][row], behind every copy and product of the CTA
-      if (t == 1 && count[1] && ok && working) {
-#pragma unroll
-        for (int k = 0; k < DP / 32; ++k) {
-          uint32_t o[32];
-          tmemLd32(tO + k * 32, o);
-          tmemLdWait32(o);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) const_cast<float*>(sums)[(k * 32 + e) * 128] = __uint_as_float(o[e]);
-        }
-        const_cast<float*>(ml)[0] = m;
-        const_cast<float*>(ml)[128] = l;
+      // both groups have the same rows, and the first one stores them: it can read the second's sums, not what they are to be multiplied by
+      if (t == 1 && count[1] && ok) {
+        ml[0] = m;
+        ml[128] = l;
       }
       ok = allWell<W::kCompute * 32>(1, ok);
     }
@@ -357,17 +347,21 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
 #pragma unroll
       for (int k = 0; k < DP / 32; ++k) {
-        uint32_t o[32];
+        uint32_t o[32], u[32];
         float f[32];
         if (count[t]) {
           tmemLd32(tO + k * 32, o);
+          if (!PAIRS && count[1]) {
+            tmemLd32(tO + 128 + k * 32, u);
+            tmemLdWait32(u);
+          }
           tmemLdWait32(o);
         }
         if (!exists) continue;
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           f[e] = count[t] ? __uint_as_float(o[e]) * weight : 0.0f;
-          if (!PAIRS && count[1]) f[e] += sums[(k * 32 + e) * 128] * theirs;
+          if (!PAIRS && count[1]) f[e] += __uint_as_float(u[e]) * theirs;
           f[e] = empty || !count[t] ? 0.0f : f[e] * share;
         }
         const int channel = k * 32;
