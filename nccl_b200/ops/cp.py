@@ -311,6 +311,8 @@ class ContextParallel:
         or ``offset`` + its index: a rank that holds rows from `begin` on gives ``offset=begin``. Pairs are channels (i, i + half), with ``interleaved`` (2 i, 2 i + 1).
         ``inverse`` turns back: the gradient's way. ``out``: (q, k) tensors for the results, which may be q and k themselves. Angles are reduced to a turn in 64 bits."""
         torch = self.torch
+        if not isinstance(freqs, RotaryFrequencies):
+            raise ValueError("freqs must come from rotary_frequencies")
         xs = (q,) if k is None else (q, k)
         ys = (None, None) if out is None else out
 
@@ -319,8 +321,8 @@ class ContextParallel:
                 raise ValueError("q and k must be fp16, bf16 or fp32 tensors [batch, tokens, heads, channels] that differ in heads only, not %s %s and %s" % (
                     str(q.dtype).replace("torch.", ""), list(q.shape), None if k is None else [str(k.dtype).replace("torch.", ""), list(k.shape)]))
             B, T, _, D = q.shape
-            if not isinstance(freqs, RotaryFrequencies) or 2 * freqs.half > D:
-                raise ValueError("freqs must come from rotary_frequencies, for at most %d channels" % D)
+            if 2 * freqs.half > D:
+                raise ValueError("frequencies of %d channels, and heads of %d" % (2 * freqs.half, D))
             if B * T >> 31 or abs(offset) >> 62:
                 raise ValueError("%d sequences of %d tokens, offset %r" % (B, T, offset))
             d = _Rotary(ctypes.sizeof(_Rotary), MAGIC, self._codes[q.dtype], B, T, D, freqs.half)

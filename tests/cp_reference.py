@@ -25,7 +25,9 @@ class Reference:
 
     A product's sum of n terms in fp32 is off by at most n * 2^-23 of the sum of their magnitudes (2^-23: the tensor cores may cut off instead of rounding). An
     exponential of a score is off relatively by the score's error, plus 2^-20 for the exponent's rounding and the function. A rounding to 16 bits is off by half a
-    step, `u`: one for the probabilities (or ds), one for the result."""
+    step, `u`: one for the probabilities (or ds), one for the result; or by half of the smallest step there is. In fp16 that one matters inside too: probabilities of the forward
+    pass are held as multiples of 2^-24 of a largest one of at least 2^-1 (2^7 over the lag of 2^8), those of the backward pass as multiples of 2^-39, and ds as
+    multiples of 2^-24 where the largest that could be, 2 |do| |v|, is 2^14 at least."""
 
     def __init__(self, q, k, v, causal=False, offset=None, scale=None, q_lengths=None, kv_lengths=None, join=None, dout=None, out=None, result=None, add=None):
         B, Q, H, D = q.shape
@@ -34,6 +36,8 @@ class Reference:
         scale = 1 / math.sqrt(D) if scale is None else scale
         u = half_step(q.dtype)
         ur = half_step(result or q.dtype)
+        tiny = torch.finfo(result or q.dtype).smallest_normal * ur
+        f16 = q.dtype == torch.float16
         see, there, key_there = visible(B, Q, K, causal, offset, q_lengths, kv_lengths)
         clear = lambda t, m: torch.where(m[:, :, None, None], t.detach().cpu().double(), torch.zeros((), dtype=torch.float64))   # noqa: E731
         qd, kd, vd = clear(q, there).transpose(1, 2), clear(k, key_there).transpose(1, 2).repeat_interleave(R, 1), clear(v, key_there).transpose(1, 2).repeat_interleave(R, 1)
@@ -47,7 +51,8 @@ class Reference:
         rel = 2 * (worst * (D + 4) * 2.0 ** -23 + 2.0 ** -20 + K * 2.0 ** -24)
         o = p @ vd
         oabs = p @ vd.abs()
-        e = oabs * (u + rel + K * 2.0 ** -23)
+        vmax = vd.abs().amax(-2, keepdim=True) if K else torch.zeros(B, H, 1, D, dtype=torch.float64)
+        e = oabs * (u + rel + K * 2.0 ** -23) + (K * 2.0 ** -24 * vmax if f16 else 0.0)
         self.lse, self.lse_tol = lse, rel[..., 0] + torch.where(some, lse.abs(), 0.0) * 2.0 ** -22
         if join is not None:
             o0, l0 = clear(join[0], there).transpose(1, 2), torch.where(there[:, None], join[1].cpu().double(), -math.inf)
@@ -58,7 +63,7 @@ class Reference:
             o = o * w(lse) + o0 * w(l0)
             self.lse, self.lse_tol = both, moved[..., 0] + torch.where(both > -math.inf, both.abs(), 0.0) * 2.0 ** -22
         self.out = o.transpose(1, 2)
-        self.out_tol = (e + o.abs() * ur + torch.finfo(q.dtype).smallest_normal).transpose(1, 2)
+        self.out_tol = (e + o.abs() * ur + tiny).transpose(1, 2)
         if dout is None:
             return
         do = clear(dout, there).transpose(1, 2)
@@ -68,8 +73,12 @@ class Reference:
         ds = p * (dp - delta)
         # of ds: its rounding, the probability's relative error, and the errors of dp and delta
         eds = ds.abs() * u + p * (rel * (dp.abs() + delta.abs()) + D * 2.0 ** -23 * (do.abs() @ vd.abs().mT + (do.abs() * od.abs()).sum(-1, keepdim=True)))
-        over = lambda t: t.view(B, G, R, K, D).sum(2).transpose(1, 2)   # the heads that share keys and values   # noqa: E731
-        tiny = torch.finfo(q.dtype).smallest_normal
+        least = 0.0
+        if f16:
+            norm = lambda t: t.norm(dim=-1).amax(-1).view(B, G, R).amax(-1).repeat_interleave(R, 1)[..., None, None]   # noqa: E731
+            least = 2.0 ** -25
+            eds = eds + see[:, None] * 2.0 ** -38 * 2 * norm(do) * norm(vd) if K and Q else eds
+        over = lambda t: t.reshape(B, G, R, K, D).sum(2).transpose(1, 2)   # the heads that share keys and values   # noqa: E731
         base = [torch.zeros((), dtype=torch.float64)] * 3 if add is None else [clear(a, m) for a, m in zip(add, (there, key_there, key_there))]
 
         def bound(t, a, e):   # the result's rounding (and of what it is added to)
@@ -77,7 +86,7 @@ class Reference:
         self.dq, self.dq_tol = bound((scale * ds @ kd).transpose(1, 2), base[0], (scale * (eds + K * 2.0 ** -23 * ds.abs()) @ kd.abs()).transpose(1, 2))
         n = Q * R
         self.dk, self.dk_tol = bound(over(scale * ds.mT @ qd), base[1], over(scale * (eds + n * 2.0 ** -23 * ds.abs()).mT @ qd.abs()))
-        self.dv, self.dv_tol = bound(over(p.mT @ do), base[2], over(((u + rel + n * 2.0 ** -23) * p).mT @ do.abs()))
+        self.dv, self.dv_tol = bound(over(p.mT @ do), base[2], over(((u + rel + n * 2.0 ** -23) * p + least * 2.0 ** -15 * see[:, None]).mT @ do.abs()))
 
 
 def check(name, got, want, tol):
