@@ -2,6 +2,8 @@
 //   dv_j = sum_i p_ij do_i      ds_ij = p_ij (do_i.v_j - <do_i, o_i>)      dq_i = scale sum_j ds_ij k_j      dk_j = scale sum_i ds_ij q_i
 // over the pairs that see each other; the sums for dk and dv run over the heads that share them as well.
 //
+// Where tiles are few, several CTAs share one's partners, and a third kernel adds up what they have, part by part.
+//
 // Two kernels, each with the sums of its tile in tensor memory from the first product to the last: one owns a tile of keys and walks the queries (dk, dv), one
 // owns a tile of queries and walks the keys (dq). Together they make seven products of a tile where five would do, if the tiles of dq were added up
 // in memory by whoever has a part of them: then the order of the additions, and the result, would change from run to run, or CTAs would have to wait for one another.
@@ -86,9 +88,9 @@ __device__ __forceinline__ BackwardBars backwardSetUp(uint8_t* smem, int warp) {
   return s;
 }
 
-// Rows of sums [128][DP] in tensor memory, times `factor` (and plus what is there already), become a gradient's rows; `to` names the row of this thread, null for none.
+// Rows of sums [128][DP] in tensor memory, times `factor` (and plus what is there already), become a gradient's rows.
 template <typename T, int DP>
-__device__ __forceinline__ void storeGradient(const AttnArgs& a, uint32_t tmem, bool some, float factor, bool exists, bool valid, size_t row, void* grad, const float* add) {
+__device__ __forceinline__ void storeGradient(const AttnArgs& a, uint32_t tmem, bool some, float factor, bool exists, bool valid, size_t row, void* grad, bool fp32, const float* add) {
 #pragma unroll
   for (int k = 0; k < DP / 32; ++k) {
     uint32_t o[32];
@@ -108,7 +110,7 @@ __device__ __forceinline__ void storeGradient(const AttnArgs& a, uint32_t tmem, 
         f[e] += v.x; f[e + 1] += v.y; f[e + 2] += v.z; f[e + 3] += v.w;
       }
     }
-    if (a.gradFp32) {
+    if (fp32) {
       float* to = (float*)grad + row * a.dim;
 #pragma unroll
       for (int e = 0; e < 32; e += 4)
@@ -154,14 +156,15 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   pdlEnter();
 
   const unsigned owners = a.batch * a.kvHeads, owner = blockIdx.x % owners;
-  const int kvHead = owner % a.kvHeads, b = owner / a.kvHeads, key0 = blockIdx.x / owners * 128;   // (the first keys are seen most)
+  const unsigned share = blockIdx.x / owners;
+  const int kvHead = owner % a.kvHeads, b = owner / a.kvHeads, key0 = share / a.kvParts * 128, part = share % a.kvParts;   // (the first keys are seen most)
   const Sequence seq = sequenceOf(a, b);
-  // tiles of queries: from the first that sees a key of this tile to the last
+  // tiles of queries: from the first that sees a key of this tile to the last, or this part of them
   const int all = (seq.q + a.tileTokens - 1) / a.tileTokens;
   const long long firstTok = a.causal ? max(0ll, (long long)key0 - seq.offset) : 0;
-  const int begin = (int)min((long long)all, firstTok / a.tileTokens);
-  const int n = key0 < seq.kv ? all - begin : 0;
-  const int fixRows = seq.q < a.q ? seq.q % a.tileTokens * a.group : 0;   // of the last tile, behind which rows may hold anything
+  const int first = (int)min((long long)all, firstTok / a.tileTokens), partners = key0 < seq.kv ? all - first : 0, each = (partners + a.kvParts - 1) / a.kvParts;
+  const int begin = first + min(partners, part * each), n = min(partners, (part + 1) * each) - min(partners, part * each);
+  const int fixRows = seq.q < a.q && begin + n == all ? seq.q % a.tileTokens * a.group : 0;   // of the last tile, behind which rows may hold anything
   const uint32_t smem0 = smemAddr(smem);
   auto fail = [&](uint32_t what) {
     *abortFlag = 1;
@@ -364,9 +367,11 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       tcFenceAfter();
     }
     if (!__any_sync(~0u, *abortFlag)) {
-      const size_t at = ((size_t)b * a.kv + key) * a.kvHeads + kvHead;
-      if (half == 0) storeGradient<T, DP>(a, tmem + lanes + 256, n > 0, exp2f(-Pack<T>::kBackwardBias), key < a.kv, valid, at, a.dv, a.addDv);
-      else storeGradient<T, DP>(a, tmem + lanes + 384, n > 0, a.scale / up, key < a.kv, valid, at, a.dk, a.addDk);
+      const bool whole = a.kvParts == 1;
+      const size_t at = ((size_t)b * a.kv + key) * a.kvHeads + kvHead, atPart = whole ? at : (size_t)part * a.batch * a.kv * a.kvHeads + at;
+      const float factor = half ? a.scale / up : exp2f(-Pack<T>::kBackwardBias);   // of dk, of dv
+      storeGradient<T, DP>(a, tmem + lanes + 256 + half * 128, n > 0, factor, key < a.kv, valid, atPart, whole ? (half ? a.dk : a.dv) : (half ? a.partDk : a.partDv), !whole || a.gradFp32,
+                           whole ? (half ? a.addDk : a.addDv) : nullptr);
     }
   }
 
@@ -402,11 +407,13 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 
   const int rows = a.tileTokens * a.group;
   const unsigned owners = a.batch * a.kvHeads, owner = blockIdx.x % owners;
-  const int kvHead = owner % a.kvHeads, b = owner / a.kvHeads, qTile = a.tiles - 1 - (int)(blockIdx.x / owners), tok0 = qTile * a.tileTokens;
+  const int share = blockIdx.x / owners, part = share % a.qParts;
+  const int kvHead = owner % a.kvHeads, b = owner / a.kvHeads, qTile = a.tiles - 1 - share / a.qParts, tok0 = qTile * a.tileTokens;
   const Sequence seq = sequenceOf(a, b);
   const int last = min(tok0 + a.tileTokens, seq.q) - 1;
-  const int n = last < tok0 ? 0 : (visibleOf(a, seq, last) + 127) / 128;
-  const int fixRows = seq.kv < a.kv ? seq.kv % 128 : 0, fixTile = fixRows ? seq.kv / 128 : -1;   // keys and values behind the last may be anything
+  const int partners = last < tok0 ? 0 : (visibleOf(a, seq, last) + 127) / 128, each = (partners + a.qParts - 1) / a.qParts;
+  const int begin = min(partners, part * each), n = min(partners, begin + each) - begin;   // tiles of keys: all that the last query sees, or this part of them
+  const int fixRows = seq.kv < a.kv ? seq.kv % 128 : 0, fixTile = fixRows ? seq.kv / 128 - begin : -1;   // keys and values behind the last may be anything
   const uint32_t smem0 = smemAddr(smem);
   auto fail = [&](uint32_t what) {
     *abortFlag = 1;
@@ -430,7 +437,7 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       if (lane == 0) {
         const uint32_t bar = smemAddr(&s.full[at]);
         mbarExpectTx(bar, kTileBytes);
-        loadTile<DP>(smem0 + Shape::kRing + at * kTileBytes, map, tile * 128, kvHead, b, bar);
+        loadTile<DP>(smem0 + Shape::kRing + at * kTileBytes, map, (begin + tile) * 128, kvHead, b, bar);
       }
       ++loaded[values];
     };
@@ -474,7 +481,7 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       };
       auto full = [&](int values, int tile) { return need(waitOr(smemAddr(&s.full[stageOf(values, tile)]), phaseOf(values, tile), abortFlag), 2000 + stageOf(values, tile)); };
       auto tileAt = [&](int values, int tile) { return smem0 + Shape::kRing + stageOf(values, tile) * kTileBytes; };
-      const bool fixed = fixTile == n - 1;
+      const bool fixed = fixTile >= 0 && fixTile == n - 1;
       auto scores = [&](int i) {
         if (!full(0, i)) return;
         if (fixed && i == n - 1 && !need(waitOr(smemAddr(&s.fix[0]), 0, abortFlag), 2200)) return;
@@ -541,7 +548,7 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       tcFenceBefore();
       __syncwarp();
       if (lane == 0) mbarArrive(smemAddr(s.firstDone));
-      const int k0 = i * 128 + half * 64;
+      const int k0 = (begin + i) * 128 + half * 64;
       const bool hide = __any_sync(~0u, limit < k0 + 64);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
@@ -584,7 +591,9 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     }
     if (!__any_sync(~0u, *abortFlag) && half == 0) {
       const size_t at = ((size_t)b * a.q + tok) * a.heads + head;
-      storeGradient<T, DP>(a, tmem + lanes + 384, n > 0, a.scale / up, exists, valid, at, a.dq, a.addDq);
+      const bool whole = a.qParts == 1;
+      storeGradient<T, DP>(a, tmem + lanes + 384, n > 0, a.scale / up, exists, valid, whole ? at : (size_t)part * a.batch * a.q * a.heads + at, whole ? a.dq : a.partDq, !whole || a.gradFp32,
+                           whole ? a.addDq : nullptr);
     }
   }
 
@@ -594,6 +603,39 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     tcFenceAfter();
     tmemDealloc(tmem, kTmemCols);
   }
+}
+
+// ---------------------------------------------------------------------------------------------- parts
+// dq, dk and dv from the parts' sums, added up in order, and what is there already. A thread has four channels of a row; rows behind a sequence's last are zeros in every part.
+template <typename T>
+__global__ void __launch_bounds__(256) attnSumKernel(const __grid_constant__ AttnArgs a) {
+  const int quads = a.dim / 4;
+  const size_t qRows = a.qParts > 1 ? (size_t)a.batch * a.q * a.heads : 0, kvRows = a.kvParts > 1 ? (size_t)a.batch * a.kv * a.kvHeads : 0;
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  size_t row = i / quads;
+  if (row >= qRows + 2 * kvRows) return;
+  const int which = row < qRows ? 0 : row < qRows + kvRows ? 1 : 2;   // dq, dk, dv
+  if (which) row -= qRows + (which == 2 ? kvRows : 0);
+  const int heads = which ? a.kvHeads : a.heads, tokens = which ? a.kv : a.q, parts = which ? a.kvParts : a.qParts;
+  const int tok = (int)(row / heads % tokens), b = (int)(row / heads / tokens);
+  const size_t at = row * quads + i % quads, stride = (which ? kvRows : qRows) * quads;
+  const float4* from = (const float4*)(which == 0 ? a.partDq : which == 1 ? a.partDk : a.partDv) + at;
+  const float4* add = (const float4*)(which == 0 ? a.addDq : which == 1 ? a.addDk : a.addDv);
+  pdlEnter();
+  const int* lengths = which ? a.kvLengths : a.qLengths;
+  float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) {
+    const float4 v = from[p * stride];
+    f.x += v.x; f.y += v.y; f.z += v.z; f.w += v.w;
+  }
+  if (add && (!lengths || tok < lengths[b])) {
+    const float4 v = add[at];
+    f.x += v.x; f.y += v.y; f.z += v.z; f.w += v.w;
+  }
+  void* to = which == 0 ? a.dq : which == 1 ? a.dk : a.dv;
+  if (a.gradFp32) ((float4*)to)[at] = f;
+  else ((uint2*)to)[at] = make_uint2(Pack<T>::two(f.x, f.y), Pack<T>::two(f.z, f.w));
 }
 
 // ---------------------------------------------------------------------------------------------- what both need of each row of queries
@@ -694,6 +736,7 @@ template <typename T> static const void* kvFn(int dim) { return dim <= 64 ? (con
 template <typename T> static const void* qFn(int dim) { return dim <= 64 ? (const void*)attnBackwardQKernel<T, 64> : (const void*)attnBackwardQKernel<T, 128>; }
 const void* attnBackwardKvKernelFn(int type, int dim) { return type == ATTN_F16 ? kvFn<__half>(dim) : kvFn<__nv_bfloat16>(dim); }
 const void* attnBackwardQKernelFn(int type, int dim) { return type == ATTN_F16 ? qFn<__half>(dim) : qFn<__nv_bfloat16>(dim); }
+const void* attnSumKernelFn(int type) { return type == ATTN_F16 ? (const void*)attnSumKernel<__half> : (const void*)attnSumKernel<__nv_bfloat16>; }
 int attnBackwardThreads() { return BackwardWarps::kThreads; }
 int attnBackwardRegs() { return BackwardWarps::kLaunchRegs; }
 size_t attnBackwardSmemBytes(int dim) { return dim <= 64 ? BackwardShape<64>::kBytes : BackwardShape<128>::kBytes; }

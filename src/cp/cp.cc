@@ -154,7 +154,7 @@ static ncclResult_t checkShape(const char* what, const ncclCpAttention_t* c) {
   if (c->mask != NCCL_CP_FULL && c->mask != NCCL_CP_CAUSAL && c->mask != NCCL_CP_CAUSAL_END) { WARN("%s: unknown mask %d", what, (int)c->mask); return ncclInvalidArgument; }
   if (!(c->scale > 0.0f) || !std::isfinite(c->scale)) { WARN("%s: scale must be positive and finite", what); return ncclInvalidArgument; }
   // CTAs are counted with 31 bits, rows of a result with 40
-  const double tiles = (double)c->batch * c->kv_heads * ((double)c->q_tokens * (c->heads / c->kv_heads) + c->kv_tokens) / 64 + 1;
+  const double tiles = (double)c->batch * c->kv_heads * (((double)c->q_tokens * (c->heads / c->kv_heads) + c->kv_tokens) / 64 + 2);
   if (tiles * kAttnMaxSplits > 2147483647.0) { WARN("%s: too many tiles", what); return ncclInvalidArgument; }
   return ncclSuccess;
 }
@@ -202,7 +202,8 @@ struct ForwardPlan {
   int splits;
 };
 static double estimate(double ctas, int sms, double mean, double longest, double constant) {
-  const double waves = std::ceil(ctas / sms);
+  // (CTAs of different lengths, the longest first, leave less than half of a last wave empty)
+  const double waves = mean < 0.9 * longest ? std::min(std::ceil(ctas / sms), ctas / sms + 0.5) : std::ceil(ctas / sms);
   return std::max(waves * mean, longest) + waves * constant;
 }
 static ForwardPlan forwardPlan(const ncclCpContext* cp, const ncclCpAttention_t* c) {
@@ -227,8 +228,47 @@ static size_t forwardWork(const ncclCpAttention_t* c, const ForwardPlan& p) {
   return p.splits == 1 ? 0 : (size_t)p.splits * c->batch * c->q_tokens * c->heads * (c->head_dim + 1) * 4;
 }
 
+// Into how many parts a backward call cuts the partners of its tiles: where CTAs are few, or leave much of a last wave empty. In units of what a CTA takes for a tile and
+// partner (1.1 to 1.4 us): waves of CTAs as in the forward pass's estimate, and for parts a launch and the traffic of their sums, once there and once back. Measured with inputs
+// from memory, 128 channels, us, without parts and by this rule: 2048 causal tokens of 32 heads over one 773, 146; of 32 over 8 176, 155; 4096 causal tokens of 8 heads over 2 242,
+// 129; 33 queries on 4000 keys of 28 heads over 4 73, 46; where it makes none, as for 4096 x 4096 of 32 heads over 8, the same.
+struct BackwardPlan {
+  int kvParts, qParts;
+};
+static int partsOf(int sms, double tiles, double mean, double longest, double bytesOfSums) {
+  int best = 1;
+  double least = estimate(tiles, sms, mean, longest, 4.0);
+  for (int parts : {2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+    if (parts * 2 > longest) break;
+    const double t = estimate(tiles * parts, sms, mean / parts, longest / parts, 4.0) + 2.5 + 2 * parts * bytesOfSums / 12e6;
+    if (t < 0.95 * least) {
+      least = t;
+      best = parts;
+    }
+  }
+  return best;
+}
+static BackwardPlan backwardPlan(const ncclCpContext* cp, const ncclCpAttention_t* c, const AttnArgs& a) {
+  const double owners = (double)c->batch * c->kv_heads, keyTiles = std::ceil(c->kv_tokens / 128.0);
+  const long long offset = c->mask == NCCL_CP_CAUSAL_END ? (long long)c->kv_tokens - c->q_tokens : a.offset;
+  // partners of the tile that has the most and of the one that has the fewest, all rows being there
+  const auto keys = [&](long long tok) { return std::ceil((c->mask == NCCL_CP_FULL ? c->kv_tokens : std::max(0ll, std::min<long long>(c->kv_tokens, tok + offset))) / 128.0); };
+  const auto queries = [&](long long key) { return std::ceil((c->mask == NCCL_CP_FULL ? c->q_tokens : std::max(0ll, std::min<long long>(c->q_tokens, c->q_tokens - key + offset))) / (double)a.tileTokens); };
+  BackwardPlan p;
+  const double qLongest = keys(c->q_tokens), qMean = (qLongest + keys(a.tileTokens)) / 2, kvLongest = queries(0), kvMean = (kvLongest + queries(c->kv_tokens - 128)) / 2;
+  p.qParts = partsOf(cp->smCount, owners * a.tiles, qMean, qLongest, (double)c->batch * c->q_tokens * c->heads * c->head_dim * 4);
+  p.kvParts = partsOf(cp->smCount, owners * keyTiles, kvMean, kvLongest, (double)c->batch * c->kv_tokens * c->kv_heads * c->head_dim * 8);
+  return p;
+}
+
 static size_t statsBytes(const AttnArgs& a) { return (size_t)a.batch * a.kvHeads * a.tiles * 256 * 4; }
-static size_t boundsBytes(const ncclCpAttention_t* c) { return isFp16(c) ? (size_t)c->batch * c->kv_heads * 8 : 0; }
+static size_t boundsBytes(const ncclCpAttention_t* c) { return isFp16(c) ? ((size_t)c->batch * c->kv_heads * 8 + 255) / 256 * 256 : 0; }
+static size_t dqBytes(const ncclCpAttention_t* c) { return (size_t)c->batch * c->q_tokens * c->heads * c->head_dim * 4; }
+static size_t dkBytes(const ncclCpAttention_t* c) { return (size_t)c->batch * c->kv_tokens * c->kv_heads * c->head_dim * 4; }
+// Numbers of each row, norms, and the sums of parts.
+static size_t backwardWork(const ncclCpAttention_t* c, const AttnArgs& a, const BackwardPlan& p) {
+  return statsBytes(a) + boundsBytes(c) + (p.qParts > 1 ? p.qParts * dqBytes(c) : 0) + (p.kvParts > 1 ? 2 * p.kvParts * dkBytes(c) : 0);
+}
 
 static ncclResult_t needsGpu(const ncclCpContext* cp, const char* what) {
   if (cp->comm->compCap < 100) { WARN("%s needs compute capability 10.0 (found %d)", what, cp->comm->compCap); return ncclInvalidUsage; }
@@ -348,7 +388,7 @@ size_t ncclCpAttentionBackwardWork(ncclCp_t cp, const ncclCpAttention_t* c) {
   if (!cp || checkShape("ncclCpAttentionBackwardWork", c) != ncclSuccess) return 0;
   AttnArgs a;
   fillAttention(c, nullptr, nullptr, &a);
-  return statsBytes(a) + boundsBytes(c);
+  return backwardWork(c, a, backwardPlan(cp, c, a));
 }
 
 ncclResult_t ncclCpAttentionBackward(ncclCp_t cp, const ncclCpAttention_t* c, const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
@@ -364,7 +404,8 @@ ncclResult_t ncclCpAttentionBackward(ncclCp_t cp, const ncclCpAttention_t* c, co
   const size_t size = c->result_type == ncclFloat32 ? 4 : 2, D = c->head_dim;
   AttnArgs a;
   fillAttention(c, qLengths, kvLengths, &a);
-  const size_t workBytes = statsBytes(a) + boundsBytes(c);
+  const BackwardPlan plan = backwardPlan(cp, c, a);
+  const size_t workBytes = backwardWork(c, a, plan);
   if (c->q_tokens) {
     NCCLCHECK(checkOperand(what, "q", q, c->batch, c->q_tokens, c->heads, c->q_stride));
     NCCLCHECK(checkOperand(what, "d_out", dout, c->batch, c->q_tokens, c->heads, c->dout_stride));
@@ -400,6 +441,11 @@ ncclResult_t ncclCpAttentionBackward(ncclCp_t cp, const ncclCpAttention_t* c, co
   a.addDv = addDv;
   a.stats = (const float*)work;
   a.bounds = isFp16(c) ? (const uint32_t*)((const char*)work + statsBytes(a)) : nullptr;
+  a.kvParts = plan.kvParts;
+  a.qParts = plan.qParts;
+  a.partDq = (float*)((char*)work + statsBytes(a) + boundsBytes(c));
+  a.partDk = (float*)((char*)a.partDq + (plan.qParts > 1 ? plan.qParts * dqBytes(c) : 0));
+  a.partDv = (float*)((char*)a.partDk + plan.kvParts * dkBytes(c));
   a.status = cp->comm->devStatusDev;
   B200_ON_DEVICE(cp);
   if (some) {
@@ -424,9 +470,12 @@ ncclResult_t ncclCpAttentionBackward(ncclCp_t cp, const ncclCpAttention_t* c, co
   NCCLCHECK(makeMap(&maps[3], c, v, c->kv_tokens, c->kv_heads, c->v_stride, kAttnRows, 1));
   void* args[5] = {&maps[0], &maps[1], &maps[2], &maps[3], &a};
   const unsigned owners = (unsigned)c->batch * c->kv_heads, keyTiles = (c->kv_tokens + kAttnRows - 1) / kAttnRows;
-  if (c->kv_tokens) NCCLCHECK(launchCp(cp, attnBackwardKvKernelFn(type, c->head_dim), owners * keyTiles, 1, attnBackwardThreads(), attnBackwardSmemBytes(c->head_dim), args, stream, attnBackwardRegs()));
-  if (c->q_tokens) NCCLCHECK(launchCp(cp, attnBackwardQKernelFn(type, c->head_dim), owners * a.tiles, 1, attnBackwardThreads(), attnBackwardSmemBytes(c->head_dim), args, stream, attnBackwardRegs()));
-  return ncclSuccess;
+  if (c->kv_tokens) NCCLCHECK(launchCp(cp, attnBackwardKvKernelFn(type, c->head_dim), owners * keyTiles * plan.kvParts, 1, attnBackwardThreads(), attnBackwardSmemBytes(c->head_dim), args, stream, attnBackwardRegs()));
+  if (c->q_tokens) NCCLCHECK(launchCp(cp, attnBackwardQKernelFn(type, c->head_dim), owners * a.tiles * plan.qParts, 1, attnBackwardThreads(), attnBackwardSmemBytes(c->head_dim), args, stream, attnBackwardRegs()));
+  const size_t sumRows = (plan.qParts > 1 ? rows : 0) + (plan.kvParts > 1 ? 2 * cols : 0);
+  if (!sumRows) return ncclSuccess;
+  void* sum[1] = {&a};
+  return launchCp(cp, attnSumKernelFn(type), (unsigned)((sumRows * (D / 4) + 255) / 256), 1, 256, 0, sum, stream);
 }
 
 ncclResult_t ncclCpAttentionDelta(ncclCp_t cp, const ncclCpAttention_t* c, const void* dout, const void* out, const int* qLengths, float* delta, cudaStream_t stream) {

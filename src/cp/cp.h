@@ -37,6 +37,9 @@ struct AttnArgs {
   void *dq, *dk, *dv;         // contiguous, of the inputs' type or fp32
   int gradFp32;
   const float *addDq, *addDk, *addDv;
+  int kvParts, qParts;        // CTAs that share the queries of a tile of keys, the keys of a tile of queries: above 1 their fp32 sums go to
+  float *partDk, *partDv;     // [kvParts][rows of dk][dim]
+  float* partDq;              // [qParts][rows of dq][dim]
   uint32_t* status;           // {code, kind, what, CTA} of the communicator, written when a wait runs out
 };
 
@@ -84,6 +87,7 @@ int attnForwardThreads();
 int attnBackwardThreads();
 int attnForwardRegs();     // that a thread is launched with
 int attnBackwardRegs();
+const void* attnSumKernelFn(int type);
 const void* attnStatsKernelFn(int type, int dim);
 const void* rotaryKernelFn(int type);
 
