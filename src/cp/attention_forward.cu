@@ -39,6 +39,17 @@ template <int DP, bool PAIRS> struct ForwardShape {
 template <bool PAIRS> __device__ __forceinline__ int placeOfK(int i) { return PAIRS ? 2 * i : i < 2 ? i : 2 * i - 1; }
 template <bool PAIRS> __device__ __forceinline__ int placeOfV(int i, int n) { return PAIRS ? 2 * i + 1 : min(i + 2, n) + i; }
 
+// The largest of 64 scores.
+__device__ __forceinline__ float maxOf(const uint32_t (&x)[32], const uint32_t (&y)[32]) {
+  float a = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])), b = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+#pragma unroll
+  for (int k = 2; k < 32; k += 2) {
+    a = max3(a, __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+    b = max3(b, __uint_as_float(y[k]), __uint_as_float(y[k + 1]));
+  }
+  return fmaxf(a, b);
+}
+
 template <typename T, int DP, bool PAIRS>
 __global__ void __launch_bounds__(ForwardWarps::kThreads, 1)
 attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnArgs a) {
@@ -240,24 +251,25 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       tcFenceAfter();
       if (working) {
         uint32_t s[4][32];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) tmemLd32(tS + k * 32, s[k]);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) tmemLdWait32(s[k]);
         const int k0 = (begin + (PAIRS ? i : 2 * i + t)) * 128;
-        if (__any_sync(~0u, limit < k0 + 128)) {
+        tmemLd32(tS, s[0]);
+        tmemLd32(tS + 32, s[1]);
+        tmemLdWait32(s[0]);
+        tmemLdWait32(s[1]);
+        tmemLd32(tS + 64, s[2]);
+        tmemLd32(tS + 96, s[3]);
+        // the first half's maximum while the second half is on its way, unless some of it is hidden
+        const bool hide = __any_sync(~0u, limit < k0 + 128);
+        float mx = hide ? 0.0f : maxOf(s[0], s[1]);
+        tmemLdWait32(s[2]);
+        tmemLdWait32(s[3]);
+        if (hide) {
 #pragma unroll
           for (int k = 0; k < 128; ++k)
             if (k0 + k >= limit) s[k / 32][k % 32] = __float_as_uint(-INFINITY);
+          mx = maxOf(s[0], s[1]);
         }
-        float top[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) top[u] = fmaxf(__uint_as_float(s[u][0]), __uint_as_float(s[u][1]));
-#pragma unroll
-        for (int k = 2; k < 32; k += 2)
-#pragma unroll
-          for (int u = 0; u < 4; ++u) top[u] = max3(top[u], __uint_as_float(s[u][k]), __uint_as_float(s[u][k + 1]));
-        const float mx = max3(fmaxf(top[0], top[1]), top[2], top[3]);
+        mx = fmaxf(mx, maxOf(s[2], s[3]));
         const bool raise = (mx - m) * c > kLag;   // (nothing seen so far and nothing now: NaN, no)
         if (__any_sync(~0u, raise)) {
           const float to = raise ? mx : m, factor = raise ? exp2Fast((m - to) * c) : 1.0f;
@@ -278,26 +290,34 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         const float shift = Pack<T>::kForwardBias - (m == -INFINITY ? 0.0f : m * c);
         const uint64_t shift2 = pair(shift, shift);
-        uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           uint32_t p[32];
 #pragma unroll
           for (int k = 0; k < 32; ++k) {
-            uint64_t x = fma2(packF32x2(s[half * 2 + k / 16][k % 16 * 2], s[half * 2 + k / 16][k % 16 * 2 + 1]), c2, shift2);
-            x = pair(exp2Fast(lowOf(x)), exp2Fast(highOf(x)));
-            sum[k % 2] = add2(sum[k % 2], x);
-            p[k] = Pack<T>::two(lowOf(x), highOf(x));
+            uint32_t &lo = s[half * 2 + k / 16][k % 16 * 2], &hi = s[half * 2 + k / 16][k % 16 * 2 + 1];
+            const uint64_t x = fma2(packF32x2(lo, hi), c2, shift2);
+            lo = __float_as_uint(exp2Fast(lowOf(x)));
+            hi = __float_as_uint(exp2Fast(highOf(x)));
+            p[k] = Pack<T>::two(__uint_as_float(lo), __uint_as_float(hi));
           }
           tmemSt32(tS + half * 64, p);
         }
-        sum[0] = add2(sum[0], sum[1]);
-        l += lowOf(sum[0]) + highOf(sum[0]);
         tmemStWait();
+        tcFenceBefore();
+        __syncwarp();
+        if (lane == 0) mbarArrive(smemAddr(&probBar[t]));
+        // the sum is added up while the tensor cores work on the probabilities
+        uint64_t sum[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < 64; ++k) sum[k % 4] = add2(sum[k % 4], packF32x2(s[k / 16][k % 16 * 2], s[k / 16][k % 16 * 2 + 1]));
+        sum[0] = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+        l += lowOf(sum[0]) + highOf(sum[0]);
+      } else {
+        tcFenceBefore();
+        __syncwarp();
+        if (lane == 0) mbarArrive(smemAddr(&probBar[t]));
       }
-      tcFenceBefore();
-      __syncwarp();
-      if (lane == 0) mbarArrive(smemAddr(&probBar[t]));
     }
     if (ok && count[t]) {
       ok = warpWaitOr(smemAddr(&outBar[t]), 0, abortFlag);
