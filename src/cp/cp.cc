@@ -191,10 +191,10 @@ static void fillAttention(const ncclCpAttention_t* c, const int* qLengths, const
 // How a forward call is cut up: CTAs with two tiles of queries each ("pairs"), or with one whose keys their two halves share; and there, with few CTAs, into how many parts
 // the keys of a tile.
 //
-// Pairs move half as many keys, CTAs with one tile fill the SMs better. Both are estimated in units of what a CTA takes for a tile of keys (0.6 us a tile and pair, 128 channels):
-// whole waves of CTAs, each with the mean number of tiles, the longest CTA at least, and a constant for a CTA's beginning and end. Measured with inputs from memory, us, pairs and
-// single tiles (32 heads over 8 of 128 channels where nothing else is said): 2048 x 2048 80, 96; the same, causal 49, 68; 1024 x 4096 74, 80; 1500 x 8192 250, 201; 3000 x 3000
-// of 10 heads over 2, causal 56, 43; 3 x 777 x 1013 of 12 heads over 4, 80 channels 29, 37.
+// Pairs move half as many keys, CTAs with one tile fill the SMs better. Both are estimated in units of what a pair takes for a tile of keys (2 us, 128 channels): waves of CTAs, each
+// with the mean number of tiles (of which a CTA with one tile of queries makes two at a time, for 1.15 of the time), the longest CTA at least, and a constant for a CTA's beginning
+// and end. Measured with inputs from memory, us, pairs and single tiles (32 heads over 8 of 128 channels where nothing else is said): 2048 x 2048 78, 94; the same, causal 49, 66;
+// 4096 causal 139, 168; 1024 x 4096 70, 80; 1500 x 8192 242, 205; 3000 x 3000 of 10 heads over 2, causal 55, 41; 3 x 777 x 1013 of 12 heads over 4, 80 channels 27, 37.
 // Parts cost a second kernel and the partial results, 5 us, and pay where they save more tiles than that: one query on 4096 keys, one part 41 us, 8 28, 16 26; on 512 keys (4 heads
 // of 64 channels) one part 14 us, two 20.
 struct ForwardPlan {
@@ -216,7 +216,7 @@ static ForwardPlan forwardPlan(const ncclCpContext* cp, const ncclCpAttention_t*
   const auto tilesUpTo = [&](long long tok) { return (double)((c->mask == NCCL_CP_FULL ? c->kv_tokens : std::max(0ll, std::min<long long>(c->kv_tokens, tok + offset))) + 127) / 128; };
   const double longest = std::floor(tilesUpTo(c->q_tokens)), mean = (longest + std::floor(tilesUpTo(a.tileTokens))) / 2;
   ForwardPlan p;
-  p.pairs = a.tiles > 1 && estimate(pairCtas, sms, mean, longest, 1.0) <= estimate(ctas, sms, mean / 2, longest / 2, 1.5);
+  p.pairs = a.tiles > 1 && estimate(pairCtas, sms, mean, longest, 1.0) <= estimate(ctas, sms, 1.15 * mean / 2, 1.15 * longest / 2, 2.0);
   p.splits = 1;
   if (!p.pairs && ctas && ctas < sms) {
     const int most = (int)std::min<long long>({sms / ctas, (long long)longest / 2, kAttnMaxSplits});
