@@ -2,10 +2,10 @@
 //   dv_j = sum_i p_ij do_i      ds_ij = p_ij (do_i.v_j - <do_i, o_i>)      dq_i = scale sum_j ds_ij k_j      dk_j = scale sum_i ds_ij q_i
 // over the pairs that see each other; the sums for dk and dv run over the heads that share them as well.
 //
-// Where tiles are few, several CTAs share one's partners, and a third kernel adds up what they have, part by part.
+// Where tiles are few, several CTAs share one's partners, and another kernel adds up what they have, part by part.
 //
-// Two kernels, each with the sums of its tile in tensor memory from the first product to the last: one owns a tile of keys and walks the queries (dk, dv), one
-// owns a tile of queries and walks the keys (dq). Together they make seven products of a tile where five would do, if the tiles of dq were added up
+// Two kinds of CTAs in one launch, each with the sums of its tile in tensor memory from the first product to the last: one owns a tile of keys and walks the queries (dk, dv),
+// the other owns a tile of queries and walks the keys (dq). Together they make seven products of a tile where five would do, if the tiles of dq were added up
 // in memory by whoever has a part of them: then the order of the additions, and the result, would change from run to run, or CTAs would have to wait for one another.
 //
 // Roles as in the forward pass: warps 0-7 have a row of the tile each and, in two groups, a half of its columns; warp 8 feeds the ring, warp 9 issues products. Probabilities
@@ -130,33 +130,15 @@ __device__ __forceinline__ void storeGradient(const AttnArgs& a, uint32_t tmem, 
 // at once, and the next tile's are made meanwhile: its exponentials are computed while the tensor cores add this tile's to dv and dk and make the next do.v. With the
 // probabilities over the scores, the next scores waited for their product: a third of the tensor cores' time.
 template <typename T, int DP>
-__global__ void __launch_bounds__(BackwardWarps::kThreads, 1)
-attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDo, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                     const __grid_constant__ AttnArgs a) {
+__device__ __forceinline__ void backwardKv(const CUtensorMap& tmQ, const CUtensorMap& tmDo, const CUtensorMap& tmK, const CUtensorMap& tmV, const AttnArgs& a, uint8_t* smem,
+                                           const BackwardBars& s, uint32_t tmem, unsigned block) {
   using Shape = BackwardShape<DP>;
   // Queries stay until their product with ds, two steps behind their scores; do for one step less: a ring for each.
   constexpr int kStages = Shape::kStages, kQStages = (kStages + 1) / 2, kDoStages = kStages - kQStages;
   constexpr uint32_t kTileBytes = Shape::kTileBytes;
-  extern __shared__ __align__(1024) uint8_t smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const BackwardBars s = backwardSetUp<DP>(smem, warp);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = a.tileTokens * a.group;
   volatile uint32_t* abortFlag = s.abortFlag;
-  const int rows = a.tileTokens * a.group;
-  if (warp < BackwardWarps::kCompute && rows < 128) {
-    // rows of a tile that no copy writes are operands of sums over the rows: zero, for good
-    const int each = (128 - rows) * 8;
-    for (int i = threadIdx.x; i < kStages * (DP / 64) * each; i += BackwardWarps::kCompute * 32)
-      *(uint4*)(smem + Shape::kRing + i / each * kHalfTile + rows * 128 + i % each * 16) = make_uint4(0, 0, 0, 0);
-    fenceProxyAsync();
-  }
-  tcFenceBefore();
-  __syncthreads();
-  tcFenceAfter();
-  const uint32_t tmem = *s.tmemSlot;
-  pdlEnter();
-
-  const unsigned owners = a.batch * a.kvHeads, owner = blockIdx.x % owners;
-  const unsigned share = blockIdx.x / owners;
+  const unsigned owners = a.batch * a.kvHeads, owner = block % owners, share = block / owners;
   const int kvHead = owner % a.kvHeads, b = owner / a.kvHeads, key0 = share / a.kvParts * 128, part = share % a.kvParts;   // (the first keys are seen most)
   const Sequence seq = sequenceOf(a, b);
   // tiles of queries: from the first that sees a key of this tile to the last, or this part of them
@@ -374,40 +356,23 @@ attnBackwardKvKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                            whole ? (half ? a.addDk : a.addDv) : nullptr);
     }
   }
-
-  tcFenceBefore();
-  __syncthreads();
-  if (warp == BackwardWarps::kMma) {
-    tcFenceAfter();
-    tmemDealloc(tmem, kTmemCols);
-  }
 }
 
 // ---------------------------------------------------------------------------------------------- dq
 // Tensor memory: scores [queries x keys] at 0, do.v (then ds) of two tiles at 128 and 256, dq at 384. Scores are taken into registers at once, and the next tile's are made
 // while exponentials are computed; so is its do.v, in the other place. So products and elements of a tile do not wait for one another.
 template <typename T, int DP>
-__global__ void __launch_bounds__(BackwardWarps::kThreads, 1)
-attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDo, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                    const __grid_constant__ AttnArgs a) {
+__device__ __forceinline__ void backwardQ(const CUtensorMap& tmQ, const CUtensorMap& tmDo, const CUtensorMap& tmK, const CUtensorMap& tmV, const AttnArgs& a, uint8_t* smem,
+                                          const BackwardBars& s, uint32_t tmem, unsigned block) {
   using Shape = BackwardShape<DP>;
   // Keys stay until their product with ds, values only until do.v: a ring for each, so that values come in early (in one ring of five stages the next do.v waited half of the
   // time for values that could not be asked for before the last ds was used).
   constexpr int kStages = Shape::kStages, kKeyStages = (kStages + 1) / 2, kValueStages = kStages - kKeyStages;
   constexpr uint32_t kTileBytes = Shape::kTileBytes;
-  extern __shared__ __align__(1024) uint8_t smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const BackwardBars s = backwardSetUp<DP>(smem, warp);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = a.tileTokens * a.group;
   volatile uint32_t* abortFlag = s.abortFlag;
-  tcFenceBefore();
-  __syncthreads();
-  tcFenceAfter();
-  const uint32_t tmem = *s.tmemSlot;
-  pdlEnter();
-
-  const int rows = a.tileTokens * a.group;
-  const unsigned owners = a.batch * a.kvHeads, owner = blockIdx.x % owners;
-  const int share = blockIdx.x / owners, part = share % a.qParts;
+  const unsigned owners = a.batch * a.kvHeads, owner = block % owners;
+  const int share = block / owners, part = share % a.qParts;
   const int kvHead = owner % a.kvHeads, b = owner / a.kvHeads, qTile = a.tiles - 1 - share / a.qParts, tok0 = qTile * a.tileTokens;
   const Sequence seq = sequenceOf(a, b);
   const int last = min(tok0 + a.tileTokens, seq.q) - 1;
@@ -596,7 +561,32 @@ attnBackwardQKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                            whole ? a.addDq : nullptr);
     }
   }
+}
 
+// The first CTAs own tiles of keys, the others tiles of queries: neither needs the other's, and where both are few they run beside one another.
+template <typename T, int DP>
+__global__ void __launch_bounds__(BackwardWarps::kThreads, 1)
+attnBackwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDo, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                   const __grid_constant__ AttnArgs a) {
+  using Shape = BackwardShape<DP>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, rows = a.tileTokens * a.group;
+  const bool ofKeys = blockIdx.x < a.kvCtas;
+  const BackwardBars s = backwardSetUp<DP>(smem, warp);
+  if (ofKeys && warp < BackwardWarps::kCompute && rows < 128) {
+    // rows of a tile that no copy writes are operands of sums over the rows: zero, for good
+    const int each = (128 - rows) * 8;
+    for (int i = threadIdx.x; i < Shape::kStages * (DP / 64) * each; i += BackwardWarps::kCompute * 32)
+      *(uint4*)(smem + Shape::kRing + i / each * kHalfTile + rows * 128 + i % each * 16) = make_uint4(0, 0, 0, 0);
+    fenceProxyAsync();
+  }
+  tcFenceBefore();
+  __syncthreads();
+  tcFenceAfter();
+  const uint32_t tmem = *s.tmemSlot;
+  pdlEnter();   // the set-up above overlaps the end of the kernel before
+  if (ofKeys) backwardKv<T, DP>(tmQ, tmDo, tmK, tmV, a, smem, s, tmem, blockIdx.x);
+  else backwardQ<T, DP>(tmQ, tmDo, tmK, tmV, a, smem, s, tmem, blockIdx.x - a.kvCtas);
   tcFenceBefore();
   __syncthreads();
   if (warp == BackwardWarps::kMma) {
@@ -732,10 +722,8 @@ __global__ void __launch_bounds__(256, 4) attnStatsKernel(const __grid_constant_
 
 }  // namespace
 
-template <typename T> static const void* kvFn(int dim) { return dim <= 64 ? (const void*)attnBackwardKvKernel<T, 64> : (const void*)attnBackwardKvKernel<T, 128>; }
-template <typename T> static const void* qFn(int dim) { return dim <= 64 ? (const void*)attnBackwardQKernel<T, 64> : (const void*)attnBackwardQKernel<T, 128>; }
-const void* attnBackwardKvKernelFn(int type, int dim) { return type == ATTN_F16 ? kvFn<__half>(dim) : kvFn<__nv_bfloat16>(dim); }
-const void* attnBackwardQKernelFn(int type, int dim) { return type == ATTN_F16 ? qFn<__half>(dim) : qFn<__nv_bfloat16>(dim); }
+template <typename T> static const void* backwardFn(int dim) { return dim <= 64 ? (const void*)attnBackwardKernel<T, 64> : (const void*)attnBackwardKernel<T, 128>; }
+const void* attnBackwardKernelFn(int type, int dim) { return type == ATTN_F16 ? backwardFn<__half>(dim) : backwardFn<__nv_bfloat16>(dim); }
 const void* attnSumKernelFn(int type) { return type == ATTN_F16 ? (const void*)attnSumKernel<__half> : (const void*)attnSumKernel<__nv_bfloat16>; }
 int attnBackwardThreads() { return BackwardWarps::kThreads; }
 int attnBackwardRegs() { return BackwardWarps::kLaunchRegs; }

@@ -470,8 +470,9 @@ ncclResult_t ncclCpAttentionBackward(ncclCp_t cp, const ncclCpAttention_t* c, co
   NCCLCHECK(makeMap(&maps[3], c, v, c->kv_tokens, c->kv_heads, c->v_stride, kAttnRows, 1));
   void* args[5] = {&maps[0], &maps[1], &maps[2], &maps[3], &a};
   const unsigned owners = (unsigned)c->batch * c->kv_heads, keyTiles = (c->kv_tokens + kAttnRows - 1) / kAttnRows;
-  if (c->kv_tokens) NCCLCHECK(launchCp(cp, attnBackwardKvKernelFn(type, c->head_dim), owners * keyTiles * plan.kvParts, 1, attnBackwardThreads(), attnBackwardSmemBytes(c->head_dim), args, stream, attnBackwardRegs()));
-  if (c->q_tokens) NCCLCHECK(launchCp(cp, attnBackwardQKernelFn(type, c->head_dim), owners * a.tiles * plan.qParts, 1, attnBackwardThreads(), attnBackwardSmemBytes(c->head_dim), args, stream, attnBackwardRegs()));
+  a.kvCtas = owners * keyTiles * plan.kvParts;
+  NCCLCHECK(launchCp(cp, attnBackwardKernelFn(type, c->head_dim), a.kvCtas + owners * a.tiles * plan.qParts, 1, attnBackwardThreads(), attnBackwardSmemBytes(c->head_dim), args, stream,
+                     attnBackwardRegs()));
   const size_t sumRows = (plan.qParts > 1 ? rows : 0) + (plan.kvParts > 1 ? 2 * cols : 0);
   if (!sumRows) return ncclSuccess;
   void* sum[1] = {&a};

@@ -37,6 +37,7 @@ struct AttnArgs {
   void *dq, *dk, *dv;         // contiguous, of the inputs' type or fp32
   int gradFp32;
   const float *addDq, *addDk, *addDv;
+  unsigned kvCtas;            // the first CTAs, which own tiles of keys; the others own tiles of queries
   int kvParts, qParts;        // CTAs that share the queries of a tile of keys, the keys of a tile of queries: above 1 their fp32 sums go to
   float *partDk, *partDv;     // [kvParts][rows of dk][dim]
   float* partDq;              // [qParts][rows of dq][dim]
@@ -80,8 +81,7 @@ enum AttnType : int { ATTN_F16 = 0, ATTN_BF16 = 1, ATTN_F32 = 2 };
 const void* attnForwardKernelFn(int type, int dim, bool pairs);
 size_t attnForwardSmemBytes(int dim, bool pairs);
 const void* attnJoinKernelFn(int type);
-const void* attnBackwardKvKernelFn(int type, int dim);
-const void* attnBackwardQKernelFn(int type, int dim);
+const void* attnBackwardKernelFn(int type, int dim);
 size_t attnBackwardSmemBytes(int dim);
 int attnForwardThreads();
 int attnBackwardThreads();
