@@ -228,37 +228,40 @@ static size_t forwardWork(const ncclCpAttention_t* c, const ForwardPlan& p) {
   return p.splits == 1 ? 0 : (size_t)p.splits * c->batch * c->q_tokens * c->heads * (c->head_dim + 1) * 4;
 }
 
-// Into how many parts a backward call cuts the partners of its tiles: where CTAs are few, or leave much of a last wave empty. In units of what a CTA takes for a tile and
-// partner (1.1 to 1.4 us): waves of CTAs as in the forward pass's estimate, and for parts a launch and the traffic of their sums, once there and once back. Measured with inputs
-// from memory, 128 channels, us, without parts and by this rule: 2048 causal tokens of 32 heads over one 773, 146; of 32 over 8 176, 155; 4096 causal tokens of 8 heads over 2 242,
-// 129; 33 queries on 4000 keys of 28 heads over 4 73, 46; where it makes none, as for 4096 x 4096 of 32 heads over 8, the same.
+// Into how many parts a backward call cuts the partners of its tiles: where CTAs are few, and the longest of them would be waited for. In units of what a CTA that owns queries takes
+// for a tile of keys (1.1 us; one that owns keys takes 1.3 of that for a tile of queries): what all CTAs take on all SMs and half of a last one beside others, the longest one at least, a
+// constant for a CTA's beginning and end, and for parts a launch and the traffic of their sums, once there and once back. Measured with inputs from memory, us, without parts and by
+// this rule: 2048 causal tokens of 32 heads over one 735, 135; 4096 of 8 over 2 205, 131; 128 queries on 16384 keys of 8 heads 211, 104; 33 on 4000, 28 heads over 4, causal 63, 43;
+// 512 causal tokens of 8 heads over one, 64 channels 55, 23; where it makes none parts would cost: 509 x 641, 3 times 12 heads over 4, 96 channels 53, in two parts 62 and more.
 struct BackwardPlan {
   int kvParts, qParts;
 };
-static int partsOf(int sms, double tiles, double mean, double longest, double bytesOfSums) {
-  int best = 1;
-  double least = estimate(tiles, sms, mean, longest, 4.0);
-  for (int parts : {2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-    if (parts * 2 > longest) break;
-    const double t = estimate(tiles * parts, sms, mean / parts, longest / parts, 4.0) + 2.5 + 2 * parts * bytesOfSums / 12e6;
-    if (t < 0.95 * least) {
-      least = t;
-      best = parts;
-    }
-  }
-  return best;
-}
 static BackwardPlan backwardPlan(const ncclCpContext* cp, const ncclCpAttention_t* c, const AttnArgs& a) {
-  const double owners = (double)c->batch * c->kv_heads, keyTiles = std::ceil(c->kv_tokens / 128.0);
+  const double owners = (double)c->batch * c->kv_heads, keyTiles = std::ceil(c->kv_tokens / 128.0), sms = cp->smCount;
   const long long offset = c->mask == NCCL_CP_CAUSAL_END ? (long long)c->kv_tokens - c->q_tokens : a.offset;
   // partners of the tile that has the most and of the one that has the fewest, all rows being there
   const auto keys = [&](long long tok) { return std::ceil((c->mask == NCCL_CP_FULL ? c->kv_tokens : std::max(0ll, std::min<long long>(c->kv_tokens, tok + offset))) / 128.0); };
   const auto queries = [&](long long key) { return std::ceil((c->mask == NCCL_CP_FULL ? c->q_tokens : std::max(0ll, std::min<long long>(c->q_tokens, c->q_tokens - key + offset))) / (double)a.tileTokens); };
-  BackwardPlan p;
-  const double qLongest = keys(c->q_tokens), qMean = (qLongest + keys(a.tileTokens)) / 2, kvLongest = queries(0), kvMean = (kvLongest + queries(c->kv_tokens - 128)) / 2;
-  p.qParts = partsOf(cp->smCount, owners * a.tiles, qMean, qLongest, (double)c->batch * c->q_tokens * c->heads * c->head_dim * 4);
-  p.kvParts = partsOf(cp->smCount, owners * keyTiles, kvMean, kvLongest, (double)c->batch * c->kv_tokens * c->kv_heads * c->head_dim * 8);
-  return p;
+  const double qLongest = keys(c->q_tokens), qMean = (qLongest + keys(a.tileTokens)) / 2, kvLongest = 1.3 * queries(0), kvMean = (kvLongest + 1.3 * queries(c->kv_tokens - 128)) / 2;
+  const double dq = (double)c->batch * c->q_tokens * c->heads * c->head_dim * 4, dkv = (double)c->batch * c->kv_tokens * c->kv_heads * c->head_dim * 8, constant = 4.0;
+  BackwardPlan best = {1, 1};
+  if (owners * (keyTiles + a.tiles) > 4 * sms && std::max(kvLongest, qLongest) < (owners * (keyTiles * kvMean + a.tiles * qMean)) / sms) return best;   // enough to do for all
+  double least = 0.0;
+  for (int kvParts : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+    if (kvParts > 1 && kvParts * 2.6 > kvLongest) break;
+    for (int qParts : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+      if (qParts > 1 && qParts * 2 > qLongest) break;
+      const double kvCtas = owners * keyTiles * kvParts, qCtas = owners * a.tiles * qParts, qEach = qMean / qParts + constant;
+      const double all = (kvCtas * (kvMean / kvParts + constant) + qCtas * qEach) / sms + (kvCtas + qCtas > sms ? 0.5 * qEach : 0.0);
+      double t = std::max({all, kvLongest / kvParts + constant, qLongest / qParts + constant});
+      if (kvParts > 1 || qParts > 1) t += 2.5 + 2 * ((kvParts > 1 ? kvParts * dkv : 0.0) + (qParts > 1 ? qParts * dq : 0.0)) / 12e6;
+      if (least == 0.0 || t < 0.95 * least) {
+        least = t;
+        best = {kvParts, qParts};
+      }
+    }
+  }
+  return best;
 }
 
 static size_t statsBytes(const AttnArgs& a) { return (size_t)a.batch * a.kvHeads * a.tiles * 256 * 4; }
