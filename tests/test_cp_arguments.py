@@ -80,7 +80,7 @@ def test_a_shape_in_use_outlives_the_store(cp):
     result, kept, alive = cp._result, [], []
 
     def clearing(*args):
-        kept.extend(weakref.ref(s[2][0]) for s in cp._shapes.values())
+        kept.extend(weakref.ref(s[-1][0]) for s in cp._shapes.values())
         cp._shapes.clear()
         return result(*args)
 
