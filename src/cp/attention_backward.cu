@@ -30,12 +30,18 @@ template <int DP> struct BackwardShape {
   static_assert(kBytes <= 227 * 1024 && (2 * kStages + 13) * 8 + 8 <= 1024, "shared memory");
 };
 
-// The power of two that ds is multiplied by, in fp16: |ds| <= p (|do.v| + |do.o|) <= 2 |do| |v|.
+// The power of two that ds is multiplied by, in fp16: |ds| <= p (|do.v| + |do.o|) <= 2 |do| |v|, by the longest rows of all tiles. (The bits of floats that are not negative
+// are ordered as they are, NaN on top.)
 template <typename T>
 __device__ __forceinline__ float gradScale(const AttnArgs& a, int b, int kvHead) {
   if (Pack<T>::kBackwardBias == 0.0f) return 1.0f;
-  const uint32_t* at = a.bounds + ((size_t)b * a.kvHeads + kvHead) * 2;
-  const float most = 2.0f * sqrtf(__uint_as_float(at[0])) * sqrtf(__uint_as_float(at[1]));
+  const uint32_t* at = a.bounds + ((size_t)b * a.kvHeads + kvHead) * (a.tiles + a.vTiles);
+  uint32_t longest[2] = {0, 0};   // do, v
+#pragma unroll 4
+  for (int i = threadIdx.x & 31; i < a.tiles; i += 32) longest[0] = max(longest[0], at[i]);
+#pragma unroll 4
+  for (int i = threadIdx.x & 31; i < a.vTiles; i += 32) longest[1] = max(longest[1], at[a.tiles + i]);
+  const float most = 2.0f * sqrtf(__uint_as_float(__reduce_max_sync(~0u, longest[0]))) * sqrtf(__uint_as_float(__reduce_max_sync(~0u, longest[1])));
   if (!(most > 0.0f) || most > 3.0e38f) return 1.0f;   // nothing to do, or nothing to save
   int e;
   frexpf(most, &e);                                     // most < 2^e
@@ -630,8 +636,8 @@ __global__ void __launch_bounds__(256) attnSumKernel(const __grid_constant__ Att
 
 // ---------------------------------------------------------------------------------------------- what both need of each row of queries
 // Minus <do, o> (unless that is given: minus what is), and minus the log-sum-exp in units of log 2, laid out as the tiles are. Rows that nobody has, and rows that
-// see no key, get an infinite log-sum-exp: their probabilities are zero. A CTA takes a tile, 8 or 16 lanes a row, a pack of 16 bytes each. fp16: the longest row of do, and by the CTAs behind the tiles of v. A maximum does not go
-// by the order, and the bits of floats that are not negative are ordered as they are (NaN on top).
+// see no key, get an infinite log-sum-exp: their probabilities are zero. A CTA takes a tile, 8 or 16 lanes a row, a pack of 16 bytes each. fp16: the longest row of do in it,
+// and by the CTAs behind those of every 128 rows of v.
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256, 4) attnStatsKernel(const __grid_constant__ AttnStatsArgs a) {
   constexpr int kAtOnce = 256 / LANES, kTurns = 4;   // rows of the CTA, and of a thread with loads on their way
@@ -656,11 +662,25 @@ __global__ void __launch_bounds__(256, 4) attnStatsKernel(const __grid_constant_
   const bool ofV = blockIdx.x >= qTiles;   // 128 rows of v instead of a tile
   const unsigned block = ofV ? blockIdx.x - qTiles : blockIdx.x, owner = block % owners;
   const int tile = block / owners, kvHead = owner % a.kvHeads, b = owner / a.kvHeads;
-  float most = 0.0f;   // (NaN stays)
+  uint32_t most = 0;   // the squared norm of the longest row, as bits
+  // The CTA's into place `to`.
+  auto longest = [&](int to) {
+    __shared__ uint32_t ofWarp[8];
+    most = __reduce_max_sync(~0u, most);
+    if (threadIdx.x % 32 == 0) ofWarp[threadIdx.x / 32] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < 8; ++i) most = max(most, ofWarp[i]);
+      a.bounds[(size_t)owner * (a.tiles + a.vTiles) + to] = most;
+    }
+  };
   pdlEnter();
   if (ofV) {
     const int used = a.kvLengths ? min(a.kvLengths[b], a.kv) : a.kv;
-    if (tile * 128 >= used) return;
+    if (tile * 128 >= used) {
+      longest(a.tiles + tile);
+      return;
+    }
     const long long base = b * a.vStride[0] + kvHead * a.vStride[2];
     for (int pass = 0; pass < 128; pass += kAtOnce * kTurns) {
       uint4 x[kTurns];
@@ -668,11 +688,10 @@ __global__ void __launch_bounds__(256, 4) attnStatsKernel(const __grid_constant_
       for (int n = 0; n < kTurns; ++n) x[n] = load(a.v, base + min(tile * 128 + pass + row0 + n * kAtOnce, used - 1) * a.vStride[1]);
 #pragma unroll
       for (int n = 0; n < kTurns; ++n) {
-        const float ss = dot(x[n], x[n]);
-        most = ss <= most ? most : ss;
+        most = max(most, __float_as_uint(dot(x[n], x[n])) & 0x7fffffffu);
       }
     }
-    if (lane == 0) atomicMax(a.bounds + owner * 2 + 1, __float_as_uint(most) & 0x7fffffffu);
+    longest(a.tiles + tile);
     return;
   }
   const int used = a.qLengths ? max(0, min(a.qLengths[b], a.q)) : a.q, tok0 = tile * a.tileTokens, rows = a.tileTokens * a.group;
@@ -699,10 +718,7 @@ __global__ void __launch_bounds__(256, 4) attnStatsKernel(const __grid_constant_
     for (int n = 0; n < kTurns; ++n) {
       const int row = pass + row0 + n * kAtOnce;
       if (!a.delta) delta[n] = dot(x[n], y[n]);
-      if (a.bounds) {
-        const float ss = dot(x[n], x[n]);
-        most = ss <= most ? most : ss;
-      }
+      if (a.bounds) most = max(most, __float_as_uint(dot(x[n], x[n])) & 0x7fffffffu);
       if (row >= some) {
         delta[n] = 0.0f;
         lse[n] = -INFINITY;
@@ -717,7 +733,7 @@ __global__ void __launch_bounds__(256, 4) attnStatsKernel(const __grid_constant_
       }
     }
   }
-  if (a.bounds && lane == 0) atomicMax(a.bounds + owner * 2, __float_as_uint(most) & 0x7fffffffu);
+  if (a.bounds) longest(tile);
 }
 
 }  // namespace

@@ -180,6 +180,7 @@ static void fillAttention(const ncclCpAttention_t* c, const int* qLengths, const
   a->group = c->heads / c->kv_heads;
   a->tileTokens = std::min(kAttnRows / a->group, std::max(c->q_tokens, 1));
   a->tiles = (c->q_tokens + a->tileTokens - 1) / a->tileTokens;
+  a->vTiles = (c->kv_tokens + kAttnRows - 1) / kAttnRows;
   a->causal = (int)c->mask;
   a->offset = (int)std::max<long long>(-(long long)c->q_tokens, std::min<long long>(c->offset, c->kv_tokens));   // further out nothing changes any more
   a->scale = c->scale;
@@ -265,12 +266,12 @@ static BackwardPlan backwardPlan(const ncclCpContext* cp, const ncclCpAttention_
 }
 
 static size_t statsBytes(const AttnArgs& a) { return (size_t)a.batch * a.kvHeads * a.tiles * 256 * 4; }
-static size_t boundsBytes(const ncclCpAttention_t* c) { return isFp16(c) ? ((size_t)c->batch * c->kv_heads * 8 + 255) / 256 * 256 : 0; }
+static size_t boundsBytes(const ncclCpAttention_t* c, const AttnArgs& a) { return isFp16(c) ? ((size_t)c->batch * c->kv_heads * (a.tiles + (c->kv_tokens + kAttnRows - 1) / kAttnRows) * 4 + 255) / 256 * 256 : 0; }
 static size_t dqBytes(const ncclCpAttention_t* c) { return (size_t)c->batch * c->q_tokens * c->heads * c->head_dim * 4; }
 static size_t dkBytes(const ncclCpAttention_t* c) { return (size_t)c->batch * c->kv_tokens * c->kv_heads * c->head_dim * 4; }
 // Numbers of each row, norms, and the sums of parts.
 static size_t backwardWork(const ncclCpAttention_t* c, const AttnArgs& a, const BackwardPlan& p) {
-  return statsBytes(a) + boundsBytes(c) + (p.qParts > 1 ? p.qParts * dqBytes(c) : 0) + (p.kvParts > 1 ? 2 * p.kvParts * dkBytes(c) : 0);
+  return statsBytes(a) + boundsBytes(c, a) + (p.qParts > 1 ? p.qParts * dqBytes(c) : 0) + (p.kvParts > 1 ? 2 * p.kvParts * dkBytes(c) : 0);
 }
 
 static ncclResult_t needsGpu(const ncclCpContext* cp, const char* what) {
@@ -279,7 +280,7 @@ static ncclResult_t needsGpu(const ncclCpContext* cp, const char* what) {
 }
 
 static ncclResult_t launchStats(ncclCpContext* cp, const ncclCpAttention_t* c, AttnStatsArgs* a, cudaStream_t stream) {
-  const unsigned ctas = (unsigned)a->batch * a->kvHeads * (a->tiles + (a->bounds ? (a->kv + kAttnRows - 1) / kAttnRows : 0));
+  const unsigned ctas = (unsigned)a->batch * a->kvHeads * (a->tiles + (a->bounds ? a->vTiles : 0));
   if (!ctas) return ncclSuccess;
   void* args[1] = {a};
   return launchCp(cp, attnStatsKernelFn(isFp16(c) ? ATTN_F16 : ATTN_BF16, c->head_dim), ctas, 1, 256, 0, args, stream);
@@ -296,6 +297,7 @@ static void fillStats(const ncclCpAttention_t* c, const AttnArgs& a, AttnStatsAr
   s->group = a.group;
   s->tileTokens = a.tileTokens;
   s->tiles = a.tiles;
+  s->vTiles = a.vTiles;
   s->qLengths = a.qLengths;
   s->kvLengths = a.kvLengths;
   memcpy(s->doutStride, c->dout_stride, sizeof(s->doutStride));
@@ -446,7 +448,7 @@ ncclResult_t ncclCpAttentionBackward(ncclCp_t cp, const ncclCpAttention_t* c, co
   a.bounds = isFp16(c) ? (const uint32_t*)((const char*)work + statsBytes(a)) : nullptr;
   a.kvParts = plan.kvParts;
   a.qParts = plan.qParts;
-  a.partDq = (float*)((char*)work + statsBytes(a) + boundsBytes(c));
+  a.partDq = (float*)((char*)work + statsBytes(a) + boundsBytes(c, a));
   a.partDk = (float*)((char*)a.partDq + (plan.qParts > 1 ? plan.qParts * dqBytes(c) : 0));
   a.partDv = (float*)((char*)a.partDk + plan.kvParts * dkBytes(c));
   a.status = cp->comm->devStatusDev;
@@ -461,7 +463,6 @@ ncclResult_t ncclCpAttentionBackward(ncclCp_t cp, const ncclCpAttention_t* c, co
     s.delta = delta;
     s.stats = (float*)work;
     s.bounds = (uint32_t*)a.bounds;
-    if (s.bounds) CUDACHECK(cudaMemsetAsync(s.bounds, 0, boundsBytes(c), stream));
     NCCLCHECK(launchStats(cp, c, &s, stream));
   }
   if (!c->q_tokens) q = dout = k;   // not read

@@ -33,7 +33,8 @@ struct AttnArgs {
   // backward
   const float* stats;         // [batch][kvHeads][tiles][2][128]: minus the log-sum-exp in units of log 2 and minus <d(out), out> of each row
   int tiles;                  // of the queries of a key head
-  const uint32_t* bounds;     // fp16: [batch][kvHeads][2] squared norms of the longest rows of d(out) and v, as bits
+  const uint32_t* bounds;     // fp16: [batch][kvHeads][tiles of d(out), then of v] squared norms of a tile's longest row, as bits
+  int vTiles;
   void *dq, *dk, *dv;         // contiguous, of the inputs' type or fp32
   int gradFp32;
   const float *addDq, *addDk, *addDv;
@@ -52,6 +53,7 @@ struct AttnStatsArgs {
   float* deltaOut;            // only that, or null
   float* stats;
   uint32_t* bounds;           // fp16, else null
+  int vTiles;
   int batch, q, kv, heads, kvHeads, dim, group, tileTokens, tiles;
   const int* qLengths;
   const int* kvLengths;
