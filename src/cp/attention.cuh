@@ -40,6 +40,13 @@ template <> struct Pack<__half> {
   __device__ static __forceinline__ float2 both(uint32_t u) { return __half22float2(*(__half2*)&u); }
 };
 
+// What rounding two numbers to 16 bits left, in 16 bits.
+template <typename T>
+__device__ __forceinline__ uint32_t remainderOf(uint32_t rounded, float a, float b) {
+  const float2 r = Pack<T>::both(rounded);
+  return Pack<T>::two(a - r.x, b - r.y);
+}
+
 // kind::f16, fp32 sums; B along the sum (K-major) or across it.
 template <typename T> constexpr uint32_t instr(int N, bool acrossB) {
   return (1u << 4) | (Pack<T>::kFormat << 7) | (Pack<T>::kFormat << 10) | ((acrossB ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);

@@ -10,6 +10,7 @@
 //
 // Roles as in the forward pass: warps 0-7 have a row of the tile each and, in two groups, a half of its columns; warp 8 feeds the ring, warp 9 issues products. Probabilities
 // and ds go back into tensor memory in 16 bits, each over the half it was computed from, and are the first operand of the next products from there.
+// "Fine" products, for calls that they cost little: what the rounding of probabilities and ds to 16 bits left is multiplied too. It lies over the scores, whose next tile then waits.
 // fp16: probabilities are held times 2^15, ds times a power of two that brings the largest that it could be (by the longest rows of do and v) to 2^15; the sums are in
 // fp32 and are multiplied back.
 #include "attention.cuh"
@@ -135,7 +136,7 @@ __device__ __forceinline__ void storeGradient(const AttnArgs& a, uint32_t tmem, 
 // Tensor memory: scores [keys x queries] at 0, do.v at 128 (then, over the half of a warp's columns, probabilities and ds), dv at 256, dk at 384. Scores are taken into registers
 // at once, and the next tile's are made meanwhile: its exponentials are computed while the tensor cores add this tile's to dv and dk and make the next do.v. With the
 // probabilities over the scores, the next scores waited for their product: a third of the tensor cores' time.
-template <typename T, int DP>
+template <typename T, int DP, bool FINE>
 __device__ __forceinline__ void backwardKv(const CUtensorMap& tmQ, const CUtensorMap& tmDo, const CUtensorMap& tmK, const CUtensorMap& tmV, const AttnArgs& a, uint8_t* smem,
                                            const BackwardBars& s, uint32_t tmem, unsigned block) {
   using Shape = BackwardShape<DP>;
@@ -246,18 +247,22 @@ __device__ __forceinline__ void backwardKv(const CUtensorMap& tmQ, const CUtenso
       if (need(waitOr(smemAddr(s.own), 0, abortFlag), 2100)) scores(0);
       if (ok) doV(0);
       for (int i = 0; i < n && ok; ++i) {
-        if (i + 1 < n) {
+        if (!FINE && i + 1 < n) {
           if (!need(waitOr(smemAddr(s.firstDone), i & 1, abortFlag), 2300)) break;   // scores are in registers
           scores(i + 1);
         }
         if (!ok || !need(waitOr(smemAddr(s.probDone), i & 1, abortFlag), 2400)) break;
         tcFenceAfter();
         productWithTmem<T, DP>(tmem + 256, tmem + 128, descAcross(tileAt(1, i)), i != 0);
+        if (FINE) productWithTmem<T, DP>(tmem + 256, tmem, descAcross(tileAt(1, i)), true);
         if (!need(waitOr(smemAddr(s.secondDone), i & 1, abortFlag), 2500)) break;
         tcFenceAfter();
         ummaCommit(smemAddr(&s.empty[stageOf(1, i)]));   // (its do.v was issued in front of this; the row's numbers that came with it are used up)
         productWithTmem<T, DP>(tmem + 384, tmem + 160, descAcross(tileAt(0, i)), i != 0);
+        if (FINE) productWithTmem<T, DP>(tmem + 384, tmem + 32, descAcross(tileAt(0, i)), true);
         ummaCommit(smemAddr(&s.empty[stageOf(0, i)]));
+        if (FINE && i + 1 < n) scores(i + 1);
+        if (!ok) break;
         if (i + 1 < n) doV(i + 1);   // over probabilities and ds: products are carried out in order
         else ummaCommit(smemAddr(s.outBar));
       }
@@ -323,6 +328,11 @@ __device__ __forceinline__ void backwardKv(const CUtensorMap& tmQ, const CUtenso
       tmemLdWait32(x[1]);
       // what is added to dv does not wait for ds
       tmemSt32(tDp, packed);
+      if (FINE) {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) packed[k] = remainderOf<T>(packed[k], lowOf(p[k]), highOf(p[k]));
+        tmemSt32(tS, packed);
+      }
       tmemStWait();
       tcFenceBefore();
       __syncwarp();
@@ -341,9 +351,18 @@ __device__ __forceinline__ void backwardKv(const CUtensorMap& tmQ, const CUtenso
           hi = mul2(p[q * 16 + k / 2 + 1], hi);
           packed[q * 16 + k / 2] = Pack<T>::two(lowOf(lo), highOf(lo));
           packed[q * 16 + k / 2 + 1] = Pack<T>::two(lowOf(hi), highOf(hi));
+          if (FINE) {
+            p[q * 16 + k / 2] = lo;
+            p[q * 16 + k / 2 + 1] = hi;
+          }
         }
       }
       tmemSt32(tDp + 32, packed);
+      if (FINE) {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) packed[k] = remainderOf<T>(packed[k], lowOf(p[k]), highOf(p[k]));
+        tmemSt32(tS + 32, packed);
+      }
       tmemStWait();
       tcFenceBefore();
       __syncwarp();
@@ -367,7 +386,7 @@ __device__ __forceinline__ void backwardKv(const CUtensorMap& tmQ, const CUtenso
 // ---------------------------------------------------------------------------------------------- dq
 // Tensor memory: scores [queries x keys] at 0, do.v (then ds) of two tiles at 128 and 256, dq at 384. Scores are taken into registers at once, and the next tile's are made
 // while exponentials are computed; so is its do.v, in the other place. So products and elements of a tile do not wait for one another.
-template <typename T, int DP>
+template <typename T, int DP, bool FINE>
 __device__ __forceinline__ void backwardQ(const CUtensorMap& tmQ, const CUtensorMap& tmDo, const CUtensorMap& tmK, const CUtensorMap& tmV, const AttnArgs& a, uint8_t* smem,
                                           const BackwardBars& s, uint32_t tmem, unsigned block) {
   using Shape = BackwardShape<DP>;
@@ -479,6 +498,7 @@ __device__ __forceinline__ void backwardQ(const CUtensorMap& tmQ, const CUtensor
         if (!ok || !need(waitOr(smemAddr(&s.secondDone[i & 1]), i >> 1 & 1, abortFlag), 2300)) break;
         tcFenceAfter();
         productWithTmem<T, DP>(tmem + 384, tmem + 128 + (i & 1) * 128, descAcross(tileAt(0, i)), i != 0);
+        if (FINE) productWithTmem<T, DP>(tmem + 384, tmem + 160 + (i & 1) * 128, descAcross(tileAt(0, i)), true);
         ummaCommit(smemAddr(&s.empty[stageOf(0, i)]));
       }
       if (ok) ummaCommit(smemAddr(s.outBar));
@@ -511,7 +531,7 @@ __device__ __forceinline__ void backwardQ(const CUtensorMap& tmQ, const CUtensor
         break;
       }
       tcFenceAfter();
-      uint32_t x[2][32], y[32], packed[32];
+      uint32_t x[2][32], y[32], packed[32], rest[FINE ? 32 : 1];
       tmemLd32(tS, x[0]);
       tmemLd32(tS + 32, x[1]);
       tmemLdWait32(x[0]);
@@ -546,10 +566,14 @@ __device__ __forceinline__ void backwardQ(const CUtensorMap& tmQ, const CUtensor
           for (int k = 0; k < 16; ++k) p[k] = pair(k0 + q * 32 + 2 * k < limit ? lowOf(p[k]) : 0.0f, k0 + q * 32 + 2 * k + 1 < limit ? highOf(p[k]) : 0.0f);
         }
 #pragma unroll
-        for (int k = 0; k < 16; ++k) packed[q * 16 + k] = Pack<T>::two(lowOf(p[k]), highOf(p[k]));
+        for (int k = 0; k < 16; ++k) {
+          packed[q * 16 + k] = Pack<T>::two(lowOf(p[k]), highOf(p[k]));
+          if (FINE) rest[q * 16 + k] = remainderOf<T>(packed[q * 16 + k], lowOf(p[k]), highOf(p[k]));
+        }
       }
       if (!ok) break;
       tmemSt32(tDp, packed);
+      if constexpr (FINE) tmemSt32(tDp + 32, rest);
       tmemStWait();
       tcFenceBefore();
       __syncwarp();
@@ -570,7 +594,7 @@ __device__ __forceinline__ void backwardQ(const CUtensorMap& tmQ, const CUtensor
 }
 
 // The first CTAs own tiles of keys, the others tiles of queries: neither needs the other's, and where both are few they run beside one another.
-template <typename T, int DP>
+template <typename T, int DP, bool FINE>
 __global__ void __launch_bounds__(BackwardWarps::kThreads, 1)
 attnBackwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDo, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const __grid_constant__ AttnArgs a) {
@@ -591,8 +615,8 @@ attnBackwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   tcFenceAfter();
   const uint32_t tmem = *s.tmemSlot;
   pdlEnter();   // the set-up above overlaps the end of the kernel before
-  if (ofKeys) backwardKv<T, DP>(tmQ, tmDo, tmK, tmV, a, smem, s, tmem, blockIdx.x);
-  else backwardQ<T, DP>(tmQ, tmDo, tmK, tmV, a, smem, s, tmem, blockIdx.x - a.kvCtas);
+  if (ofKeys) backwardKv<T, DP, FINE>(tmQ, tmDo, tmK, tmV, a, smem, s, tmem, blockIdx.x);
+  else backwardQ<T, DP, FINE>(tmQ, tmDo, tmK, tmV, a, smem, s, tmem, blockIdx.x - a.kvCtas);
   tcFenceBefore();
   __syncthreads();
   if (warp == BackwardWarps::kMma) {
@@ -738,8 +762,11 @@ __global__ void __launch_bounds__(256, 4) attnStatsKernel(const __grid_constant_
 
 }  // namespace
 
-template <typename T> static const void* backwardFn(int dim) { return dim <= 64 ? (const void*)attnBackwardKernel<T, 64> : (const void*)attnBackwardKernel<T, 128>; }
-const void* attnBackwardKernelFn(int type, int dim) { return type == ATTN_F16 ? backwardFn<__half>(dim) : backwardFn<__nv_bfloat16>(dim); }
+template <typename T> static const void* backwardFn(int dim, bool fine) {
+  if (dim <= 64) return fine ? (const void*)attnBackwardKernel<T, 64, true> : (const void*)attnBackwardKernel<T, 64, false>;
+  return fine ? (const void*)attnBackwardKernel<T, 128, true> : (const void*)attnBackwardKernel<T, 128, false>;
+}
+const void* attnBackwardKernelFn(int type, int dim, bool fine) { return type == ATTN_F16 ? backwardFn<__half>(dim, fine) : backwardFn<__nv_bfloat16>(dim, fine); }
 const void* attnSumKernelFn(int type) { return type == ATTN_F16 ? (const void*)attnSumKernel<__half> : (const void*)attnSumKernel<__nv_bfloat16>; }
 int attnBackwardThreads() { return BackwardWarps::kThreads; }
 int attnBackwardRegs() { return BackwardWarps::kLaunchRegs; }

@@ -234,9 +234,16 @@ static size_t forwardWork(const ncclCpAttention_t* c, const ForwardPlan& p) {
 // constant for a CTA's beginning and end, and for parts a launch and the traffic of their sums, once there and once back. Measured with inputs from memory, us, without parts and by
 // this rule: 2048 causal tokens of 32 heads over one 735, 135; 4096 of 8 over 2 205, 131; 128 queries on 16384 keys of 8 heads 211, 104; 33 on 4000, 28 heads over 4, causal 63, 43;
 // 512 causal tokens of 8 heads over one, 64 channels 55, 23; where it makes none parts would cost: 509 x 641, 3 times 12 heads over 4, 96 channels 53, in two parts 62 and more.
+//
+// Gradients have two roundings to 16 bits: of ds (dv: of the probabilities) and of what is stored, 1.4 times the second alone on average. Where an output has few rows, or few terms
+// that cancel, that is 1.55 times now and then. Calls of few products multiply what the first rounding left as well ("fine"): one query on 512 keys 14.6 us instead of 12.5, 2 x 256
+// causal tokens of 8 heads of 64 12.8 instead of 10.8; beyond that it would cost more (512 causal tokens of 8 heads 23.8 instead of 17.9, 1024 of 4 36.4 instead of 23.6).
 struct BackwardPlan {
   int kvParts, qParts;
 };
+static bool fineProducts(const ncclCpAttention_t* c, const AttnArgs& a) {
+  return (double)c->batch * c->kv_heads * a.tiles * std::ceil(c->kv_tokens / 128.0) <= 64;   // products of 128 x 128
+}
 static BackwardPlan backwardPlan(const ncclCpContext* cp, const ncclCpAttention_t* c, const AttnArgs& a) {
   const double owners = (double)c->batch * c->kv_heads, keyTiles = std::ceil(c->kv_tokens / 128.0), sms = cp->smCount;
   const long long offset = c->mask == NCCL_CP_CAUSAL_END ? (long long)c->kv_tokens - c->q_tokens : a.offset;
@@ -475,8 +482,8 @@ ncclResult_t ncclCpAttentionBackward(ncclCp_t cp, const ncclCpAttention_t* c, co
   void* args[5] = {&maps[0], &maps[1], &maps[2], &maps[3], &a};
   const unsigned owners = (unsigned)c->batch * c->kv_heads, keyTiles = (c->kv_tokens + kAttnRows - 1) / kAttnRows;
   a.kvCtas = owners * keyTiles * plan.kvParts;
-  NCCLCHECK(launchCp(cp, attnBackwardKernelFn(type, c->head_dim), a.kvCtas + owners * a.tiles * plan.qParts, 1, attnBackwardThreads(), attnBackwardSmemBytes(c->head_dim), args, stream,
-                     attnBackwardRegs()));
+  NCCLCHECK(launchCp(cp, attnBackwardKernelFn(type, c->head_dim, fineProducts(c, a)), a.kvCtas + owners * a.tiles * plan.qParts, 1, attnBackwardThreads(),
+                     attnBackwardSmemBytes(c->head_dim), args, stream, attnBackwardRegs()));
   const size_t sumRows = (plan.qParts > 1 ? rows : 0) + (plan.kvParts > 1 ? 2 * cols : 0);
   if (!sumRows) return ncclSuccess;
   void* sum[1] = {&a};

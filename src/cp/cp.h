@@ -83,7 +83,7 @@ enum AttnType : int { ATTN_F16 = 0, ATTN_BF16 = 1, ATTN_F32 = 2 };
 const void* attnForwardKernelFn(int type, int dim, bool pairs);
 size_t attnForwardSmemBytes(int dim, bool pairs);
 const void* attnJoinKernelFn(int type);
-const void* attnBackwardKernelFn(int type, int dim);
+const void* attnBackwardKernelFn(int type, int dim, bool fine);
 size_t attnBackwardSmemBytes(int dim);
 int attnForwardThreads();
 int attnBackwardThreads();

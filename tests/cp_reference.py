@@ -29,12 +29,13 @@ class Reference:
     pass are held as multiples of 2^-24 of a largest one of at least 2^-1 (2^7 over the lag of 2^8), those of the backward pass as multiples of 2^-39, and ds as
     multiples of 2^-24 where the largest that could be, 2 |do| |v|, is 2^14 at least."""
 
-    def __init__(self, q, k, v, causal=False, offset=None, scale=None, q_lengths=None, kv_lengths=None, join=None, dout=None, out=None, result=None, add=None):
+    def __init__(self, q, k, v, causal=False, offset=None, scale=None, q_lengths=None, kv_lengths=None, join=None, dout=None, out=None, result=None, add=None, fine=False):
         B, Q, H, D = q.shape
         K, G = k.shape[1:3]
         R = H // G
         scale = 1 / math.sqrt(D) if scale is None else scale
         u = half_step(q.dtype)
+        inner = u * u if fine else u   # with "fine" products, what the first rounding of probabilities and ds left is rounded and counted too
         ur = half_step(result or q.dtype)
         tiny = torch.finfo(result or q.dtype).smallest_normal * ur
         f16 = q.dtype == torch.float16
@@ -72,7 +73,7 @@ class Reference:
         dp = do @ vd.mT
         ds = p * (dp - delta)
         # of ds: its rounding, the probability's relative error, and the errors of dp and delta
-        eds = ds.abs() * u + p * (rel * (dp.abs() + delta.abs()) + D * 2.0 ** -23 * (do.abs() @ vd.abs().mT + (do.abs() * od.abs()).sum(-1, keepdim=True)))
+        eds = ds.abs() * inner + p * (rel * (dp.abs() + delta.abs()) + D * 2.0 ** -23 * (do.abs() @ vd.abs().mT + (do.abs() * od.abs()).sum(-1, keepdim=True)))
         least = 0.0
         if f16:
             norm = lambda t: t.norm(dim=-1).amax(-1).view(B, G, R).amax(-1).repeat_interleave(R, 1)[..., None, None]   # noqa: E731
@@ -86,7 +87,7 @@ class Reference:
         self.dq, self.dq_tol = bound((scale * ds @ kd).transpose(1, 2), base[0], (scale * (eds + K * 2.0 ** -23 * ds.abs()) @ kd.abs()).transpose(1, 2))
         n = Q * R
         self.dk, self.dk_tol = bound(over(scale * ds.mT @ qd), base[1], over(scale * (eds + n * 2.0 ** -23 * ds.abs()).mT @ qd.abs()))
-        self.dv, self.dv_tol = bound(over(p.mT @ do), base[2], over(((u + rel + n * 2.0 ** -23) * p + least * 2.0 ** -15 * see[:, None]).mT @ do.abs()))
+        self.dv, self.dv_tol = bound(over(p.mT @ do), base[2], over(((inner + rel + n * 2.0 ** -23) * p + least * 2.0 ** -15 * see[:, None]).mT @ do.abs()))
 
 
 def check(name, got, want, tol):

@@ -91,6 +91,19 @@ def test_add(cp):
     assert all(torch.equal(a, b) for a, b in zip(mine, got))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("B,Q,K,H,G,D", [(1, 1, 1, 1, 1, 8), (1, 3, 500, 8, 2, 128), (2, 200, 70, 4, 4, 64), (1, 1000, 300, 4, 2, 96), (1, 5, 3000, 2, 2, 128)])
+def test_small_calls_lose_nothing_inside(cp, dtype, B, Q, K, H, G, D):
+    q, k, v = operands(B, Q, K, H, G, D, dtype)
+    dout = randn(B, Q, H, D, dtype=dtype, seed=9)
+    out, lse = cp.attention(q, k, v, causal=True)
+    got = cp.attention_backward(dout, q, k, v, out, lse, causal=True, dtype=F32)
+    few = B * G * -(-Q // (128 // (H // G))) * -(-K // 128) <= 64   # products of 128 x 128 (1000 queries on 300 keys are 2 * 16 * 3 = 96: the ordinary bound)
+    ref = Reference(q, k, v, True, dout=dout, out=out, result=F32, fine=few)
+    for name, t in zip(("dv", "dk", "dq"), got[::-1]):
+        check(name, t, getattr(ref, name), getattr(ref, name + "_tol"))
+
+
 # ------------------------------------------------------------------------------------------------ padding
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("junk", [math.nan, math.inf, "lowest"])
