@@ -421,8 +421,8 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 // Joins the parts of the keys: out = sum_s exp(lse_s - L) out_s with L = ln sum_s exp(lse_s); what `join` names is one more part. quads * a.joinShares threads take a row: four
 // channels of every joinShares-th part each, all of them on their way at once, and the first of those with the same channels joins the others' (with a thread for four channels that
 // walked the parts one after the other, 16 parts of 32 rows took 8.6 us).
-constexpr int kJoinTurns = 8;
-static_assert(kAttnMaxSplits <= kJoinTurns * (256 / (kAttnMaxDim / 4)), "parts of a thread");
+constexpr int kJoinTurns = kAttnJoinTurns;
+static_assert(kAttnMaxSplits <= kJoinTurns * (256 / (kAttnMaxDim / 4)), "parts of a thread");   // (256 / ... is a power of two)
 template <typename T>
 __global__ void __launch_bounds__(256) attnJoinKernel(const __grid_constant__ AttnArgs a) {
   __shared__ float4 sums[256];
@@ -457,7 +457,14 @@ __global__ void __launch_bounds__(256) attnJoinKernel(const __grid_constant__ At
     top = m;
   };
 #pragma unroll
-  for (int i = 0; i < kJoinTurns; ++i) add(lse[i], 1.0f, v[i]);
+  for (int i = 0; i < kJoinTurns; ++i) top = fmaxf(top, lse[i]);
+  const float shift = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+  for (int i = 0; i < kJoinTurns; ++i) {
+    const float weight = expf(lse[i] - shift);
+    total += weight;
+    f.x += v[i].x * weight; f.y += v[i].y * weight; f.z += v[i].z * weight; f.w += v[i].w * weight;
+  }
   if (share) {
     sums[threadIdx.x] = f;
     heads[threadIdx.x] = make_float2(top, total);

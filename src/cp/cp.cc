@@ -196,8 +196,9 @@ static void fillAttention(const ncclCpAttention_t* c, const int* qLengths, const
 // with the mean number of tiles (of which a CTA with one tile of queries makes two at a time, for 1.15 of the time), the longest CTA at least, and a constant for a CTA's beginning
 // and end. Measured with inputs from memory, us, pairs and single tiles (32 heads over 8 of 128 channels where nothing else is said): 2048 x 2048 78, 94; the same, causal 49, 66;
 // 4096 causal 139, 168; 1024 x 4096 70, 80; 1500 x 8192 242, 205; 3000 x 3000 of 10 heads over 2, causal 55, 41; 3 x 777 x 1013 of 12 heads over 4, 80 channels 27, 37.
-// Parts cost a second kernel and the partial results, 5 us, and pay where they save more tiles than that: one query on 4096 keys, one part 41 us, 8 28, 16 26; on 512 keys (4 heads
-// of 64 channels) one part 14 us, two 20.
+// Parts cost a second kernel and the partial results, 5 us, and pay where they save more tiles than that; then as many as there are SMs for. Measured on inputs in L2, us, one part and
+// by the rule: one head of 2048 x 2048 21.5, 16.1; 33 on 4000, 28 heads over 4 35.3, 16.6; 300 on 4000, 4 heads 35.6, 17.9; 128 on 65536, one head 445, 20.5 (32 parts 27); two on
+// 16384, 2 heads 118, 13.6; one on 512 keys, 4 heads of 64 channels 8.7 in one part, which stays so.
 struct ForwardPlan {
   bool pairs;
   int splits;
@@ -224,6 +225,13 @@ static ForwardPlan forwardPlan(const ncclCpContext* cp, const ncclCpAttention_t*
     if (most > 1 && longest * (1.0 - 1.0 / most) > 8.0) p.splits = most;
   }
   return p;
+}
+// How many threads share four channels of a row's parts in the kernel that joins them: as many as there are parts while that makes no more than 512 threads for an SM, and for each no
+// more than kAttnJoinTurns parts. One head of 2048 x 2048 in 8 parts takes 16.1 us so, with up to 1024 threads 17.2, with 2048 20.0, with a thread for each part 26.4.
+static int joinShares(const ncclCpContext* cp, size_t rows, int quads, int splits) {
+  int shares = 1;
+  while (shares * kAttnJoinTurns < splits || (2 * shares <= std::min(256 / quads, splits) && 2 * shares * rows * quads <= (size_t)cp->smCount * 512)) shares *= 2;
+  return shares;
 }
 static size_t forwardWork(const ncclCpAttention_t* c, const ForwardPlan& p) {
   return p.splits == 1 ? 0 : (size_t)p.splits * c->batch * c->q_tokens * c->heads * (c->head_dim + 1) * 4;
@@ -390,7 +398,7 @@ ncclResult_t ncclCpAttention(ncclCp_t cp, const ncclCpAttention_t* c, const void
   NCCLCHECK(launchCp(cp, attnForwardKernelFn(type, c->head_dim, plan.pairs), grid, 1, attnForwardThreads(), attnForwardSmemBytes(c->head_dim, plan.pairs), args, stream, attnForwardRegs()));
   if (plan.splits == 1) return ncclSuccess;
   const int quads = c->head_dim / 4;
-  a.joinShares = std::min(256 / quads, plan.splits);
+  a.joinShares = joinShares(cp, rows, quads, plan.splits);
   const int perCta = 256 / (quads * a.joinShares);
   void* join[1] = {&a};
   return launchCp(cp, attnJoinKernelFn(type), (unsigned)((rows + perCta - 1) / perCta), 1, 256, 0, join, stream);

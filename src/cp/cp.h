@@ -9,6 +9,7 @@ constexpr int kAttnRows = 128;       // rows of a tile: (token, head of a group)
 constexpr int kAttnMaxDim = 128;     // channels of a head
 constexpr int kAttnMaxTokens = 1 << 30;
 constexpr int kAttnMaxSplits = 64;   // parts of the keys that CTAs work on at the same time
+constexpr int kAttnJoinTurns = 8;    // of them, that a thread joins
 
 // Rows of queries are packed: the heads that share keys and values lie next to each other, so that a tile holds `tileTokens` tokens of the `group` heads
 // of one key head, row = token * group + head. tileTokens * group <= 128; rows behind that are nobody's.
