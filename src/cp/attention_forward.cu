@@ -10,6 +10,11 @@
 // While one group works on its scores the tensor cores work for the other. In the form for many rows ("pairs") the groups have a tile of 128 rows of
 // queries each; in the form for few rows they share one and take the tiles of keys in turn, and their results are joined at the end. There the keys may also be cut into
 // parts for several CTAs, whose results a second kernel joins.
+//
+// What bounds it: at 128 channels a tile of 128 x 128 scores is 1024 cycles for the tensor cores and as many for its exponentials (16 a cycle), and takes 1800: a group's products, maximum
+// and exponentials depend on one another, and two groups hide that in part. 8192 x 8192 of 32 heads over 8, everything seen, 822 to 850 us (1.3 PFLOP/s), causal 441 to 453; the products
+// alone 635, all but the products 709. Single queries are bound by memory: 8 on 16384 keys each, 32 heads over 8, 94 us under a profiler, 71 % of memory's rate.
+//
 // Rows behind a tile's last are whatever shared memory held: they reach only results that nobody stores. Values behind a sequence's last key may be
 // anything (0 * NaN is NaN): zeros are written over them in shared memory.
 // Every wait is bounded; on expiry the kernel records a status, waits for its copies and products in flight, frees its tensor memory and returns.
@@ -419,8 +424,8 @@ attnForwardKernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 }
 
 // Joins the parts of the keys: out = sum_s exp(lse_s - L) out_s with L = ln sum_s exp(lse_s); what `join` names is one more part. quads * a.joinShares threads take a row: four
-// channels of every joinShares-th part each, all of them on their way at once, and the first of those with the same channels joins the others' (with a thread for four channels that
-// walked the parts one after the other, 16 parts of 32 rows took 8.6 us).
+// channels of every joinShares-th part each, all of them on their way at once, and the first of those with the same channels joins the others'. Its time is that of a launch and a
+// load: 16 parts of 32 rows 3.3 us (a thread for four channels that walked the parts one after the other took 8.6).
 constexpr int kJoinTurns = kAttnJoinTurns;
 static_assert(kAttnMaxSplits <= kJoinTurns * (256 / (kAttnMaxDim / 4)), "parts of a thread");   // (256 / ... is a power of two)
 template <typename T>
