@@ -18,12 +18,13 @@ A block of keys that another rank sent joins what is there already, in fp32, and
 A cache is read by the same call, one query or more for each sequence: ``cp.attention(q, k_cache, v_cache, causal=True, kv_lengths=lengths)``.
 
 Every call is local to the communicator's GPU, runs on its current stream and keeps nothing: results and workspaces come from the framework's allocator, so that calls may be
-captured, replayed, and made on several streams at once. Reference parity: the reference has no compute kernels; programs like these use its send / receive and all-to-all
+captured, replayed, and made on several streams at once; no call keeps a history for autograd (gradients come from the backward calls). Reference parity: the reference has no compute kernels; programs like these use its send / receive and all-to-all
 (src/collectives.cc) around their own.
 """
 import ctypes
 import functools
 import math
+import operator
 
 from .. import _lib
 from ..core import BF16, FP16, FP32, current_stream
@@ -178,16 +179,21 @@ class ContextParallel:
         return B, Q, K, H, G, D
 
     @staticmethod
+    def _numbers(causal, offset, scale):
+        """What a call is remembered by: numbers, where a caller has given a tensor that may hold another one next time."""
+        return bool(causal), None if offset is None else operator.index(offset), None if scale is None else float(scale)
+
+    @staticmethod
     def _mask(causal, offset, scale, D):
         """(mask, offset, scale) as the library takes them."""
         if offset is not None and not causal:
             raise ValueError("offset says where a causal mask lies: without one there is nothing to offset")
-        scale = 1 / math.sqrt(D) if scale is None else float(scale)
+        scale = 1 / math.sqrt(D) if scale is None else scale
         if not 0 < scale < math.inf or not 0 < ctypes.c_float(scale).value < math.inf:
             raise ValueError("scale = %r must be positive and finite" % (scale,))
         if offset is not None and abs(offset) >> 62:
             raise ValueError("offset = %r" % (offset,))
-        return (0 if not causal else 2 if offset is None else 1), (0 if offset is None else int(offset)), scale
+        return (0 if not causal else 2 if offset is None else 1), (0 if offset is None else offset), scale
 
     def _describe(self, sizes, dtype, result, mask, strides, work):
         """The library's description of a call, its address, and the bytes of workspace that it takes."""
@@ -221,6 +227,7 @@ class ContextParallel:
 
         Sums and statistics are fp32; probabilities are rounded to q's type (by at most half a step each) before they meet v."""
         torch = self.torch
+        causal, offset, scale = self._numbers(causal, offset, scale)
 
         def make():
             sizes = B, Q, K, H, G, D = self._sizes(q, k, v)
@@ -267,6 +274,7 @@ class ContextParallel:
         ``out`` and ``lse`` are the result over all keys of the queries: where blocks were joined, the last one's. ``delta``: what ``attention_delta`` gives (out may then be
         None). ``add``: fp32 (dq, dk, dv) so far, to which these are added; they may be the results' tensors. The same call gives the same bits."""
         torch = self.torch
+        causal, offset, scale = self._numbers(causal, offset, scale)
 
         def make():
             sizes = B, Q, K, H, G, D = self._sizes(q, k, v)
@@ -316,6 +324,7 @@ class ContextParallel:
         if not isinstance(freqs, RotaryFrequencies):
             raise ValueError("freqs must come from rotary_frequencies")
         yq, yk = (None, None) if out is None else out
+        offset, interleaved, inverse = operator.index(offset), bool(interleaved), bool(inverse)
 
         def make():
             if q.dim() != 4 or q.dtype not in self._codes or (k is not None and (k.dim() != 4 or k.dtype is not q.dtype or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
@@ -327,7 +336,7 @@ class ContextParallel:
             if B * T >> 31 or abs(offset) >> 62:
                 raise ValueError("%d sequences of %d tokens, offset %r" % (B, T, offset))
             d = _Rotary(ctypes.sizeof(_Rotary), MAGIC, self._codes[q.dtype], B, T, D, freqs.half)
-            d.interleaved, d.inverse, d.amplitude, d.offset = bool(interleaved), bool(inverse), freqs.amplitude, offset
+            d.interleaved, d.inverse, d.amplitude, d.offset = interleaved, inverse, freqs.amplitude, offset
             if positions is not None:
                 if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (B, T) or min(positions.stride()) < 0:
                     raise ValueError("positions must be an int32 or int64 tensor [%d, %d], not %s %s" % (B, T, str(positions.dtype).replace("torch.", ""), list(positions.shape)))

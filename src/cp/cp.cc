@@ -109,6 +109,50 @@ static Span spanOf(const void* p, int batch, int tokens, int heads, int dim, con
   return {p, ((size_t)(batch - 1) * stride[0] + (size_t)(tokens - 1) * stride[1] + (size_t)(heads - 1) * stride[2] + dim) * size};
 }
 
+// Rows of a tensor that is turned: [batch][tokens][heads], strides in elements (0 where there is one).
+struct Rows {
+  const void* at;
+  const int* sizes;
+  const long long* stride;
+};
+// Whether rows of that many elements at these places never meet: each dimension steps over all that the smaller ones reach.
+static bool nest(const int* sizes, const long long* stride, unsigned dims, __int128 extent) {
+  for (int i = 0; i < 3; ++i)
+    if (sizes[i] <= 1) dims &= ~(1u << i);
+  while (dims) {
+    int least = -1;
+    for (int i = 0; i < 3; ++i)
+      if (dims >> i & 1 && (least < 0 || stride[i] < stride[least])) least = i;
+    if (stride[least] < extent) return false;
+    extent += (__int128)(sizes[least] - 1) * stride[least];
+    dims &= ~(1u << least);
+  }
+  return true;
+}
+// Whether rows of two tensors of the same batch and tokens never meet: with some dimensions stepping alike, what the others reach is apart (a projection's queries and keys).
+static bool apart(Rows a, Rows b, int dim, int size) {
+  if ((uintptr_t)a.at > (uintptr_t)b.at) std::swap(a, b);
+  const __int128 distance = (__int128)((uintptr_t)b.at - (uintptr_t)a.at) / size;
+  for (unsigned alike = 0; alike < 8; ++alike) {
+    __int128 reachA = dim, reachB = dim;
+    int sizes[3];
+    long long stride[3];
+    bool same = true;
+    for (int i = 0; i < 3; ++i) {
+      sizes[i] = std::max(a.sizes[i], b.sizes[i]);
+      stride[i] = std::max(a.stride[i], b.stride[i]);
+      if (alike >> i & 1) {
+        same = same && (a.sizes[i] == 1 || b.sizes[i] == 1 || a.stride[i] == b.stride[i]);
+      } else {
+        reachA += (__int128)(a.sizes[i] - 1) * a.stride[i];
+        reachB += (__int128)(b.sizes[i] - 1) * b.stride[i];
+      }
+    }
+    if (same && reachA <= distance && nest(sizes, stride, alike, distance + reachB)) return true;
+  }
+  return false;
+}
+
 // ---------------------------------------------------------------- attention
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                   CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -545,24 +589,26 @@ ncclResult_t ncclCpRotary(ncclCp_t cp, const ncclCpRotary_t* c, const void* x0, 
   memset(&a, 0, sizeof(a));
   Span in[2] = {}, out[2] = {};
   bool inPlace[2] = {};
+  int sizes[2][3];
   a.wide = c->head_dim % E == 0 && (c->interleaved ? 2 * c->half : c->half) % E == 0;
   const int tensors = c->heads[1] ? 2 : 1;
   for (int t = 0; t < tensors; ++t) {
     a.x[t] = t ? x1 : x0;
     a.y[t] = t ? y1 : y0;
     a.heads[t] = c->heads[t];
-    const int sizes[3] = {c->batch, c->tokens, c->heads[t]};
+    for (int i = 0; i < 3; ++i) sizes[t][i] = i == 0 ? c->batch : i == 1 ? c->tokens : c->heads[t];
     inPlace[t] = a.x[t] == a.y[t];
     for (int i = 0; i < 3; ++i) {
       const long long xs = c->x_stride[t][i], ys = c->y_stride[t][i];
-      if (sizes[i] > 1) {
+      if (sizes[t][i] > 1) {
         if (xs < 0 || xs >= 1ll << 40 || ys < c->head_dim || ys >= 1ll << 40) { WARN("%s: strides must not be negative, and rows of a result not overlap", what); return ncclInvalidArgument; }
         a.wide = a.wide && xs % E == 0 && ys % E == 0;
         inPlace[t] = inPlace[t] && xs == ys;
       }
-      a.inStride[t][i] = sizes[i] > 1 ? xs : 0;
-      a.outStride[t][i] = sizes[i] > 1 ? ys : 0;
+      a.inStride[t][i] = sizes[t][i] > 1 ? xs : 0;
+      a.outStride[t][i] = sizes[t][i] > 1 ? ys : 0;
     }
+    if (!nest(sizes[t], a.outStride[t], 7, c->head_dim)) { WARN("%s: rows of a result overlap", what); return ncclInvalidArgument; }
     a.wide = a.wide && aligned({a.x[t], a.y[t]}, 16);
     in[t] = spanOf(a.x[t], c->batch, c->tokens, c->heads[t], c->head_dim, a.inStride[t], size);
     out[t] = spanOf(a.y[t], c->batch, c->tokens, c->heads[t], c->head_dim, a.outStride[t], size);
@@ -575,9 +621,10 @@ ncclResult_t ncclCpRotary(ncclCp_t cp, const ncclCpRotary_t* c, const void* x0, 
       if (s0 < 0 || s1 < 0 || s0 >= 1ll << 40 || s1 >= 1ll << 40) { WARN("%s: strides must not be negative", what); return ncclInvalidArgument; }
       bad = bad || meets(out[t], {positions, ((size_t)(c->batch - 1) * s0 + (size_t)(c->tokens - 1) * s1 + 1) * (c->positions64 ? 8 : 4)});
     }
-    // a tensor that is turned in place may lie between another's rows (one projection's queries and keys)
+    // a tensor that is turned in place may lie between another's rows (one projection's queries and keys), not on them
     for (int u = 0; u < tensors; ++u) {
       if (!inPlace[t]) bad = bad || meets(out[t], in[u]);
+      else if (u != t) bad = bad || !apart({a.y[t], sizes[t], a.outStride[t]}, {a.x[u], sizes[u], a.inStride[u]}, c->head_dim, size);
       if (u != t && !(inPlace[t] && inPlace[u])) bad = bad || meets(out[t], out[u]);
     }
     if (bad) { WARN("%s: an output shares memory with another tensor", what); return ncclInvalidArgument; }

@@ -284,6 +284,46 @@ def test_outputs_that_share_memory_are_refused(cp):
     torch.cuda.synchronize()
 
 
+def test_turned_in_place(cp):
+    from nccl_b200._lib import NcclError
+    freqs = cp.rotary_frequencies(64)
+
+    def layouts():   # a storage, and two tensors in it whose rows lie between one another
+        x = randn(2, 9, 6, 64)
+        yield x, x[:, :, :4], x[:, :, 4:]
+        yield x, x[:, :, ::2], x[:, :, 1::2]
+        x = randn(2, 6, 9, 64).transpose(1, 2)
+        yield x, x[:, :, 2:], x[:, :, :2]
+        x = randn(9, 2, 6, 64).transpose(0, 1)
+        yield x, x[:, :, :3], x[:, :, 3:]
+    for x, q, k in layouts():
+        wq, wk = cp.rotary(q.clone(), k.clone(), freqs, offset=5)
+        before = x.clone()
+        aside = torch.empty(k.shape, device="cuda", dtype=k.dtype)
+        cp.rotary(q, k, freqs, offset=5, out=(q, aside))   # the other only read
+        assert torch.equal(q, wq) and torch.equal(aside, wk)
+        x.copy_(before)
+        cp.rotary(q, k, freqs, offset=5, out=(q, k))
+        assert torch.equal(q, wq) and torch.equal(k, wk)
+    x, y = randn(1, 9, 6, 64), randn(1, 9, 6, 64)
+    for q, k, out in ((x, x, (x, x)), (x, x, (x, y)), (x, x, (y, x)), (x[:, :, :4], x[:, :, 3:], (x[:, :, :4], x[:, :, 3:])), (x[:, :5], x[:, 4:], (x[:, :5], x[:, 4:])),
+                      (x, y, (x, x.as_strided(x.shape, (0, 128, 64, 1))))):
+        with pytest.raises(NcclError):
+            cp.rotary(q, k, freqs, out=out)
+
+
+def test_numbers_in_tensors_are_read_by_every_call(cp):
+    q, k, v = operands(1, 40, 90, 2, 2, 64)
+    scale, offset = torch.tensor(0.5), torch.tensor(3)
+    for s, o in ((0.5, 3), (0.25, 40)):
+        scale.fill_(s)
+        offset.fill_(o)
+        got, want = cp.attention(q, k, v, causal=True, offset=offset, scale=scale), cp.attention(q, k, v, causal=True, offset=o, scale=s)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(TypeError):
+        cp.attention(q, k, v, causal=True, offset=2.5)
+
+
 # ------------------------------------------------------------------------------------------------ graphs, streams, threads
 def test_graphs_and_streams(cp):
     """Two captured calls with workspaces of their own, replayed in turn with new inputs, beside eager ones on another stream."""
