@@ -240,8 +240,9 @@ static void fillAttention(const ncclCpAttention_t* c, const int* qLengths, const
 // with the mean number of tiles (of which a CTA with one tile of queries makes two at a time, for 1.15 of the time), the longest CTA at least, and a constant for a CTA's beginning
 // and end. Measured with inputs from memory, us, pairs and single tiles (32 heads over 8 of 128 channels where nothing else is said): 2048 x 2048 78, 94; the same, causal 49, 66;
 // 4096 causal 139, 168; 1024 x 4096 70, 80; 1500 x 8192 242, 205; 3000 x 3000 of 10 heads over 2, causal 55, 41; 3 x 777 x 1013 of 12 heads over 4, 80 channels 27, 37.
-// Parts cost a second kernel and the partial results, 5 us, and pay where they save more tiles than that; then as many as there are SMs for. Measured on inputs in L2, us, one part and
-// by the rule: one head of 2048 x 2048 21.5, 16.1; 33 on 4000, 28 heads over 4 35.3, 16.6; 300 on 4000, 4 heads 35.6, 17.9; 128 on 65536, one head 445, 20.5 (32 parts 27); two on
+// Parts cost a second kernel and the partial results, and pay where they save more tiles than that, 5 to 9 by the number of rows; then as many as there are SMs for. Measured on inputs
+// in L2, us, one part and by the rule (where it makes none: in parts): one query of 32 heads over 8 on 1024 keys 14.1, 12.3, on 768 (12.0); 256 of 4 heads over 2 on 1024 (14.6; 15.6), on
+// 1280 16.1, 15.4; 1024 of 4 heads on 1024 (14.8; 16.9), on 2048 21.8, 19.2; one head of 2048 x 2048 21.5, 16.1; 33 on 4000, 28 heads over 4 35.3, 16.6; 300 on 4000, 4 heads 35.6, 17.9; 128 on 65536, one head 445, 20.5 (32 parts 27); two on
 // 16384, 2 heads 118, 13.6; one on 512 keys, 4 heads of 64 channels 8.7 in one part, which stays so.
 struct ForwardPlan {
   bool pairs;
@@ -266,7 +267,7 @@ static ForwardPlan forwardPlan(const ncclCpContext* cp, const ncclCpAttention_t*
   p.splits = 1;
   if (!p.pairs && ctas && ctas < sms) {
     const int most = (int)std::min<long long>({sms / ctas, (long long)longest / 2, kAttnMaxSplits});
-    if (most > 1 && longest * (1.0 - 1.0 / most) > 8.0) p.splits = most;
+    if (most > 1 && longest * (1.0 - 1.0 / most) > 5.0 + std::min(4.0, (double)c->batch * c->q_tokens * c->heads / 500)) p.splits = most;
   }
   return p;
 }
