@@ -79,13 +79,13 @@ __device__ __forceinline__ void mmaTS(uint32_t d, uint32_t aTmem, uint32_t b, ui
       ::"r"(d), "r"(aTmem), "r"(b), "r"(idesc), "r"(kDescHigh), "r"(accumulate) : "memory");
 }
 // D[128 x N] = A B^T over DP channels of two tiles in shared memory, from the lower words of their descriptors (descAlong).
-template <typename T, int DP, int N = 128>
+// AHalf: bytes from A's first 64 channels to the next.
+template <typename T, int DP, int N = 128, uint32_t AHalf = kHalfTile>
 __device__ __forceinline__ void productOfTiles(uint32_t d, uint32_t a, uint32_t b) {
   mmaSS<true>(d, a, b, instr<T>(N, false));
 #pragma unroll
   for (int k = 1; k < DP / 16; ++k) {
-    const uint32_t at = ((k / 4) * kHalfTile + (k % 4) * 32) >> 4;
-    mmaSS<false>(d, a + at, b + at, instr<T>(N, false));
+    mmaSS<false>(d, a + (((k / 4) * AHalf + (k % 4) * 32) >> 4), b + (((k / 4) * kHalfTile + (k % 4) * 32) >> 4), instr<T>(N, false));
   }
 }
 // D[128 x DP] (+)= A B with A [128 x 128] in tensor memory, 16 bits a value, columns [0, 64) of the sum at `a`, the others 64 columns on; B (descAcross) 128 rows of DP channels.

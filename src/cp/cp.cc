@@ -18,7 +18,7 @@ using namespace b200;
 struct ncclCpContext {
   ncclComm* comm = nullptr;
   int smCount = 0;
-  std::atomic<const void*> ready[16] = {};   // kernels with tiles that have been set up on this GPU
+  std::atomic<const void*> ready[32] = {};   // kernels with tiles that have been set up on this GPU
 };
 
 // The context's GPU is the current one while this lives.
@@ -233,19 +233,24 @@ static void fillAttention(const ncclCpAttention_t* c, const int* qLengths, const
   a->splits = 1;
 }
 
-// How a forward call is cut up: CTAs with two tiles of queries each ("pairs"), or with one whose keys their two halves share; and there, with few CTAs, into how many parts
-// the keys of a tile.
+// How a forward call is cut up: CTAs with two tiles of queries each ("pairs"), with one whose keys their two halves share, or with at most 32 rows, two to an SM ("few"); and with few
+// CTAs, or long keys, into how many parts the keys of a tile.
 //
 // Pairs move half as many keys, CTAs with one tile fill the SMs better. Both are estimated in units of what a pair takes for a tile of keys (2 us, 128 channels): waves of CTAs, each
 // with the mean number of tiles (of which a CTA with one tile of queries makes two at a time, for 1.15 of the time), the longest CTA at least, and a constant for a CTA's beginning
 // and end. Measured with inputs from memory, us, pairs and single tiles (32 heads over 8 of 128 channels where nothing else is said): 2048 x 2048 78, 94; the same, causal 49, 66;
 // 4096 causal 139, 168; 1024 x 4096 70, 80; 1500 x 8192 242, 205; 3000 x 3000 of 10 heads over 2, causal 55, 41; 3 x 777 x 1013 of 12 heads over 4, 80 channels 27, 37.
-// Parts cost a second kernel and the partial results, and pay where they save more tiles than that, 5 to 9 by the number of rows; then as many as there are SMs for. Measured on inputs
-// in L2, us, one part and by the rule (where it makes none: in parts): one query of 32 heads over 8 on 1024 keys 14.1, 12.3, on 768 (12.0); 256 of 4 heads over 2 on 1024 (14.6; 15.6), on
-// 1280 16.1, 15.4; 1024 of 4 heads on 1024 (14.8; 16.9), on 2048 21.8, 19.2; one head of 2048 x 2048 21.5, 16.1; 33 on 4000, 28 heads over 4 35.3, 16.6; 300 on 4000, 4 heads 35.6, 17.9; 128 on 65536, one head 445, 20.5 (32 parts 27); two on
-// 16384, 2 heads 118, 13.6; one on 512 keys, 4 heads of 64 channels 8.7 in one part, which stays so.
+// Parts cost a second kernel and the partial results, and pay where they save more tiles than that, 5 to 9 by the number of rows (few: 3 to 7); then as many as there are places for.
+// Measured on inputs in L2, us, one part and by the rule (where it makes none: in parts): 256 of 4 heads over 2 on 1024 (14.6; 15.6), on 1280 16.1, 15.4; 1024 of 4 heads on 1024
+// (14.8; 16.9), on 2048 21.8, 19.2; one head of 2048 x 2048 21.5, 16.1; 33 on 4000, 28 heads over 4 35.3, 16.6; 300 on 4000, 4 heads 35.6, 17.9; 128 on 65536, one head 445, 20.5 (32
+// parts 27).
+//
+// Few rows, 32 heads over 8: the single form and this one, single queries on keys for all lengths from one on: 128 on up to 1024 92, 68; 64 on up to 8192 186, 183; 20 on up to 16384 134, 123;
+// 16 on up to 4096 39, 41; 8 heads of 64 channels, 256 on up to 2048 184, 125. On 4096 keys one query 15, 12; 16 each 50, 50. Where lengths differ a CTA of a long sequence
+// would be waited for, hence parts of about 16 tiles there, for no more than 7 CTAs to a place, whatever the lengths, which only the GPU knows: in one part 64 on up to 8192 198 and 20 on
+// up to 16384 211, but of 8192 keys each 64 take 316 and not 327. One query on 768 keys in one part 13.6, by the rule 10.2; on 512 10.5 in one, which stays so.
 struct ForwardPlan {
-  bool pairs;
+  AttnForm form;
   int splits;
 };
 static double estimate(double ctas, int sms, double mean, double longest, double constant) {
@@ -263,12 +268,15 @@ static ForwardPlan forwardPlan(const ncclCpContext* cp, const ncclCpAttention_t*
   const auto tilesUpTo = [&](long long tok) { return (double)((c->mask == NCCL_CP_FULL ? c->kv_tokens : std::max(0ll, std::min<long long>(c->kv_tokens, tok + offset))) + 127) / 128; };
   const double longest = std::floor(tilesUpTo(c->q_tokens)), mean = (longest + std::floor(tilesUpTo(a.tileTokens))) / 2;
   ForwardPlan p;
-  p.pairs = a.tiles > 1 && estimate(pairCtas, sms, mean, longest, 1.0) <= estimate(ctas, sms, 1.15 * mean / 2, 1.15 * longest / 2, 2.0);
+  const bool pairs = a.tiles > 1 && estimate(pairCtas, sms, mean, longest, 1.0) <= estimate(ctas, sms, 1.15 * mean / 2, 1.15 * longest / 2, 2.0);
+  p.form = pairs ? ATTN_PAIRS : a.tiles * a.tileTokens * a.group <= kFewRows ? ATTN_FEW : ATTN_SINGLE;
   p.splits = 1;
-  if (!p.pairs && ctas && ctas < sms) {
-    const int most = (int)std::min<long long>({sms / ctas, (long long)longest / 2, kAttnMaxSplits});
-    if (most > 1 && longest * (1.0 - 1.0 / most) > 5.0 + std::min(4.0, (double)c->batch * c->q_tokens * c->heads / 500)) p.splits = most;
-  }
+  const int places = p.form == ATTN_FEW ? 2 * sms : sms;
+  if (pairs || !ctas) return p;
+  long long most = places / ctas;
+  if (p.form == ATTN_FEW) most = std::max(most, std::min((long long)longest / 16, 7 * places / ctas));
+  most = std::min({most, (long long)longest / 2, (long long)kAttnMaxSplits});
+  if (most > 1 && longest * (1.0 - 1.0 / most) > (p.form == ATTN_FEW ? 3.0 : 5.0) + std::min(4.0, (double)c->batch * c->q_tokens * c->heads / 500)) p.splits = (int)most;
   return p;
 }
 // How many threads share four channels of a row's parts in the kernel that joins them: as many as there are parts while that makes no more than 512 threads for an SM, and for each no
@@ -439,8 +447,9 @@ ncclResult_t ncclCpAttention(ncclCp_t cp, const ncclCpAttention_t* c, const void
   NCCLCHECK(makeMap(&maps[1], c, k, c->kv_tokens, c->kv_heads, c->k_stride, kAttnRows, 1));
   NCCLCHECK(makeMap(&maps[2], c, v, c->kv_tokens, c->kv_heads, c->v_stride, kAttnRows, 1));
   void* args[4] = {&maps[0], &maps[1], &maps[2], &a};
-  const unsigned grid = (unsigned)c->batch * c->kv_heads * (plan.pairs ? (a.tiles + 1) / 2 : a.tiles) * plan.splits;
-  NCCLCHECK(launchCp(cp, attnForwardKernelFn(type, c->head_dim, plan.pairs), grid, 1, attnForwardThreads(), attnForwardSmemBytes(c->head_dim, plan.pairs), args, stream, attnForwardRegs()));
+  const unsigned grid = (unsigned)c->batch * c->kv_heads * (plan.form == ATTN_PAIRS ? (a.tiles + 1) / 2 : a.tiles) * plan.splits;
+  NCCLCHECK(launchCp(cp, attnForwardKernelFn(type, c->head_dim, plan.form), grid, 1, attnForwardThreads(plan.form), attnForwardSmemBytes(c->head_dim, plan.form), args, stream,
+                     attnForwardRegs(plan.form)));
   if (plan.splits == 1) return ncclSuccess;
   const int quads = c->head_dim / 4;
   a.joinShares = joinShares(cp, rows, quads, plan.splits);

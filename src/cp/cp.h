@@ -80,15 +80,18 @@ struct RotaryArgs {
 constexpr int kRotaryAngles = 256;   // of a CTA at a time
 
 enum AttnType : int { ATTN_F16 = 0, ATTN_BF16 = 1, ATTN_F32 = 2 };
-// dim <= 64 or <= 128. `pairs`: two tiles of queries for each CTA; else one, whose keys its two halves share.
-const void* attnForwardKernelFn(int type, int dim, bool pairs);
-size_t attnForwardSmemBytes(int dim, bool pairs);
+// Two tiles of queries for each CTA; one, whose keys its two halves share; or one of at most kFewRows rows, for two CTAs to an SM.
+enum AttnForm : int { ATTN_PAIRS = 0, ATTN_SINGLE = 1, ATTN_FEW = 2 };
+constexpr int kFewRows = 32;
+// dim <= 64 or <= 128.
+const void* attnForwardKernelFn(int type, int dim, AttnForm form);
+size_t attnForwardSmemBytes(int dim, AttnForm form);
 const void* attnJoinKernelFn(int type);
 const void* attnBackwardKernelFn(int type, int dim, bool fine);
 size_t attnBackwardSmemBytes(int dim);
-int attnForwardThreads();
+int attnForwardThreads(AttnForm form);
 int attnBackwardThreads();
-int attnForwardRegs();     // that a thread is launched with
+int attnForwardRegs(AttnForm form);   // that a thread is launched with
 int attnBackwardRegs();
 const void* attnSumKernelFn(int type);
 const void* attnStatsKernelFn(int type, int dim);

@@ -62,6 +62,29 @@ def test_join(cp, Q, K, dtype):
     check("out in place", mine[0], wide.out, wide.out_tol)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("B,Q,K,H,G,D,causal,q_lengths,kv_lengths", [
+    (3, 4, 1000, 16, 2, 128, True, (4, 0, 2), (1000, 0, 129)), (2, 32, 300, 1, 1, 64, True, None, (300, 17)), (2, 33, 300, 2, 2, 64, True, None, (300, 17)),
+    (2, 6, 260, 15, 3, 40, False, (6, 1), (1, 260)), (40, 1, 2200, 32, 8, 128, True, None, None), (1, 1, 9000, 2, 1, 96, False, None, (8999,)), (4, 1, 5000, 32, 1, 16, True, None, (1, 128, 4097, 4999)),
+    (300, 1, 140, 2, 2, 64, True, None, None)])
+def test_few_rows(cp, dtype, B, Q, K, H, G, D, causal, q_lengths, kv_lengths):
+    q, k, v = operands(B, Q, K, H, G, D, dtype)
+    if B == 40:
+        kv_lengths = [(i * 977) % (K + 1) for i in range(B)]
+    ql, kl = None if q_lengths is None else lens(*q_lengths), None if kv_lengths is None else lens(*kv_lengths)
+    rule = dict(causal=causal, q_lengths=ql, kv_lengths=kl)
+    got = cp.attention(q, k, v, **rule)
+    ref = Reference(q, k, v, causal, None, None, ql, kl)
+    check("lse", got[1], ref.lse, ref.lse_tol)
+    check("out", got[0], ref.out, ref.out_tol)
+    join = randn(B, Q, H, D, dtype=F32, seed=5), randn(B, H, Q, dtype=F32, seed=6)
+    for result in (dtype, F32):
+        got = cp.attention(q, k, v, join=join, dtype=result, **rule)
+        ref = Reference(q, k, v, causal, None, None, ql, kl, join=join, result=result)
+        check("lse", got[1], ref.lse, ref.lse_tol)
+        check("out", got[0], ref.out, ref.out_tol)
+
+
 def test_join_of_blocks_is_the_whole(cp):
     """What a ring does: keys in three blocks, the middle one seen in part, the last by no one."""
     q, k, v = operands(2, 300, 900, 6, 3, 96)
