@@ -15,8 +15,8 @@
 // What bounds it: products and elements of a tile alternate in part; a tile takes about 2900 cycles (keys) and 2450 (queries), of which the tensor cores work 2048 and 1536 at 128 channels. 8192 causal tokens of
 // 32 heads over 8 take 1372 us after a rest, 4096 383 under a profiler, tensor cores busy 69 % of it; five products of what is seen would be 837 and 209.
 //
-// fp16: probabilities are held times 2^15, ds times a power of two that brings the largest that it could be (by the longest rows of do and v) to 2^15; the sums are in
-// fp32 and are multiplied back.
+// fp16: probabilities are held times 2^15, ds times a power of two that brings the largest that it could be (by the longest rows of do and v, and the largest delta) to 2^15; the sums
+// are in fp32 and are multiplied back.
 #include "attention.cuh"
 
 namespace b200 {
@@ -35,22 +35,28 @@ template <int DP> struct BackwardShape {
   static_assert(kBytes <= 227 * 1024 && (2 * kStages + 13) * 8 + 8 <= 1024, "shared memory");
 };
 
-// The power of two that ds is multiplied by, in fp16: |ds| <= p (|do.v| + |do.o|) <= 2 |do| |v|, by the longest rows of all tiles. (The bits of floats that are not negative
+// The power of two that ds is multiplied by, in fp16: |ds| <= p (|do.v| + |delta|) <= |do| |v| + |delta|, by the longest rows and the largest delta of all tiles. delta is not bounded by
+// |do| |v|: o is a mean of values of all of a row's keys, of which a call may have a block, and a gradient of the log-sum-exp may be in it. (The bits of floats that are not negative
 // are ordered as they are, NaN on top.)
 template <typename T>
 __device__ __forceinline__ float gradScale(const AttnArgs& a, int b, int kvHead) {
   if (Pack<T>::kBackwardBias == 0.0f) return 1.0f;
-  const uint32_t* at = a.bounds + ((size_t)b * a.kvHeads + kvHead) * (a.tiles + a.vTiles);
-  uint32_t longest[2] = {0, 0};   // do, v
+  const uint32_t* at = a.bounds + ((size_t)b * a.kvHeads + kvHead) * (2 * a.tiles + a.vTiles);
+  uint32_t largest[3] = {0, 0, 0};   // |do|^2, |delta|, |v|^2
 #pragma unroll 4
-  for (int i = threadIdx.x & 31; i < a.tiles; i += 32) longest[0] = max(longest[0], at[i]);
+  for (int i = threadIdx.x & 31; i < a.tiles; i += 32) {
+    largest[0] = max(largest[0], at[2 * i]);
+    largest[1] = max(largest[1], at[2 * i + 1]);
+  }
 #pragma unroll 4
-  for (int i = threadIdx.x & 31; i < a.vTiles; i += 32) longest[1] = max(longest[1], at[a.tiles + i]);
-  const float most = 2.0f * sqrtf(__uint_as_float(__reduce_max_sync(~0u, longest[0]))) * sqrtf(__uint_as_float(__reduce_max_sync(~0u, longest[1])));
+  for (int i = threadIdx.x & 31; i < a.vTiles; i += 32) largest[2] = max(largest[2], at[2 * a.tiles + i]);
+#pragma unroll
+  for (uint32_t& x : largest) x = __reduce_max_sync(~0u, x);
+  const float most = fmaf(sqrtf(__uint_as_float(largest[0])), sqrtf(__uint_as_float(largest[2])), __uint_as_float(largest[1]));
   if (!(most > 0.0f) || most > 3.0e38f) return 1.0f;   // nothing to do, or nothing to save
   int e;
   frexpf(most, &e);                                     // most < 2^e
-  return exp2f((float)max(-100, min(100, 15 - e)));
+  return exp2f((float)max(-113, min(100, 15 - e)));
 }
 
 struct BackwardBars {
@@ -665,8 +671,8 @@ __global__ void __launch_bounds__(256) attnSumKernel(const __grid_constant__ Att
 
 // ---------------------------------------------------------------------------------------------- what both need of each row of queries
 // Minus <do, o> (unless that is given: minus what is), and minus the log-sum-exp in units of log 2, laid out as the tiles are. Rows that nobody has, and rows that
-// see no key, get an infinite log-sum-exp: their probabilities are zero. A CTA takes a tile, 8 or 16 lanes a row, a pack of 16 bytes each. fp16: the longest row of do in it,
-// and by the CTAs behind those of every 128 rows of v. Bound by its loads and their first use: 4096 tokens of 32 heads of 128 channels 20 us (68 MB, 42 % of memory's rate), 8192 33 us; with loads
+// see no key, get an infinite log-sum-exp and a delta of zero: their probabilities and ds are zero. A CTA takes a tile, 8 or 16 lanes a row, a pack of 16 bytes each. fp16: the longest
+// row of do and the largest delta in it, and by the CTAs behind those the longest of every 128 rows of v. Bound by its loads and their first use: 4096 tokens of 32 heads of 128 channels 20 us (68 MB, 42 % of memory's rate), 8192 33 us; with loads
 // that a condition guards row by row it took twice that.
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256, 4) attnStatsKernel(const __grid_constant__ AttnStatsArgs a) {
@@ -692,23 +698,28 @@ __global__ void __launch_bounds__(256, 4) attnStatsKernel(const __grid_constant_
   const bool ofV = blockIdx.x >= qTiles;   // 128 rows of v instead of a tile
   const unsigned block = ofV ? blockIdx.x - qTiles : blockIdx.x, owner = block % owners;
   const int tile = block / owners, kvHead = owner % a.kvHeads, b = owner / a.kvHeads;
-  uint32_t most = 0;   // the squared norm of the longest row, as bits
-  // The CTA's into place `to`.
-  auto longest = [&](int to) {
-    __shared__ uint32_t ofWarp[8];
+  uint32_t most = 0, mostDelta = 0;   // the squared norm of the longest row, and the largest |delta|, as bits
+  // The CTA's into their places.
+  auto largest = [&] {
+    __shared__ uint32_t ofWarp[2][8];
     most = __reduce_max_sync(~0u, most);
-    if (threadIdx.x % 32 == 0) ofWarp[threadIdx.x / 32] = most;
+    mostDelta = __reduce_max_sync(~0u, mostDelta);
+    if (threadIdx.x % 32 == 0) {
+      ofWarp[0][threadIdx.x / 32] = most;
+      ofWarp[1][threadIdx.x / 32] = mostDelta;
+    }
     __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int i = 1; i < 8; ++i) most = max(most, ofWarp[i]);
-      a.bounds[(size_t)owner * (a.tiles + a.vTiles) + to] = most;
+    if (threadIdx.x < (ofV ? 1 : 2)) {
+      uint32_t all = 0;
+      for (int i = 0; i < 8; ++i) all = max(all, ofWarp[threadIdx.x][i]);
+      a.bounds[(size_t)owner * (2 * a.tiles + a.vTiles) + (ofV ? 2 * a.tiles + tile : 2 * tile + threadIdx.x)] = all;
     }
   };
   pdlEnter();
   if (ofV) {
     const int used = a.kvLengths ? min(a.kvLengths[b], a.kv) : a.kv;
     if (tile * 128 >= used) {
-      longest(a.tiles + tile);
+      largest();
       return;
     }
     const long long base = b * a.vStride[0] + kvHead * a.vStride[2];
@@ -721,7 +732,7 @@ __global__ void __launch_bounds__(256, 4) attnStatsKernel(const __grid_constant_
         most = max(most, __float_as_uint(dot(x[n], x[n])) & 0x7fffffffu);
       }
     }
-    longest(a.tiles + tile);
+    largest();
     return;
   }
   const int used = a.qLengths ? max(0, min(a.qLengths[b], a.q)) : a.q, tok0 = tile * a.tileTokens, rows = a.tileTokens * a.group;
@@ -753,6 +764,8 @@ __global__ void __launch_bounds__(256, 4) attnStatsKernel(const __grid_constant_
         delta[n] = 0.0f;
         lse[n] = -INFINITY;
       }
+      if (a.stats && lse[n] == -INFINITY) delta[n] = 0.0f;   // (of a row that sees no key it may have been given as anything)
+      if (a.bounds) mostDelta = max(mostDelta, __float_as_uint(delta[n]) & 0x7fffffffu);
       if (a.stats && lane == 0) {
         to[row - row0] = lse[n] == -INFINITY ? -INFINITY : fmaf(lse[n], -kLog2e, Pack<T>::kBackwardBias);
         to[row - row0 + 128] = -delta[n];
@@ -763,7 +776,7 @@ __global__ void __launch_bounds__(256, 4) attnStatsKernel(const __grid_constant_
       }
     }
   }
-  if (a.bounds) longest(tile);
+  if (a.bounds) largest();
 }
 
 }  // namespace

@@ -334,7 +334,7 @@ static BackwardPlan backwardPlan(const ncclCpContext* cp, const ncclCpAttention_
 }
 
 static size_t statsBytes(const AttnArgs& a) { return (size_t)a.batch * a.kvHeads * a.tiles * 256 * 4; }
-static size_t boundsBytes(const ncclCpAttention_t* c, const AttnArgs& a) { return isFp16(c) ? ((size_t)c->batch * c->kv_heads * (a.tiles + (c->kv_tokens + kAttnRows - 1) / kAttnRows) * 4 + 255) / 256 * 256 : 0; }
+static size_t boundsBytes(const ncclCpAttention_t* c, const AttnArgs& a) { return isFp16(c) ? ((size_t)c->batch * c->kv_heads * (2 * a.tiles + a.vTiles) * 4 + 255) / 256 * 256 : 0; }
 static size_t dqBytes(const ncclCpAttention_t* c) { return (size_t)c->batch * c->q_tokens * c->heads * c->head_dim * 4; }
 static size_t dkBytes(const ncclCpAttention_t* c) { return (size_t)c->batch * c->kv_tokens * c->kv_heads * c->head_dim * 4; }
 // Numbers of each row, norms, and the sums of parts.

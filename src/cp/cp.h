@@ -34,7 +34,7 @@ struct AttnArgs {
   // backward
   const float* stats;         // [batch][kvHeads][tiles][2][128]: minus the log-sum-exp in units of log 2 and minus <d(out), out> of each row
   int tiles;                  // of the queries of a key head
-  const uint32_t* bounds;     // fp16: [batch][kvHeads][tiles of d(out), then of v] squared norms of a tile's longest row, as bits
+  const uint32_t* bounds;     // fp16: [batch][kvHeads][tiles of queries: squared norm of the longest row of d(out), largest |delta|; then tiles of v: squared norm], as bits
   int vTiles;
   void *dq, *dk, *dv;         // contiguous, of the inputs' type or fp32
   int gradFp32;
