@@ -160,6 +160,13 @@ class ContextParallel:
             raise ValueError("%s must be on cuda:%d, at a multiple of 16 bytes, not on %s at %#x" % (name, self._device, t.device, p))
         return p
 
+    @staticmethod
+    def _tuple(name, given, n):
+        given = tuple(given)
+        if len(given) != n:
+            raise ValueError("%s must be %d tensors, not %d" % (name, n, len(given)))
+        return given
+
     def _lengths(self, name, t, batch):
         if t is None:
             return None
@@ -241,6 +248,7 @@ class ContextParallel:
         nq, nk = self._lengths("q_lengths", q_lengths, B), self._lengths("kv_lengths", kv_lengths, B)
         join_out = join_lse = None
         if join is not None:
+            join = self._tuple("join", join, 2)
             self._need("join[0]", join[0], torch.float32, (B, Q, H, D))
             self._need("join[1]", join[1], torch.float32, (B, H, Q))
             join_out, join_lse = join[0].data_ptr(), join[1].data_ptr()
@@ -295,6 +303,7 @@ class ContextParallel:
         sq, sk = (B, Q, H, D), (B, K, G, D)
         given = (None, None, None)
         if add is not None:
+            add = self._tuple("add", add, 3)
             for name, t, shape in zip(("add[0]", "add[1]", "add[2]"), add, (sq, sk, sk)):
                 self._need(name, t, torch.float32, shape)
             given = [t.data_ptr() for t in add]
