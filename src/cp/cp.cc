@@ -297,13 +297,15 @@ static size_t forwardWork(const ncclCpAttention_t* c, const ForwardPlan& p) {
 // 512 causal tokens of 8 heads over one, 64 channels 55, 23; where it makes none parts would cost: 509 x 641, 3 times 12 heads over 4, 96 channels 53, in two parts 62 and more.
 //
 // Gradients have two roundings to 16 bits: of ds (dv: of the probabilities) and of what is stored, 1.4 times the second alone on average. Where an output has few rows, or few terms
-// that cancel, that is 1.55 times now and then. Calls of few products multiply what the first rounding left as well ("fine"): one query on 512 keys 14.6 us instead of 12.5, 2 x 256
-// causal tokens of 8 heads of 64 12.8 instead of 10.8; beyond that it would cost more (512 causal tokens of 8 heads 23.8 instead of 17.9, 1024 of 4 36.4 instead of 23.6).
+// that cancel, that is 1.55 times now and then. Calls that do not fill the GPU multiply what the first rounding left as well ("fine"). Each product of tiles is made by two CTAs, one that
+// owns the keys and one that owns the queries: while the SMs have a place for each of them, more products only make a CTA longer; beyond they add to what all SMs have to do. us, without
+// and with, on 148 SMs: 1 query on 512 keys 16.0, 17.7; 2 x 256 causal tokens of 8 heads of 64 10.9, 12.7; 250 of 18 heads of 64 (72 products, with by this rule) 10.8, 12.8, of 19 (76,
+// without) 10.8, 12.9; 512 of 8 heads (128) 18.5, 23.6, of 64 channels 13.4, 17.3; 1024 of 4 heads (256) 23.6, 36.4.
 struct BackwardPlan {
   int kvParts, qParts;
 };
-static bool fineProducts(const ncclCpAttention_t* c, const AttnArgs& a) {
-  return (double)c->batch * c->kv_heads * a.tiles * std::ceil(c->kv_tokens / 128.0) <= 64;   // products of 128 x 128
+static bool fineProducts(const ncclCpContext* cp, const ncclCpAttention_t* c, const AttnArgs& a) {
+  return 2.0 * c->batch * c->kv_heads * a.tiles * a.vTiles <= cp->smCount;   // tiles of queries and of keys that meet, masks aside
 }
 static BackwardPlan backwardPlan(const ncclCpContext* cp, const ncclCpAttention_t* c, const AttnArgs& a) {
   const double owners = (double)c->batch * c->kv_heads, keyTiles = std::ceil(c->kv_tokens / 128.0), sms = cp->smCount;
@@ -544,7 +546,7 @@ ncclResult_t ncclCpAttentionBackward(ncclCp_t cp, const ncclCpAttention_t* c, co
   void* args[5] = {&maps[0], &maps[1], &maps[2], &maps[3], &a};
   const unsigned owners = (unsigned)c->batch * c->kv_heads, keyTiles = (c->kv_tokens + kAttnRows - 1) / kAttnRows;
   a.kvCtas = owners * keyTiles * plan.kvParts;
-  NCCLCHECK(launchCp(cp, attnBackwardKernelFn(type, c->head_dim, fineProducts(c, a)), a.kvCtas + owners * a.tiles * plan.qParts, 1, attnBackwardThreads(),
+  NCCLCHECK(launchCp(cp, attnBackwardKernelFn(type, c->head_dim, fineProducts(cp, c, a)), a.kvCtas + owners * a.tiles * plan.qParts, 1, attnBackwardThreads(),
                      attnBackwardSmemBytes(c->head_dim), args, stream, attnBackwardRegs()));
   const size_t sumRows = (plan.qParts > 1 ? rows : 0) + (plan.kvParts > 1 ? 2 * cols : 0);
   if (!sumRows) return ncclSuccess;
