@@ -660,7 +660,7 @@ ncclResult_t ncclCpRotary(ncclCp_t cp, const ncclCpRotary_t* c, const void* x0, 
   a.items = (a.interleaved && a.wide ? 2 * a.half : a.half) / width + (a.dim - 2 * a.half) / width;
   const int most = std::max(1, kRotaryAngles / a.half);
   a.tokensAtOnce = std::max(1, std::min(most, tokens / (4 * cp->smCount)));
-  const int blocks = (tokens + a.tokensAtOnce - 1) / a.tokensAtOnce;
+  const int blocks = (tokens - 1) / a.tokensAtOnce + 1;   // (tokens may be 2^31 - 1)
   const int shares = std::max(1, std::min({cp->smCount / blocks, (heads * a.items + 255) / 256, 64}));
   void* args[1] = {&a};
   return launchCp(cp, rotaryKernelFn(type), (unsigned)blocks, (unsigned)shares, 256, 0, args, stream);

@@ -35,7 +35,10 @@ __device__ __forceinline__ void turnHeads(const RotaryArgs& a, int token0, int t
   const int paired = neighbours ? 2 * a.half / E : a.half / E, heads = a.heads[0] + a.heads[1];
   const int stride = gridDim.y * blockDim.x, first = blockIdx.y * blockDim.x + threadIdx.x;
   const int stepRows = stride / a.items, stepP = stride % a.items, stepTokens = stepRows / heads, stepHeads = stepRows % heads;
-  int p = first % a.items, row = first / a.items, local = row / heads, head = row % heads, b = (token0 + local) / a.tokens, tok = token0 + local - b * a.tokens;
+  int p = first % a.items, row = first / a.items, local = row / heads, head = row % heads;
+  const unsigned each = a.tokens, token = (unsigned)token0 + local;   // (one behind the last may be 2^31 or more)
+  unsigned tok = token % each;
+  int b = token / each;
   while (local < tokens) {
     const int which = head >= a.heads[0];
     const long long h = which ? head - a.heads[0] : head;
@@ -80,7 +83,7 @@ __device__ __forceinline__ void turnHeads(const RotaryArgs& a, int token0, int t
       ++more;
     }
     local += more;
-    for (tok += more; tok >= a.tokens; tok -= a.tokens) ++b;
+    for (tok += more; tok >= each; tok -= each) ++b;
   }
 }
 
