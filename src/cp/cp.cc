@@ -170,11 +170,12 @@ static EncodeTiledFn encodeFn() {
 
 static bool isFp16(const ncclCpAttention_t* c) { return c->type == ncclFloat16; }
 
-// [batch][tokens][heads][dim], boxes of `boxTokens` tokens x `boxHeads` heads x 64 channels with 128-byte swizzle. A tensor without tokens is never read: its map names one.
+// [batch][tokens][heads][dim], boxes of `boxTokens` tokens x `boxHeads` heads x 64 channels with 128-byte swizzle. A tensor without tokens is never read, and its strides are anything:
+// its map names one row.
 static ncclResult_t makeMap(CUtensorMap* map, const ncclCpAttention_t* c, const void* base, int tokens, int heads, const long long* stride, int boxTokens, int boxHeads) {
   EncodeTiledFn enc = encodeFn();
   if (!enc) { WARN("cuTensorMapEncodeTiled is not available"); return ncclUnhandledCudaError; }
-  const int sizes[3] = {heads, std::max(tokens, 1), c->batch};
+  const int sizes[3] = {tokens ? heads : 1, tokens ? tokens : 1, tokens ? c->batch : 1};
   cuuint64_t dims[4] = {(cuuint64_t)c->head_dim, (cuuint64_t)sizes[0], (cuuint64_t)sizes[1], (cuuint64_t)sizes[2]};
   cuuint64_t strides[3];
   for (int i = 0; i < 3; ++i) strides[i] = sizes[i] > 1 ? (cuuint64_t)stride[2 - i] * 2 : (cuuint64_t)c->head_dim * 2;   // (of one there is no next)
