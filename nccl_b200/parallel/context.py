@@ -56,15 +56,15 @@ def _rows(t):
 
 
 class _Ring:
-    """Passes a tensor on to the next rank and takes the previous one's into another, on a GPU on a stream of its own."""
+    """Passes a tensor on to the next rank and takes the previous one's into another, on a GPU on a stream of its own. `device`: the tensors', which need not be the current one."""
 
     def __init__(self, comm, cuda, device, stream):
-        self.comm, self.cuda = comm, cuda
+        self.comm, self.cuda, self.device = comm, cuda, device
         self.nxt, self.prv = (comm.rank + 1) % comm.nranks, (comm.rank - 1) % comm.nranks
         self.stream = stream if stream is not None else (torch.cuda.Stream(device=device) if cuda and comm.nranks > 1 else None)
 
     def pass_on(self, send, recv):
-        """Behind what the current stream has been given so far; gives what to wait for before `recv` is read or `send` written (None: it is done)."""
+        """Behind what the device's current stream has been given so far; gives what to wait for before `recv` is read or `send` written (None: it is done)."""
         comm = self.comm
         if not self.cuda:
             with group(comm.lib):
@@ -72,7 +72,7 @@ class _Ring:
                 comm.recv(recv, self.prv)
             return None
         ready = torch.cuda.Event()
-        ready.record()                      # `recv` is no longer read, `send` is complete
+        ready.record(torch.cuda.current_stream(self.device))   # `recv` is no longer read, `send` is complete
         with torch.cuda.stream(self.stream):
             self.stream.wait_event(ready)
             with group(comm.lib):
@@ -82,10 +82,9 @@ class _Ring:
             done.record(self.stream)
         return done
 
-
-def _wait(done):
-    if done is not None:
-        torch.cuda.current_stream().wait_event(done)
+    def wait(self, done):
+        if done is not None:
+            torch.cuda.current_stream(self.device).wait_event(done)
 
 
 def ring_attention(comm, q, k, v, causal=False, stream=None, cp=None, with_lse=False):
@@ -125,7 +124,7 @@ def ring_attention(comm, q, k, v, causal=False, stream=None, cp=None, with_lse=F
             l_run = l_run * a_old + l_blk * a_blk
             o_run = o_run * a_old + o_blk * a_blk
             m_run = m_new
-        _wait(done)
+        ring.wait(done)
     if cp is not None:
         out, lse = joined[0].transpose(1, 2), joined[1]
         return (out, lse) if with_lse else out
@@ -160,7 +159,7 @@ def ring_attention_backward(comm, dout, q, k, v, out, lse, causal=False, stream=
         g = grads[step % 2]
         done = ring.pass_on(cur, other) if step + 1 < n else None
         src = (rank - step) % n
-        _wait(grads_done)
+        ring.wait(grads_done)
         if causal and src > rank:
             pass                                    # nothing of this block is visible here: its gradients only pass through
         elif cp is not None:
@@ -178,8 +177,8 @@ def ring_attention_backward(comm, dout, q, k, v, out, lse, causal=False, stream=
                 g[1].copy_(add[2])
         if n > 1:
             grads_done = ring.pass_on(g, grads[(step + 1) % 2])
-        _wait(done)
-    _wait(grads_done)
+        ring.wait(done)
+    ring.wait(grads_done)
     g = grads[n % 2 if n > 1 else 0].to(q.dtype)
     dq = dq.to(q.dtype)
     return (dq, g[0], g[1]) if cp is None else (dq.transpose(1, 2), g[0].transpose(1, 2), g[1].transpose(1, 2))

@@ -1,0 +1,61 @@
+"""What the ring and the Ulysses swap hand on, without a GPU: streams and events recorded, the kernels' calls recorded."""
+import contextlib
+import types
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+class FakeStream:
+    def __init__(self, name, log):
+        self.name, self.log = name, log
+
+    def wait_event(self, event):
+        self.log.append((self.name, "waits for", event.on))
+
+
+class FakeComm:
+    nranks, rank, lib = 2, 0, None
+
+    def __init__(self, log):
+        self.log = log
+
+    def send(self, t, peer, stream=None):
+        self.log.append(("send", stream.name))
+
+    def recv(self, t, peer, stream=None):
+        self.log.append(("recv", stream.name))
+
+
+def test_the_ring_is_ordered_with_the_streams_of_its_own_gpu(monkeypatch):
+    """The exchange waits for what the tensors' GPU has been given, and that GPU's stream for the exchange, whichever GPU is the current one."""
+    from nccl_b200.parallel import context
+    log, entered = [], []
+    place = torch.device("cuda", 3)
+
+    class FakeEvent:
+        on = None
+
+        def record(self, stream=None):
+            self.on = (stream or torch.cuda.current_stream()).name
+
+    @contextlib.contextmanager
+    def enter(stream):
+        entered.append(stream)
+        yield
+        entered.pop()
+
+    def current_stream(device=None):
+        return entered[-1] if entered else FakeStream("main of %s" % ("the current GPU" if device is None else torch.device(device)), log)
+
+    monkeypatch.setattr(torch.cuda, "Event", FakeEvent)
+    monkeypatch.setattr(torch.cuda, "stream", enter)
+    monkeypatch.setattr(torch.cuda, "current_stream", current_stream)
+    monkeypatch.setattr(context, "group", lambda lib: contextlib.nullcontext())
+    ring = context._Ring(FakeComm(log), True, place, FakeStream("side", log))
+    done = ring.pass_on(torch.zeros(1), torch.zeros(1))
+    ring.wait(done)
+    assert log == [("side", "waits for", "main of cuda:3"), ("send", "side"), ("recv", "side"), ("main of cuda:3", "waits for", "side")]
+    ring.wait(None)
+    assert len(log) == 4
