@@ -228,6 +228,7 @@ def ulysses_attention(comm, q, k, v, causal=False, cp=None, with_state=False):
     have fewer heads (a multiple of the number of ranks)."""
     whole = [ulysses_scatter_heads(comm, t) for t in (q, k, v)]                           # [B, S_all, H/n, D]
     if cp is not None:
+        whole = [_rows(t.transpose(1, 2)) for t in whole]                                 # (of one rank: as they were given)
         o, lse = cp.attention(*whole, causal=causal, offset=0 if causal else None)
     else:
         qh, kh, vh = (t.transpose(1, 2) for t in whole)

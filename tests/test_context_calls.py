@@ -6,6 +6,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+from test_cp_arguments import cp, shape_at  # noqa: E402, F401
+
 
 class FakeStream:
     def __init__(self, name, log):
@@ -59,3 +61,21 @@ def test_the_ring_is_ordered_with_the_streams_of_its_own_gpu(monkeypatch):
     assert log == [("side", "waits for", "main of cuda:3"), ("send", "side"), ("recv", "side"), ("main of cuda:3", "waits for", "side")]
     ring.wait(None)
     assert len(log) == 4
+
+
+def test_ulysses_of_one_rank_takes_any_strides(cp):   # noqa: F811
+    """As with more ranks, where the swap lays the tensors out anew."""
+    from nccl_b200.parallel.context import ulysses_attention, ulysses_attention_backward
+    comm = types.SimpleNamespace(nranks=1, rank=0)
+    wide = [torch.randn(2, 5, heads, 20).bfloat16() for heads in (4, 2, 2)]
+    q, k, v = (t[..., :16] for t in wide)
+    out, state = ulysses_attention(comm, q, k, v, causal=True, cp=cp, with_state=True)
+    assert out.shape == q.shape
+    d = shape_at(cp.calls[0][2])
+    assert list(d.q_stride) == [320, 64, 16] and list(d.k_stride) == list(d.v_stride) == [160, 32, 16]
+    assert all(torch.equal(a, b) for a, b in zip(state[:3], (q, k, v)))
+    grads = ulysses_attention_backward(comm, wide[0][..., 4:], state, causal=True, cp=cp)
+    assert [g.shape for g in grads] == [t.shape for t in (q, k, v)] and cp.calls[1][0] == "ncclCpAttentionBackward"
+    fits = [t.contiguous() for t in (q, k, v)]
+    ulysses_attention(comm, *fits, cp=cp)
+    assert cp.calls[2][3:6] == tuple(t.data_ptr() for t in fits)   # what fits is read where it is
