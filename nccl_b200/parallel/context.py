@@ -52,7 +52,7 @@ def _rows(t):
     """[batch, heads, sequence, dim] as the kernels take it, [batch, sequence, heads, dim]; a copy where its rows are not where they can be read."""
     t = t.transpose(1, 2)
     fits = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape, t.stride()[:3]))
-    return t if fits else t.contiguous()
+    return t if fits else t.clone(memory_format=torch.contiguous_format)   # (a contiguous tensor may be off the grid)
 
 
 class _Ring:

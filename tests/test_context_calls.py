@@ -79,3 +79,26 @@ def test_ulysses_of_one_rank_takes_any_strides(cp):   # noqa: F811
     fits = [t.contiguous() for t in (q, k, v)]
     ulysses_attention(comm, *fits, cp=cp)
     assert cp.calls[2][3:6] == tuple(t.data_ptr() for t in fits)   # what fits is read where it is
+
+
+@pytest.mark.parametrize("recipe", ["ring", "ulysses"])
+def test_rows_off_the_16_byte_grid_are_copied(cp, recipe):   # noqa: F811
+    """Contiguous tensors, too, that begin where the kernels' copies cannot."""
+    from nccl_b200.parallel.context import ring_attention, ring_attention_backward, ulysses_attention, ulysses_attention_backward
+    comm = types.SimpleNamespace(nranks=1, rank=0, lib=None)
+
+    def off(*shape):   # [batch, sequence, heads, dim]
+        n = torch.Size(shape).numel()
+        flat = torch.randn(n + 8).bfloat16()
+        begin = next(i for i in range(1, 8) if (flat.data_ptr() + 2 * i) % 16)
+        return flat[begin:begin + n].view(shape)
+    q, k, v, dout = off(2, 5, 4, 16), off(2, 5, 2, 16), off(2, 5, 2, 16), off(2, 5, 4, 16)
+    if recipe == "ring":
+        q, k, v, dout = (t.transpose(1, 2) for t in (q, k, v, dout))
+        out, lse = ring_attention(comm, q, k, v, cp=cp, with_lse=True)
+        grads = ring_attention_backward(comm, dout, q, k, v, out, lse, cp=cp)
+    else:
+        out, state = ulysses_attention(comm, q, k, v, cp=cp, with_state=True)
+        grads = ulysses_attention_backward(comm, dout, state, cp=cp)
+    assert [g.shape for g in grads] == [t.shape for t in (q, k, v)]
+    assert all(p % 16 == 0 for call in cp.calls for p in call[3:5])
