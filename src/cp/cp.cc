@@ -227,7 +227,8 @@ static void fillAttention(const ncclCpAttention_t* c, const int* qLengths, const
   a->tiles = (c->q_tokens + a->tileTokens - 1) / a->tileTokens;
   a->vTiles = (c->kv_tokens + kAttnRows - 1) / kAttnRows;
   a->causal = (int)c->mask;
-  a->offset = (int)std::max<long long>(-(long long)c->q_tokens, std::min<long long>(c->offset, c->kv_tokens));   // further out nothing changes any more
+  // further out nothing changes any more (and a query's token, its offset and one more stay within 31 bits)
+  a->offset = (int)std::max<long long>(-(long long)c->q_tokens, std::min<long long>(c->offset, std::max(c->kv_tokens - 1, 0)));
   a->scale = c->scale;
   a->qLengths = qLengths;
   a->kvLengths = kvLengths;
