@@ -66,7 +66,7 @@ size_t ncclCpAttentionBackwardWork(ncclCp_t cp, const ncclCpAttention_t* shape);
 ncclResult_t ncclCpAttentionBackward(ncclCp_t cp, const ncclCpAttention_t* shape, const void* d_out, const void* q, const void* k, const void* v, const void* out, const float* lse,
                                      const float* delta, const int* q_lengths, const int* kv_lengths, const float* add_dq, const float* add_dk, const float* add_dv, void* d_q,
                                      void* d_k, void* d_v, void* work, cudaStream_t stream);
-/* delta = <d_out, out> of each row (zero behind the lengths). A gradient of lse itself is subtracted from it. */
+/* delta = <d_out, out> of each row (zero behind the lengths). A gradient of lse itself is subtracted from it, whatever its size; of queries that see no key delta is not used. */
 ncclResult_t ncclCpAttentionDelta(ncclCp_t cp, const ncclCpAttention_t* shape, const void* d_out, const void* out, const int* q_lengths, float* delta, cudaStream_t stream);
 
 /* Rotary positions. The first 2 * half channels of a head are pairs (i, i + half), with `interleaved` (2 i, 2 i + 1); pair (a, b) becomes

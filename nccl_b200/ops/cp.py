@@ -259,7 +259,8 @@ class ContextParallel:
         return out, lse
 
     def attention_delta(self, dout, out, q_lengths=None, delta=None):
-        """fp32 [batch, heads, queries]: <dout, out> of each row, which every backward call of these queries needs. Where the log-sum-exp has a gradient of its own, subtract it."""
+        """fp32 [batch, heads, queries]: <dout, out> of each row, which every backward call of these queries needs. Where the log-sum-exp has a gradient of its own, subtract it:
+        of any size, also in fp16. (Of queries that see no key what is here is not used.)"""
         if out.dim() != 4 or out.dtype not in (self.torch.float16, self.torch.bfloat16):
             raise ValueError("out must be an fp16 or bf16 tensor [batch, tokens, heads, channels], not %s %s" % (str(out.dtype).replace("torch.", ""), list(out.shape)))
         B, Q, H, D = out.shape
@@ -280,7 +281,7 @@ class ContextParallel:
         from ``lse``. Mask, scale and lengths as the forward call had them; rows behind the lengths get zeros.
 
         ``out`` and ``lse`` are the result over all keys of the queries: where blocks were joined, the last one's. ``delta``: what ``attention_delta`` gives (out may then be
-        None). ``add``: fp32 (dq, dk, dv) so far, to which these are added; they may be the results' tensors. The same call gives the same bits."""
+        None). A ``delta`` of any size, and one that the keys of other calls have a part in, are taken in fp16 too. ``add``: fp32 (dq, dk, dv) so far, to which these are added; they may be the results' tensors. The same call gives the same bits."""
         torch = self.torch
         causal, offset, scale = self._numbers(causal, offset, scale)
 

@@ -16,6 +16,9 @@ communicator's GPU), which never hold a block's scores in memory. Either way the
     out, state = ulysses_attention(comm, q, k, v, causal=True, cp=cp, with_state=True)
     dq, dk, dv = ulysses_attention_backward(comm, dout, state, causal=True, cp=cp)
 
+With ``cp`` results have no history for autograd, also where inputs require gradients: those come from the backward calls. (Without it they have the local one, which knows
+nothing of what other ranks do with this rank's keys and values.)
+
 Reference parity: the reference ships the primitives only (grouped ncclSend / ncclRecv ring of docs/examples/02_point_to_point/01_ring_pattern,
 ncclAlltoAll of src/collectives.cc).
 """

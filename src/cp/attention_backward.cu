@@ -13,7 +13,7 @@
 // "Fine" products, for calls that they cost little: what the rounding of probabilities and ds to 16 bits left is multiplied too. It lies over the scores, whose next tile then waits.
 //
 // What bounds it: products and elements of a tile alternate in part; a tile takes about 2900 cycles (keys) and 2450 (queries), of which the tensor cores work 2048 and 1536 at 128 channels. 8192 causal tokens of
-// 32 heads over 8 take 1372 us after a rest, 4096 383 under a profiler, tensor cores busy 69 % of it; five products of what is seen would be 837 and 209.
+// 32 heads over 8 take 1372 us after a rest and 1546 to 1631 pass after pass, 4096 383 under a profiler, tensor cores busy 69 % of it; five products of what is seen would be 837 and 209.
 //
 // fp16: probabilities are held times 2^15, ds times a power of two that brings the largest that it could be (by the longest rows of do and v, and the largest delta) to 2^15; the sums
 // are in fp32 and are multiplied back.
@@ -672,8 +672,9 @@ __global__ void __launch_bounds__(256) attnSumKernel(const __grid_constant__ Att
 // ---------------------------------------------------------------------------------------------- what both need of each row of queries
 // Minus <do, o> (unless that is given: minus what is), and minus the log-sum-exp in units of log 2, laid out as the tiles are. Rows that nobody has, and rows that
 // see no key, get an infinite log-sum-exp and a delta of zero: their probabilities and ds are zero. A CTA takes a tile, 8 or 16 lanes a row, a pack of 16 bytes each. fp16: the longest
-// row of do and the largest delta in it, and by the CTAs behind those the longest of every 128 rows of v. Bound by its loads and their first use: 4096 tokens of 32 heads of 128 channels 20 us (68 MB, 42 % of memory's rate), 8192 33 us; with loads
-// that a condition guards row by row it took twice that.
+// row of do and the largest delta in it, and by the CTAs behind those the longest of every 128 rows of v. Bound by its instructions, of which 73 % of the slots are issued: a reduction over the lanes for each row (fp16: two), divisions
+// by the group and addresses. 4096 tokens of 32 heads of 128 channels 19.6 us (68 MB, 43 % of memory's rate; fp16, with 8 key heads' values, 22.5), 8192 33 us; with loads that a condition
+// guards row by row it took twice that.
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256, 4) attnStatsKernel(const __grid_constant__ AttnStatsArgs a) {
   constexpr int kAtOnce = 256 / LANES, kTurns = 4;   // rows of the CTA, and of a thread with loads on their way

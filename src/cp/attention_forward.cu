@@ -12,8 +12,8 @@
 // parts for several CTAs, whose results a second kernel joins; so they may in the form for a decoder's few rows, below.
 //
 // What bounds it: at 128 channels a tile of 128 x 128 scores is 1024 cycles for the tensor cores and as many for its exponentials (16 a cycle), and takes 1800: a group's products, maximum
-// and exponentials depend on one another, and two groups hide that in part. 8192 x 8192 of 32 heads over 8, everything seen, 822 to 850 us (1.3 PFLOP/s), causal 441 to 453; the products
-// alone 635, all but the products 709. Single queries are bound by memory: 64 on 8192 keys each, 32 heads over 8, 2.1 GB, 316 to 327 us.
+// and exponentials depend on one another, and two groups hide that in part. 8192 x 8192 of 32 heads over 8, everything seen, 822 to 850 us after a rest (1.3 PFLOP/s), causal 441 to 453; the
+// products alone 635, all but the products 709. Pass after pass the power limit has the clock down, and it is 999 and 515 to 531 us. Single queries are bound by memory: 64 on 8192 keys each, 32 heads over 8, 2.1 GB, 316 to 327 us.
 //
 // Rows behind a tile's last are whatever shared memory held: they reach only results that nobody stores. Values behind a sequence's last key may be
 // anything (0 * NaN is NaN): zeros are written over them in shared memory.

@@ -238,6 +238,7 @@ static void fillAttention(const ncclCpAttention_t* c, const int* qLengths, const
 // How a forward call is cut up: CTAs with two tiles of queries each ("pairs"), with one whose keys their two halves share, or with at most 32 rows, two to an SM ("few"); and with few
 // CTAs, or long keys, into how many parts the keys of a tile.
 //
+// (All of it measured at 128 channels where nothing else is said; at 64 a tile costs half, and the units with it.)
 // Pairs move half as many keys, CTAs with one tile fill the SMs better. Both are estimated in units of what a pair takes for a tile of keys (2 us, 128 channels): waves of CTAs, each
 // with the mean number of tiles (of which a CTA with one tile of queries makes two at a time, for 1.15 of the time), the longest CTA at least, and a constant for a CTA's beginning
 // and end. Measured with inputs from memory, us, pairs and single tiles (32 heads over 8 of 128 channels where nothing else is said): 2048 x 2048 78, 94; the same, causal 49, 66;
